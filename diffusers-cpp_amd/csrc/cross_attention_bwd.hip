@@ -1,0 +1,618 @@
+// cross_attention_bwd.hip -- the gradients of cross_attention.hip's attention:
+//   P_ij = exp(s_ij - lse_i),  dP_ij = <dO_i, v_j>,  delta_i = sum_j P_ij dP_ij,
+//   dS = P (dP - delta),  dQ_i = scale sum_j dS_ij k_j,
+//   dK_j = scale sum_i dS_ij q_i,  dV_j = sum_i P_ij dO_i  (i over the query heads
+//   that share the key head),  dtable[t][h] = sum of dS over the pairs of bucket t.
+//
+// Two kernels recompute P instead of one that adds into dQ with atomics, so every sum
+// has a fixed order and a call gives the same bits each time:
+//  * queries: 128 rows per workgroup, a query per lane, keys streamed -- dQ, delta
+//    and the table's gradient (transposed products, dS^T straight into dQ^T += K^T dS^T);
+//  * keys: 128 keys per workgroup, a key per lane, queries streamed -- dK and dV
+//    (S = Q K^T, P and dS straight into dV^T += dO^T P and dK^T += Q^T dS).
+//    Too few key blocks for the chip share the queries in ranges, whose fp32 partial
+//    sums are added in range order by a third launch.
+#include "attn_tiles.hpp"
+
+namespace dit {
+namespace attn {
+namespace {
+
+struct BwdArgs {
+    AttnIn in;
+    const void* d_o;
+    const void* o;
+    int64_t dos[3], os[3];
+    const float* lse;   // [batch][heads][seq_q]
+    void* dq;
+    void* dk;
+    void* dv;
+    int64_t dqs[3], dks[3], dvs[3];
+    float* ref;         // [batch][heads][seq_q]: lse in log2, +inf for a query without kept keys
+    float* delta;       // [batch][heads][seq_q]
+    float* part_table;  // [batch][heads][row_blocks][buckets]
+    float* part_kv;     // [ranges][2][batch][kv_heads][seq_kv][DP]
+    float* d_table;
+    int64_t d_table_stride;
+    int32_t row_blocks, key_blocks, ranges, buckets;
+};
+
+template <typename T, int DP>
+constexpr int tile_rows() {
+    return sizeof(T) == 4 && DP == 128 ? 32 : 64;
+}
+
+// Floats of a wave's table-gradient line: offsets -(reach + 62) .. reach + 62, all
+// that a 32 x 32 block with an offset inside +-reach has.
+__host__ __device__ inline int grad_line(int reach) { return 2 * (reach + 62) + 1; }
+constexpr int kScratch = 32 * 33;  // a wave's dS block, rows padded
+
+// ---- dQ, delta, the table's gradient ---------------------------------------------------
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const BwdArgs a) {
+    typedef Tile<T, DP> Tl;
+    constexpr int KB = tile_rows<T, DP>(), HALVES = KB / 32, TILE = KB * Tl::RB, NW = 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][K | V], bias line, gradient lines, scratch
+    const AttnIn& in = a.in;
+    const int reach = in.rel.reach;
+    float* const line = reinterpret_cast<float*>(smem + 4 * TILE);
+    float* const grad = line + 2 * reach + 1;
+    float* const scratch = grad + NW * grad_line(reach);
+    __shared__ float far_sum[2][NW];
+
+    const uint32_t bid = xcd_block();
+    const int blk = (int)(bid % (uint32_t)a.row_blocks), bh = (int)(bid / (uint32_t)a.row_blocks);
+    const int h = bh % in.heads, b = bh / in.heads, kvh = h / in.shared;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    const int row = blk * 128 + wave * 32 + r;
+    const bool live = row < in.seq_q;
+    const int tok = live ? row : 0;
+    float* const my_grad = grad + wave * grad_line(reach);
+    float* const my_scratch = scratch + wave * kScratch;
+
+    const T* Kp = reinterpret_cast<const T*>(in.k) + b * in.ks[0] + kvh * in.ks[2];
+    const T* Vp = reinterpret_cast<const T*>(in.v) + b * in.vs[0] + kvh * in.vs[2];
+    if (in.dim < DP) Tl::clear(smem, 4 * TILE, tid, 256);
+    if constexpr (BIAS) {
+        rel_line(in.rel, h, line, tid, 256);
+        for (int i = tid; i < NW * grad_line(reach); i += 256) grad[i] = 0.f;
+    }
+    if (BIAS || in.dim < DP) __syncthreads();
+
+    auto issue = [&](int t, uint64_t word, int buf) {
+        uint8_t* kb = smem + buf * 2 * TILE;
+        const T* ks = Kp + (int64_t)t * KB * in.ks[1];
+        const T* vs = Vp + (int64_t)t * KB * in.vs[1];
+        if (all_kept<KB>(word)) {
+            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [](int i) { return i; });
+            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [](int i) { return i; });
+        } else {
+            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [&](int i) { return kept_row(word, i); });
+            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [&](int i) { return kept_row(word, i); });
+        }
+    };
+
+    typename Tl::Frag qf[Tl::STEPS], of[Tl::STEPS];
+    const int64_t stat = ((int64_t)b * in.heads + h) * in.seq_q + tok;
+    float ref = a.lse[stat] * kLog2e;
+    if (!live || ref == -INFINITY) ref = INFINITY;
+    float delta = 0.f;
+    {
+        const T* qp = reinterpret_cast<const T*>(in.q) + b * in.qs[0] + (int64_t)tok * in.qs[1] + h * in.qs[2];
+        const T* gp = reinterpret_cast<const T*>(a.d_o) + b * a.dos[0] + (int64_t)tok * a.dos[1] + h * a.dos[2];
+        const T* op = reinterpret_cast<const T*>(a.o) + b * a.os[0] + (int64_t)tok * a.os[1] + h * a.os[2];
+#pragma unroll
+        for (int c = 0; c < Tl::STEPS; ++c) {
+            qf[c] = live ? frag_global<T>(qp, c, g, in.dim) : frag_zero<T>();
+            of[c] = live ? frag_global<T>(gp, c, g, in.dim) : frag_zero<T>();
+            delta += frag_dot(of[c], live ? frag_global<T>(op, c, g, in.dim) : frag_zero<T>());
+        }
+        delta += __shfl_xor(delta, 32);
+    }
+    const typename Tl::Cols cols = Tl::cols(lane);
+    const int at = tok + (BIAS ? rel_position(in.rel, b) : 0);
+    const int len = kept_len(in, b);
+
+    // P and dS of one 32-key half of tile t (P in s, dS in d).
+    auto half = [&](const uint8_t* Kt, const uint8_t* Vt, int t, int hh, uint64_t word, f32x16_t& s, f32x16_t& d) {
+        s = zero16();
+        d = zero16();
+#pragma unroll
+        for (int c = 0; c < Tl::STEPS; ++c) {
+            s = mma(Tl::row_frag(Kt, 32 * hh + r, c, g), qf[c], s);
+            d = mma(Tl::row_frag(Vt, 32 * hh + r, c, g), of[c], d);
+        }
+        const int lo = t * KB + 32 * hh + 4 * g - at;
+        const uint32_t w = (uint32_t)(word >> (32 * hh)) >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float bias = -ref;
+            if constexpr (BIAS) bias += line[reach + min(max(lo + 8 * (i >> 2) + (i & 3), -reach), reach)];
+            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], in.scale_log2, bias));
+            const bool keep = w & (1u << (8 * (i >> 2) + (i & 3)));
+            s[i] = keep ? p : 0.f;
+            d[i] = keep ? p * (d[i] - delta) : 0.f;
+        }
+    };
+    // Tiles with a kept key, the next one's DMA in flight behind each.
+    auto walk = [&](auto body) {
+        Kept<KB> kept;
+        kept.start(in, b, len, 0, in.seq_kv, 1, lane);
+        int t = kept.next(lane), buf = 0;
+        uint64_t word = kept.word;
+        if (t >= 0) issue(t, word, 0);
+        while (t >= 0) {
+            wait_vmem<0>();
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            const int t_next = kept.next(lane);
+            const uint64_t word_next = kept.word;
+            if (t_next >= 0) issue(t_next, word_next, buf ^ 1);
+            body(smem + buf * 2 * TILE, smem + buf * 2 * TILE + TILE, t, word);
+            t = t_next;
+            word = word_next;
+            buf ^= 1;
+        }
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+    };
+
+    // The table's gradient is kept in fp32, and a whole row's dS cancels in it: delta
+    // from the rounded output (off by its rounding and P's) would show there, so it is
+    // summed from P and dP first.
+    if constexpr (BIAS && sizeof(T) == 2) {
+        float sum = 0.f;
+        delta = 0.f;
+        walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+#pragma unroll
+            for (int hh = 0; hh < HALVES; ++hh) {
+                f32x16_t s, d;
+                half(Kt, Vt, t, hh, word, s, d);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += d[i];
+            }
+        });
+        delta = sum + __shfl_xor(sum, 32);
+    }
+    if (live && g == 0) {
+        a.ref[stat] = ref;
+        a.delta[stat] = delta;
+    }
+
+    f32x16_t dq[Tl::BLOCKS];
+#pragma unroll
+    for (int d = 0; d < Tl::BLOCKS; ++d) dq[d] = zero16();
+    float far[2] = {0.f, 0.f};  // keys behind, keys ahead, out of reach
+    walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+#pragma unroll
+        for (int hh = 0; hh < HALVES; ++hh) {
+            f32x16_t s, ds;
+            half(Kt, Vt, t, hh, word, s, ds);
+            if constexpr (BIAS) {
+                // Offsets of this 32 x 32 block: off0 + [-31, 31].  A block that is out
+                // of reach as a whole has one bucket (per side: reach may be small).
+                const int off0 = t * KB + 32 * hh - (blk * 128 + wave * 32) - (at - tok);
+                if (off0 - 31 >= reach || off0 + 31 <= -reach) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum += ds[i];
+                    far[0] += off0 > 0 ? 0.f : sum;
+                    far[1] += off0 > 0 ? sum : 0.f;
+                } else {
+                    // Key-major block in LDS, then a diagonal per lane, in row order.
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) my_scratch[(8 * (i >> 2) + 4 * g + (i & 3)) * 33 + r] = ds[i];
+                    wait_lds();
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int diag = lane - 31;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int key = i + diag;
+                        if (key >= 0 && key < 32) sum += my_scratch[key * 33 + i];
+                    }
+                    if (lane < 63) my_grad[reach + 62 + off0 + diag] += sum;
+                    wait_lds();
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = ds[8 * j + e];
+                typename Tl::Frag f;
+                to_frag(v, f);
+#pragma unroll
+                for (int d = 0; d < Tl::BLOCKS; ++d) dq[d] = mma(Tl::col_frag(Kt, 32 * hh + 16 * j, d, cols), f, dq[d]);
+            }
+        }
+    });
+
+    if (live) {
+        T* op = reinterpret_cast<T*>(a.dq) + b * a.dqs[0] + (int64_t)tok * a.dqs[1] + h * a.dqs[2];
+#pragma unroll
+        for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const int e0 = 32 * d + 8 * i4 + 4 * g;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = dq[d][4 * i4 + e] * in.scale;
+                if (e0 < in.dim) put4(op + e0, v);
+            }
+    }
+    if constexpr (BIAS) {
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+            const float f = wave_sum(far[side]);
+            if (lane == 0) far_sum[side][wave] = f;
+        }
+        __syncthreads();
+        // The waves' lines, in wave order, into the first.
+        const int n = grad_line(reach);
+        for (int i = tid; i < n; i += 256) {
+            float sum = grad[i];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) sum += grad[w * n + i];
+            grad[i] = sum;
+        }
+        __syncthreads();
+        // A bucket per wave at a time: its offsets over the lanes.
+        float* out = a.part_table + ((int64_t)bh * a.row_blocks + blk) * a.buckets;
+        for (int t = wave; t < a.buckets; t += NW) {
+            const bool ahead = in.rel.two_sided && t >= in.rel.side;
+            const int u = ahead ? t - in.rel.side : t;
+            const bool last = u == in.rel.side - 1;
+            // Distances [lo, hi) of the bucket.  Without the two sides every key ahead is at distance 0.
+            const int lo = in.rel.start[u], hi = last ? reach + 63 : in.rel.start[u + 1];
+            float sum = 0.f;
+            for (int dist = lo + lane; dist < hi; dist += 64)
+                if (!ahead || dist > 0) sum += grad[reach + 62 + (ahead ? dist : -dist)];
+            if (!in.rel.two_sided && u == 0)
+                for (int dist = 1 + lane; dist < reach + 63; dist += 64) sum += grad[reach + 62 + dist];
+            sum = wave_sum(sum);
+            if (lane == 0) {
+                if (last)
+                    for (int w = 0; w < NW; ++w) sum += far_sum[ahead][w];
+                if (!in.rel.two_sided && u == 0)
+                    for (int w = 0; w < NW; ++w) sum += far_sum[1][w];
+                out[t] = sum;
+            }
+        }
+    }
+}
+
+// dtable[t][h] = the sum of its partial sums over batch entries and row blocks: a wave per (t, h), in 64 bits.
+__global__ __launch_bounds__(64) void attn_dtable_kernel(const BwdArgs a) {
+    const int t = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, lane = threadIdx.x;
+    double sum = 0.0;
+    const int n = a.in.batch * a.row_blocks;
+    for (int i = lane; i < n; i += 64) {
+        const int b = i / a.row_blocks, blk = i - b * a.row_blocks;
+        sum += (double)a.part_table[(((int64_t)b * a.in.heads + h) * a.row_blocks + blk) * a.buckets + t];
+    }
+    sum = wave_sum_f64(sum);
+    if (lane == 0) a.d_table[t * a.d_table_stride + h] = (float)sum;
+}
+
+// ---- dK, dV ----------------------------------------------------------------------------
+template <typename T, int DP, bool BIAS>
+__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const BwdArgs a) {
+    typedef Tile<T, DP> Tl;
+    constexpr int QB = tile_rows<T, DP>(), HALVES = QB / 32, TILE = QB * Tl::RB, NW = 4;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][Q | dO], [buffer][ref | delta], bias line
+    const AttnIn& in = a.in;
+    float* const stats = reinterpret_cast<float*>(smem + 4 * TILE);  // [buffer][2][64]
+    float* const line = stats + 2 * 2 * 64;
+
+    const uint32_t bid = xcd_block();
+    const int blk = (int)(bid % (uint32_t)a.key_blocks), rest = (int)(bid / (uint32_t)a.key_blocks);
+    const int range = rest % a.ranges, bh = rest / a.ranges, kvh = bh % in.kv_heads, b = bh / in.kv_heads;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5;
+    const int key = blk * 128 + wave * 32 + r, len = kept_len(in, b);
+    const bool keep = key < len && (!in.kv_mask || in.kv_mask[b * in.mask_stride + key] != 0);
+    const bool inside = key < in.seq_kv;
+
+    typename Tl::Frag kf[Tl::STEPS], vf[Tl::STEPS];
+    {
+        // A key that is not kept is taken as zeros: what it holds reaches no product.
+        const int64_t n = keep ? key : 0;
+        const T* kp = reinterpret_cast<const T*>(in.k) + b * in.ks[0] + n * in.ks[1] + kvh * in.ks[2];
+        const T* vp = reinterpret_cast<const T*>(in.v) + b * in.vs[0] + n * in.vs[1] + kvh * in.vs[2];
+#pragma unroll
+        for (int c = 0; c < Tl::STEPS; ++c) {
+            kf[c] = keep ? frag_global<T>(kp, c, g, in.dim) : frag_zero<T>();
+            vf[c] = keep ? frag_global<T>(vp, c, g, in.dim) : frag_zero<T>();
+        }
+    }
+    f32x16_t dk[Tl::BLOCKS], dv[Tl::BLOCKS];
+#pragma unroll
+    for (int d = 0; d < Tl::BLOCKS; ++d) dk[d] = dv[d] = zero16();
+    const typename Tl::Cols cols = Tl::cols(lane);
+
+    // Query tiles of the heads that share this key head, one after another; this range's.
+    const int tiles = (in.seq_q + QB - 1) / QB;
+    const int64_t total = (int64_t)tiles * in.shared;
+    int first = (int)(total * range / a.ranges), last = (int)(total * (range + 1) / a.ranges);
+    if (__syncthreads_or(keep) == 0) last = first;  // no kept key in the block
+    const int pos = BIAS ? rel_position(in.rel, b) : 0;
+
+    if (in.dim < DP) {
+        Tl::clear(smem, 4 * TILE, tid, 256);
+        __syncthreads();
+    }
+    auto issue = [&](int n, int buf) {
+        const int h = kvh * in.shared + n / tiles, q0 = (n % tiles) * QB;
+        const int left = in.seq_q - q0;
+        uint8_t* qb = smem + buf * 2 * TILE;
+        const T* qp = reinterpret_cast<const T*>(in.q) + b * in.qs[0] + (int64_t)q0 * in.qs[1] + h * in.qs[2];
+        const T* gp = reinterpret_cast<const T*>(a.d_o) + b * a.dos[0] + (int64_t)q0 * a.dos[1] + h * a.dos[2];
+        Tl::template load<QB, NW>(qp, in.qs[1], in.dim, qb, wave, lane, [&](int i) { return min(i, left - 1); });
+        Tl::template load<QB, NW>(gp, a.dos[1], in.dim, qb + TILE, wave, lane, [&](int i) { return min(i, left - 1); });
+        if (wave < 2) {  // 64 floats each
+            const float* src = (wave == 0 ? a.ref : a.delta) + ((int64_t)b * in.heads + h) * in.seq_q + q0;
+            __builtin_amdgcn_global_load_lds(src + min(lane, left - 1), stats + (buf * 2 + wave) * 64, 4, 0, 0);
+        }
+    };
+    int cur = -1, buf = 0;
+    if (first < last) issue(first, 0);
+    for (int n = first; n < last; ++n) {
+        wait_vmem<0>();
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (BIAS) {
+            if (n / tiles != cur) {  // every wave has finished with the last head's line
+                cur = n / tiles;
+                rel_line(in.rel, kvh * in.shared + cur, line, tid, 256);
+                __syncthreads();
+            }
+        }
+        if (n + 1 < last) issue(n + 1, buf ^ 1);
+        const uint8_t* Qt = smem + buf * 2 * TILE;
+        const uint8_t* Gt = Qt + TILE;
+        const float* st = stats + buf * 2 * 64;
+        const int q0 = (n % tiles) * QB, left = in.seq_q - q0;
+#pragma unroll
+        for (int hh = 0; hh < HALVES; ++hh) {
+            f32x16_t s = zero16(), ds = zero16();
+#pragma unroll
+            for (int c = 0; c < Tl::STEPS; ++c) {
+                s = mma(Tl::row_frag(Qt, 32 * hh + r, c, g), kf[c], s);
+                ds = mma(Tl::row_frag(Gt, 32 * hh + r, c, g), vf[c], ds);
+            }
+            // Element i: query q0 + 32 hh + 8 (i / 4) + 4 g + i % 4.
+            const int i0 = 32 * hh + 4 * g;
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const float4 rf = *reinterpret_cast<const float4*>(st + i0 + 8 * i4);
+                const float4 dl = *reinterpret_cast<const float4*>(st + 64 + i0 + 8 * i4);
+                const float ref[4] = {rf.x, rf.y, rf.z, rf.w}, delta[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int q = i0 + 8 * i4 + e;
+                    float bias = -ref[e];
+                    if constexpr (BIAS) {
+                        const int off = key - (q0 + q) - pos;
+                        bias += line[in.rel.reach + min(max(off, -in.rel.reach), in.rel.reach)];
+                    }
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], in.scale_log2, bias));
+                    const bool on = keep && q < left;
+                    s[4 * i4 + e] = on ? p : 0.f;
+                    ds[4 * i4 + e] = on ? p * (ds[4 * i4 + e] - delta[e]) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float pv[8], dsv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    pv[e] = s[8 * j + e];
+                    dsv[e] = ds[8 * j + e];
+                }
+                typename Tl::Frag pf, df;
+                to_frag(pv, pf);
+                to_frag(dsv, df);
+#pragma unroll
+                for (int d = 0; d < Tl::BLOCKS; ++d) {
+                    dv[d] = mma(Tl::col_frag(Gt, 32 * hh + 16 * j, d, cols), pf, dv[d]);
+                    dk[d] = mma(Tl::col_frag(Qt, 32 * hh + 16 * j, d, cols), df, dk[d]);
+                }
+            }
+        }
+        buf ^= 1;
+    }
+    if (!inside) return;
+    if (a.ranges > 1) {
+        const int64_t plane = (int64_t)in.batch * in.kv_heads * in.seq_kv * DP;
+        float* pk = a.part_kv + (int64_t)range * 2 * plane + ((int64_t)bh * in.seq_kv + key) * DP;
+#pragma unroll
+        for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const int e0 = 32 * d + 8 * i4 + 4 * g;
+                const float x[4] = {dk[d][4 * i4], dk[d][4 * i4 + 1], dk[d][4 * i4 + 2], dk[d][4 * i4 + 3]};
+                const float y[4] = {dv[d][4 * i4], dv[d][4 * i4 + 1], dv[d][4 * i4 + 2], dv[d][4 * i4 + 3]};
+                if (e0 < in.dim) {
+                    put4(pk + e0, x);
+                    put4(pk + plane + e0, y);
+                }
+            }
+        return;
+    }
+    T* kp = reinterpret_cast<T*>(a.dk) + b * a.dks[0] + (int64_t)key * a.dks[1] + kvh * a.dks[2];
+    T* vp = reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + (int64_t)key * a.dvs[1] + kvh * a.dvs[2];
+#pragma unroll
+    for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            const int e0 = 32 * d + 8 * i4 + 4 * g;
+            float x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = dk[d][4 * i4 + e] * in.scale;
+                y[e] = dv[d][4 * i4 + e];
+            }
+            if (e0 < in.dim) {
+                put4(kp + e0, x);
+                put4(vp + e0, y);
+            }
+        }
+}
+
+// The ranges' dK and dV of one key, added in range order: a thread per four elements.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(const BwdArgs a) {
+    const AttnIn& in = a.in;
+    constexpr int TPR = DP / 4;
+    const int64_t n = (int64_t)in.batch * in.kv_heads * in.seq_kv, id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR;
+    const int d = (int)(threadIdx.x % TPR) * 4;
+    if (id >= n || d >= in.dim) return;
+    const int key = (int)(id % in.seq_kv), bh = (int)(id / in.seq_kv), kvh = bh % in.kv_heads, b = bh / in.kv_heads;
+    float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.ranges; ++s) {
+        const float* p = a.part_kv + ((int64_t)s * 2 * n + id) * DP + d;
+        const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + n * DP);
+        x[0] += u.x;
+        x[1] += u.y;
+        x[2] += u.z;
+        x[3] += u.w;
+        y[0] += w.x;
+        y[1] += w.y;
+        y[2] += w.z;
+        y[3] += w.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] *= in.scale;
+    put4(reinterpret_cast<T*>(a.dk) + b * a.dks[0] + (int64_t)key * a.dks[1] + kvh * a.dks[2] + d, x);
+    put4(reinterpret_cast<T*>(a.dv) + b * a.dvs[0] + (int64_t)key * a.dvs[1] + kvh * a.dvs[2] + d, y);
+}
+
+// ---- launch ------------------------------------------------------------------------------
+struct Plan {
+    int row_blocks, key_blocks, ranges;
+    int64_t stat_floats, table_floats, kv_floats;  // workspace, in this order (ref and delta first)
+};
+
+int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
+
+Plan plan(const AttnIn& in, int buckets, int cus) {
+    Plan p{};
+    const int dp = in.dim <= 64 ? 64 : 128;
+    p.row_blocks = (in.seq_q + 127) / 128;
+    p.key_blocks = (in.seq_kv + 127) / 128;
+    const int64_t blocks = (int64_t)p.key_blocks * in.kv_heads * in.batch, tiles = (int64_t)((in.seq_q + 63) / 64) * in.shared;
+    // Ranges of the queries until every CU has a workgroup, each of at least two tiles.
+    int64_t s = blocks > 0 ? cus / blocks : 1;
+    if (s > tiles / 2) s = tiles / 2;
+    if (s > 16) s = 16;
+    p.ranges = s < 2 ? 1 : (int)s;
+    p.stat_floats = up4((int64_t)in.batch * in.heads * in.seq_q);
+    p.table_floats = buckets ? up4((int64_t)in.batch * in.heads * p.row_blocks * buckets) : 0;
+    p.kv_floats = p.ranges > 1 ? (int64_t)p.ranges * 2 * in.batch * in.kv_heads * in.seq_kv * dp : 0;
+    return p;
+}
+
+template <typename T, int DP, bool BIAS>
+int launch(const BwdArgs& a, const Plan& p, hipStream_t st) {
+    const char* who = "dt_attn_bwd";
+    const AttnIn& in = a.in;
+    const size_t tiles = 4 * tile_rows<T, DP>() * Tile<T, DP>::RB;
+    const int line = rel_line_floats(in.rel);
+    const int64_t dq_blocks = (int64_t)p.row_blocks * in.heads * in.batch;
+    const int64_t dkv_blocks = (int64_t)p.key_blocks * p.ranges * in.kv_heads * in.batch;
+    DT_REQUIRE(dq_blocks < (1ll << 31) && dkv_blocks < (1ll << 31), "%s: grid too large", who);
+    int rc = DT_OK;
+    if (dq_blocks > 0) {
+        const size_t lds = tiles + (BIAS ? line + 4 * (grad_line(in.rel.reach) + kScratch) : 0) * sizeof(float);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, BIAS>), dim3((unsigned)dq_blocks), dim3(256), lds, st, a);
+        rc = check_launch(who);
+    }
+    if (!rc && BIAS && a.d_table && in.heads > 0) {
+        hipLaunchKernelGGL(attn_dtable_kernel, dim3((unsigned)(a.buckets * in.heads)), dim3(64), 0, st, a);
+        rc = check_launch(who);
+    }
+    if (rc || dkv_blocks == 0) return rc;
+    const size_t lds = tiles + (4 * 64 + (BIAS ? line : 0)) * sizeof(float);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, BIAS>), dim3((unsigned)dkv_blocks), dim3(256), lds, st, a);
+    rc = check_launch(who);
+    if (rc || p.ranges == 1) return rc;
+    const int64_t n = (int64_t)in.batch * in.kv_heads * in.seq_kv * (DP / 4);
+    hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    return check_launch(who);
+}
+
+template <typename T, int DP>
+int launch_bias(const BwdArgs& a, const Plan& p, hipStream_t st) {
+    return a.in.rel.table ? launch<T, DP, true>(a, p, st) : launch<T, DP, false>(a, p, st);
+}
+
+int64_t total_floats(const Plan& p) { return 2 * p.stat_floats + p.table_floats + p.kv_floats; }
+
+}  // namespace
+}  // namespace attn
+}  // namespace dit
+
+extern "C" size_t dt_attn_bwd_workspace_bytes(const dt_attn_args* x) {
+    using namespace dit;
+    using namespace dit::attn;
+    AttnIn in;
+    if (prepare_in(x, "dt_attn_bwd_workspace_bytes", &in)) return 0;
+    return (size_t)total_floats(plan(in, x->rel_table ? x->rel_buckets : 0, cu_count())) * sizeof(float);
+}
+
+extern "C" int dt_attn_bwd(const dt_attn_args* x, const dt_attn_grads* y, void* workspace, size_t workspace_bytes,
+                           dt_stream_t stream) {
+    using namespace dit;
+    using namespace dit::attn;
+    const char* who = "dt_attn_bwd";
+    BwdArgs a{};
+    int rc = prepare_in(x, who, &a.in);
+    if (rc) return rc;
+    DT_REQUIRE(y != nullptr, "%s: null gradients", who);
+    rc = check_rows(x, y->d_o, y->d_o_strides, x->heads, x->seq_q, false, "d_o", who);
+    if (!rc) rc = check_rows(x, y->o, y->o_strides, x->heads, x->seq_q, false, "o", who);
+    if (!rc) rc = check_rows(x, y->dq, y->dq_strides, x->heads, x->seq_q, true, "dq", who);
+    if (!rc) rc = check_rows(x, y->dk, y->dk_strides, x->kv_heads, x->seq_kv, true, "dk", who);
+    if (!rc) rc = check_rows(x, y->dv, y->dv_strides, x->kv_heads, x->seq_kv, true, "dv", who);
+    if (rc) return rc;
+    const AttnIn& in = a.in;
+    const bool rows = in.batch > 0 && in.heads > 0 && in.seq_q > 0;
+    DT_REQUIRE(!rows || (y->lse && ((uintptr_t)y->lse & 3) == 0), "%s: lse must be given, 4-byte aligned", who);
+    DT_REQUIRE(!x->rel_table || !y->d_rel_table || (((uintptr_t)y->d_rel_table & 3) == 0 && y->d_rel_table_stride >= x->heads),
+               "%s: d_rel_table must be 4-byte aligned with rows of at least heads", who);
+    a.buckets = x->rel_table ? x->rel_buckets : 0;
+    const Plan p = plan(in, a.buckets, cu_count());
+    const size_t need = (size_t)total_floats(p) * sizeof(float);
+    DT_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need, workspace ? workspace_bytes : 0);
+    a.d_o = y->d_o;
+    a.o = y->o;
+    a.lse = y->lse;
+    a.dq = y->dq;
+    a.dk = y->dk;
+    a.dv = y->dv;
+    for (int i = 0; i < 3; ++i) {
+        a.dos[i] = y->d_o_strides[i];
+        a.os[i] = y->o_strides[i];
+        a.dqs[i] = y->dq_strides[i];
+        a.dks[i] = y->dk_strides[i];
+        a.dvs[i] = y->dv_strides[i];
+    }
+    a.ref = (float*)workspace;
+    a.delta = a.ref + p.stat_floats;
+    a.part_table = a.delta + p.stat_floats;
+    a.part_kv = a.part_table + p.table_floats;
+    a.d_table = y->d_rel_table;
+    a.d_table_stride = y->d_rel_table_stride;
+    a.row_blocks = p.row_blocks;
+    a.key_blocks = p.key_blocks;
+    a.ranges = p.ranges;
+    const hipStream_t st = (hipStream_t)stream;
+    if (x->io_type == DT_TYPE_F32) return in.dim <= 64 ? launch_bias<float, 64>(a, p, st) : launch_bias<float, 128>(a, p, st);
+    return in.dim <= 64 ? launch_bias<bf16, 64>(a, p, st) : launch_bias<bf16, 128>(a, p, st);
+}

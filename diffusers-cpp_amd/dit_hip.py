@@ -135,6 +135,11 @@ _SIGS = {
     "dt_flash_attn_bf16": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                      c_int64, c_int64, c_int64, POINTER(c_int64), POINTER(c_int64),
                                      POINTER(c_int64), POINTER(c_int64), c_float, c_int32, _S]),
+    "dt_rel_bucket_fill": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32]),
+    "dt_attn_fwd_workspace_bytes": (ctypes.c_size_t, [c_void_p]),
+    "dt_attn_fwd": (c_int32, [c_void_p, c_void_p, _I64P, c_void_p, c_void_p, ctypes.c_size_t, _S]),
+    "dt_attn_bwd_workspace_bytes": (ctypes.c_size_t, [c_void_p]),
+    "dt_attn_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, ctypes.c_size_t, _S]),
     "dt_op_binary": (c_int32, [c_int32, POINTER(DtTensor), POINTER(DtTensor), POINTER(DtTensor), _S]),
     "dt_op_unary": (c_int32, [c_int32, POINTER(DtTensor), POINTER(DtTensor), c_float, c_float, _S]),
     "dt_op_norm": (c_int32, [POINTER(DtTensor), POINTER(DtTensor), c_float, _S]),
@@ -763,6 +768,169 @@ def flash_attn_qk(q_segments, k, v, pos, axis_dim, freq_base, eps=1e-6, table=No
         eps, _p(pos), pos.stride(0), pos.shape[1], axis_dim, freq_base, _p(table), n_pos, _p(k), _p(v), _p(out),
         B, H, Sq, Skv, D, st(k), st(v), st(out), scale, io_type(out), stream()), "dt_flash_attn_qk_bf16")
     return out
+
+
+class AttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_strides", _I64x3), ("k_strides", _I64x3),
+                ("v_strides", _I64x3), ("batch", c_int64), ("heads", c_int64), ("kv_heads", c_int64),
+                ("seq_q", c_int64), ("seq_kv", c_int64), ("head_dim", c_int64), ("kv_len", c_void_p),
+                ("kv_mask", c_void_p), ("kv_mask_stride", c_int64), ("rel_table", c_void_p),
+                ("rel_table_stride", c_int64), ("q_pos", c_void_p), ("rel_buckets", c_int32),
+                ("rel_distance", c_int32), ("rel_two_sided", c_int32), ("io_type", c_int32), ("scale", c_float)]
+
+
+class AttnGrads(ctypes.Structure):
+    _fields_ = [("d_o", c_void_p), ("o", c_void_p), ("lse", c_void_p), ("dq", c_void_p), ("dk", c_void_p),
+                ("dv", c_void_p), ("d_o_strides", _I64x3), ("o_strides", _I64x3), ("dq_strides", _I64x3),
+                ("dk_strides", _I64x3), ("dv_strides", _I64x3), ("d_rel_table", c_void_p),
+                ("d_rel_table_stride", c_int64)]
+
+
+class RelBias:
+    """A learned relative position bias: table fp32 [buckets, heads]; key - query
+    falls into the buckets rel_buckets() lists."""
+
+    def __init__(self, table, distance, two_sided=True):
+        self.table, self.distance, self.two_sided = table, distance, two_sided
+
+
+def rel_buckets(n, buckets, distance, two_sided=True):
+    """The bucket of every offset key - query in (-n, n), as a host int32 tensor [2 n - 1]."""
+    torch = _torch()
+    out = torch.empty(max(2 * n - 1, 0), dtype=torch.int32)
+    check(load().dt_rel_bucket_fill(c_void_p(out.data_ptr()), n, buckets, distance, 1 if two_sided else 0),
+          "dt_rel_bucket_fill")
+    return out
+
+
+def _same_device(first, *others):
+    """The launch goes to the current device's current stream: every tensor has to be there."""
+    at = first.device
+    for t in others:
+        if t is not None and t.device != at:
+            raise DtError(f"tensors on {at} and {t.device}")
+    if at.type != "cuda":
+        raise DtError(f"tensors must be on a HIP device, not {at}")
+    if at.index != _torch().cuda.current_device():
+        raise DtError(f"tensors on {at}, which is not the current device")
+
+
+def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos):
+    torch = _torch()
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise DtError("q must be [B, Sq, H, D], k and v [B, Skv, Hkv, D]")
+    B, Sq, H, D = q.shape
+    Bk, Skv, Hkv, Dk = k.shape
+    if Bk != B or Dk != D:
+        raise DtError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise DtError("q, k and v must share a dtype")
+    st = (q.stride(), k.stride(), v.stride())
+    if st[0][3] != 1 or st[1][3] != 1 or st[2][3] != 1:
+        raise DtError("the head dim must be contiguous")
+    a = AttnArgs()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_strides[:], a.k_strides[:], a.v_strides[:] = st[0][:3], st[1][:3], st[2][:3]
+    a.batch, a.heads, a.kv_heads, a.seq_q, a.seq_kv, a.head_dim = B, H, Hkv, Sq, Skv, D
+    a.io_type = io_type(q)
+    a.scale = 1.0 / D ** 0.5 if scale is None else scale
+    table = None
+    if kv_len is not None:
+        if kv_len.dtype != torch.int32 or kv_len.shape != (B,) or (B > 1 and kv_len.stride(0) != 1):
+            raise DtError("kv_len must be contiguous int32 [B]")
+        a.kv_len = kv_len.data_ptr()
+    if kv_mask is not None:
+        if kv_mask.dtype not in (torch.uint8, torch.bool) or kv_mask.shape != (B, Skv) or \
+                (Skv > 1 and kv_mask.stride(1) != 1):
+            raise DtError("kv_mask must be uint8 or bool [B, Skv] with contiguous rows")
+        a.kv_mask, a.kv_mask_stride = kv_mask.data_ptr(), kv_mask.stride(0)
+    if rel is not None:
+        table = rel.table
+        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != H or (H > 1 and table.stride(1) != 1):
+            raise DtError("the bias table must be fp32 [buckets, H] with contiguous rows")
+        a.rel_table, a.rel_table_stride = table.data_ptr(), table.stride(0) if table.shape[0] > 1 else H
+        a.rel_buckets, a.rel_distance, a.rel_two_sided = table.shape[0], rel.distance, 1 if rel.two_sided else 0
+        if q_pos is not None:
+            if q_pos.dtype != torch.int32 or q_pos.shape != (B,) or (B > 1 and q_pos.stride(0) != 1):
+                raise DtError("q_pos must be contiguous int32 [B]")
+            a.q_pos = q_pos.data_ptr()
+    _same_device(q, k, v, kv_len, kv_mask, table, q_pos)
+    return a
+
+
+def _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse):
+    torch = _torch()
+    a = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
+        raise DtError("out must have q's shape, dtype and device, its head dim contiguous")
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if return_lse else None
+    lib = load()
+    p = ctypes.addressof(a)
+    n = lib.dt_attn_fwd_workspace_bytes(p)
+    ws = _scratch(n, q.device) if n else None
+    check(lib.dt_attn_fwd(p, out.data_ptr(), _strides3(out), _p(lse), _p(ws), n, stream()), "dt_attn_fwd")
+    if isinstance(lib, _Recorder):
+        lib.keep.append(a)
+    return (out, lse) if return_lse else out
+
+
+def _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos):
+    torch = _torch()
+    a = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos)
+    for t, name in ((d_o, "d_o"), (o, "o")):
+        if t.shape != q.shape or t.dtype != q.dtype or t.stride(3) != 1:
+            raise DtError(f"{name} must have q's shape and dtype, its head dim contiguous")
+    B, Sq, H, _ = q.shape
+    if lse.dtype != torch.float32 or lse.shape != (B, H, Sq) or not lse.is_contiguous():
+        raise DtError("lse must be the forward pass's: contiguous fp32 [B, H, Sq]")
+    _same_device(q, d_o, o, lse)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dt = None if rel is None else torch.empty(rel.table.shape, dtype=torch.float32, device=q.device)
+    y = AttnGrads()
+    y.d_o, y.o, y.lse = d_o.data_ptr(), o.data_ptr(), lse.data_ptr()
+    y.dq, y.dk, y.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    y.d_o_strides[:], y.o_strides[:] = d_o.stride()[:3], o.stride()[:3]
+    y.dq_strides[:], y.dk_strides[:], y.dv_strides[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+    if dt is not None:
+        y.d_rel_table, y.d_rel_table_stride = dt.data_ptr(), H
+    lib = load()
+    p = ctypes.addressof(a)
+    n = lib.dt_attn_bwd_workspace_bytes(p)
+    ws = _scratch(n, q.device) if n else None
+    check(lib.dt_attn_bwd(p, ctypes.addressof(y), _p(ws), n, stream()), "dt_attn_bwd")
+    if isinstance(lib, _Recorder):
+        lib.keep.extend((a, y))
+    return (dq, dk, dv) if rel is None else (dq, dk, dv, dt)
+
+
+def cross_attn(q, k, v, kv_len=None, kv_mask=None, scale=None, out=None, return_lse=False):
+    """softmax over the kept keys of scale q k^T, times v: q [B, Sq, H, D], k and v
+    [B, Skv, Hkv, D] (bf16 or fp32, Hkv a divisor of H, D a multiple of 8 up to 128,
+    any strides with d contiguous) -> [B, Sq, H, D].  kv_len int32 [B] keeps keys
+    below it, kv_mask uint8 or bool [B, Skv] those that are set.  return_lse: also
+    the log of each softmax's sum, fp32 [B, H, Sq], for cross_attn_bwd."""
+    return _attn(q, k, v, kv_len, kv_mask, scale, None, None, out, return_lse)
+
+
+def cross_attn_bwd(d_o, q, k, v, o, lse, kv_len=None, kv_mask=None, scale=None):
+    """(dq, dk, dv) of cross_attn's o for its gradient d_o."""
+    return _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, None, None)
+
+
+def rel_attn(q, k, v, rel, q_pos=None, kv_len=None, kv_mask=None, scale=None, out=None, return_lse=False):
+    """cross_attn with the bias rel.table[bucket(key - query)] of each head (RelBias)
+    added to the scores; query i of batch entry b is at position q_pos[b] + i (int32
+    [B]; None: 0), key j at j."""
+    return _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse)
+
+
+def rel_attn_bwd(d_o, q, k, v, o, lse, rel, q_pos=None, kv_len=None, kv_mask=None, scale=None):
+    """(dq, dk, dv, dtable) of rel_attn's o for its gradient d_o; dtable fp32 [buckets, H]."""
+    return _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos)
 
 
 # --------------------------------------------------------------------------

@@ -461,6 +461,80 @@ int dt_flash_attn_f32(const float *q, const float *k, const float *v, float *o, 
                       const int64_t *k_strides, const int64_t *v_strides, const int64_t *o_strides, float scale,
                       void *workspace, size_t workspace_bytes, dt_stream_t stream);
 
+/* ---- text conditioning: masked attention, its gradients, adapters --------- */
+
+/* Attention of queries to keys whose number differs per batch entry, e.g. the
+ * states of a text encoder (or the encoder's own attention):
+ *   s_ij = scale <q_i, k_j> (+ rel_table[bucket(j - i - q_pos)][h]), j kept,
+ *   o_i = sum_j softmax_j(s_ij) v_j.
+ * Element (b, s, h, d) of q is q[b*q_strides[0] + s*q_strides[1] +
+ * h*q_strides[2] + d]; likewise k and v with kv_heads heads, query head h
+ * reading key head h / (heads / kv_heads).  io_type BF16 or F32 (q, k, v, o and
+ * the gradients; products of bf16 operands, or of fp32 ones on the fp32 matrix
+ * cores, sums in fp32), head_dim a multiple of 8 up to 128, pointers and rows
+ * 16-byte aligned (strides of dimensions of one element are not read; stride 0
+ * repeats an input).
+ * kv_len (int32 [batch], device) keeps keys below kv_len[b] (clamped to
+ * [0, seq_kv]); kv_mask (uint8, key j of entry b at kv_mask[b*kv_mask_stride +
+ * j], device) keeps keys with a nonzero byte; both given: both.  What a key that
+ * is not kept holds is not used (it may be NaN).  A query without kept keys, or
+ * whose scores are all -inf, has o = 0 and lse = -inf.
+ * rel_table (fp32 [rel_buckets][heads], rows rel_table_stride apart) adds a learned
+ * bias by the bucket (dt_rel_bucket_fill) of key position j - query position
+ * q_pos[b] + i (q_pos: int32 [batch], device, or NULL: 0).  rel_table NULL: none.
+ * No counterpart in the reference, whose FlashAttentionOp passes no mask
+ * (src/nn/attention/FlashAttentionOp.cpp:84-94). */
+typedef struct dt_attn_args {
+    const void *q, *k, *v;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    int64_t batch, heads, kv_heads, seq_q, seq_kv, head_dim;
+    const int32_t *kv_len;
+    const uint8_t *kv_mask;
+    int64_t kv_mask_stride;
+    const float *rel_table;
+    int64_t rel_table_stride;
+    const int32_t *q_pos;
+    int32_t rel_buckets, rel_distance, rel_two_sided;
+    int32_t io_type;
+    float scale;
+} dt_attn_args;
+
+/* Host-side: bucket[n - 1 + off] = the bucket of offset off = key - query for
+ * |off| < n (`bucket` is HOST memory of 2 n - 1 values).  With nb buckets a side
+ * (buckets / 2 when two_sided, where keys after the query take the upper half, else
+ * buckets, and keys after the query are at distance 0) and near = nb / 2, distance
+ * d is bucket d below near, then near + floor(log(d / near) / log(distance / near)
+ * * (nb - near)), at most nb - 1, in exact arithmetic.  2 to 64 buckets a side,
+ * near < distance <= 1024. */
+int dt_rel_bucket_fill(int32_t *bucket, int64_t n, int32_t buckets, int32_t distance, int32_t two_sided);
+
+/* The forward pass: o (strides as q's) and, when lse is not NULL, lse_i = log
+ * sum_j exp(s_ij) as fp32 [batch][heads][seq_q], which the gradients need.  Few
+ * rows take their keys in ranges whose partial results go through `workspace`
+ * (dt_attn_fwd_workspace_bytes, 0 for most calls; 16-byte aligned); with less,
+ * or none, the ranges are one.  Same results for the same call: no atomics. */
+size_t dt_attn_fwd_workspace_bytes(const dt_attn_args *args);
+int dt_attn_fwd(const dt_attn_args *args, void *o, const int64_t *o_strides, float *lse, void *workspace,
+                size_t workspace_bytes, dt_stream_t stream);
+
+/* The gradients of dt_attn_fwd's o for d_o: of q, of k and v (zeros for a key that
+ * is not kept; summed over the query heads that share a key head) and, with a
+ * rel_table and d_rel_table not NULL, of the table (fp32, summed over batch entries).
+ * o and lse are dt_attn_fwd's for the same arguments.  `workspace` of
+ * dt_attn_bwd_workspace_bytes (16-byte aligned) is needed.  No atomics: the same
+ * call gives the same bits.  Outputs must not overlap inputs or each other. */
+typedef struct dt_attn_grads {
+    const void *d_o, *o;
+    const float *lse;
+    void *dq, *dk, *dv;
+    int64_t d_o_strides[3], o_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+    float *d_rel_table;
+    int64_t d_rel_table_stride;
+} dt_attn_grads;
+size_t dt_attn_bwd_workspace_bytes(const dt_attn_args *args);
+int dt_attn_bwd(const dt_attn_args *args, const dt_attn_grads *grads, void *workspace, size_t workspace_bytes,
+                dt_stream_t stream);
+
 /* ======================================================================== */
 /* (iii) unfused ggml-op kernels on ggml-shaped descriptors                 */
 /* ======================================================================== */
