@@ -484,6 +484,9 @@ struct Wide {
     }
 };
 bool reaches(int n, int near, int max, int far, int j) {
+    // By logarithms where they are not next to each other (they are off by 1e-13 at most).
+    const double d = far * log((double)n) - (far - j) * log((double)near) - j * log((double)max);
+    if (fabs(d) > 1e-9) return d > 0;
     Wide a, b;
     for (int i = 0; i < far; ++i) {
         a.times((uint32_t)n);

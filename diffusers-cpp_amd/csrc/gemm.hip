@@ -161,6 +161,94 @@ __device__ __forceinline__ void epilogue(const Problem& p, const f32x16_t (&acc)
     }
 }
 
+// ---- low-rank adapters beside the product (dt_lora_gemm) ---------------------
+// C[m, n] += sum_r T[m, r] U_a[n, r], a = adapter of row m: T = scale (A A_a^T) from
+// lora_down_kernel (lora.hip), U_a the adapter's up weights.  It is added to a
+// tile's accumulators after its last k-step, so the sum is rounded once.  T is held
+// as two bf16 parts (16 significant bits), each a product of its own: beside K of
+// some thousands the second costs nothing that shows, and an fp32 C keeps its accuracy.
+// NoLora leaves a kernel as it is without.
+struct NoLora {
+    static constexpr bool on = false;
+};
+struct LoraTile {
+    static constexpr bool on = true;
+    const uint16_t* t;  // [M][2][rp]: the two parts, zeros from rank to rp
+    const uint16_t* u;  // [adapters][N][rank]
+    int64_t ldu, u_stride;
+    const int32_t* row_adapter;
+    int adapters, rank, rp;
+    int vec;  // u's rows in 16-byte chunks of 8 ranks
+};
+
+// Ranks r .. r + 7 of the up row; zeros past the rank.
+__device__ __forceinline__ bf16x8_t lora_up(const LoraTile& l, const uint16_t* row, int r) {
+    if (l.vec)
+        return __builtin_bit_cast(bf16x8_t, r < l.rank ? *reinterpret_cast<const uint4*>(row + r) : make_uint4(0, 0, 0, 0));
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = r + 2 * e < l.rank ? row[r + 2 * e] : 0u, hi = r + 2 * e + 1 < l.rank ? row[r + 2 * e + 1] : 0u;
+        w[e] = lo | hi << 16;
+    }
+    return __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+}
+__device__ __forceinline__ bf16x8_t lora_t(const uint16_t* p) {
+    return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(p));
+}
+
+// The wave's FM x FN blocks of 32 x 32.  A 32-row block whose rows share an adapter (any
+// request of 32 rows or more) goes straight into the accumulators; one with several takes
+// each adapter's product apart and keeps it in that adapter's rows alone, so what
+// an adapter holds reaches no other request's rows.
+template <int FM, int FN>
+__device__ __forceinline__ void lora_add(const LoraTile& l, const Problem& p, f32x16_t (&acc)[FN][FM], int mw, int nw,
+                                         int lane) {
+    const int lrow = lane & 31, g = lane >> 5;
+    const uint16_t* u0[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) u0[j] = l.u + (int64_t)min(nw + 32 * j + lrow, p.N - 1) * l.ldu;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = mw + 32 * i + lrow;
+        const bool row = m < p.M;
+        const int mine = row ? l.row_adapter[m] : -1;
+        const uint16_t* t = l.t + (int64_t)min(m, p.M - 1) * 2 * l.rp + 8 * g;
+        uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < l.adapters);
+        while (left) {
+            const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(left));
+            const uint64_t of = __builtin_amdgcn_ballot_w64(mine == a);
+            left &= ~of;
+            const int64_t at = a * l.u_stride;
+            if (__builtin_amdgcn_ballot_w64(row && mine != a) == 0) {
+                for (int r = 0; r < l.rank; r += 16) {
+                    const bf16x8_t hi = lora_t(t + r), lo = lora_t(t + l.rp + r);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) {
+                        const bf16x8_t u = lora_up(l, u0[j] + at, r + 8 * g);
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, hi, acc[j][i], 0, 0, 0);
+                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lo, acc[j][i], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    f32x16_t d;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) d[e] = 0.f;
+                    for (int r = 0; r < l.rank; r += 16) {
+                        const bf16x8_t u = lora_up(l, u0[j] + at, r + 8 * g);
+                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lora_t(t + r), d, 0, 0, 0);
+                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lora_t(t + l.rp + r), d, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[j][i][e] += mine == a ? d[e] : 0.f;
+                }
+            }
+        }
+    }
+}
+
 // ---- 256 x 256, direct global -> LDS, 4 stages ------------------------------
 constexpr int DBK = 32, DSTAGES = 4, DROWB = DBK * 2, DOPB = 256 * DROWB, DSTAGEB = 2 * DOPB;
 
@@ -301,8 +389,8 @@ __device__ __forceinline__ int swz8(int r) { return (r ^ (r >> 3)) & 7; }
 // dt_dequant followed by the bf16 GEMM bit for bit.  Each code is converted
 // once per workgroup (the eight-wave gemm_q8_kernel converts each twice, after
 // the LDS read); measured 4-16% faster than it on the step's products.
-template <typename TC, bool SCHED, int BM, bool Q8 = false, int NW = 4, int BN = 256, int KG = 1>
-__global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp) {
+template <typename TC, bool SCHED, int BM, bool Q8 = false, int NW = 4, int BN = 256, int KG = 1, typename L = NoLora>
+__global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp, const L lora) {
     static_assert(BN == 128 || BM == 256 || BM == 224, "tile height");
     static_assert(NW == 4 || (NW == 8 && BM == 256), "eight waves: 256-row tiles");
     static_assert((BN == 256 && KG == 1) || (BM == 128 && BN == 128 && NW == 4), "K groups: 128 x 128 tiles");
@@ -551,6 +639,8 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp)
                     for (int e = 0; e < 16; ++e)
                         acc[j][i][e] += part[(q * NW + wave) * PW + ((j * FM + i) * 16 + e) * 64 + lane];
     }
+    if constexpr (L::on)
+        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
@@ -764,8 +854,8 @@ __global__ __launch_bounds__(512) void gemm_q8_kernel(const Group grp) {
 constexpr int SBK = 64;
 constexpr int SLDSW = SBK + 8;  // padded LDS row, in bf16 elements
 
-template <typename TC, bool Q8 = false>
-__global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp) {
+template <typename TC, bool Q8 = false, typename L = NoLora>
+__global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L lora) {
     constexpr int FM = 2, FN = 2, T = 256;
     constexpr int CH = 128 * (SBK / 8) / T;  // 16-byte chunks per thread per operand
     constexpr int STAGE = 256 * SLDSW;
@@ -892,6 +982,8 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp) {
         if (more) stash(s ^ 1);
         __syncthreads();
     }
+    if constexpr (L::on)
+        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
@@ -913,8 +1005,8 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp) {
 // bf16, the value dt_dequant writes.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-template <typename TC, bool Q8, int KS>
-__global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp) {
+template <typename TC, bool Q8, int KS, typename L = NoLora>
+__global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, const L lora) {
     constexpr int UNR = 4;      // 64-k blocks loaded together
     constexpr int LD = 16 + 4;  // padded row of the partial sums
     __shared__ float part[KS][16 * LD];
@@ -979,6 +1071,26 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp) {
     for (; b + UNR <= b1; b += UNR) step(b, std::integral_constant<int, UNR>{});
     for (; b < b1; ++b) step(b, std::integral_constant<int, 1>{});
 
+    if constexpr (L::on) {
+        // The rows' adapters over the waves, each product kept in its own rows.
+        const int mine = r < p.M ? lora.row_adapter[r] : -1;
+        const uint16_t* t = lora.t + (int64_t)min(r, p.M - 1) * 2 * lora.rp + 8 * g;
+        const uint16_t* u0 = lora.u + n * lora.ldu;
+        uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < lora.adapters);
+        for (int turn = 0; left; ++turn) {
+            const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(left));
+            left &= ~__builtin_amdgcn_ballot_w64(mine == a);
+            if (turn % KS != wave) continue;
+            f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < lora.rank; k += 32) {
+                const bf16x8_t u = lora_up(lora, u0 + a * lora.u_stride, k + 8 * g);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, lora_t(t + k), d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, lora_t(t + lora.rp + k), d, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += mine == a ? d[e] : 0.f;
+        }
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[wave][r * LD + 4 * g + e] = acc[e];
     __syncthreads();
@@ -1006,8 +1118,8 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp) {
 // value dt_dequant writes.  Four waves of 64 x 64 on the same MFMA as the
 // kernels above.  These shapes are small (they occur outside the step's
 // projections), so the kernel is written for coverage, not rate.
-template <typename TC, bool Q8>
-__global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp) {
+template <typename TC, bool Q8, typename L = NoLora>
+__global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp, const L lora) {
     constexpr int FM = 2, FN = 2, LDW = 24;  // LDS row: 16 bf16 + 8 of padding (48 bytes)
     __shared__ __attribute__((aligned(16))) uint16_t sa[128 * LDW];
     __shared__ __attribute__((aligned(16))) uint16_t sb[128 * LDW];
@@ -1072,6 +1184,8 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp) {
             for (int i = 0; i < FM; ++i)
                 acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[j], xf[i], acc[j][i], 0, 0, 0);
     }
+    if constexpr (L::on)
+        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
@@ -1177,8 +1291,22 @@ int pick_config(const Problem* ps, int n, int cus, bool ranges) {
     return ranges ? pick_by_waves(ps, n, cus, {8, 1, kSplitConfig}) : pick_by_waves(ps, n, cus, {8, 1});
 }
 
-template <typename TC, bool Q8>
-int launch_skinny(const Problem* ps, int n, hipStream_t st) {
+// The configuration of a group when the caller names none.
+int pick_of(const Problem* ps, int n, bool all_tiled) {
+    int m_max = 0;
+    bool ranges = true;
+    for (int i = 0; i < n; ++i) {
+        m_max = m_max > ps[i].M ? m_max : ps[i].M;
+        ranges = ranges && sums_ranges(ps[i].N, ps[i].K);
+    }
+    return !all_tiled                    ? kAnyConfig
+           : ranges && m_max <= kSkinnyM ? kSkinnyConfig
+           : ps[0].Bs                    ? pick_config_q8(ps, n, cu_count(), ranges)
+                                         : pick_config(ps, n, cu_count(), ranges);
+}
+
+template <typename TC, bool Q8, typename L>
+int launch_skinny(const Problem* ps, int n, const L& lora, hipStream_t st) {
     Group g{};
     g.count = n;
     int64_t total = 0;
@@ -1191,16 +1319,39 @@ int launch_skinny(const Problem* ps, int n, hipStream_t st) {
     g.tile_start[n] = (int)total;
     // Eight waves a workgroup until there are four workgroups per CU.
     if (total >= 4 * cu_count())
-        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 4>), dim3((unsigned)total), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 4, L>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
     else
-        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8>), dim3((unsigned)total), dim3(512), 0, st, g);
+        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8, L>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
     return check_launch("dt_gemm_bf16");
 }
 
-template <typename TC>
-int launch(const Problem* ps, int n, int cfg, hipStream_t st) {
+// The configurations that a size picks, with or without adapters.
+template <typename TC, typename L>
+int launch_picked(const Group& g, int cfg, dim3 grid, dim3 block, const L& lora, hipStream_t st) {
+    const bool q8 = g.p[0].Bs != nullptr;
+    if (cfg == 8)
+        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, false, 8, 256, 1, L>), grid, block, 0, st, g, lora);
+    else if (cfg == 9)
+        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, true, 8, 256, 1, L>), grid, block, 0, st, g, lora);
+    else if (cfg == kSplitConfig && q8)
+        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 128, true, 4, 128, 2, L>), grid, block, 0, st, g, lora);
+    else if (cfg == kSplitConfig)
+        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 128, false, 4, 128, 2, L>), grid, block, 0, st, g, lora);
+    else if (cfg == kAnyConfig && q8)
+        hipLaunchKernelGGL((gemm_any_kernel<TC, true, L>), grid, block, 0, st, g, lora);
+    else if (cfg == kAnyConfig)
+        hipLaunchKernelGGL((gemm_any_kernel<TC, false, L>), grid, block, 0, st, g, lora);
+    else if (q8)
+        hipLaunchKernelGGL((gemm_128_kernel<TC, true, L>), grid, block, 0, st, g, lora);
+    else
+        hipLaunchKernelGGL((gemm_128_kernel<TC, false, L>), grid, block, 0, st, g, lora);
+    return check_launch("dt_gemm_bf16");
+}
+
+template <typename TC, typename L = NoLora>
+int launch(const Problem* ps, int n, int cfg, hipStream_t st, const L& lora = L{}) {
     if (cfg == kSkinnyConfig)
-        return ps[0].Bs ? launch_skinny<TC, true>(ps, n, st) : launch_skinny<TC, false>(ps, n, st);
+        return ps[0].Bs ? launch_skinny<TC, true>(ps, n, lora, st) : launch_skinny<TC, false>(ps, n, lora, st);
     Group g{};
     g.count = n;
     int64_t total = 0;
@@ -1213,35 +1364,25 @@ int launch(const Problem* ps, int n, int cfg, hipStream_t st) {
     g.tile_start[n] = (int)total;
     if (total == 0) return DT_OK;
     const dim3 grid((unsigned)total), block((unsigned)kConfigs[cfg].threads);
-    if (cfg == 0)
-        hipLaunchKernelGGL((gemm_dma256_kernel<TC>), grid, block, 0, st, g);
-    else if (cfg == 2)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, false, 256>), grid, block, 0, st, g);
-    else if (cfg == 5)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256>), grid, block, 0, st, g);
-    else if (cfg == 6)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 224>), grid, block, 0, st, g);
-    else if (cfg == 7)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, true>), grid, block, 0, st, g);
-    else if (cfg == 8)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, false, 8>), grid, block, 0, st, g);
-    else if (cfg == 9)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, true, 8>), grid, block, 0, st, g);
-    else if (cfg == 3)
-        hipLaunchKernelGGL((gemm_q8_kernel<TC>), grid, block, 0, st, g);
-    else if (cfg == kSplitConfig && ps[0].Bs)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 128, true, 4, 128, 2>), grid, block, 0, st, g);
-    else if (cfg == kSplitConfig)
-        hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 128, false, 4, 128, 2>), grid, block, 0, st, g);
-    else if (cfg == kAnyConfig && ps[0].Bs)
-        hipLaunchKernelGGL((gemm_any_kernel<TC, true>), grid, block, 0, st, g);
-    else if (cfg == kAnyConfig)
-        hipLaunchKernelGGL((gemm_any_kernel<TC, false>), grid, block, 0, st, g);
-    else if (ps[0].Bs)
-        hipLaunchKernelGGL((gemm_128_kernel<TC, true>), grid, block, 0, st, g);
-    else
-        hipLaunchKernelGGL((gemm_128_kernel<TC>), grid, block, 0, st, g);
-    return check_launch("dt_gemm_bf16");
+    if constexpr (!L::on) {
+        if (cfg == 0)
+            hipLaunchKernelGGL((gemm_dma256_kernel<TC>), grid, block, 0, st, g);
+        else if (cfg == 2)
+            hipLaunchKernelGGL((gemm_k64_kernel<TC, false, 256>), grid, block, 0, st, g, lora);
+        else if (cfg == 3)
+            hipLaunchKernelGGL((gemm_q8_kernel<TC>), grid, block, 0, st, g);
+        else if (cfg == 5)
+            hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256>), grid, block, 0, st, g, lora);
+        else if (cfg == 6)
+            hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 224>), grid, block, 0, st, g, lora);
+        else if (cfg == 7)
+            hipLaunchKernelGGL((gemm_k64_kernel<TC, true, 256, true>), grid, block, 0, st, g, lora);
+        else
+            return launch_picked<TC>(g, cfg, grid, block, lora, st);
+        return check_launch("dt_gemm_bf16");
+    } else {
+        return launch_picked<TC>(g, cfg, grid, block, lora, st);
+    }
 }
 
 // Checks a problem and says whether the tiled kernels take it (K % 64 == 0,
@@ -1378,17 +1519,7 @@ extern "C" int dt_gemm_bf16_grouped(const dt_gemm_problem* problems, int32_t cou
     DT_REQUIRE(config == -1 || config == kAnyConfig || all_tiled,
                "dt_gemm_bf16: config %d needs K %% 64 == 0 and 16-byte aligned rows", config);
     if (n == 0) return DT_OK;
-    int m_max = 0;
-    bool ranges = true;
-    for (int i = 0; i < n; ++i) {
-        m_max = m_max > ps[i].M ? m_max : ps[i].M;
-        ranges = ranges && sums_ranges(ps[i].N, ps[i].K);
-    }
-    const int cfg = config >= 0      ? config
-                    : !all_tiled     ? kAnyConfig
-                    : ranges && m_max <= kSkinnyM ? kSkinnyConfig
-                    : n_q8           ? pick_config_q8(ps, n, cu_count(), ranges)
-                                     : pick_config(ps, n, cu_count(), ranges);
+    const int cfg = config >= 0 ? config : pick_of(ps, n, all_tiled);
     hipStream_t st = (hipStream_t)stream;
     return c_type == DT_TYPE_F32 ? launch<float>(ps, n, cfg, st) : launch<bf16>(ps, n, cfg, st);
 }
@@ -1421,6 +1552,34 @@ extern "C" size_t dt_gemm_bf16_workspace_bytes(int64_t M, int64_t N, int64_t K) 
     return s > 1 ? (size_t)(s * M * gemm_split_ld(N)) * sizeof(float) : 0;
 }
 
+namespace dit {
+namespace {
+// One product over split_count's K ranges (validated, tiled, within reach): partial sums
+// in `part`, the adapters (if any) in the first range's, joined by a second launch.
+template <typename L = NoLora>
+int launch_ranges(const Problem& p, int32_t c_type, float* part, hipStream_t st, const L& lora = L{}) {
+    const int S = split_count(p.M, p.N, p.K, cu_count());
+    const int64_t ldp = gemm_split_ld(p.N), blocks = p.K / 64;
+    Problem ps[kMaxGroup];
+    for (int s = 0; s < S; ++s) {
+        const int64_t k0 = blocks * s / S * 64, k1 = blocks * (s + 1) / S * 64;
+        ps[s] = p;
+        ps[s].A = p.A + k0;
+        ps[s].B = p.Bs ? reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(p.B) + k0) : p.B + k0;
+        if (p.Bs) ps[s].Bs = p.Bs + k0 / 32 * p.ldbs;
+        ps[s].K = (int)(k1 - k0);
+        ps[s].C = part + s * (int64_t)p.M * ldp;
+        ps[s].ldc = ldp;
+        ps[s].D = nullptr;
+        ps[s].bias = nullptr;
+    }
+    const int rc = launch<float>(ps, S, kSplitConfig, st, lora);
+    if (rc) return rc;
+    return gemm_reduce(part, S, p.M, p.N, p.C, p.ldc, p.bias, p.D, p.ldd, c_type, st);
+}
+}  // namespace
+}  // namespace dit
+
 extern "C" int dt_gemm_bf16_ws(const dt_gemm_problem* problem, int32_t c_type, void* workspace, size_t workspace_bytes,
                                dt_stream_t stream) {
     using namespace dit;
@@ -1435,23 +1594,68 @@ extern "C" int dt_gemm_bf16_ws(const dt_gemm_problem* problem, int32_t c_type, v
     const int rc = validate(q, c_type, &p, &tiled);
     if (rc) return rc;
     if (!tiled || !reaches(&p, 1, kSplitConfig)) return dt_gemm_bf16_grouped(problem, 1, c_type, -1, stream);
-    const int S = split_count(q.M, q.N, q.K, cu_count());
-    const int64_t ldp = gemm_split_ld(q.N), blocks = q.K / 64;
-    Problem ps[kMaxGroup];
-    float* part = (float*)workspace;
-    for (int s = 0; s < S; ++s) {
-        const int64_t k0 = blocks * s / S * 64, k1 = blocks * (s + 1) / S * 64;
-        ps[s] = p;
-        ps[s].A = p.A + k0;
-        ps[s].B = p.Bs ? reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(p.B) + k0) : p.B + k0;
-        if (p.Bs) ps[s].Bs = p.Bs + k0 / 32 * p.ldbs;
-        ps[s].K = (int)(k1 - k0);
-        ps[s].C = part + s * q.M * ldp;
-        ps[s].ldc = ldp;
-        ps[s].D = nullptr;
-        ps[s].bias = nullptr;
-    }
-    const int rl = launch<float>(ps, S, kSplitConfig, (hipStream_t)stream);
-    if (rl) return rl;
-    return gemm_reduce(part, S, q.M, q.N, q.C, q.ldc, q.bias, q.addend, q.ldd, c_type, (hipStream_t)stream);
+    return launch_ranges(p, c_type, (float*)workspace, (hipStream_t)stream);
+}
+
+namespace dit {
+namespace {
+// Checks the adapters of a product of N columns and K terms.
+int validate_lora(const dt_lora& l, int64_t M, int64_t N, int64_t K, const char* who) {
+    DT_REQUIRE(l.adapters >= 0 && l.rank >= 0, "%s: negative size", who);
+    DT_REQUIRE(l.adapters < (1 << 24) && l.rank <= kMaxLoraRank, "%s: rank %lld above %d or too many adapters", who,
+               (long long)l.rank, kMaxLoraRank);
+    if (M == 0 || N == 0 || l.adapters == 0 || l.rank == 0) return DT_OK;
+    DT_REQUIRE(l.a && l.b && l.row_adapter, "%s: null adapter pointer", who);
+    DT_REQUIRE(((uintptr_t)l.a & 1) == 0 && ((uintptr_t)l.b & 1) == 0, "%s: adapters must be 2-byte aligned", who);
+    DT_REQUIRE(((uintptr_t)l.scale & 3) == 0 && ((uintptr_t)l.row_adapter & 3) == 0,
+               "%s: scale and row_adapter must be 4-byte aligned", who);
+    DT_REQUIRE(l.lda >= K && l.ldb >= l.rank, "%s: leading dimensions must cover the adapters' rows", who);
+    DT_REQUIRE(l.a_stride >= 0 && l.b_stride >= 0, "%s: negative adapter stride", who);
+    return DT_OK;
+}
+size_t lora_t_bytes(int64_t M, int64_t rank) { return (size_t)((M * 2 * lora_rank_padded(rank) * 2 + 15) / 16 * 16); }
+}  // namespace
+}  // namespace dit
+
+extern "C" size_t dt_lora_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t rank) {
+    using namespace dit;
+    if (M <= 0 || N <= 0 || K <= 0 || rank < 0 || rank > kMaxLoraRank || M >= (1ll << 31)) return 0;
+    return (rank ? lora_t_bytes(M, rank) : 0) + dt_gemm_bf16_workspace_bytes(M, N, K);
+}
+
+extern "C" int dt_lora_gemm(const dt_gemm_problem* problem, const dt_lora* lora, int32_t c_type, void* workspace,
+                            size_t workspace_bytes, dt_stream_t stream) {
+    using namespace dit;
+    const char* who = "dt_lora_gemm";
+    DT_REQUIRE(problem != nullptr && lora != nullptr, "%s: null arguments", who);
+    DT_REQUIRE(is_io_type(c_type), "%s: c_type %d unsupported", who, c_type);
+    Problem p;
+    bool tiled = false;
+    int rc = validate(*problem, c_type, &p, &tiled);
+    if (!rc) rc = validate_lora(*lora, p.M, p.N, p.K, who);
+    if (rc || p.M == 0 || p.N == 0) return rc;
+    if (lora->adapters == 0 || lora->rank == 0) return dt_gemm_bf16_ws(problem, c_type, workspace, workspace_bytes, stream);
+    const size_t t_bytes = lora_t_bytes(p.M, lora->rank);
+    DT_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= t_bytes,
+               "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, t_bytes, workspace ? workspace_bytes : 0);
+    const hipStream_t st = (hipStream_t)stream;
+    uint16_t* t = (uint16_t*)workspace;
+    rc = lora_down(p.A, p.lda, p.M, p.K, *lora, t, st);
+    if (rc) return rc;
+    LoraTile l{};
+    l.t = t;
+    l.u = (const uint16_t*)lora->b;
+    l.ldu = lora->ldb;
+    l.u_stride = lora->b_stride;
+    l.row_adapter = lora->row_adapter;
+    l.adapters = (int)lora->adapters;
+    l.rank = (int)lora->rank;
+    l.rp = (int)lora_rank_padded(lora->rank);
+    l.vec = lora->rank % 8 == 0 && lora->ldb % 8 == 0 && (lora->b_stride % 8 == 0 || lora->adapters == 1) && aligned16(lora->b);
+    // The product's own choice (dt_gemm_bf16_ws).
+    const size_t need = dt_gemm_bf16_workspace_bytes(p.M, p.N, p.K);
+    if (need && tiled && workspace_bytes >= t_bytes + need && reaches(&p, 1, kSplitConfig))
+        return launch_ranges(p, c_type, (float*)((uint8_t*)workspace + t_bytes), st, l);
+    const int cfg = pick_of(&p, 1, tiled);
+    return c_type == DT_TYPE_F32 ? launch<float>(&p, 1, cfg, st, l) : launch<bf16>(&p, 1, cfg, st, l);
 }

@@ -88,6 +88,12 @@ inline int64_t gemm_split_ld(int64_t N) { return (N + 3) / 4 * 4; }
 int gemm_reduce(const float* part, int S, int64_t M, int64_t N, void* C, int64_t ldc, const float* bias,
                 const void* addend, int64_t ldd, int32_t c_type, hipStream_t st);
 
+// T = scale (x A_a^T) of each row's adapter a as two bf16 parts, [M][2][lora_rank_padded(rank)]
+// (zeros past the rank and for a row without adapter), lora.hip.
+constexpr int kMaxLoraRank = 512;
+inline int64_t lora_rank_padded(int64_t rank) { return (rank + 31) / 32 * 32; }
+int lora_down(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, const dt_lora& lora, uint16_t* t, hipStream_t st);
+
 // Fused fp32 attention (attention_f32.hip) for head_dim 128 with 16-byte rows:
 // whether it takes a call, the (batch, head) pairs it takes per launch within a
 // workspace limit, their workspace, the launches.

@@ -135,6 +135,8 @@ _SIGS = {
     "dt_flash_attn_bf16": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                      c_int64, c_int64, c_int64, POINTER(c_int64), POINTER(c_int64),
                                      POINTER(c_int64), POINTER(c_int64), c_float, c_int32, _S]),
+    "dt_lora_gemm_workspace_bytes": (ctypes.c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "dt_lora_gemm": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, ctypes.c_size_t, _S]),
     "dt_rel_bucket_fill": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32]),
     "dt_attn_fwd_workspace_bytes": (ctypes.c_size_t, [c_void_p]),
     "dt_attn_fwd": (c_int32, [c_void_p, c_void_p, _I64P, c_void_p, c_void_p, ctypes.c_size_t, _S]),
@@ -767,6 +769,70 @@ def flash_attn_qk(q_segments, k, v, pos, axis_dim, freq_base, eps=1e-6, table=No
         _p(q0), st(q0), _p(w0), _p(q1), st(q1) if q1 is not None else None, _p(w1), S0 if q1 is not None else Sq,
         eps, _p(pos), pos.stride(0), pos.shape[1], axis_dim, freq_base, _p(table), n_pos, _p(k), _p(v), _p(out),
         B, H, Sq, Skv, D, st(k), st(v), st(out), scale, io_type(out), stream()), "dt_flash_attn_qk_bf16")
+    return out
+
+
+class LoraArgs(ctypes.Structure):
+    _fields_ = [("a", c_void_p), ("lda", c_int64), ("a_stride", c_int64), ("b", c_void_p), ("ldb", c_int64),
+                ("b_stride", c_int64), ("scale", c_void_p), ("row_adapter", c_void_p), ("adapters", c_int64),
+                ("rank", c_int64)]
+
+
+class Lora:
+    """Low-rank adapters of one Linear, side by side: a bf16 [adapters, rank, K] (down),
+    b bf16 [adapters, N, rank] (up), scale fp32 [adapters] or None (1)."""
+
+    def __init__(self, a, b, scale=None):
+        self.a, self.b, self.scale = a, b, scale
+
+
+def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dtype=None):
+    """x: bf16 [M, K], w: bf16 [N, K] or Q8Weight -> x @ w.T (+ bias) (+ addend) +
+    scale[a] * (x @ a[a].T) @ b[a].T, each row with the adapter a = row_adapter[m]
+    (int32 [M]; outside the adapters: none)."""
+    torch = _torch()
+    M, K = x.shape
+    N = w.shape[0]
+    q8 = isinstance(w, Q8Weight)
+    a, b, scale = lora.a, lora.b, lora.scale
+    n, rank = a.shape[0], a.shape[1]
+    codes = w.codes if q8 else w
+    if x.dtype != torch.bfloat16 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16 or \
+            codes.dtype != (torch.uint8 if q8 else torch.bfloat16):
+        raise DtError("x, w (or its codes) and the adapters must be bf16 (codes uint8)")
+    if w.shape[1] != K or a.shape != (n, rank, K) or b.shape != (n, N, rank):
+        raise DtError(f"adapters {tuple(a.shape)}, {tuple(b.shape)} do not fit x {tuple(x.shape)} and w {tuple(w.shape)}")
+    if (K > 1 and (x.stride(1) != 1 or codes.stride(1) != 1 or a.stride(2) != 1)) or (rank > 1 and b.stride(2) != 1):
+        raise DtError("rows of x, w and the adapters must be contiguous")
+    if row_adapter.dtype != torch.int32 or row_adapter.shape != (M,) or (M > 1 and row_adapter.stride(0) != 1):
+        raise DtError("row_adapter must be contiguous int32 [M]")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (n,) or (n > 1 and scale.stride(0) != 1)):
+        raise DtError("scale must be contiguous fp32 [adapters]")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+        raise DtError("bias must be contiguous fp32 [N]")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
+    for t in (out, addend):
+        if t is not None and (t.shape != (M, N) or t.dtype != out.dtype or (N > 1 and t.stride(1) != 1)):
+            raise DtError("out and addend must be [M, N] of one dtype with contiguous rows")
+    _same_device(x, codes, w.scales if q8 else None, a, b, scale, row_adapter, bias, addend, out)
+
+    def ld(t, cols):  # the row stride of a tensor of one row is not used
+        return max(t.stride(-2), cols) if t.shape[-2] <= 1 else t.stride(-2)
+
+    p = GemmProblem(x.data_ptr(), ld(x, K), codes.data_ptr(), ld(codes, K), out.data_ptr(), ld(out, N),
+                    None if addend is None else addend.data_ptr(), 0 if addend is None else ld(addend, N),
+                    None if bias is None else bias.data_ptr(), M, N, K, w.scales.data_ptr() if q8 else None,
+                    ld(w.scales, N) if q8 else 0)
+    s = LoraArgs(a.data_ptr(), ld(a, K), a.stride(0), b.data_ptr(), ld(b, rank), b.stride(0),
+                 None if scale is None else scale.data_ptr(), row_adapter.data_ptr(), n, rank)
+    lib = load()
+    nbytes = lib.dt_lora_gemm_workspace_bytes(M, N, K, rank)
+    ws = _scratch(nbytes, x.device) if nbytes else None
+    check(lib.dt_lora_gemm(ctypes.addressof(p), ctypes.addressof(s), io_type(out), _p(ws), nbytes, stream()),
+          "dt_lora_gemm")
+    if isinstance(lib, _Recorder):
+        lib.keep.extend((p, s))
     return out
 
 

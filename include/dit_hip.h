@@ -535,6 +535,33 @@ size_t dt_attn_bwd_workspace_bytes(const dt_attn_args *args);
 int dt_attn_bwd(const dt_attn_args *args, const dt_attn_grads *grads, void *workspace, size_t workspace_bytes,
                 dt_stream_t stream);
 
+/* Low-rank adapters of many requests beside a shared Linear:
+ *   C[m][n] = (dt_gemm_bf16 / dt_gemm_q8_0 of `problem`) +
+ *             scale[a] * sum_r (sum_k A[m][k] a[a][r][k]) b[a][n][r],  a = row_adapter[m],
+ * summed in fp32 and rounded once; a row whose row_adapter is outside [0,
+ * adapters) has the shared product alone, and no adapter reaches another
+ * adapter's rows.  a: bf16 [adapters][rank][K] (rows lda apart, adapters a_stride),
+ * b: bf16 [adapters][N][rank] (rows ldb, adapters b_stride), scale: fp32 [adapters]
+ * or NULL (1), row_adapter: int32 [M]; all device memory.  Any rank up to 512
+ * (adapters of smaller ranks are filled up with zeros); ranks, K and strides in
+ * multiples of 8 with 16-byte aligned pointers are read fastest.  `workspace`
+ * (dt_lora_gemm_workspace_bytes, 16-byte aligned) holds the rows' rank-space
+ * values, and the partial sums of a product that dt_gemm_bf16_ws would split;
+ * without room for those the product is not split.  The reference has no
+ * adapters: Linear::forward is one mul_mat (src/nn/Linear.cpp:17-36). */
+typedef struct dt_lora {
+    const void *a;
+    int64_t lda, a_stride;
+    const void *b;
+    int64_t ldb, b_stride;
+    const float *scale;
+    const int32_t *row_adapter;
+    int64_t adapters, rank;
+} dt_lora;
+size_t dt_lora_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t rank);
+int dt_lora_gemm(const dt_gemm_problem *problem, const dt_lora *lora, int32_t c_type, void *workspace,
+                 size_t workspace_bytes, dt_stream_t stream);
+
 /* ======================================================================== */
 /* (iii) unfused ggml-op kernels on ggml-shaped descriptors                 */
 /* ======================================================================== */
