@@ -88,6 +88,14 @@ __device__ __forceinline__ void to_frag(const float (&p)[8], Elem<float>::Frag& 
     for (int e = 0; e < 8; ++e) f.v[e] = p[e];
 }
 
+template <typename T>
+__device__ __forceinline__ void acc_frag(const f32x16_t& p, int j, typename Elem<T>::Frag& f) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = p[8 * j + e];
+    to_frag(v, f);
+}
+
 __device__ __forceinline__ float frag_dot(const bf16x8_t& a, const bf16x8_t& b) {
     float s = 0.f;
 #pragma unroll
@@ -138,6 +146,17 @@ __device__ __forceinline__ void wait_vmem() {
 }
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+constexpr uint32_t kOut = 0x80000000u;  // an offset out of every buffer's range
+// 16 bytes a lane from base + off (zeros where off is out of range) to lds + 16 lane; base and lds uniform.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint8_t* lds) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
+}__device__ __forceinline__ void dma4(const void* base, uint32_t off, void* lds) {  // 4 bytes a lane
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
+}
+
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t* lds_short4_p;
 __device__ __forceinline__ uint2 read_tr16(const uint8_t* p) {
@@ -157,27 +176,37 @@ struct Tile {
         return CPR == 8 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
     }
 
-    // ROWS rows by NW waves (this one is `wave`): row(r) gives the source row.
-    // Chunks past the head width are not written: the tile is cleared once
-    // before its first use (clear()).
-    template <int ROWS, int NW, typename Row>
-    __device__ __forceinline__ static void load(const T* src, int64_t stride, int dim, uint8_t* lds, int wave, int lane,
-                                                Row row) {
-        constexpr int J = ROWS * CPR / 64 / NW;
+    // ROWS rows by NW waves (this one is `wave`) as buffer loads to LDS: a scalar base
+    // per tile, the lane's rows and chunks as 32-bit offsets for all tiles.  An offset out of
+    // the buffer's range gives zeros: chunks past the head width, and rows that are not
+    // kept (keep), whose values then reach no product (a mask may hide NaN, a tail
+    // lies outside the tensor).
+    template <int ROWS, int NW>
+    struct Loads {
+        static constexpr int J = ROWS * CPR / 64 / NW;
         static_assert(J >= 1 && ROWS * CPR % (64 * NW) == 0, "tile");
-        const int chunks = dim / Elem<T>::EPC;
+        uint32_t at[J];
+
+        __device__ __forceinline__ void init(int64_t stride, int dim, int wave, int lane) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int at = (wave * J + j) * 64, r = (at + lane) / CPR, c = ((at + lane) % CPR) ^ swz(r);
-            const T* p = src + (int64_t)row(r) * stride + c * Elem<T>::EPC;
-            if (chunks == CPR || c < chunks) __builtin_amdgcn_global_load_lds(p, lds + at * 16, 16, 0, 0);
+            for (int j = 0; j < J; ++j) {
+                const int i = (wave * J + j) * 64 + lane, r = i / CPR, c = (i % CPR) ^ swz(r);
+                at[j] = c * Elem<T>::EPC < dim ? (uint32_t)((r * stride + c * Elem<T>::EPC) * (int64_t)sizeof(T)) : kOut;
+            }
         }
-    }
+        __device__ __forceinline__ static int row(int wave, int lane, int j) { return ((wave * J + j) * 64 + lane) / CPR; }
 
-    __device__ __forceinline__ static void clear(uint8_t* lds, int bytes, int tid, int threads) {
-        for (int i = tid * 16; i < bytes; i += threads * 16) *reinterpret_cast<uint4*>(lds + i) = make_uint4(0, 0, 0, 0);
-    }
-
+        // base: the tile's first row.
+        __device__ __forceinline__ void issue_all(const T* base, uint8_t* lds, int wave) const {
+#pragma unroll
+            for (int j = 0; j < J; ++j) dma16(base, at[j], lds + (wave * J + j) * 1024);
+        }
+        template <typename Keep>
+        __device__ __forceinline__ void issue(const T* base, uint8_t* lds, int wave, int lane, Keep keep) const {
+#pragma unroll
+            for (int j = 0; j < J; ++j) dma16(base, keep(row(wave, lane, j)) ? at[j] : kOut, lds + (wave * J + j) * 1024);
+        }
+    };
     // Row operand: elements 16 c + 8 g .. + 7 of row r.
     __device__ __forceinline__ static Frag row_frag(const uint8_t* t, int r, int c, int g) {
         Frag f;
@@ -238,6 +267,81 @@ struct Tile {
     }
 };
 
+// N products whose first operands come from LDS: read(i) gives one, mul(i, f) uses it, and
+// side(n, of) is other work for the n-th of `of` parts, of V vector instructions for each
+// product (0: none).  bf16 reads four operands ahead, R LDS instructions each, while the
+// four before are multiplied, and spreads the other work between the products: left alone
+// the compiler reads each operand right before its product, into the same registers, and
+// every product waits for LDS.  An fp32 operand lasts eight instructions of 64 cycles: it is
+// read when it is needed.
+struct NoSide {
+    __device__ __forceinline__ void operator()(int, int) const {}
+};
+template <typename T, int N, int R, int V = 0, typename Read, typename Mul, typename Side = NoSide>
+__device__ __forceinline__ void products(Read read, Mul mul, Side side = Side{}) {
+    constexpr int G = 4;
+    static_assert(N % G == 0, "groups");
+    if constexpr (sizeof(T) == 2) {
+        typename Elem<T>::Frag f[2][G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) f[0][i] = read(i);
+#pragma unroll
+        for (int n = 0; n < N / G; ++n) {
+            if (n + 1 < N / G) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) f[(n + 1) & 1][i] = read((n + 1) * G + i);
+            }
+#pragma unroll
+            for (int i = 0; i < G; ++i) mul(n * G + i, f[n & 1][i]);
+            side(n, N / G);
+            if (n == 0) __builtin_amdgcn_sched_group_barrier(0x100, R * G, 0);
+            if constexpr (V == 0) {
+                __builtin_amdgcn_sched_group_barrier(0x100, R * G, 0);  // LDS reads
+                __builtin_amdgcn_sched_group_barrier(0x008, G, 0);      // MFMA
+            } else {
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x402, V, 0);  // vector and transcendental ALU
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            mul(i, read(i));
+            if (i % G == G - 1) side(i / G, N / G);
+        }
+    }
+}
+
+// An operand put together from four accumulator elements at a time (see to_frag).
+template <typename T> struct FragParts;
+template <> struct FragParts<bf16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void set(int half, const float (&v)[4]) {
+        w[2 * half] = pack_bf16x2(v[0], v[1]);
+        w[2 * half + 1] = pack_bf16x2(v[2], v[3]);
+    }
+    __device__ __forceinline__ bf16x8_t frag() const { return __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3])); }
+};
+template <> struct FragParts<float> {
+    Elem<float>::Frag f;
+    __device__ __forceinline__ void set(int half, const float (&v)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f.v[4 * half + e] = v[e];
+    }
+    __device__ __forceinline__ const Elem<float>::Frag& frag() const { return f; }
+};
+
+// The other lane half's value (lane ^ 32).
+__device__ __forceinline__ float swap32(float v) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
+}
+
 // ---- kept keys --------------------------------------------------------------------
 __device__ __forceinline__ int kept_len(const AttnIn& a, int b) {
     int n = a.seq_kv;
@@ -245,18 +349,22 @@ __device__ __forceinline__ int kept_len(const AttnIn& a, int b) {
     return n;
 }
 
-// Walks the tiles of N keys (32 or 64) that hold a kept key, from `t` on by
+// Walks the tiles of N keys (32, 64 or 128) that hold a kept key, from `t` on by
 // `step` to `end`, the mask bytes of the tile after read ahead.  Uniform in the wave.
 template <int N>
 struct Kept {
+    static constexpr int W = (N + 63) / 64;
     const uint8_t* mask;
     int len, t, end, step;
-    uint32_t ahead;  // mask byte of key N t + lane
-    uint64_t word;   // kept keys of the tile next() returned
+    uint32_t ahead[W];  // mask byte of key N t + 64 w + lane
+    uint64_t word[W];   // kept keys of the tile next() returned
 
     __device__ __forceinline__ void fetch(int lane) {
-        const int key = t * N + lane;
-        ahead = t < end && lane < N && key < len ? (mask ? mask[key] : 1u) : 0u;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int key = t * N + 64 * w + lane;
+            ahead[w] = t < end && (N >= 64 || lane < N) && key < len ? (mask ? mask[key] : 1u) : 0u;
+        }
     }
     __device__ __forceinline__ void start(const AttnIn& a, int b, int n, int first, int last, int by, int lane) {
         mask = a.kv_mask ? a.kv_mask + b * a.mask_stride : nullptr;
@@ -269,40 +377,53 @@ struct Kept {
     // The next tile with a kept key, or -1.
     __device__ __forceinline__ int next(int lane) {
         while (t < end) {
-            word = __builtin_amdgcn_ballot_w64(ahead != 0);
+            uint64_t any = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) any |= word[w] = __builtin_amdgcn_ballot_w64(ahead[w] != 0);
             const int at = t;
             t += step;
             fetch(lane);
-            if (word) return at;
+            if (any) return at;
         }
         return -1;
     }
 };
 template <int N>
-__device__ __forceinline__ bool all_kept(uint64_t word) {
-    return N == 64 ? word == ~0ull : (uint32_t)word == 0xFFFFFFFFu;
+__device__ __forceinline__ bool all_kept(const uint64_t (&word)[(N + 63) / 64]) {
+    if constexpr (N == 32) return (uint32_t)word[0] == 0xFFFFFFFFu;
+    if constexpr (N == 64) return word[0] == ~0ull;
+    return (word[0] & word[N / 64 - 1]) == ~0ull;
 }
-// Source row of tile row r: itself, or the tile's first kept row where it is not
-// kept, whose values (a mask may hide NaN, a tail lies outside the tensor)
-// then never reach a product.
-__device__ __forceinline__ int kept_row(uint64_t word, int r) {
-    return (word >> r) & 1 ? r : (int)__builtin_ctzll(word);
+template <int W>
+__device__ __forceinline__ bool kept_row(const uint64_t (&word)[W], int r) {
+    return ((W == 1 || r < 64 ? word[0] : word[W - 1]) >> (r & 63)) & 1;
 }
 
 // ---- bias -------------------------------------------------------------------------
-// Offset key - query, clamped to +-reach, to its bucket.
+// Offset key - query to its bucket.
 __device__ __forceinline__ int rel_bucket(const RelArgs& r, int off) {
     const int dist = off > 0 ? (r.two_sided ? off : 0) : -off;
     int t = 0;
     for (int i = 1; i < r.side; ++i) t += dist >= r.start[i];
     return t + (r.two_sided && off > 0 ? r.side : 0);
 }
-// line[reach + off] = the bias of that offset in units of log2, for one head.
+// line[reach + kMargin + off] = the bias of that offset in units of log2, for one head.  The
+// margins are what a 32 x 32 block with some |offset| < reach can have beyond it: no offset
+// is clamped.
+constexpr int kMargin = 62;
+__host__ __device__ inline int rel_line_len(int reach) { return 2 * (reach + kMargin) + 1; }
 __device__ __forceinline__ void rel_line(const RelArgs& r, int head, float* line, int tid, int threads) {
-    for (int i = tid; i < 2 * r.reach + 1; i += threads)
-        line[i] = r.table[rel_bucket(r, i - r.reach) * r.table_stride + head] * kLog2e;
+    const int mid = r.reach + kMargin;
+    for (int i = tid; i < 2 * mid + 1; i += threads)
+        line[i] = r.table[rel_bucket(r, i - mid) * r.table_stride + head] * kLog2e;
 }
-inline int rel_line_floats(const RelArgs& r) { return r.table ? 2 * r.reach + 1 : 0; }
+inline int rel_line_floats(const RelArgs& r) { return r.table ? rel_line_len(r.reach) : 0; }
+// Where a lane reads the bias of offsets lo + {0 .. 27}: in a block out of reach the end of the
+// line on its side, which holds one value.
+__device__ __forceinline__ const float* rel_at(const float* line, int reach, int lo) {
+    const int mid = reach + kMargin;
+    return line + mid + min(max(lo, -mid), mid - 27);
+}
 // Position of query 0 of batch entry b.  Positions far from every key differ only in
 // being far: the bound keeps offsets in 32 bits.
 __device__ __forceinline__ int rel_position(const RelArgs& r, int b) {
@@ -311,6 +432,7 @@ __device__ __forceinline__ int rel_position(const RelArgs& r, int b) {
 
 // ---- host ---------------------------------------------------------------------------
 constexpr int64_t kMaxSeq = 1 << 28;
+constexpr int64_t kMaxRowStride = (1 << 23) - 128;  // 64 fp32 rows stay below kOut bytes
 // Checks the shared arguments and fills `in` (cross_attention.hip).
 int prepare_in(const dt_attn_args* args, const char* who, AttnIn* in);
 // Checks one strided operand [batch][seq][heads][head_dim]; `out`: no element twice.

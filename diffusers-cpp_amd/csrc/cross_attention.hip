@@ -11,7 +11,10 @@
 // 2 reach + 1 values per head in LDS (offsets beyond the last bucket's start are
 // clamped), read by offset for each score of a tile that the band |offset| < reach
 // meets and once for any other.
+#include <float.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "attn_tiles.hpp"
 
@@ -32,143 +35,150 @@ struct FwdArgs {
     float* part_ml;  // [splits][batch * groups][rows][2]: their reference (log2) and sum
 };
 
-// Scores in units of log2 with the bias, -inf for a key that is not kept.
-// Element i of s[hh] is key 32 hh + 8 (i / 4) + 4 g + i % 4 of the tile.
-template <int HALVES, bool BIAS>
-__device__ __forceinline__ void finish_scores(f32x16_t (&s)[HALVES], float sc, uint64_t word, bool full,
-                                              const float* line, int reach, int off0, int g) {
+// With a bias: scores in units of log2, the bias added.  Without: as they are (the scale
+// is folded into the exponent).  -inf for a key that is not kept.  Element i of s is key
+// 8 (i / 4) + 4 g + i % 4 of the 32 whose kept ones `word` says.
+template <bool BIAS>
+__device__ __forceinline__ void finish_scores(f32x16_t& s, float sc, uint32_t word, const float* line, int reach, int off0,
+                                              int g) {
+    if constexpr (BIAS) {
+        // off0 + r: offset of key r to this lane's query.
+        const int lo = off0 + 4 * g;
+        const float* at = line + reach + kMargin + lo;
+        if (__builtin_amdgcn_ballot_w64(lo < reach && lo + 28 > -reach) == 0) {
+            const float far = line[lo > 0 ? 2 * (reach + kMargin) : 0];
 #pragma unroll
-    for (int hh = 0; hh < HALVES; ++hh) {
-        if constexpr (BIAS) {
-            // off0 + r: offset of the tile's key r to this lane's query.
-            const int lo = off0 + 32 * hh + 4 * g;
-            if (__builtin_amdgcn_ballot_w64(lo < reach && lo + 28 > -reach) == 0) {
-                const float far = line[lo > 0 ? 2 * reach : 0];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[hh][i] = __builtin_fmaf(s[hh][i], sc, far);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int off = min(max(lo + 8 * (i >> 2) + (i & 3), -reach), reach);
-                    s[hh][i] = __builtin_fmaf(s[hh][i], sc, line[reach + off]);
-                }
-            }
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sc, far);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[hh][i] *= sc;
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(s[i], sc, at[8 * (i >> 2) + (i & 3)]);
         }
-        if (!full) {
-            const uint32_t w = (uint32_t)(word >> (32 * hh)) >> (4 * g);
+    }
+    if (word != 0xFFFFFFFFu) {
+        const uint32_t w = word >> (4 * g);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (!(w & (1u << (8 * (i >> 2) + (i & 3))))) s[hh][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+            if (!(w & (1u << (8 * (i >> 2) + (i & 3))))) s[i] = -INFINITY;
     }
 }
 
 // The running softmax of one query: reference m (log2), this lane's half of the sum.
-template <int BLOCKS>
+// Scores are in units of 1 / sc of log2 (sc > 0; 1 with a bias).
+template <typename T, int BLOCKS>
 struct Running {
-    float m = -INFINITY, l = 0.f;
+    float m, l;
     f32x16_t o[BLOCKS];
 
     __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) o[b] = zero16();
     }
-    // The reference moves only when a score exceeds it by more than 2^8, so most
-    // tiles skip the rescale and every P stays <= 256.
-    template <int HALVES>
-    __device__ __forceinline__ void take(f32x16_t (&s)[HALVES]) {
-        float mx = s[0][0];
+    // Whether the reference moved.  It does only when a score exceeds it by more than 2^8, so
+    // most tiles skip the rescale, and every weight stays <= 256.
+    __device__ __forceinline__ bool look(const f32x16_t& s, float sc) {
+        float mx = s[0];
 #pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[hh][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, swap32(mx)) * sc;
         const bool move = mx > m + 8.0f;
-        if (__builtin_amdgcn_ballot_w64(move)) {
-            const float to = move ? mx : m;
-            const float alpha = move ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
-            l *= alpha;
+        if (__builtin_amdgcn_ballot_w64(move) == 0) return false;
+        const float to = move ? mx : m;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        l *= alpha;
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
+        for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
-            m = to;
-        }
+            for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+        m = to;
+        return true;
+    }
+    // The weights of elements 4 i4 .. + 3 into their operand, and added to `sum` before that
+    // rounds them: lse, from which the gradients' weights come, stays fp32.
+    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i4, FragParts<T> (&p)[2], float& sum) const {
         const float ref = m == -INFINITY ? 0.f : m;  // scores of -inf only, so far: weight 0
+        float v[4];
 #pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh)
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], sc, -ref));
+        p[i4 / 2].set(i4 & 1, v);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[hh][i] = __builtin_amdgcn_exp2f(s[hh][i] - ref);
-                l += s[hh][i];
-            }
+        for (int e = 0; e < 4; ++e) sum += v[e];
     }
 };
 
-template <typename T, int N>
-__device__ __forceinline__ void p_frag(const f32x16_t (&p)[N], int j, typename Elem<T>::Frag& f) {
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = p[j >> 1][8 * (j & 1) + e];
-    to_frag(v, f);
-}
+// The lane's row of a row block.
+struct Row {
+    int tok, h;
+    bool live;
+    __device__ __forceinline__ Row(const FwdArgs& a, int row, int h0) {
+        live = row < a.rows;
+        tok = live ? (int)fdiv((uint32_t)row, a.pack_div) : 0;
+        h = h0 + (live ? row - tok * a.pack : 0);
+    }
+};
 
-// ---- many rows: 128 rows per workgroup, 32 per wave, 64-key tiles shared ------------
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const FwdArgs a) {
+// ---- many rows: 128 rows per workgroup, 32 per wave, tiles of 64 KG keys shared --------
+// A tile's two 32-key halves are staggered, so that one half's weights (vector and
+// exponential instructions) run between the other half's products.
+// KG = 1: four waves, two workgroups per CU.
+// KG = 2: for at most one block per CU eight waves, two per SIMD; each half of them
+// takes half of a 128-key tile, and the halves' results are joined through LDS (2048
+// queries x 16 heads x 128 to 1500 keys: 52 -> 39 us).
+template <typename T, int DP, bool BIAS, int KG>
+__global__ __launch_bounds__(256 * KG, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(const FwdArgs a) {
     typedef Tile<T, DP> Tl;
-    constexpr int KB = 64, TILE = KB * Tl::RB, NW = 4;
+    constexpr int KB = 64 * KG, TILE = KB * Tl::RB, NW = 4 * KG;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][K | V], then the bias line
     float* const line = reinterpret_cast<float*>(smem + 4 * TILE);
     const AttnIn& in = a.in;
 
+    // Batch entries innermost: their lengths differ, and every XCD gets some of each.
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.row_blocks), bg = (int)(bid / (uint32_t)a.row_blocks);
-    const int grp = bg % a.groups, b = bg / a.groups, h0 = grp * a.pack, kvh = h0 / in.shared;
+    const int b = bg % in.batch, h0 = bg / in.batch * a.pack, kvh = h0 / in.shared;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
-    const int row = blk * 128 + wave * 32 + r;
-    const bool live = row < a.rows;
-    const int tok = live ? (int)fdiv((uint32_t)row, a.pack_div) : 0, h = h0 + (live ? row - tok * a.pack : 0);
+    const int r = lane & 31, g = lane >> 5, kg = wave >> 2;
+    const int row = blk * 128 + (wave & 3) * 32 + r;
+    const Row w(a, row, h0);
 
     const T* Kp = reinterpret_cast<const T*>(in.k) + b * in.ks[0] + kvh * in.ks[2];
     const T* Vp = reinterpret_cast<const T*>(in.v) + b * in.vs[0] + kvh * in.vs[2];
-    if (in.dim < DP) Tl::clear(smem, 4 * TILE, tid, 256);
-    if constexpr (BIAS) rel_line(in.rel, h0, line, tid, 256);
-    if (BIAS || in.dim < DP) __syncthreads();
-
     Kept<KB> kept;
-    const int len = kept_len(in, b);
-    kept.start(in, b, len, 0, in.seq_kv, 1, lane);
-    auto issue = [&](int t, uint64_t word, int buf) {
+    kept.start(in, b, kept_len(in, b), 0, in.seq_kv, 1, lane);
+    typename Tl::template Loads<KB, NW> kl, vl;
+    kl.init(in.ks[1], in.dim, wave, lane);
+    vl.init(in.vs[1], in.dim, wave, lane);
+    auto issue = [&](int t, int buf) {
         uint8_t* kb = smem + buf * 2 * TILE;
         const T* ks = Kp + (int64_t)t * KB * in.ks[1];
         const T* vs = Vp + (int64_t)t * KB * in.vs[1];
-        if (all_kept<KB>(word)) {
-            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [](int i) { return i; });
-            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [](int i) { return i; });
+        if (all_kept<KB>(kept.word)) {
+            kl.issue_all(ks, kb, wave);
+            vl.issue_all(vs, kb + TILE, wave);
         } else {
-            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [&](int i) { return kept_row(word, i); });
-            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [&](int i) { return kept_row(word, i); });
+            const auto keep = [&](int i) { return kept_row(kept.word, i); };
+            kl.issue(ks, kb, wave, lane, keep);
+            vl.issue(vs, kb + TILE, wave, lane, keep);
         }
     };
     int t = kept.next(lane);
-    uint64_t word = kept.word;
-    if (t >= 0) issue(t, word, 0);
+    uint64_t word = kg ? kept.word[KG - 1] : kept.word[0];
+    if (t >= 0) issue(t, 0);
 
     typename Tl::Frag qf[Tl::STEPS];
     {
-        const T* qp = reinterpret_cast<const T*>(in.q) + b * in.qs[0] + (int64_t)tok * in.qs[1] + h * in.qs[2];
+        const T* qp = reinterpret_cast<const T*>(in.q) + b * in.qs[0] + (int64_t)w.tok * in.qs[1] + w.h * in.qs[2];
 #pragma unroll
-        for (int c = 0; c < Tl::STEPS; ++c) qf[c] = live ? frag_global<T>(qp, c, g, in.dim) : frag_zero<T>();
+        for (int c = 0; c < Tl::STEPS; ++c) qf[c] = w.live ? frag_global<T>(qp, c, g, in.dim) : frag_zero<T>();
     }
+    if constexpr (BIAS) rel_line(in.rel, h0, line, tid, 64 * NW);  // read after the first tile's barrier
     const typename Tl::Cols cols = Tl::cols(lane);
-    Running<Tl::BLOCKS> run;
+    Running<T, Tl::BLOCKS> run;
     run.clear();
-    const int at = tok + (BIAS ? rel_position(in.rel, b) : 0);
+    const float sc = BIAS ? 1.0f : in.scale_log2;
+    // With a bias a row is a token; rows past the last one too, so the block's offsets stay together.
+    const int at = BIAS ? row + rel_position(in.rel, b) : 0;
 
     int buf = 0;
     while (t >= 0) {
@@ -177,34 +187,86 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         const int t_next = kept.next(lane);
-        const uint64_t word_next = kept.word;
-        if (t_next >= 0) issue(t_next, word_next, buf ^ 1);
-        const uint8_t* Kt = smem + buf * 2 * TILE;
+        if (t_next >= 0) issue(t_next, buf ^ 1);
+        const uint8_t* Kt = smem + buf * 2 * TILE + kg * 64 * Tl::RB;
         const uint8_t* Vt = Kt + TILE;
-
-        f32x16_t s[2] = {zero16(), zero16()};
+        if (KG == 1 || word) {
+            f32x16_t s[2] = {zero16(), zero16()};
+            FragParts<T> p[2][2];
+            float sum[2] = {0.f, 0.f};
+            auto scores = [&](auto hc, auto vc, auto side) {
+                constexpr int hh = decltype(hc)::value;
+                products<T, Tl::STEPS, 1, decltype(vc)::value>(
+                    [&](int i) { return Tl::row_frag(Kt, 32 * hh + r, i, g); },
+                    [&](int i, const typename Tl::Frag& f) { s[hh] = mma(f, qf[i], s[hh]); }, side);
+            };
+            auto finish = [&](int hh) {
+                finish_scores<BIAS>(s[hh], in.scale_log2, (uint32_t)(word >> (32 * hh)), line, in.rel.reach,
+                                    t * KB + kg * 64 + 32 * hh - at, g);
+            };
+            auto weights = [&](auto hc) {
+                return [&, hc](int part, int of) {
 #pragma unroll
-        for (int c = 0; c < Tl::STEPS; ++c)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) s[hh] = mma(Tl::row_frag(Kt, 32 * hh + r, c, g), qf[c], s[hh]);
-        finish_scores<2, BIAS>(s, in.scale_log2, word, all_kept<KB>(word), line, in.rel.reach, t * KB - at, g);
-        run.take(s);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            typename Tl::Frag pf;
-            p_frag<T>(s, j, pf);
-#pragma unroll
-            for (int d = 0; d < Tl::BLOCKS; ++d) run.o[d] = mma(Tl::col_frag(Vt, 16 * j, d, cols), pf, run.o[d]);
+                    for (int i4 = 0; i4 < 4; ++i4)
+                        if (i4 * of / 4 == part) run.weigh(s[hc], sc, i4, p[hc], sum[hc]);
+                };
+            };
+            auto values = [&](auto hc, auto vc, auto side) {
+                constexpr int hh = decltype(hc)::value;
+                products<T, 2 * Tl::BLOCKS, 2, decltype(vc)::value>(
+                    [&](int i) { return Tl::col_frag(Vt, 32 * hh + 16 * (i / Tl::BLOCKS), i % Tl::BLOCKS, cols); },
+                    [&](int i, const typename Tl::Frag& f) {
+                        run.o[i % Tl::BLOCKS] = mma(f, p[hh][i / Tl::BLOCKS].frag(), run.o[i % Tl::BLOCKS]);
+                    },
+                    side);
+            };
+            using H0 = std::integral_constant<int, 0>;
+            using H1 = std::integral_constant<int, 1>;
+            using V = std::integral_constant<int, DP == 64 ? 12 : 6>;  // vector instructions per product
+            scores(H0{}, H0{}, NoSide{});
+            finish(0);
+            run.look(s[0], sc);
+            scores(H1{}, V{}, weights(H0{}));
+            finish(1);
+            if (run.look(s[1], sc)) {  // the first half's weights again, by the new reference
+                sum[0] = 0.f;
+                weights(H0{})(0, 1);
+            }
+            values(H0{}, V{}, weights(H1{}));
+            values(H1{}, H0{}, NoSide{});
+            run.l += sum[0] + sum[1];
         }
         t = t_next;
-        word = word_next;
+        word = kg ? kept.word[KG - 1] : kept.word[0];
         buf ^= 1;
     }
-
-    const float l = run.l + __shfl_xor(run.l, 32);
+    if constexpr (KG == 2) {
+        // The second half's waves hand theirs over in the tiles' place, lane for lane.
+        __syncthreads();
+        float* part = reinterpret_cast<float*>(smem) + (wave & 3) * (Tl::BLOCKS * 16 + 2) * 64 + lane;
+        if (kg == 1) {
+            part[0] = run.m;
+            part[64] = run.l;
+#pragma unroll
+            for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[(2 + 16 * d + e) * 64] = run.o[d][e];
+        }
+        __syncthreads();
+        if (kg == 1) return;
+        const float m1 = part[0], m = fmaxf(run.m, m1), ref = m == -INFINITY ? 0.f : m;
+        const float w0 = __builtin_amdgcn_exp2f(run.m - ref), w1 = __builtin_amdgcn_exp2f(m1 - ref);
+        run.m = m;
+        run.l = run.l * w0 + part[64] * w1;
+#pragma unroll
+        for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) run.o[d][e] = run.o[d][e] * w0 + part[(2 + 16 * d + e) * 64] * w1;
+    }
+    const float l = run.l + swap32(run.l);
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no kept key: 0; NaN stays
-    if (!live) return;
-    T* op = reinterpret_cast<T*>(a.o) + b * a.os[0] + (int64_t)tok * a.os[1] + h * a.os[2];
+    if (!w.live) return;
+    T* op = reinterpret_cast<T*>(a.o) + b * a.os[0] + (int64_t)w.tok * a.os[1] + w.h * a.os[2];
 #pragma unroll
     for (int d = 0; d < Tl::BLOCKS; ++d)
 #pragma unroll
@@ -216,7 +278,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_rows_kernel(
             if (e0 < in.dim) put4(op + e0, v);
         }
     if (a.lse && g == 0)
-        a.lse[((int64_t)b * in.heads + h) * in.seq_q + tok] = l == 0.f ? -INFINITY : (run.m + __builtin_amdgcn_logf(l)) * kLn2;
+        a.lse[((int64_t)b * in.heads + w.h) * in.seq_q + w.tok] =
+            l == 0.f ? -INFINITY : (run.m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // ---- few rows: 32 rows per workgroup, keys over its waves and over workgroups --------
@@ -237,36 +300,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_few_kernel(c
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.row_blocks), rest = (int)(bid / (uint32_t)a.row_blocks);
     const int split = rest % a.splits, bg = rest / a.splits;
-    const int grp = bg % a.groups, b = bg / a.groups, h0 = grp * a.pack, kvh = h0 / in.shared;
+    const int b = bg % in.batch, h0 = bg / in.batch * a.pack, kvh = h0 / in.shared;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5;
     const int row = blk * 32 + r;
-    const bool live = row < a.rows;
-    const int tok = live ? (int)fdiv((uint32_t)row, a.pack_div) : 0, h = h0 + (live ? row - tok * a.pack : 0);
+    const Row w(a, row, h0);
+    const int tok = w.tok, h = w.h;
+    const bool live = w.live;
 
     const T* Kp = reinterpret_cast<const T*>(in.k) + b * in.ks[0] + kvh * in.ks[2];
     const T* Vp = reinterpret_cast<const T*>(in.v) + b * in.vs[0] + kvh * in.vs[2];
     uint8_t* const Kt = smem + wave * 2 * TILE;
     uint8_t* const Vt = Kt + TILE;
-    if (in.dim < DP) Tl::clear(smem, NW * 2 * TILE, tid, 256);
-    if constexpr (BIAS) rel_line(in.rel, h0, line, tid, 256);
-    if (BIAS || in.dim < DP) __syncthreads();
-
     // This range's tiles of the entry's own kept length: ranges stay even however
     // the lengths differ.
     const int len = kept_len(in, b), tiles = (len + KB - 1) / KB;
     const int first = (int)((int64_t)tiles * split / a.splits), last = (int)((int64_t)tiles * (split + 1) / a.splits);
     Kept<KB> kept;
     kept.start(in, b, len, first + wave, last, NW, lane);
-    auto issue = [&](const T* src, int64_t stride, int t, uint64_t word, uint8_t* lds) {
+    typename Tl::template Loads<KB, 1> kl, vl;
+    kl.init(in.ks[1], in.dim, 0, lane);
+    vl.init(in.vs[1], in.dim, 0, lane);
+    auto issue = [&](const auto& loads, const T* src, int64_t stride, int t, uint32_t word, uint8_t* lds) {
         const T* p = src + (int64_t)t * KB * stride;
-        if (all_kept<KB>(word)) Tl::template load<KB, 1>(p, stride, in.dim, lds, 0, lane, [](int i) { return i; });
-        else Tl::template load<KB, 1>(p, stride, in.dim, lds, 0, lane, [&](int i) { return kept_row(word, i); });
+        if (word == 0xFFFFFFFFu) loads.issue_all(p, lds, 0);
+        else loads.issue(p, lds, 0, lane, [&](int i) { return (word >> i) & 1; });
     };
     constexpr int VL = KB * Tl::CPR / 64;  // loads of one tile
     int t = kept.next(lane);
-    uint64_t word = kept.word;
-    if (t >= 0) issue(Kp, in.ks[1], t, word, Kt);
+    uint32_t word = (uint32_t)kept.word[0];
+    if (t >= 0) issue(kl, Kp, in.ks[1], t, word, Kt);
 
     typename Tl::Frag qf[Tl::STEPS];
     {
@@ -274,50 +337,58 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_few_kernel(c
 #pragma unroll
         for (int c = 0; c < Tl::STEPS; ++c) qf[c] = live ? frag_global<T>(qp, c, g, in.dim) : frag_zero<T>();
     }
-    if (t >= 0) issue(Vp, in.vs[1], t, word, Vt);
+    if constexpr (BIAS) {
+        rel_line(in.rel, h0, line, tid, 256);
+        wait_lds();  // not __syncthreads: K's DMA stays in flight
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (t >= 0) issue(vl, Vp, in.vs[1], t, word, Vt);
     const typename Tl::Cols cols = Tl::cols(lane);
-    Running<Tl::BLOCKS> run;
+    Running<T, Tl::BLOCKS> run;
     run.clear();
-    const int at = tok + (BIAS ? rel_position(in.rel, b) : 0);
+    // With a bias a row is a token; rows past the last one too, so the block's offsets stay together.
+    const int at = BIAS ? row + rel_position(in.rel, b) : 0;
 
     while (t >= 0) {
         wait_vmem<VL>();  // K (V's loads are younger)
         __builtin_amdgcn_sched_barrier(0);
         f32x16_t s[1] = {zero16()}, s2 = zero16();
-#pragma unroll
-        for (int c = 0; c < Tl::STEPS; c += 2) {
-            s[0] = mma(Tl::row_frag(Kt, r, c, g), qf[c], s[0]);
-            s2 = mma(Tl::row_frag(Kt, r, c + 1, g), qf[c + 1], s2);
-        }
+        products<T, Tl::STEPS, 1>([&](int i) { return Tl::row_frag(Kt, r, i, g); },
+                                  [&](int i, const typename Tl::Frag& f) {
+                                      if (i & 1) s2 = mma(f, qf[i], s2);
+                                      else s[0] = mma(f, qf[i], s[0]);
+                                  });
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[0][i] += s2[i];
         wait_lds();  // K is read: its buffer is free
         __builtin_amdgcn_sched_barrier(0);
         const int t_next = kept.next(lane);
-        const uint64_t word_next = kept.word;
-        if (t_next >= 0) issue(Kp, in.ks[1], t_next, word_next, Kt);
-        finish_scores<1, BIAS>(s, in.scale_log2, word, all_kept<KB>(word), line, in.rel.reach, t * KB - at, g);
-        run.take(s);
+        const uint32_t word_next = (uint32_t)kept.word[0];
+        if (t_next >= 0) issue(kl, Kp, in.ks[1], t_next, word_next, Kt);
+        finish_scores<BIAS>(s[0], in.scale_log2, word, line, in.rel.reach, t * KB - at, g);
+        run.look(s[0], BIAS ? 1.0f : in.scale_log2);
+        FragParts<T> p[2];
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) run.weigh(s[0], BIAS ? 1.0f : in.scale_log2, i4, p, run.l);
         // V (the next K's loads, and the mask byte read ahead, are younger).
         if (t_next >= 0) wait_vmem<VL>();
         else wait_vmem<0>();
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            typename Tl::Frag pf;
-            p_frag<T>(s, j, pf);
-#pragma unroll
-            for (int d = 0; d < Tl::BLOCKS; ++d) run.o[d] = mma(Tl::col_frag(Vt, 16 * j, d, cols), pf, run.o[d]);
-        }
+        products<T, 2 * Tl::BLOCKS, 2>(
+            [&](int i) { return Tl::col_frag(Vt, 16 * (i / Tl::BLOCKS), i % Tl::BLOCKS, cols); },
+            [&](int i, const typename Tl::Frag& f) {
+                run.o[i % Tl::BLOCKS] = mma(f, p[i / Tl::BLOCKS].frag(), run.o[i % Tl::BLOCKS]);
+            });
         wait_lds();
         __builtin_amdgcn_sched_barrier(0);
-        if (t_next >= 0) issue(Vp, in.vs[1], t_next, word_next, Vt);
+        if (t_next >= 0) issue(vl, Vp, in.vs[1], t_next, word_next, Vt);
         t = t_next;
         word = word_next;
     }
 
     // The waves' results under the largest reference.
-    const float l = run.l + __shfl_xor(run.l, 32);
+    const float l = run.l + swap32(run.l);
     if (g == 0) {
         ml[0][wave][r] = run.m;
         ml[1][wave][r] = l;
@@ -386,7 +457,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const FwdArgs a) {
     const int64_t n = (int64_t)in.batch * a.groups * a.rows;
     if (id >= n) return;
     const int row = (int)(id % a.rows), bg = (int)(id / a.rows);
-    const int tok = (int)fdiv((uint32_t)row, a.pack_div), h = (bg % a.groups) * a.pack + row - tok * a.pack, b = bg / a.groups;
+    const Row r(a, row, bg / in.batch * a.pack);
+    const int tok = r.tok, h = r.h, b = bg % in.batch;
     float m = -INFINITY;
     for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[((int64_t)s * n + id) * 2]);
     const float ref = m == -INFINITY ? 0.f : m;
@@ -414,7 +486,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(const FwdArgs a) {
 // ---- choice and launch --------------------------------------------------------------
 struct Plan {
     bool few;
-    int pack, groups, rows, row_blocks, splits;
+    int kg, pack, groups, rows, row_blocks, splits;
     int64_t part_floats;  // workspace
 };
 
@@ -422,7 +494,7 @@ int padded_dim(int64_t dim) { return dim <= 64 ? 64 : 128; }
 
 // Query heads that share a key head lie side by side as rows (their keys are then
 // read once), but with a bias, whose line belongs to one head.
-Plan plan(const AttnIn& in, int cus) {
+Plan plan(const AttnIn& in, bool bf16_io, int cus) {
     Plan p{};
     const int64_t batch = in.batch;
     p.pack = in.rel.table ? 1 : in.shared;
@@ -430,11 +502,13 @@ Plan plan(const AttnIn& in, int cus) {
     p.rows = in.seq_q * p.pack;
     const int64_t wide = (int64_t)((p.rows + 127) / 128) * p.groups * batch;
     const int64_t narrow = (int64_t)((p.rows + 31) / 32) * p.groups * batch;
-    // Blocks of 128 rows while they give every CU one.
-    p.few = wide < cus;
-    p.splits = 1;
+    // Blocks of 128 rows while they give every CU one, and are not three quarters empty.
+    p.few = wide < cus || p.rows <= 32;
+    p.splits = p.kg = 1;
     if (!p.few) {
         p.row_blocks = (p.rows + 127) / 128;
+        // bf16 leaves room for a second workgroup, or twice the waves, on a CU.
+        if (wide <= cus && in.seq_kv > 64 && bf16_io) p.kg = 2;
         return p;
     }
     p.row_blocks = (p.rows + 31) / 32;
@@ -449,14 +523,20 @@ Plan plan(const AttnIn& in, int cus) {
 
 template <typename T, int DP, bool BIAS>
 int launch(const FwdArgs& a, const Plan& p, hipStream_t st) {
-    const int64_t blocks = (int64_t)p.row_blocks * p.splits * p.groups * a.in.batch;
-    const size_t tiles = p.few ? 4 * 2 * 32 * Tile<T, DP>::RB : 4 * 64 * Tile<T, DP>::RB;
+    const size_t tiles = p.few ? 4 * 2 * 32 * Tile<T, DP>::RB : p.kg * 4 * 64 * Tile<T, DP>::RB;
     const size_t lds = tiles + rel_line_floats(a.in.rel) * sizeof(float);
-    if (p.few) hipLaunchKernelGGL((attn_few_kernel<T, DP, BIAS>), dim3((unsigned)blocks), dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((attn_rows_kernel<T, DP, BIAS>), dim3((unsigned)blocks), dim3(256), lds, st, a);
+    const int64_t bg = (int64_t)p.groups * a.in.batch;
+    const int64_t wide = p.row_blocks * bg;
+    if (p.few) {
+        hipLaunchKernelGGL((attn_few_kernel<T, DP, BIAS>), dim3((unsigned)(p.row_blocks * p.splits * bg)), dim3(256), lds, st, a);
+    } else {
+        if constexpr (sizeof(T) == 2)
+            if (p.kg == 2) hipLaunchKernelGGL((attn_rows_kernel<T, DP, BIAS, 2>), dim3((unsigned)wide), dim3(512), lds, st, a);
+        if (p.kg == 1) hipLaunchKernelGGL((attn_rows_kernel<T, DP, BIAS, 1>), dim3((unsigned)wide), dim3(256), lds, st, a);
+    }
     int rc = check_launch("dt_attn_fwd");
     if (rc || p.splits == 1) return rc;
-    const int64_t n = (int64_t)a.in.batch * p.groups * p.rows * (DP / 4);
+    const int64_t n = bg * p.rows * (DP / 4);
     hipLaunchKernelGGL((attn_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     return check_launch("dt_attn_fwd");
 }
@@ -537,7 +617,7 @@ int check_rows(const dt_attn_args* x, const void* p, const int64_t* strides, int
         if (n[at] == 1) continue;
         const int64_t s = strides[at];
         DT_REQUIRE(s % step == 0, "%s: %s strides must keep rows 16-byte aligned", who, name);
-        DT_REQUIRE(s >= 0 && s < (1ll << 40), "%s: %s stride %lld unsupported", who, name, (long long)s);
+        DT_REQUIRE(s >= 0 && s < (at == 1 ? kMaxRowStride : 1ll << 40), "%s: %s stride %lld unsupported", who, name, (long long)s);
         if (!out) continue;
         DT_REQUIRE(s >= reach, "%s: elements of %s overlap", who, name);
         reach = s * (n[at] - 1) + reach;
@@ -582,7 +662,9 @@ int prepare_in(const dt_attn_args* x, const char* who, AttnIn* out) {
     a.kv_mask = x->kv_mask;
     a.mask_stride = x->kv_mask_stride;
     a.scale = x->scale;
-    a.scale_log2 = x->scale * kLog2e;
+    // A scale of 0 as the least normal number: -inf times it is still -inf, and every finite
+    // score still next to 0.
+    a.scale_log2 = x->scale * kLog2e > FLT_MIN ? x->scale * kLog2e : FLT_MIN;
     if (x->rel_table) {
         rc = check_rel(x->rel_buckets, x->rel_distance, x->rel_two_sided, who);
         if (rc) return rc;
@@ -629,7 +711,7 @@ extern "C" size_t dt_attn_fwd_workspace_bytes(const dt_attn_args* x) {
     AttnIn in;
     if (prepare_in(x, "dt_attn_fwd_workspace_bytes", &in)) return 0;
     if (in.batch == 0 || in.heads == 0 || in.seq_q == 0) return 0;
-    return (size_t)plan(in, cu_count()).part_floats * sizeof(float);
+    return (size_t)plan(in, x->io_type == DT_TYPE_BF16, cu_count()).part_floats * sizeof(float);
 }
 
 extern "C" int dt_attn_fwd(const dt_attn_args* x, void* o, const int64_t* o_strides, float* lse, void* workspace,
@@ -646,7 +728,7 @@ extern "C" int dt_attn_fwd(const dt_attn_args* x, void* o, const int64_t* o_stri
     a.o = o;
     for (int i = 0; i < 3; ++i) a.os[i] = o_strides[i];
     a.lse = lse;
-    Plan p = plan(a.in, cu_count());
+    Plan p = plan(a.in, x->io_type == DT_TYPE_BF16, cu_count());
     if (p.splits > 1 && (!workspace || workspace_bytes < (size_t)p.part_floats * sizeof(float) || !aligned16(workspace))) p.splits = 1;
     DT_REQUIRE((int64_t)a.in.seq_q * p.pack < (1ll << 31) &&
                    (int64_t)p.row_blocks * p.splits * p.groups * a.in.batch < (1ll << 31) &&

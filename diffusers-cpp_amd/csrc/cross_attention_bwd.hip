@@ -12,6 +12,8 @@
 //    (S = Q K^T, P and dS straight into dV^T += dO^T P and dK^T += Q^T dS).
 //    Too few key blocks for the chip share the queries in ranges, whose fp32 partial
 //    sums are added in range order by a third launch.
+#include <type_traits>
+
 #include "attn_tiles.hpp"
 
 namespace dit {
@@ -42,54 +44,53 @@ constexpr int tile_rows() {
     return sizeof(T) == 4 && DP == 128 ? 32 : 64;
 }
 
-// Floats of a wave's table-gradient line: offsets -(reach + 62) .. reach + 62, all
-// that a 32 x 32 block with an offset inside +-reach has.
-__host__ __device__ inline int grad_line(int reach) { return 2 * (reach + 62) + 1; }
-constexpr int kScratch = 32 * 33;  // a wave's dS block, rows padded
+// A wave's dS block as its 63 diagonals (offsets -31 .. 31), each a row of 32 queries; what
+// lies outside the block stays 0.  Rows padded to 36: the block's writes (a step of 35
+// floats a lane) and a lane's reads of its row in 16 bytes spread over all banks.
+constexpr int kDiag = 36, kScratch = 63 * kDiag;
 
 // ---- dQ, delta, the table's gradient ---------------------------------------------------
 template <typename T, int DP, bool BIAS>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const BwdArgs a) {
     typedef Tile<T, DP> Tl;
     constexpr int KB = tile_rows<T, DP>(), HALVES = KB / 32, TILE = KB * Tl::RB, NW = 4;
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][K | V], bias line, gradient lines, scratch
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][K | V], scratch, bias line, gradient lines
     const AttnIn& in = a.in;
     const int reach = in.rel.reach;
-    float* const line = reinterpret_cast<float*>(smem + 4 * TILE);
-    float* const grad = line + 2 * reach + 1;
-    float* const scratch = grad + NW * grad_line(reach);
+    const int line_len = rel_line_len(reach), mid = reach + kMargin;
+    float* const scratch = reinterpret_cast<float*>(smem + 4 * TILE);
+    float* const line = scratch + NW * kScratch;
+    // Then the waves' table gradients, a line each as the bias's; scratch first, for its alignment.
+    float* const grad = line + line_len;
     __shared__ float far_sum[2][NW];
 
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.row_blocks), bh = (int)(bid / (uint32_t)a.row_blocks);
-    const int h = bh % in.heads, b = bh / in.heads, kvh = h / in.shared;
+    const int b = bh % in.batch, h = bh / in.batch, kvh = h / in.shared;  // batch entries innermost, as in the forward pass
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5;
     const int row = blk * 128 + wave * 32 + r;
     const bool live = row < in.seq_q;
     const int tok = live ? row : 0;
-    float* const my_grad = grad + wave * grad_line(reach);
+    float* const my_grad = grad + wave * line_len;
     float* const my_scratch = scratch + wave * kScratch;
 
     const T* Kp = reinterpret_cast<const T*>(in.k) + b * in.ks[0] + kvh * in.ks[2];
     const T* Vp = reinterpret_cast<const T*>(in.v) + b * in.vs[0] + kvh * in.vs[2];
-    if (in.dim < DP) Tl::clear(smem, 4 * TILE, tid, 256);
-    if constexpr (BIAS) {
-        rel_line(in.rel, h, line, tid, 256);
-        for (int i = tid; i < NW * grad_line(reach); i += 256) grad[i] = 0.f;
-    }
-    if (BIAS || in.dim < DP) __syncthreads();
-
+    typename Tl::template Loads<KB, NW> kl, vl;
+    kl.init(in.ks[1], in.dim, wave, lane);
+    vl.init(in.vs[1], in.dim, wave, lane);
     auto issue = [&](int t, uint64_t word, int buf) {
         uint8_t* kb = smem + buf * 2 * TILE;
         const T* ks = Kp + (int64_t)t * KB * in.ks[1];
         const T* vs = Vp + (int64_t)t * KB * in.vs[1];
-        if (all_kept<KB>(word)) {
-            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [](int i) { return i; });
-            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [](int i) { return i; });
+        if (KB == 64 ? word == ~0ull : (uint32_t)word == 0xFFFFFFFFu) {
+            kl.issue_all(ks, kb, wave);
+            vl.issue_all(vs, kb + TILE, wave);
         } else {
-            Tl::template load<KB, NW>(ks, in.ks[1], in.dim, kb, wave, lane, [&](int i) { return kept_row(word, i); });
-            Tl::template load<KB, NW>(vs, in.vs[1], in.dim, kb + TILE, wave, lane, [&](int i) { return kept_row(word, i); });
+            const auto keep = [&](int i) { return (word >> i) & 1; };
+            kl.issue(ks, kb, wave, lane, keep);
+            vl.issue(vs, kb + TILE, wave, lane, keep);
         }
     };
 
@@ -108,39 +109,52 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
             of[c] = live ? frag_global<T>(gp, c, g, in.dim) : frag_zero<T>();
             delta += frag_dot(of[c], live ? frag_global<T>(op, c, g, in.dim) : frag_zero<T>());
         }
-        delta += __shfl_xor(delta, 32);
+        delta += swap32(delta);
+    }
+    if constexpr (BIAS) {  // read after the first tile's barrier
+        rel_line(in.rel, h, line, tid, 256);
+        for (int i = tid; i < NW * line_len; i += 256) grad[i] = 0.f;
+        for (int i = tid; i < NW * kScratch; i += 256) scratch[i] = 0.f;
     }
     const typename Tl::Cols cols = Tl::cols(lane);
-    const int at = tok + (BIAS ? rel_position(in.rel, b) : 0);
+    const int at = row + (BIAS ? rel_position(in.rel, b) : 0);  // rows past the last one too: the block's offsets stay together
     const int len = kept_len(in, b);
 
-    // P and dS of one 32-key half of tile t (P in s, dS in d).
-    auto half = [&](const uint8_t* Kt, const uint8_t* Vt, int t, int hh, uint64_t word, f32x16_t& s, f32x16_t& d) {
-        s = zero16();
-        d = zero16();
+    // S and dP of one 32-key half of a tile.
+    auto scores = [&](const uint8_t* Kt, const uint8_t* Vt, int hh, f32x16_t& s, f32x16_t& d, auto vc, auto side) {
+        s = d = zero16();
+        products<T, 2 * Tl::STEPS, 1, decltype(vc)::value>(
+            [&](int i) { return Tl::row_frag(i & 1 ? Vt : Kt, 32 * hh + r, i / 2, g); },
+            [&](int i, const typename Tl::Frag& f) {
+                if (i & 1) d = mma(f, of[i / 2], d);
+                else s = mma(f, qf[i / 2], s);
+            },
+            side);
+    };
+    // dS in d from S and dP, elements 4 i4 .. + 3: keys 8 i4 + 4 g + e of the 32 from offset `off`.
+    auto weights = [&](const f32x16_t& s, f32x16_t& d, int off, int i4) {
 #pragma unroll
-        for (int c = 0; c < Tl::STEPS; ++c) {
-            s = mma(Tl::row_frag(Kt, 32 * hh + r, c, g), qf[c], s);
-            d = mma(Tl::row_frag(Vt, 32 * hh + r, c, g), of[c], d);
+        for (int e = 0; e < 4; ++e) {
+            const int i = 4 * i4 + e;
+            float c = -ref;
+            if constexpr (BIAS) c += rel_at(line, reach, off + 4 * g)[8 * i4 + e];
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], in.scale_log2, c));
+            d[i] = p * (d[i] - delta);
         }
-        const int lo = t * KB + 32 * hh + 4 * g - at;
-        const uint32_t w = (uint32_t)(word >> (32 * hh)) >> (4 * g);
+    };
+    auto drop = [&](f32x16_t& d, uint32_t word) {  // keys that are not kept
+        if (word == 0xFFFFFFFFu) return;
+        const uint32_t w = word >> (4 * g);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float bias = -ref;
-            if constexpr (BIAS) bias += line[reach + min(max(lo + 8 * (i >> 2) + (i & 3), -reach), reach)];
-            float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], in.scale_log2, bias));
-            const bool keep = w & (1u << (8 * (i >> 2) + (i & 3)));
-            s[i] = keep ? p : 0.f;
-            d[i] = keep ? p * (d[i] - delta) : 0.f;
-        }
+        for (int i = 0; i < 16; ++i)
+            if (!(w & (1u << (8 * (i >> 2) + (i & 3))))) d[i] = 0.f;
     };
     // Tiles with a kept key, the next one's DMA in flight behind each.
     auto walk = [&](auto body) {
         Kept<KB> kept;
         kept.start(in, b, len, 0, in.seq_kv, 1, lane);
         int t = kept.next(lane), buf = 0;
-        uint64_t word = kept.word;
+        uint64_t word = kept.word[0];
         if (t >= 0) issue(t, word, 0);
         while (t >= 0) {
             wait_vmem<0>();
@@ -148,7 +162,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             const int t_next = kept.next(lane);
-            const uint64_t word_next = kept.word;
+            const uint64_t word_next = kept.word[0];
             if (t_next >= 0) issue(t_next, word_next, buf ^ 1);
             body(smem + buf * 2 * TILE, smem + buf * 2 * TILE + TILE, t, word);
             t = t_next;
@@ -159,6 +173,22 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         __builtin_amdgcn_s_barrier();
     };
 
+    // dS of a tile's halves: the first half's weights between the second one's products.
+    using None = std::integral_constant<int, 0>;
+    using SV = std::integral_constant<int, DP == 64 ? 18 : 9>;  // vector instructions per product
+    auto each = [&](const uint8_t* Kt, const uint8_t* Vt, int t, f32x16_t (&s)[HALVES], f32x16_t (&d)[HALVES]) {
+        const int off = t * KB - at;
+        scores(Kt, Vt, 0, s[0], d[0], None{}, NoSide{});
+        if constexpr (HALVES == 2)
+            scores(Kt, Vt, 1, s[1], d[1], SV{}, [&](int part, int of) {
+#pragma unroll
+                for (int i4 = 0; i4 < 4; ++i4)
+                    if (i4 * of / 4 == part) weights(s[0], d[0], off, i4);
+            });
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) weights(s[HALVES - 1], d[HALVES - 1], off + 32 * (HALVES - 1), i4);
+    };
+
     // The table's gradient is kept in fp32, and a whole row's dS cancels in it: delta
     // from the rounded output (off by its rounding and P's) would show there, so it is
     // summed from P and dP first.
@@ -166,15 +196,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         float sum = 0.f;
         delta = 0.f;
         walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+            f32x16_t s[HALVES], d[HALVES];
+            each(Kt, Vt, t, s, d);
 #pragma unroll
             for (int hh = 0; hh < HALVES; ++hh) {
-                f32x16_t s, d;
-                half(Kt, Vt, t, hh, word, s, d);
+                drop(d[hh], (uint32_t)(word >> (32 * hh)));
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum += d[i];
+                for (int i = 0; i < 16; ++i) sum += d[hh][i];
             }
         });
-        delta = sum + __shfl_xor(sum, 32);
+        delta = sum + swap32(sum);
     }
     if (live && g == 0) {
         a.ref[stat] = ref;
@@ -186,14 +217,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     for (int d = 0; d < Tl::BLOCKS; ++d) dq[d] = zero16();
     float far[2] = {0.f, 0.f};  // keys behind, keys ahead, out of reach
     walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+        f32x16_t s[HALVES], dsv[HALVES];
+        each(Kt, Vt, t, s, dsv);
 #pragma unroll
         for (int hh = 0; hh < HALVES; ++hh) {
-            f32x16_t s, ds;
-            half(Kt, Vt, t, hh, word, s, ds);
+            f32x16_t& ds = dsv[hh];
+            drop(ds, (uint32_t)(word >> (32 * hh)));
             if constexpr (BIAS) {
                 // Offsets of this 32 x 32 block: off0 + [-31, 31].  A block that is out
                 // of reach as a whole has one bucket (per side: reach may be small).
-                const int off0 = t * KB + 32 * hh - (blk * 128 + wave * 32) - (at - tok);
+                const int off0 = t * KB + 32 * hh - (blk * 128 + wave * 32) - (at - row);
                 if (off0 - 31 >= reach || off0 + 31 <= -reach) {
                     float sum = 0.f;
 #pragma unroll
@@ -201,33 +234,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
                     far[0] += off0 > 0 ? 0.f : sum;
                     far[1] += off0 > 0 ? sum : 0.f;
                 } else {
-                    // Key-major block in LDS, then a diagonal per lane, in row order.
+                    // Diagonal key - query + 31 of each element, then a lane sums its diagonal in four parts.
+                    float* to = my_scratch + (31 + 4 * g) * kDiag - (kDiag - 1) * r;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) my_scratch[(8 * (i >> 2) + 4 * g + (i & 3)) * 33 + r] = ds[i];
+                    for (int i = 0; i < 16; ++i) to[(8 * (i >> 2) + (i & 3)) * kDiag] = ds[i];
                     wait_lds();
                     __builtin_amdgcn_sched_barrier(0);
-                    const int diag = lane - 31;
-                    float sum = 0.f;
+                    const float4* from = reinterpret_cast<const float4*>(my_scratch + min(lane, 62) * kDiag);
+                    float4 sum = from[0];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int key = i + diag;
-                        if (key >= 0 && key < 32) sum += my_scratch[key * 33 + i];
+                    for (int i = 1; i < 8; ++i) {
+                        const float4 x = from[i];
+                        sum.x += x.x;
+                        sum.y += x.y;
+                        sum.z += x.z;
+                        sum.w += x.w;
                     }
-                    if (lane < 63) my_grad[reach + 62 + off0 + diag] += sum;
+                    if (lane < 63) my_grad[mid + off0 + lane - 31] += (sum.x + sum.y) + (sum.z + sum.w);
                     wait_lds();
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            typename Tl::Frag f2[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float v[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = ds[8 * j + e];
-                typename Tl::Frag f;
-                to_frag(v, f);
-#pragma unroll
-                for (int d = 0; d < Tl::BLOCKS; ++d) dq[d] = mma(Tl::col_frag(Kt, 32 * hh + 16 * j, d, cols), f, dq[d]);
-            }
+            for (int j = 0; j < 2; ++j) acc_frag<T>(ds, j, f2[j]);
+            products<T, 2 * Tl::BLOCKS, 2>(
+                [&](int i) { return Tl::col_frag(Kt, 32 * hh + 16 * (i / Tl::BLOCKS), i % Tl::BLOCKS, cols); },
+                [&](int i, const typename Tl::Frag& f) { dq[i % Tl::BLOCKS] = mma(f, f2[i / Tl::BLOCKS], dq[i % Tl::BLOCKS]); });
         }
     });
 
@@ -252,7 +285,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
         __syncthreads();
         // The waves' lines, in wave order, into the first.
-        const int n = grad_line(reach);
+        const int n = line_len;
         for (int i = tid; i < n; i += 256) {
             float sum = grad[i];
 #pragma unroll
@@ -261,18 +294,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
         __syncthreads();
         // A bucket per wave at a time: its offsets over the lanes.
-        float* out = a.part_table + ((int64_t)bh * a.row_blocks + blk) * a.buckets;
+        float* out = a.part_table + (((int64_t)b * in.heads + h) * a.row_blocks + blk) * a.buckets;
         for (int t = wave; t < a.buckets; t += NW) {
             const bool ahead = in.rel.two_sided && t >= in.rel.side;
             const int u = ahead ? t - in.rel.side : t;
             const bool last = u == in.rel.side - 1;
             // Distances [lo, hi) of the bucket.  Without the two sides every key ahead is at distance 0.
-            const int lo = in.rel.start[u], hi = last ? reach + 63 : in.rel.start[u + 1];
+            const int lo = in.rel.start[u], hi = last ? mid + 1 : in.rel.start[u + 1];
             float sum = 0.f;
             for (int dist = lo + lane; dist < hi; dist += 64)
-                if (!ahead || dist > 0) sum += grad[reach + 62 + (ahead ? dist : -dist)];
+                if (!ahead || dist > 0) sum += grad[mid + (ahead ? dist : -dist)];
             if (!in.rel.two_sided && u == 0)
-                for (int dist = 1 + lane; dist < reach + 63; dist += 64) sum += grad[reach + 62 + dist];
+                for (int dist = 1 + lane; dist <= mid; dist += 64) sum += grad[mid + dist];
             sum = wave_sum(sum);
             if (lane == 0) {
                 if (last)
@@ -300,7 +333,7 @@ __global__ __launch_bounds__(64) void attn_dtable_kernel(const BwdArgs a) {
 
 // ---- dK, dV ----------------------------------------------------------------------------
 template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const BwdArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_dkv_kernel(const BwdArgs a) {
     typedef Tile<T, DP> Tl;
     constexpr int QB = tile_rows<T, DP>(), HALVES = QB / 32, TILE = QB * Tl::RB, NW = 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][Q | dO], [buffer][ref | delta], bias line
@@ -310,7 +343,7 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const BwdArgs a) {
 
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.key_blocks), rest = (int)(bid / (uint32_t)a.key_blocks);
-    const int range = rest % a.ranges, bh = rest / a.ranges, kvh = bh % in.kv_heads, b = bh / in.kv_heads;
+    const int range = rest % a.ranges, bh = rest / a.ranges, b = bh % in.batch, kvh = bh / in.batch;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5;
     const int key = blk * 128 + wave * 32 + r, len = kept_len(in, b);
@@ -341,21 +374,26 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const BwdArgs a) {
     if (__syncthreads_or(keep) == 0) last = first;  // no kept key in the block
     const int pos = BIAS ? rel_position(in.rel, b) : 0;
 
-    if (in.dim < DP) {
-        Tl::clear(smem, 4 * TILE, tid, 256);
-        __syncthreads();
-    }
+    typename Tl::template Loads<QB, NW> ql, gl;
+    ql.init(in.qs[1], in.dim, wave, lane);
+    gl.init(a.dos[1], in.dim, wave, lane);
     auto issue = [&](int n, int buf) {
         const int h = kvh * in.shared + n / tiles, q0 = (n % tiles) * QB;
         const int left = in.seq_q - q0;
         uint8_t* qb = smem + buf * 2 * TILE;
         const T* qp = reinterpret_cast<const T*>(in.q) + b * in.qs[0] + (int64_t)q0 * in.qs[1] + h * in.qs[2];
         const T* gp = reinterpret_cast<const T*>(a.d_o) + b * a.dos[0] + (int64_t)q0 * a.dos[1] + h * a.dos[2];
-        Tl::template load<QB, NW>(qp, in.qs[1], in.dim, qb, wave, lane, [&](int i) { return min(i, left - 1); });
-        Tl::template load<QB, NW>(gp, a.dos[1], in.dim, qb + TILE, wave, lane, [&](int i) { return min(i, left - 1); });
+        if (left >= QB) {
+            ql.issue_all(qp, qb, wave);
+            gl.issue_all(gp, qb + TILE, wave);
+        } else {
+            const auto keep = [&](int i) { return i < left; };
+            ql.issue(qp, qb, wave, lane, keep);
+            gl.issue(gp, qb + TILE, wave, lane, keep);
+        }
         if (wave < 2) {  // 64 floats each
             const float* src = (wave == 0 ? a.ref : a.delta) + ((int64_t)b * in.heads + h) * in.seq_q + q0;
-            __builtin_amdgcn_global_load_lds(src + min(lane, left - 1), stats + (buf * 2 + wave) * 64, 4, 0, 0);
+            dma4(src, lane < min(left, QB) ? 4 * lane : kOut, stats + (buf * 2 + wave) * 64);
         }
     };
     int cur = -1, buf = 0;
@@ -376,60 +414,84 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(const BwdArgs a) {
         const uint8_t* Qt = smem + buf * 2 * TILE;
         const uint8_t* Gt = Qt + TILE;
         const float* st = stats + buf * 2 * 64;
-        const int q0 = (n % tiles) * QB, left = in.seq_q - q0;
+        const int q0 = (n % tiles) * QB;
+        f32x16_t s[HALVES], ds[HALVES];
+        FragParts<T> pf[HALVES][2], df[HALVES][2];
+        auto scores = [&](auto hc, auto vc, auto side) {
+            constexpr int hh = decltype(hc)::value;
+            s[hh] = ds[hh] = zero16();
+            products<T, 2 * Tl::STEPS, 1, decltype(vc)::value>(
+                [&](int i) { return Tl::row_frag(i & 1 ? Gt : Qt, 32 * hh + r, i / 2, g); },
+                [&](int i, const typename Tl::Frag& f) {
+                    if (i & 1) ds[hh] = mma(f, vf[i / 2], ds[hh]);
+                    else s[hh] = mma(f, kf[i / 2], s[hh]);
+                },
+                side);
+        };
+        // P and dS of elements 4 i4 .. + 3: queries q0 + 32 hh + 8 i4 + 4 g + e.  A query past the
+        // last one is all zeros (row, ref and delta), and so is what it adds; a key that is
+        // not kept has a lane of its own, which is not stored.
+        auto weights = [&](auto hc, int i4) {
+            constexpr int hh = decltype(hc)::value;
+            const int i0 = 32 * hh + 4 * g + 8 * i4;
+            const float4 rf = *reinterpret_cast<const float4*>(st + i0);
+            const float4 dl = *reinterpret_cast<const float4*>(st + 64 + i0);
+            const float ref[4] = {rf.x, rf.y, rf.z, rf.w}, delta[4] = {dl.x, dl.y, dl.z, dl.w};
+            float p[4], d[4];
 #pragma unroll
-        for (int hh = 0; hh < HALVES; ++hh) {
-            f32x16_t s = zero16(), ds = zero16();
-#pragma unroll
-            for (int c = 0; c < Tl::STEPS; ++c) {
-                s = mma(Tl::row_frag(Qt, 32 * hh + r, c, g), kf[c], s);
-                ds = mma(Tl::row_frag(Gt, 32 * hh + r, c, g), vf[c], ds);
+            for (int e = 0; e < 4; ++e) {
+                float c = -ref[e];
+                // Offsets fall by one from query to query.
+                if constexpr (BIAS) c += rel_at(line, in.rel.reach, key - (q0 + 32 * hh + 4 * g) - pos - 27)[27 - 8 * i4 - e];
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hh][4 * i4 + e], in.scale_log2, c));
+                d[e] = p[e] * (ds[hh][4 * i4 + e] - delta[e]);
             }
-            // Element i: query q0 + 32 hh + 8 (i / 4) + 4 g + i % 4.
-            const int i0 = 32 * hh + 4 * g;
+            pf[hh][i4 / 2].set(i4 & 1, p);
+            df[hh][i4 / 2].set(i4 & 1, d);
+        };
+        auto some = [&](auto hc) {
+            return [&, hc](int part, int of) {
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                const float4 rf = *reinterpret_cast<const float4*>(st + i0 + 8 * i4);
-                const float4 dl = *reinterpret_cast<const float4*>(st + 64 + i0 + 8 * i4);
-                const float ref[4] = {rf.x, rf.y, rf.z, rf.w}, delta[4] = {dl.x, dl.y, dl.z, dl.w};
+                for (int i4 = 0; i4 < 4; ++i4)
+                    if (i4 * of / 4 == part) weights(hc, i4);
+            };
+        };
+        auto grads = [&](auto hc, auto vc, auto side) {
+            constexpr int hh = decltype(hc)::value;
+            products<T, 4 * Tl::BLOCKS, 2, decltype(vc)::value>(
+                [&](int i) { return Tl::col_frag(i & 1 ? Qt : Gt, 32 * hh + 16 * (i / 2 / Tl::BLOCKS), i / 2 % Tl::BLOCKS, cols); },
+                [&](int i, const typename Tl::Frag& f) {
+                    const int j = i / 2 / Tl::BLOCKS, d = i / 2 % Tl::BLOCKS;
+                    if (i & 1) dk[d] = mma(f, df[hh][j].frag(), dk[d]);
+                    else dv[d] = mma(f, pf[hh][j].frag(), dv[d]);
+                },
+                side);
+        };
+        // One half's weights between the other half's products.
+        using H0 = std::integral_constant<int, 0>;
+        using H1 = std::integral_constant<int, HALVES - 1>;
+        using None = std::integral_constant<int, 0>;
+        using SV = std::integral_constant<int, DP == 64 ? 18 : 9>;   // vector instructions per product
+        using GV = std::integral_constant<int, DP == 64 ? 18 : 9>;
+        scores(H0{}, None{}, NoSide{});
+        if constexpr (HALVES == 2) {
+            scores(H1{}, SV{}, some(H0{}));
+            grads(H0{}, GV{}, some(H1{}));
+        } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int q = i0 + 8 * i4 + e;
-                    float bias = -ref[e];
-                    if constexpr (BIAS) {
-                        const int off = key - (q0 + q) - pos;
-                        bias += line[in.rel.reach + min(max(off, -in.rel.reach), in.rel.reach)];
-                    }
-                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], in.scale_log2, bias));
-                    const bool on = keep && q < left;
-                    s[4 * i4 + e] = on ? p : 0.f;
-                    ds[4 * i4 + e] = on ? p * (ds[4 * i4 + e] - delta[e]) : 0.f;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float pv[8], dsv[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    pv[e] = s[8 * j + e];
-                    dsv[e] = ds[8 * j + e];
-                }
-                typename Tl::Frag pf, df;
-                to_frag(pv, pf);
-                to_frag(dsv, df);
-#pragma unroll
-                for (int d = 0; d < Tl::BLOCKS; ++d) {
-                    dv[d] = mma(Tl::col_frag(Gt, 32 * hh + 16 * j, d, cols), pf, dv[d]);
-                    dk[d] = mma(Tl::col_frag(Qt, 32 * hh + 16 * j, d, cols), df, dk[d]);
-                }
-            }
+            for (int i4 = 0; i4 < 4; ++i4) weights(H0{}, i4);
         }
+        grads(H1{}, None{}, NoSide{});
         buf ^= 1;
     }
     if (!inside) return;
+    if (!keep) {
+#pragma unroll
+        for (int d = 0; d < Tl::BLOCKS; ++d) dk[d] = dv[d] = zero16();
+    }
     if (a.ranges > 1) {
         const int64_t plane = (int64_t)in.batch * in.kv_heads * in.seq_kv * DP;
-        float* pk = a.part_kv + (int64_t)range * 2 * plane + ((int64_t)bh * in.seq_kv + key) * DP;
+        float* pk = a.part_kv + (int64_t)range * 2 * plane + (((int64_t)b * in.kv_heads + kvh) * in.seq_kv + key) * DP;
 #pragma unroll
         for (int d = 0; d < Tl::BLOCKS; ++d)
 #pragma unroll
@@ -528,7 +590,7 @@ int launch(const BwdArgs& a, const Plan& p, hipStream_t st) {
     DT_REQUIRE(dq_blocks < (1ll << 31) && dkv_blocks < (1ll << 31), "%s: grid too large", who);
     int rc = DT_OK;
     if (dq_blocks > 0) {
-        const size_t lds = tiles + (BIAS ? line + 4 * (grad_line(in.rel.reach) + kScratch) : 0) * sizeof(float);
+        const size_t lds = tiles + (BIAS ? 5 * line + 4 * kScratch : 0) * sizeof(float);
         hipLaunchKernelGGL((attn_dq_kernel<T, DP, BIAS>), dim3((unsigned)dq_blocks), dim3(256), lds, st, a);
         rc = check_launch(who);
     }
