@@ -163,8 +163,10 @@ __device__ __forceinline__ void epilogue(const Problem& p, const f32x16_t (&acc)
 
 // ---- low-rank adapters beside the product (dt_lora_gemm) ---------------------
 // C[m, n] += sum_r T[m, r] U_a[n, r], a = adapter of row m: T = scale (A A_a^T) from
-// lora_down_kernel (lora.hip), U_a the adapter's up weights.  It is added to a
-// tile's accumulators after its last k-step, so the sum is rounded once.  T is held
+// lora_down_kernel (lora.hip), U_a the adapter's up weights.  A tile's accumulators
+// start from it instead of 0, so the sum is rounded once, and its operands load
+// beside the first stages' (after the last k-step they found no registers, and each
+// tile waited for them: 4608 x 12288 x 4096 503-559 us instead of 420).  T is held
 // as two bf16 parts (16 significant bits), each a product of its own: beside K of
 // some thousands the second costs nothing that shows, and an fp32 C keeps its accuracy.
 // NoLora leaves a kernel as it is without.
@@ -197,54 +199,98 @@ __device__ __forceinline__ bf16x8_t lora_t(const uint16_t* p) {
     return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(p));
 }
 
-// The wave's FM x FN blocks of 32 x 32.  A 32-row block whose rows share an adapter (any
-// request of 32 rows or more) goes straight into the accumulators; one with several takes
-// each adapter's product apart and keeps it in that adapter's rows alone, so what
-// an adapter holds reaches no other request's rows.
+// The adapter of each of this lane's rows (-1: none), read before the product's k-loop.
+template <int FM>
+__device__ __forceinline__ void lora_rows(const LoraTile& l, const Problem& p, int mw, int lane, int (&mine)[FM]) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = mw + 32 * i + (lane & 31);
+        const int a = m < p.M ? l.row_adapter[m] : -1;
+        mine[i] = a >= 0 && a < l.adapters ? a : -1;
+    }
+}
+
+// The wave's FM x FN blocks of 32 x 32, which hold zeros.  Rows that all share an adapter:
+// the operands of 32 ranks at once.  Else block by block, an adapter at a time, each
+// kept in its own rows alone: what an adapter holds reaches no other request's rows.
 template <int FM, int FN>
-__device__ __forceinline__ void lora_add(const LoraTile& l, const Problem& p, f32x16_t (&acc)[FN][FM], int mw, int nw,
-                                         int lane) {
+__device__ __forceinline__ void lora_start(const LoraTile& l, const Problem& p, f32x16_t (&acc)[FN][FM],
+                                           const int (&mine)[FM], int mw, int nw, int lane) {
     const int lrow = lane & 31, g = lane >> 5;
     const uint16_t* u0[FN];
 #pragma unroll
     for (int j = 0; j < FN; ++j) u0[j] = l.u + (int64_t)min(nw + 32 * j + lrow, p.N - 1) * l.ldu;
+    const uint16_t* t0[FM];
+#pragma unroll
+    for (int i = 0; i < FM; ++i) t0[i] = l.t + (int64_t)min(mw + 32 * i + lrow, p.M - 1) * 2 * l.rp + 8 * g;
+    const int first = __builtin_amdgcn_readfirstlane(mine[0]);
+    bool other = false, any = false;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int m = mw + 32 * i + lrow;
-        const bool row = m < p.M;
-        const int mine = row ? l.row_adapter[m] : -1;
-        const uint16_t* t = l.t + (int64_t)min(m, p.M - 1) * 2 * l.rp + 8 * g;
-        uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < l.adapters);
-        while (left) {
-            const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(left));
-            const uint64_t of = __builtin_amdgcn_ballot_w64(mine == a);
-            left &= ~of;
-            const int64_t at = a * l.u_stride;
-            if (__builtin_amdgcn_ballot_w64(row && mine != a) == 0) {
-                for (int r = 0; r < l.rank; r += 16) {
-                    const bf16x8_t hi = lora_t(t + r), lo = lora_t(t + l.rp + r);
+        other = other || (mw + 32 * i + lrow < p.M && mine[i] != first);
+        any = any || mine[i] >= 0;
+    }
+    if (__builtin_amdgcn_ballot_w64(any) == 0) return;
+    if (__builtin_amdgcn_ballot_w64(other) == 0) {
+        const int64_t at = first * l.u_stride;
+        for (int r = 0; r < l.rank; r += 32) {
+            bf16x8_t u[FN][2], t[FM][2][2];
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) {
-                        const bf16x8_t u = lora_up(l, u0[j] + at, r + 8 * g);
-                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, hi, acc[j][i], 0, 0, 0);
-                        acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lo, acc[j][i], 0, 0, 0);
-                    }
-                }
-            } else {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    f32x16_t d;
+                for (int j = 0; j < FN; ++j) u[j][h] = lora_up(l, u0[j] + at, r + 16 * h + 8 * g);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) d[e] = 0.f;
-                    for (int r = 0; r < l.rank; r += 16) {
-                        const bf16x8_t u = lora_up(l, u0[j] + at, r + 8 * g);
-                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lora_t(t + r), d, 0, 0, 0);
-                        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u, lora_t(t + l.rp + r), d, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[j][i][e] += mine == a ? d[e] : 0.f;
+                for (int i = 0; i < FM; ++i) {
+                    t[i][h][0] = lora_t(t0[i] + r + 16 * h);
+                    t[i][h][1] = lora_t(t0[i] + l.rp + r + 16 * h);
                 }
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int i = 0; i < FM; ++i)
+                            acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[j][h], t[i][h][part], acc[j][i], 0, 0, 0);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        uint64_t left = __builtin_amdgcn_ballot_w64(mine[i] >= 0);
+        while (left) {
+            const int a = __builtin_amdgcn_readlane(mine[i], (int)__builtin_ctzll(left));
+            left &= ~__builtin_amdgcn_ballot_w64(mine[i] == a);
+            const int64_t at = a * l.u_stride;
+            f32x16_t d[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) d[j][e] = 0.f;
+            for (int r = 0; r < l.rank; r += 32) {
+                bf16x8_t u[FN][2], t[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) u[j][h] = lora_up(l, u0[j] + at, r + 16 * h + 8 * g);
+                    t[h][0] = lora_t(t0[i] + r + 16 * h);
+                    t[h][1] = lora_t(t0[i] + l.rp + r + 16 * h);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+                            d[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[j][h], t[h][part], d[j], 0, 0, 0);
+            }
+            const bool keep = mine[i] == a;
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[j][i][e] = keep ? d[j][e] : acc[j][i][e];
         }
     }
 }
@@ -413,6 +459,8 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp,
     const Problem& p = locate<BM, BN>(grp, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int wm = (wave / WAVES_N) * (BM / WAVES_M), wn = (wave % WAVES_N) * (BN / WAVES_N);
+    int mine[FM];
+    if constexpr (L::on) lora_rows<FM>(lora, p, m0 + wm, lane, mine);
 
     // DMA sources: wave w fills A rows [BM/NW w, +BM/NW) and B rows
     // [256/NW w, +256/NW), instructions of 8 rows each; lane i covers row +
@@ -557,6 +605,8 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp,
     issue(ktile(0), 0);
     if constexpr (Q8) qwrite(0);
     if (nk > 1) issue(ktile(1), 1);
+    if constexpr (L::on)  // of several K ranges, and groups, in the first
+        if (&p == grp.p && kg == 0) lora_start<FM, FN>(lora, p, acc, mine, m0 + wm, n0 + wn, lane);
     if (nk > 1) wait_vm<A_DMA + B_DMA>();  // Q8: QJ code and QJ scale loads stand in for the B_DMA B DMAs
     else wait_vm<0>();
     if constexpr (Q8) __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the B rows written
@@ -639,8 +689,6 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp,
                     for (int e = 0; e < 16; ++e)
                         acc[j][i][e] += part[(q * NW + wave) * PW + ((j * FM + i) * 16 + e) * 64 + lane];
     }
-    if constexpr (L::on)
-        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
@@ -866,6 +914,8 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
     const Problem& p = locate<128, 128>(grp, &tm, &tn);
     const int m0 = tm * 128, n0 = tn * 128;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    int mine[FM];
+    if constexpr (L::on) lora_rows<FM>(lora, p, m0 + wm, lane, mine);
 
     const uint16_t* Ap = p.A;
     const uint16_t* Bp = p.B;
@@ -952,6 +1002,7 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+    if constexpr (L::on) lora_start<FM, FN>(lora, p, acc, mine, m0 + wm, n0 + wn, lane);
 
     const int lrow = lane & 31, lk = (lane >> 5) * 8;
     const int nk = p.K / SBK;
@@ -982,8 +1033,6 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
         if (more) stash(s ^ 1);
         __syncthreads();
     }
-    if constexpr (L::on)
-        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 
@@ -1016,6 +1065,8 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
     const Problem& p = grp.p[pi];
     const int n0 = ((int)blockIdx.x - grp.tile_start[pi]) * 16;
     const int r = lane & 15, g = lane >> 4;
+    int mine = -1;  // the adapter of row r, read ahead of the weights
+    if constexpr (L::on) mine = r < p.M ? lora.row_adapter[r] : -1;
 
     const int nblk = p.K / 64, per = (nblk + KS - 1) / KS;
     const int b0 = min(wave * per, nblk), b1 = min(b0 + per, nblk);
@@ -1073,7 +1124,6 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 
     if constexpr (L::on) {
         // The rows' adapters over the waves, each product kept in its own rows.
-        const int mine = r < p.M ? lora.row_adapter[r] : -1;
         const uint16_t* t = lora.t + (int64_t)min(r, p.M - 1) * 2 * lora.rp + 8 * g;
         const uint16_t* u0 = lora.u + n * lora.ldu;
         uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < lora.adapters);
@@ -1129,6 +1179,8 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp, const L 
     const Problem& p = locate<128, 128>(grp, &tm, &tn);
     const int m0 = tm * 128, n0 = tn * 128;
     const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
+    int mine[FM];
+    if constexpr (L::on) lora_rows<FM>(lora, p, m0 + wm, lane, mine);
     const int row = tid >> 1, kh = (tid & 1) * 8;
     const int64_t am = min(m0 + row, p.M - 1), bn = min(n0 + row, p.N - 1);
     const uint16_t* arow = p.A + am * p.lda;
@@ -1142,6 +1194,7 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp, const L 
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[j][i][e] = 0.f;
+    if constexpr (L::on) lora_start<FM, FN>(lora, p, acc, mine, m0 + wm, n0 + wn, lane);
 
     const int lrow = lane & 31, lk = (lane >> 5) * 8;
     for (int k0 = 0; k0 < p.K; k0 += 16) {
@@ -1184,8 +1237,6 @@ __global__ __launch_bounds__(256) void gemm_any_kernel(const Group grp, const L 
             for (int i = 0; i < FM; ++i)
                 acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[j], xf[i], acc[j][i], 0, 0, 0);
     }
-    if constexpr (L::on)
-        if (&p == grp.p) lora_add<FM, FN>(lora, p, acc, m0 + wm, n0 + wn, lane);  // of several K ranges the first
     epilogue<FM, FN, TC>(p, acc, m0 + wm, n0 + wn, lane);
 }
 

@@ -2,11 +2,14 @@
 // A_a[r, k], a = adapter of row m, as two bf16 parts for the product's epilogue
 // (lora_add in gemm.hip).
 //
-// A stream of x and of the used adapters with next to no arithmetic.  A workgroup takes 32
-// rows and 32 ranks; its sixteen waves share K, read both operands straight into
-// the MFMA's registers (v_mfma_f32_32x32x16_bf16, the adapter's rows as A, the rows of x
-// as B) and meet in LDS, in wave order.  The adapters of the 32 rows are found by ballot
-// and taken one after another, or, when there are few rows, by workgroups of their own.
+// A stream of x and of the used adapters with next to no arithmetic.  A workgroup takes 16
+// rows and 32 ranks; its waves take every NW-th 64 k and meet in LDS, in wave order.  Each
+// streams its 16 x 64 of x and 32 x 64 of the adapter through LDS buffers of its own by
+// direct DMA, whole 128-byte lines of a row side by side: read straight into the MFMA's
+// registers, lanes next to each other lie in different rows, and the vector cache
+// looks up every lane for itself, 16 bytes a cycle (4608 rows x 4096, rank 32: 27 us).
+// The adapters of the 16 rows are found by ballot and taken one after another, or,
+// when there are few rows, by workgroups of their own.
 #include "capi_util.hpp"
 #include "common.hpp"
 #include "kernels.hpp"
@@ -15,7 +18,7 @@ namespace dit {
 namespace {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct DownArgs {
     const uint16_t* x;
@@ -29,9 +32,7 @@ struct DownArgs {
 };
 
 // Elements k .. k + 7 of a row of K; zeros past its end.
-template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
-    if constexpr (VEC) return k < K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -41,66 +42,150 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <bool VEC>
-__global__ __launch_bounds__(1024) void lora_down_kernel(const DownArgs p) {
-    constexpr int NW = 16, STEPS = 4;  // waves; 16-k steps loaded together (a 128-byte line of each row)
-    __shared__ float part[NW][32][33];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
-    const int m0 = blockIdx.x * 32, r0 = blockIdx.y * 32, slot = blockIdx.z;
-    const bool row = m0 + r < p.M;
-    const int mine = row ? p.row_adapter[m0 + r] : -1;
-    const bool valid = mine >= 0 && mine < p.adapters;
-    const uint16_t* xr = p.x + (int64_t)min(m0 + r, p.M - 1) * p.ldx;
-    // A thread's output: row tid / 32, rank tid % 32.
-    const int om = tid >> 5, orank = tid & 31;
-    const int theirs = __shfl(mine, om);
-    auto put = [&](float v) {
+constexpr int kRanks = 32;  // of a workgroup
+constexpr int kLine = 64;               // k a wave takes at a time
+
+struct Out {  // a thread's element of T: row tid / 32, rank tid % 32
+    const DownArgs& p;
+    int m, rank, theirs;
+    __device__ __forceinline__ void put(float v) const {
         const uint32_t hi = f32_to_bf16_bits(v);
         const float h = __uint_as_float(hi << 16);
         // The rest; none behind a value beyond bf16's range.
         const float lo = (hi & 0x7FFFu) < 0x7F80u ? v - h : 0.f;
-        uint16_t* o = p.t + (int64_t)(m0 + om) * 2 * p.rp + r0 + orank;
+        uint16_t* o = p.t + (int64_t)m * 2 * p.rp + rank;
         o[0] = (uint16_t)hi;
         o[p.rp] = (uint16_t)f32_to_bf16_bits(lo);
-    };
-    if (slot == 0 && m0 + om < p.M && !(theirs >= 0 && theirs < p.adapters)) put(0.f);
+    }
+};
 
-    // Whole lines per wave: K in ranges of 64.
-    const int lines = (p.K + 63) / 64, per = (lines + NW - 1) / NW;
-    const int k0 = wave * per * 64, k1 = min(k0 + per * 64, p.K);
-    uint64_t left = __builtin_amdgcn_ballot_w64(valid) & 0xFFFFFFFFull;
+constexpr uint32_t kZero = 0x80000000u;  // an offset out of every buffer's range: reads zeros
+// 16 bytes a lane from base + off to lds + 16 lane; base and lds uniform.
+__device__ __forceinline__ void down_dma(const void* base, uint32_t off, uint8_t* lds) {
+    typedef __attribute__((address_space(3))) void* lds_ptr_t;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
+}
+
+// VEC: rows in whole 16-byte chunks, through LDS.  Else element by element, for any layout.
+template <bool VEC, int ROWS, int NW, int NB>
+__global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
+    constexpr int ROWB = kLine * 2, BUF = (ROWS + kRanks) * ROWB, RF = ROWS / 16;  // NB buffers of a wave
+    constexpr int DMAS = BUF / 1024, PARTB = NW * ROWS * (kRanks + 1) * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[VEC && NW * NB * BUF > PARTB ? NW * NB * BUF : PARTB];
+    float(*const part)[ROWS][kRanks + 1] = reinterpret_cast<float(*)[ROWS][kRanks + 1]>(smem);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int m0 = blockIdx.x * ROWS, r0 = blockIdx.y * kRanks, slot = blockIdx.z;
+    // Lane i < ROWS has row i's adapter.
+    int mine = lane < ROWS && m0 + lane < p.M ? p.row_adapter[m0 + lane] : -1;
+    if (mine >= p.adapters) mine = -1;
+    const int lines = (p.K + kLine - 1) / kLine;
+    constexpr int OUTS = ROWS / (2 * NW) > 1 ? ROWS / (2 * NW) : 1;  // elements of T a thread has
+    auto each_out = [&](auto f) {
+#pragma unroll
+        for (int o = 0; o < OUTS; ++o) {
+            const int row = (tid >> 5) + 2 * NW * o;
+            const int theirs = __shfl(mine, row & (ROWS - 1));
+            if (row < ROWS && m0 + row < p.M) f(Out{p, m0 + row, r0 + (tid & 31), theirs}, row);
+        }
+    };
+    if (slot == 0)
+        each_out([](const Out& o, int) {
+            if (o.theirs < 0) o.put(0.f);
+        });
+
+    uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0);
     for (int turn = 0; left; ++turn) {
         const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(left));
-        left &= ~__builtin_amdgcn_ballot_w64(mine == a);
+        const uint64_t of = __builtin_amdgcn_ballot_w64(mine == a);
+        left &= ~of;
         if (turn % p.slots != slot) continue;
-        const uint16_t* ar = p.a + a * p.a_stride + (int64_t)min(r0 + r, p.rank - 1) * p.lda;
-        f32x16_t acc;
+        f32x4_t acc[RF][2];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-        for (int k = k0; k < k1; k += 16 * STEPS) {
-            uint4 xv[STEPS], av[STEPS];
+        for (int f = 0; f < RF; ++f) acc[f][0] = acc[f][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        auto multiply = [&](const uint4 (&v)[RF + 2]) {  // 16 rows of x each, then 16 of the adapter each
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                xv[s] = load8<VEC>(xr, k + 16 * s + 8 * g, p.K);
-                av[s] = load8<VEC>(ar, k + 16 * s + 8 * g, p.K);
+            for (int f = 0; f < RF; ++f)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    acc[f][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v[RF + h]),
+                                                                        __builtin_bit_cast(bf16x8_t, v[f]), acc[f][h], 0, 0, 0);
+        };
+        if constexpr (VEC) {
+            // Instruction j covers buffer rows 8 j .. + 7 (x, then the adapter), lane i chunk
+            // i % 8 of row i / 8, stored at chunk ^ (row & 7).  Rows past the ends, of other
+            // adapters, and k past K are zeros.
+            uint8_t* const mem = smem + wave * NB * BUF;
+            const uint16_t* xb = p.x + (int64_t)m0 * p.ldx;
+            const uint16_t* ab = p.a + a * p.a_stride + (int64_t)r0 * p.lda;
+            const int chunk = (lane & 7) ^ (lane >> 3);
+            uint32_t off[DMAS];
+#pragma unroll
+            for (int j = 0; j < DMAS; ++j) {
+                const int row = 8 * j + (lane >> 3), rank = row - ROWS;
+                const bool there = row < ROWS ? (of >> row) & 1 : r0 + rank < p.rank;
+                off[j] = there ? (uint32_t)((row < ROWS ? row * p.ldx : rank * p.lda) * 2 + chunk * 16) : kZero;
             }
+            auto issue = [&](int line, int buf) {
+                const bool tail = line * kLine + chunk * 8 >= p.K;  // lines past the last one too
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-                acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av[s]),
-                                                              __builtin_bit_cast(bf16x8_t, xv[s]), acc, 0, 0, 0);
+                for (int j = 0; j < DMAS; ++j)
+                    down_dma((8 * j < ROWS ? xb : ab) + (int64_t)line * kLine, tail ? kZero : off[j], mem + buf * BUF + 1024 * j);
+            };
+#pragma unroll
+            for (int i = 0; i < NB - 1; ++i) issue(wave + i * NW, i);
+            int buf = 0;
+            for (int line = wave; line < lines; line += NW) {
+                issue(line + (NB - 1) * NW, buf == 0 ? NB - 1 : buf - 1);  // the one read last
+                __builtin_amdgcn_s_waitcnt(((NB - 1) * DMAS & 15) | (((NB - 1) * DMAS >> 4) << 14) | 0x0F70);
+                __builtin_amdgcn_sched_barrier(0);
+                const uint8_t* t = mem + buf * BUF;
+                uint4 v[2][RF + 2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int h = 0; h < RF + 2; ++h)
+                        v[s][h] = *reinterpret_cast<const uint4*>(t + (16 * h + r) * ROWB + (((4 * s + g) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int s = 0; s < 2; ++s) multiply(v[s]);
+                __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the buffer is read
+                __builtin_amdgcn_sched_barrier(0);
+                buf = buf == NB - 1 ? 0 : buf + 1;
+            }
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the DMA past the end is in LDS before it is used again
+        } else {
+            const uint16_t* row[RF + 2];
+#pragma unroll
+            for (int h = 0; h < RF + 2; ++h)
+                row[h] = h < RF ? p.x + (int64_t)min(m0 + 16 * h + r, p.M - 1) * p.ldx
+                                : p.a + a * p.a_stride + (int64_t)min(r0 + 16 * (h - RF) + r, p.rank - 1) * p.lda;
+            for (int line = wave; line < lines; line += NW)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    uint4 v[RF + 2];
+#pragma unroll
+                    for (int h = 0; h < RF + 2; ++h) v[h] = load8(row[h], line * kLine + 32 * s + 8 * g, p.K);
+                    multiply(v);
+                }
         }
-        __syncthreads();  // the last adapter's sums have been read
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[wave][r][8 * (i >> 2) + 4 * g + (i & 3)] = acc[i];
         __syncthreads();
-        if (theirs == a && m0 + om < p.M) {
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) part[wave][16 * f + r][16 * h + 4 * g + i] = acc[f][h][i];
+        __syncthreads();
+        each_out([&](const Out& o, int row) {
+            if (o.theirs != a) return;
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += part[w][om][orank];
-            if (r0 + orank >= p.rank) v = 0.f;
-            put(p.scale ? v * p.scale[a] : v);
-        }
+            for (int w = 0; w < NW; ++w) v += part[w][row][tid & 31];
+            if (o.rank >= p.rank) v = 0.f;
+            o.put(p.scale ? v * p.scale[a] : v);
+        });
+        __syncthreads();  // the sums have been read
     }
 }
 
@@ -121,17 +206,23 @@ int lora_down(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, const dt_lor
     p.adapters = (int)l.adapters;
     p.rank = (int)l.rank;
     p.rp = (int)lora_rank_padded(l.rank);
-    const int64_t tiles = (M + 31) / 32, blocks = p.rp / 32;
-    // Adapters of a tile side by side until the chip is full: at most the 32 its rows can have.
+    // 16 rows a workgroup while that gives each CU one at most, else 32: the adapter is read
+    // again for every workgroup.
+    const int64_t blocks = p.rp / kRanks;
+    const bool small = (M + 15) / 16 * blocks <= cu_count();
+    const int64_t high = small ? 16 : 32, tiles = (M + high - 1) / high;
+    // Adapters of a tile side by side until the chip is full: at most one for each of its rows.
     int64_t slots = cu_count() / (tiles * blocks);
-    const int64_t most = l.adapters < (M < 32 ? M : 32) ? l.adapters : (M < 32 ? M : 32);
+    const int64_t rows = M < high ? M : high, most = l.adapters < rows ? l.adapters : rows;
     slots = slots < 1 ? 1 : slots < most ? slots : most;
     p.slots = (int)slots;
+    // Rows in whole chunks, a tile's within 2^31 bytes.
     const bool vec = K % 8 == 0 && ldx % 8 == 0 && l.lda % 8 == 0 && (l.a_stride % 8 == 0 || l.adapters == 1) &&
-                     aligned16(x) && aligned16(l.a);
+                     aligned16(x) && aligned16(l.a) && ldx < (1 << 25) && l.lda < (1 << 25);
     const dim3 grid((unsigned)tiles, (unsigned)blocks, (unsigned)slots);
-    if (vec) hipLaunchKernelGGL((lora_down_kernel<true>), grid, dim3(1024), 0, st, p);
-    else hipLaunchKernelGGL((lora_down_kernel<false>), grid, dim3(1024), 0, st, p);
+    if (!vec) hipLaunchKernelGGL((lora_down_kernel<false, 32, 8, 1>), dim3((unsigned)((M + 31) / 32), (unsigned)blocks, (unsigned)slots), dim3(512), 0, st, p);
+    else if (small) hipLaunchKernelGGL((lora_down_kernel<true, 16, 8, 3>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((lora_down_kernel<true, 32, 8, 2>), grid, dim3(64 * 8), 0, st, p);
     return check_launch("dt_lora_gemm");
 }
 
