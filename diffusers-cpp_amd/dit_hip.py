@@ -786,51 +786,89 @@ class Lora:
         self.a, self.b, self.scale = a, b, scale
 
 
+# The calls below check what their tensors are like (types, shapes, strides, devices) once
+# for each such description, and keep the arguments' structure without its pointers: of a
+# call around a 9 us kernel the checks took 10 us.
+
+def _meta(t):
+    return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
+
+
+def _on_device(metas):
+    """The launch goes to the current device's current stream: every tensor has to be there."""
+    here = _torch().cuda.current_device()
+    for m in metas:
+        if m is not None and m[3] != here:
+            raise DtError(f"a tensor is on {'the host' if m[3] < 0 else 'device %d' % m[3]}, not on the current device {here}")
+
+
+def _vector(m, dtype, n, what):
+    if m is not None and (m[0] != dtype or m[1] != (n,) or (n > 1 and m[2][0] != 1)):
+        raise DtError(f"{what} must be contiguous {dtype} [{n}]")
+
+
+@functools.lru_cache(maxsize=512)
+def _lora_plan(x, w, scales, a, b, scale, rows, bias, addend, out, here):
+    torch = _torch()
+    q8 = scales is not None
+    if len(x[1]) != 2 or len(w[1]) != 2 or len(a[1]) != 3 or len(b[1]) != 3 or len(out[1]) != 2:
+        raise DtError("x and w must have two dimensions, the adapters three")
+    (M, K), N, (n, rank) = x[1], w[1][0], a[1][:2]
+    if x[0] != torch.bfloat16 or a[0] != torch.bfloat16 or b[0] != torch.bfloat16 or \
+            w[0] != (torch.uint8 if q8 else torch.bfloat16) or (q8 and scales[0] != torch.float32):
+        raise DtError("x, w and the adapters must be bf16 (a Q8Weight: uint8 codes, fp32 scales)")
+    if w[1][1] != K or a[1] != (n, rank, K) or b[1] != (n, N, rank) or (q8 and scales[1] != (K // 32, N)):
+        raise DtError(f"adapters {tuple(a[1])}, {tuple(b[1])} do not fit x {tuple(x[1])} and w {tuple(w[1])}")
+    if (K > 1 and (x[2][1] != 1 or w[2][1] != 1 or a[2][2] != 1)) or (rank > 1 and b[2][2] != 1) or \
+            (q8 and N > 1 and scales[2][1] != 1):
+        raise DtError("rows of x, w and the adapters must be contiguous")
+    _vector(rows, torch.int32, M, "row_adapter")
+    _vector(scale, torch.float32, n, "scale")
+    _vector(bias, torch.float32, N, "bias")
+    for t in (out, addend):
+        if t is not None and (t[1] != (M, N) or t[0] != out[0] or (N > 1 and t[2][1] != 1)):
+            raise DtError("out and addend must be [M, N] of one dtype with contiguous rows")
+    if out[0] not in (torch.bfloat16, torch.float32):
+        raise DtError(f"out must be bf16 or fp32, not {out[0]}")
+    _on_device((x, w, scales, a, b, scale, rows, bias, addend, out))
+
+    def ld(m, cols):  # the row stride of a tensor of one row is not used
+        return max(m[2][-2], cols) if m[1][-2] <= 1 else m[2][-2]
+
+    p = GemmProblem(None, ld(x, K), None, ld(w, K), None, ld(out, N), None, 0 if addend is None else ld(addend, N), None, M,
+                    N, K, None, ld(scales, N) if q8 else 0)
+    s = LoraArgs(None, ld(a, K), a[2][0], None, ld(b, rank), b[2][0], None, None, n, rank)
+    return bytes(p), bytes(s), load().dt_lora_gemm_workspace_bytes(M, N, K, rank), _IO_TYPES[out[0]]
+
+
 def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dtype=None):
     """x: bf16 [M, K], w: bf16 [N, K] or Q8Weight -> x @ w.T (+ bias) (+ addend) +
     scale[a] * (x @ a[a].T) @ b[a].T, each row with the adapter a = row_adapter[m]
     (int32 [M]; outside the adapters: none)."""
     torch = _torch()
-    M, K = x.shape
-    N = w.shape[0]
     q8 = isinstance(w, Q8Weight)
+    codes, scales = (w.codes, w.scales) if q8 else (w, None)
     a, b, scale = lora.a, lora.b, lora.scale
-    n, rank = a.shape[0], a.shape[1]
-    codes = w.codes if q8 else w
-    if x.dtype != torch.bfloat16 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16 or \
-            codes.dtype != (torch.uint8 if q8 else torch.bfloat16):
-        raise DtError("x, w (or its codes) and the adapters must be bf16 (codes uint8)")
-    if w.shape[1] != K or a.shape != (n, rank, K) or b.shape != (n, N, rank):
-        raise DtError(f"adapters {tuple(a.shape)}, {tuple(b.shape)} do not fit x {tuple(x.shape)} and w {tuple(w.shape)}")
-    if (K > 1 and (x.stride(1) != 1 or codes.stride(1) != 1 or a.stride(2) != 1)) or (rank > 1 and b.stride(2) != 1):
-        raise DtError("rows of x, w and the adapters must be contiguous")
-    if row_adapter.dtype != torch.int32 or row_adapter.shape != (M,) or (M > 1 and row_adapter.stride(0) != 1):
-        raise DtError("row_adapter must be contiguous int32 [M]")
-    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (n,) or (n > 1 and scale.stride(0) != 1)):
-        raise DtError("scale must be contiguous fp32 [adapters]")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
-        raise DtError("bias must be contiguous fp32 [N]")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype or torch.bfloat16, device=x.device)
-    for t in (out, addend):
-        if t is not None and (t.shape != (M, N) or t.dtype != out.dtype or (N > 1 and t.stride(1) != 1)):
-            raise DtError("out and addend must be [M, N] of one dtype with contiguous rows")
-    _same_device(x, codes, w.scales if q8 else None, a, b, scale, row_adapter, bias, addend, out)
-
-    def ld(t, cols):  # the row stride of a tensor of one row is not used
-        return max(t.stride(-2), cols) if t.shape[-2] <= 1 else t.stride(-2)
-
-    p = GemmProblem(x.data_ptr(), ld(x, K), codes.data_ptr(), ld(codes, K), out.data_ptr(), ld(out, N),
-                    None if addend is None else addend.data_ptr(), 0 if addend is None else ld(addend, N),
-                    None if bias is None else bias.data_ptr(), M, N, K, w.scales.data_ptr() if q8 else None,
-                    ld(w.scales, N) if q8 else 0)
-    s = LoraArgs(a.data_ptr(), ld(a, K), a.stride(0), b.data_ptr(), ld(b, rank), b.stride(0),
-                 None if scale is None else scale.data_ptr(), row_adapter.data_ptr(), n, rank)
-    lib = load()
-    nbytes = lib.dt_lora_gemm_workspace_bytes(M, N, K, rank)
+        out = torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype or torch.bfloat16, device=x.device)
+    p, s, nbytes, out_type = _lora_plan(_meta(x), _meta(codes), _meta(scales), _meta(a), _meta(b), _meta(scale),
+                                        _meta(row_adapter), _meta(bias), _meta(addend), _meta(out),
+                                        torch.cuda.current_device())
+    p, s = GemmProblem.from_buffer_copy(p), LoraArgs.from_buffer_copy(s)
+    p.A, p.B, p.C = x.data_ptr(), codes.data_ptr(), out.data_ptr()
+    s.a, s.b, s.row_adapter = a.data_ptr(), b.data_ptr(), row_adapter.data_ptr()
+    if bias is not None:
+        p.bias = bias.data_ptr()
+    if addend is not None:
+        p.addend = addend.data_ptr()
+    if q8:
+        p.b_scale = scales.data_ptr()
+    if scale is not None:
+        s.scale = scale.data_ptr()
     ws = _scratch(nbytes, x.device) if nbytes else None
-    check(lib.dt_lora_gemm(ctypes.addressof(p), ctypes.addressof(s), io_type(out), _p(ws), nbytes, stream()),
-          "dt_lora_gemm")
+    lib = load()
+    check(lib.dt_lora_gemm(ctypes.addressof(p), ctypes.addressof(s), out_type, None if ws is None else ws.data_ptr(),
+                           nbytes, stream()), "dt_lora_gemm")
     if isinstance(lib, _Recorder):
         lib.keep.extend((p, s))
     return out
@@ -869,105 +907,116 @@ def rel_buckets(n, buckets, distance, two_sided=True):
     return out
 
 
-def _same_device(first, *others):
-    """The launch goes to the current device's current stream: every tensor has to be there."""
-    at = first.device
-    for t in others:
-        if t is not None and t.device != at:
-            raise DtError(f"tensors on {at} and {t.device}")
-    if at.type != "cuda":
-        raise DtError(f"tensors must be on a HIP device, not {at}")
-    if at.index != _torch().cuda.current_device():
-        raise DtError(f"tensors on {at}, which is not the current device")
-
-
-def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos):
+@functools.lru_cache(maxsize=512)
+def _attn_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, out, here):
     torch = _torch()
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+    if len(q[1]) != 4 or len(k[1]) != 4 or v[1] != k[1]:
         raise DtError("q must be [B, Sq, H, D], k and v [B, Skv, Hkv, D]")
-    B, Sq, H, D = q.shape
-    Bk, Skv, Hkv, Dk = k.shape
+    B, Sq, H, D = q[1]
+    Bk, Skv, Hkv, Dk = k[1]
     if Bk != B or Dk != D:
-        raise DtError(f"k {tuple(k.shape)} does not fit q {tuple(q.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise DtError("q, k and v must share a dtype")
-    st = (q.stride(), k.stride(), v.stride())
-    if st[0][3] != 1 or st[1][3] != 1 or st[2][3] != 1:
+        raise DtError(f"k {tuple(k[1])} does not fit q {tuple(q[1])}")
+    if q[0] not in (torch.bfloat16, torch.float32) or k[0] != q[0] or v[0] != q[0]:
+        raise DtError("q, k and v must share a dtype, bf16 or fp32")
+    if q[2][3] != 1 or k[2][3] != 1 or v[2][3] != 1:
         raise DtError("the head dim must be contiguous")
+    if out[1] != q[1] or out[0] != q[0] or out[2][3] != 1:
+        raise DtError("out must have q's shape and dtype, its head dim contiguous")
     a = AttnArgs()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_strides[:], a.k_strides[:], a.v_strides[:] = st[0][:3], st[1][:3], st[2][:3]
+    a.q_strides[:], a.k_strides[:], a.v_strides[:] = q[2][:3], k[2][:3], v[2][:3]
     a.batch, a.heads, a.kv_heads, a.seq_q, a.seq_kv, a.head_dim = B, H, Hkv, Sq, Skv, D
-    a.io_type = io_type(q)
-    a.scale = 1.0 / D ** 0.5 if scale is None else scale
-    table = None
+    a.io_type = _IO_TYPES[q[0]]
+    _vector(kv_len, torch.int32, B, "kv_len")
+    if kv_mask is not None:
+        if kv_mask[0] not in (torch.uint8, torch.bool) or kv_mask[1] != (B, Skv) or (Skv > 1 and kv_mask[2][1] != 1):
+            raise DtError("kv_mask must be uint8 or bool [B, Skv] with contiguous rows")
+        a.kv_mask_stride = kv_mask[2][0]
+    if table is not None:
+        if table[0] != torch.float32 or len(table[1]) != 2 or table[1][1] != H or (H > 1 and table[2][1] != 1):
+            raise DtError("the bias table must be fp32 [buckets, H] with contiguous rows")
+        a.rel_table_stride = table[2][0] if table[1][0] > 1 else H
+        a.rel_buckets, a.rel_distance, a.rel_two_sided = table[1][0], distance, 1 if two_sided else 0
+        _vector(q_pos, torch.int32, B, "q_pos")
+    _on_device((q, k, v, kv_len, kv_mask, table, q_pos, out))
+    a.scale = 1.0 / D ** 0.5
+    # The workspaces go by sizes alone; the pointers stand for the call's own.
+    a.q = a.k = a.v = 16
+    a.rel_table = None if table is None else 16
+    lib, p = load(), ctypes.addressof(a)
+    sizes = lib.dt_attn_fwd_workspace_bytes(p), lib.dt_attn_bwd_workspace_bytes(p)
+    return bytes(a), *sizes, _i64x3(*out[2][:3])
+
+
+def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out):
+    table = None if rel is None else rel.table
+    plan, fwd, bwd, o_strides = _attn_plan(_meta(q), _meta(k), _meta(v), _meta(kv_len), _meta(kv_mask), _meta(table), _meta(q_pos),
+                      None if rel is None else rel.distance, None if rel is None else rel.two_sided, _meta(out),
+                      _torch().cuda.current_device())
+    a = AttnArgs.from_buffer_copy(plan)
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if scale is not None:
+        a.scale = scale
     if kv_len is not None:
-        if kv_len.dtype != torch.int32 or kv_len.shape != (B,) or (B > 1 and kv_len.stride(0) != 1):
-            raise DtError("kv_len must be contiguous int32 [B]")
         a.kv_len = kv_len.data_ptr()
     if kv_mask is not None:
-        if kv_mask.dtype not in (torch.uint8, torch.bool) or kv_mask.shape != (B, Skv) or \
-                (Skv > 1 and kv_mask.stride(1) != 1):
-            raise DtError("kv_mask must be uint8 or bool [B, Skv] with contiguous rows")
-        a.kv_mask, a.kv_mask_stride = kv_mask.data_ptr(), kv_mask.stride(0)
-    if rel is not None:
-        table = rel.table
-        if table.dtype != torch.float32 or table.dim() != 2 or table.shape[1] != H or (H > 1 and table.stride(1) != 1):
-            raise DtError("the bias table must be fp32 [buckets, H] with contiguous rows")
-        a.rel_table, a.rel_table_stride = table.data_ptr(), table.stride(0) if table.shape[0] > 1 else H
-        a.rel_buckets, a.rel_distance, a.rel_two_sided = table.shape[0], rel.distance, 1 if rel.two_sided else 0
+        a.kv_mask = kv_mask.data_ptr()
+    if table is not None:
+        a.rel_table = table.data_ptr()
         if q_pos is not None:
-            if q_pos.dtype != torch.int32 or q_pos.shape != (B,) or (B > 1 and q_pos.stride(0) != 1):
-                raise DtError("q_pos must be contiguous int32 [B]")
             a.q_pos = q_pos.data_ptr()
-    _same_device(q, k, v, kv_len, kv_mask, table, q_pos)
-    return a
+    return a, fwd, bwd, o_strides
 
 
 def _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse):
     torch = _torch()
-    a = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(3) != 1:
-        raise DtError("out must have q's shape, dtype and device, its head dim contiguous")
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if return_lse else None
+    a, n, _, o_strides = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out)
+    lse = torch.empty((a.batch, a.heads, a.seq_q), dtype=torch.float32, device=q.device) if return_lse else None
     lib = load()
-    p = ctypes.addressof(a)
-    n = lib.dt_attn_fwd_workspace_bytes(p)
     ws = _scratch(n, q.device) if n else None
-    check(lib.dt_attn_fwd(p, out.data_ptr(), _strides3(out), _p(lse), _p(ws), n, stream()), "dt_attn_fwd")
+    check(lib.dt_attn_fwd(ctypes.addressof(a), out.data_ptr(), o_strides, None if lse is None else lse.data_ptr(),
+                          None if ws is None else ws.data_ptr(), n, stream()), "dt_attn_fwd")
     if isinstance(lib, _Recorder):
         lib.keep.append(a)
     return (out, lse) if return_lse else out
 
 
+@functools.lru_cache(maxsize=512)
+def _grads_plan(q, d_o, o, lse, k, here):
+    for m, name in ((d_o, "d_o"), (o, "o")):
+        if m[1] != q[1] or m[0] != q[0] or m[2][3] != 1:
+            raise DtError(f"{name} must have q's shape and dtype, its head dim contiguous")
+    B, Sq, H, D = q[1]
+    if lse[0] != _torch().float32 or lse[1] != (B, H, Sq) or lse[2] != (H * Sq, Sq, 1) and 0 not in lse[1]:
+        raise DtError("lse must be the forward pass's: contiguous fp32 [B, H, Sq]")
+    _on_device((d_o, o, lse))
+    y = AttnGrads()
+    y.d_o_strides[:], y.o_strides[:] = d_o[2][:3], o[2][:3]
+    y.dq_strides[:] = (Sq * H * D, H * D, D)
+    y.dk_strides[:] = y.dv_strides[:] = (k[1][1] * k[1][2] * D, k[1][2] * D, D)
+    y.d_rel_table_stride = H
+    return bytes(y)
+
+
 def _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos):
     torch = _torch()
-    a = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos)
-    for t, name in ((d_o, "d_o"), (o, "o")):
-        if t.shape != q.shape or t.dtype != q.dtype or t.stride(3) != 1:
-            raise DtError(f"{name} must have q's shape and dtype, its head dim contiguous")
-    B, Sq, H, _ = q.shape
-    if lse.dtype != torch.float32 or lse.shape != (B, H, Sq) or not lse.is_contiguous():
-        raise DtError("lse must be the forward pass's: contiguous fp32 [B, H, Sq]")
-    _same_device(q, d_o, o, lse)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    dt = None if rel is None else torch.empty(rel.table.shape, dtype=torch.float32, device=q.device)
-    y = AttnGrads()
+    a, _, n, _ = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, o)
+    y = AttnGrads.from_buffer_copy(_grads_plan(_meta(q), _meta(d_o), _meta(o), _meta(lse), _meta(k),
+                                               torch.cuda.current_device()))
+    dtype, device = q.dtype, q.device
+    dq = torch.empty(q.shape, dtype=dtype, device=device)
+    dk = torch.empty(k.shape, dtype=dtype, device=device)
+    dv = torch.empty(k.shape, dtype=dtype, device=device)
     y.d_o, y.o, y.lse = d_o.data_ptr(), o.data_ptr(), lse.data_ptr()
     y.dq, y.dk, y.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    y.d_o_strides[:], y.o_strides[:] = d_o.stride()[:3], o.stride()[:3]
-    y.dq_strides[:], y.dk_strides[:], y.dv_strides[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
-    if dt is not None:
-        y.d_rel_table, y.d_rel_table_stride = dt.data_ptr(), H
+    dt = None
+    if rel is not None:
+        dt = torch.empty(rel.table.shape, dtype=torch.float32, device=device)
+        y.d_rel_table = dt.data_ptr()
     lib = load()
-    p = ctypes.addressof(a)
-    n = lib.dt_attn_bwd_workspace_bytes(p)
-    ws = _scratch(n, q.device) if n else None
-    check(lib.dt_attn_bwd(p, ctypes.addressof(y), _p(ws), n, stream()), "dt_attn_bwd")
+    ws = _scratch(n, device) if n else None
+    check(lib.dt_attn_bwd(ctypes.addressof(a), ctypes.addressof(y), None if ws is None else ws.data_ptr(), n, stream()), "dt_attn_bwd")
     if isinstance(lib, _Recorder):
         lib.keep.extend((a, y))
     return (dq, dk, dv) if rel is None else (dq, dk, dv, dt)

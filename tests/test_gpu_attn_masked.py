@@ -277,10 +277,10 @@ def test_same_bits_each_time_on_other_streams_and_without_workspace():
         got = dh.cross_attn(q, k, v)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want)
-    a = dh._attn_args(q, k, v, None, None, None, None, None)
-    lib = dh.load()
-    assert lib.dt_attn_fwd_workspace_bytes(dh.ctypes.addressof(a)) > 0
     out = torch.empty_like(q)
+    a, room, _, _ = dh._attn_args(q, k, v, None, None, None, None, None, out)
+    lib = dh.load()
+    assert room == lib.dt_attn_fwd_workspace_bytes(dh.ctypes.addressof(a)) > 0
     dh.check(lib.dt_attn_fwd(dh.ctypes.addressof(a), out.data_ptr(), dh._strides3(out), None, None, 0, dh.stream()))
     hold("o", out, oracle(q, k, v), BF16, Skv)
 
