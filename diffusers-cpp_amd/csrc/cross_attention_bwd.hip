@@ -39,9 +39,15 @@ struct BwdArgs {
     int32_t row_blocks, key_blocks, ranges, buckets;
 };
 
+// 32-row halves of a wave's part of a tile with four waves side by side; waves that share rows
+// when there are few.
 template <typename T, int DP>
-constexpr int tile_rows() {
-    return sizeof(T) == 4 && DP == 128 ? 32 : 64;
+constexpr int halves() {
+    return sizeof(T) == 4 && DP == 128 ? 1 : 2;
+}
+template <typename T, int DP, bool BIAS>
+constexpr int few_waves() {
+    return Tile<T, DP>::RB <= 128 || (Tile<T, DP>::RB == 256 && !BIAS) ? 4 : Tile<T, DP>::RB == 256 || !BIAS ? 2 : 1;
 }
 
 // A wave's dS block as its 63 diagonals (offsets -31 .. 31), each a row of 32 queries; what
@@ -50,10 +56,13 @@ constexpr int tile_rows() {
 constexpr int kDiag = 36, kScratch = 63 * kDiag;
 
 // ---- dQ, delta, the table's gradient ---------------------------------------------------
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const BwdArgs a) {
+// WR waves of 32 rows each, times WK that share the rows and take HALVES x 32 keys each of
+// a tile; their results meet in LDS in wave order.
+template <typename T, int DP, bool BIAS, int WR, int WK, int HALVES>
+__global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(const BwdArgs a) {
     typedef Tile<T, DP> Tl;
-    constexpr int KB = tile_rows<T, DP>(), HALVES = KB / 32, TILE = KB * Tl::RB, NW = 4;
+    constexpr int MY = 32 * HALVES, KB = MY * WK, TILE = KB * Tl::RB, NW = WR * WK;
+    static_assert(WR * (WK - 1) * (Tl::BLOCKS * 16 + 1) * 256 <= 4 * TILE, "the waves' results take the tiles' place");
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][K | V], scratch, bias line, gradient lines
     const AttnIn& in = a.in;
     const int reach = in.rel.reach;
@@ -68,8 +77,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     const int blk = (int)(bid % (uint32_t)a.row_blocks), bh = (int)(bid / (uint32_t)a.row_blocks);
     const int b = bh % in.batch, h = bh / in.batch, kvh = h / in.shared;  // batch entries innermost, as in the forward pass
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
-    const int row = blk * 128 + wave * 32 + r;
+    const int r = lane & 31, g = lane >> 5, wr = wave % WR, wk = wave / WR;
+    const int row0 = (blk * WR + wr) * 32, row = row0 + r;
     const bool live = row < in.seq_q;
     const int tok = live ? row : 0;
     float* const my_grad = grad + wave * line_len;
@@ -80,15 +89,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     typename Tl::template Loads<KB, NW> kl, vl;
     kl.init(in.ks[1], in.dim, wave, lane);
     vl.init(in.vs[1], in.dim, wave, lane);
-    auto issue = [&](int t, uint64_t word, int buf) {
+    auto issue = [&](int t, const uint64_t (&word)[(KB + 63) / 64], int buf) {
         uint8_t* kb = smem + buf * 2 * TILE;
         const T* ks = Kp + (int64_t)t * KB * in.ks[1];
         const T* vs = Vp + (int64_t)t * KB * in.vs[1];
-        if (KB == 64 ? word == ~0ull : (uint32_t)word == 0xFFFFFFFFu) {
+        if (all_kept<KB>(word)) {
             kl.issue_all(ks, kb, wave);
             vl.issue_all(vs, kb + TILE, wave);
         } else {
-            const auto keep = [&](int i) { return (word >> i) & 1; };
+            const auto keep = [&](int i) { return kept_row(word, i); };
             kl.issue(ks, kb, wave, lane, keep);
             vl.issue(vs, kb + TILE, wave, lane, keep);
         }
@@ -112,9 +121,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         delta += swap32(delta);
     }
     if constexpr (BIAS) {  // read after the first tile's barrier
-        rel_line(in.rel, h, line, tid, 256);
-        for (int i = tid; i < NW * line_len; i += 256) grad[i] = 0.f;
-        for (int i = tid; i < NW * kScratch; i += 256) scratch[i] = 0.f;
+        rel_line(in.rel, h, line, tid, 64 * NW);
+        for (int i = tid; i < NW * line_len; i += 64 * NW) grad[i] = 0.f;
+        for (int i = tid; i < NW * kScratch; i += 64 * NW) scratch[i] = 0.f;
     }
     const typename Tl::Cols cols = Tl::cols(lane);
     const int at = row + (BIAS ? rel_position(in.rel, b) : 0);  // rows past the last one too: the block's offsets stay together
@@ -149,24 +158,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         for (int i = 0; i < 16; ++i)
             if (!(w & (1u << (8 * (i >> 2) + (i & 3))))) d[i] = 0.f;
     };
-    // Tiles with a kept key, the next one's DMA in flight behind each.
+    // Tiles with a kept key, the next one's DMA in flight behind each; body has this wave's
+    // rows of K and V, its first key and which of its keys are kept.
     auto walk = [&](auto body) {
         Kept<KB> kept;
         kept.start(in, b, len, 0, in.seq_kv, 1, lane);
         int t = kept.next(lane), buf = 0;
-        uint64_t word = kept.word[0];
-        if (t >= 0) issue(t, word, 0);
+        auto mine = [&]() {
+            return (MY * wk < 64 ? kept.word[0] : kept.word[Kept<KB>::W - 1]) >> (MY * wk & 63);
+        };
+        uint64_t word = mine();
+        if (t >= 0) issue(t, kept.word, 0);
         while (t >= 0) {
             wait_vmem<0>();
             wait_lds();
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             const int t_next = kept.next(lane);
-            const uint64_t word_next = kept.word[0];
-            if (t_next >= 0) issue(t_next, word_next, buf ^ 1);
-            body(smem + buf * 2 * TILE, smem + buf * 2 * TILE + TILE, t, word);
+            if (t_next >= 0) issue(t_next, kept.word, buf ^ 1);
+            const uint8_t* Kt = smem + buf * 2 * TILE + MY * wk * Tl::RB;
+            if (WK == 1 || (HALVES == 2 ? word != 0 : (uint32_t)word != 0)) body(Kt, Kt + TILE, t * KB + MY * wk, word);
             t = t_next;
-            word = word_next;
+            word = mine();
             buf ^= 1;
         }
         wait_lds();
@@ -176,8 +189,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     // dS of a tile's halves: the first half's weights between the second one's products.
     using None = std::integral_constant<int, 0>;
     using SV = std::integral_constant<int, DP == 64 ? 18 : 9>;  // vector instructions per product
-    auto each = [&](const uint8_t* Kt, const uint8_t* Vt, int t, f32x16_t (&s)[HALVES], f32x16_t (&d)[HALVES]) {
-        const int off = t * KB - at;
+    auto each = [&](const uint8_t* Kt, const uint8_t* Vt, int key, f32x16_t (&s)[HALVES], f32x16_t (&d)[HALVES]) {
+        const int off = key - at;
         scores(Kt, Vt, 0, s[0], d[0], None{}, NoSide{});
         if constexpr (HALVES == 2)
             scores(Kt, Vt, 1, s[1], d[1], SV{}, [&](int part, int of) {
@@ -195,9 +208,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
     if constexpr (BIAS && sizeof(T) == 2) {
         float sum = 0.f;
         delta = 0.f;
-        walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+        walk([&](const uint8_t* Kt, const uint8_t* Vt, int key, uint64_t word) {
             f32x16_t s[HALVES], d[HALVES];
-            each(Kt, Vt, t, s, d);
+            each(Kt, Vt, key, s, d);
 #pragma unroll
             for (int hh = 0; hh < HALVES; ++hh) {
                 drop(d[hh], (uint32_t)(word >> (32 * hh)));
@@ -206,8 +219,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
             }
         });
         delta = sum + swap32(sum);
+        if constexpr (WK > 1) {  // of all keys, in wave order (the tiles are free)
+            float* part = reinterpret_cast<float*>(smem);
+            if (g == 0) part[wave * 32 + r] = delta;
+            __syncthreads();
+            delta = part[wr * 32 + r];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) delta += part[(w * WR + wr) * 32 + r];
+            __syncthreads();
+        }
     }
-    if (live && g == 0) {
+    if (live && g == 0 && wk == 0) {
         a.ref[stat] = ref;
         a.delta[stat] = delta;
     }
@@ -216,9 +238,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
 #pragma unroll
     for (int d = 0; d < Tl::BLOCKS; ++d) dq[d] = zero16();
     float far[2] = {0.f, 0.f};  // keys behind, keys ahead, out of reach
-    walk([&](const uint8_t* Kt, const uint8_t* Vt, int t, uint64_t word) {
+    walk([&](const uint8_t* Kt, const uint8_t* Vt, int key, uint64_t word) {
         f32x16_t s[HALVES], dsv[HALVES];
-        each(Kt, Vt, t, s, dsv);
+        each(Kt, Vt, key, s, dsv);
 #pragma unroll
         for (int hh = 0; hh < HALVES; ++hh) {
             f32x16_t& ds = dsv[hh];
@@ -226,7 +248,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
             if constexpr (BIAS) {
                 // Offsets of this 32 x 32 block: off0 + [-31, 31].  A block that is out
                 // of reach as a whole has one bucket (per side: reach may be small).
-                const int off0 = t * KB + 32 * hh - (blk * 128 + wave * 32) - (at - row);
+                const int off0 = key + 32 * hh - row0 - (at - row);
                 if (off0 - 31 >= reach || off0 + 31 <= -reach) {
                     float sum = 0.f;
 #pragma unroll
@@ -264,7 +286,26 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         }
     });
 
-    if (live) {
+    if constexpr (WK > 1) {  // the other waves' sums, in wave order
+        float* part = reinterpret_cast<float*>(smem) + lane;
+        constexpr int N = Tl::BLOCKS * 16 * 64;
+        if (wk > 0) {
+#pragma unroll
+            for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[((wk - 1) * WR + wr) * N + (16 * d + e) * 64] = dq[d][e];
+        }
+        __syncthreads();
+        if (wk == 0) {
+#pragma unroll
+            for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+                for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) dq[d][e] += part[(w * WR + wr) * N + (16 * d + e) * 64];
+        }
+    }
+    if (live && wk == 0) {
         T* op = reinterpret_cast<T*>(a.dq) + b * a.dqs[0] + (int64_t)tok * a.dqs[1] + h * a.dqs[2];
 #pragma unroll
         for (int d = 0; d < Tl::BLOCKS; ++d)
@@ -286,7 +327,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_dq_kernel(co
         __syncthreads();
         // The waves' lines, in wave order, into the first.
         const int n = line_len;
-        for (int i = tid; i < n; i += 256) {
+        for (int i = tid; i < n; i += 64 * NW) {
             float sum = grad[i];
 #pragma unroll
             for (int w = 1; w < NW; ++w) sum += grad[w * n + i];
@@ -332,21 +373,24 @@ __global__ __launch_bounds__(64) void attn_dtable_kernel(const BwdArgs a) {
 }
 
 // ---- dK, dV ----------------------------------------------------------------------------
-template <typename T, int DP, bool BIAS>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_dkv_kernel(const BwdArgs a) {
+// WR waves of 32 keys each, times WK that share the keys and take HALVES x 32 queries each
+// of a tile; their results meet in LDS in wave order.
+template <typename T, int DP, bool BIAS, int WR, int WK, int HALVES>
+__global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_dkv_kernel(const BwdArgs a) {
     typedef Tile<T, DP> Tl;
-    constexpr int QB = tile_rows<T, DP>(), HALVES = QB / 32, TILE = QB * Tl::RB, NW = 4;
+    constexpr int MY = 32 * HALVES, QB = MY * WK, TILE = QB * Tl::RB, NW = WR * WK, SL = QB < 64 ? 64 : QB;
+    static_assert(WR * (WK - 1) * 2 * Tl::BLOCKS * 16 * 256 <= 4 * TILE, "the waves' results take the tiles' place");
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];  // [buffer][Q | dO], [buffer][ref | delta], bias line
     const AttnIn& in = a.in;
-    float* const stats = reinterpret_cast<float*>(smem + 4 * TILE);  // [buffer][2][64]
-    float* const line = stats + 2 * 2 * 64;
+    float* const stats = reinterpret_cast<float*>(smem + 4 * TILE);  // [buffer][2][SL]
+    float* const line = stats + 2 * 2 * SL;
 
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.key_blocks), rest = (int)(bid / (uint32_t)a.key_blocks);
     const int range = rest % a.ranges, bh = rest / a.ranges, b = bh % in.batch, kvh = bh / in.batch;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, g = lane >> 5;
-    const int key = blk * 128 + wave * 32 + r, len = kept_len(in, b);
+    const int r = lane & 31, g = lane >> 5, wr = wave % WR, wk = wave / WR;
+    const int key = (blk * WR + wr) * 32 + r, len = kept_len(in, b);
     const bool keep = key < len && (!in.kv_mask || in.kv_mask[b * in.mask_stride + key] != 0);
     const bool inside = key < in.seq_kv;
 
@@ -391,9 +435,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_
             ql.issue(qp, qb, wave, lane, keep);
             gl.issue(gp, qb + TILE, wave, lane, keep);
         }
-        if (wave < 2) {  // 64 floats each
-            const float* src = (wave == 0 ? a.ref : a.delta) + ((int64_t)b * in.heads + h) * in.seq_q + q0;
-            dma4(src, lane < min(left, QB) ? 4 * lane : kOut, stats + (buf * 2 + wave) * 64);
+#pragma unroll
+        for (int i = 0; i < 2 * SL / 64; ++i) {  // 64 floats an instruction: ref's, then delta's
+            if (i % NW != wave) continue;
+            const int which = i / (SL / 64), at = i % (SL / 64) * 64 + lane;
+            const float* src = (which == 0 ? a.ref : a.delta) + ((int64_t)b * in.heads + h) * in.seq_q + q0;
+            dma4(src, at < min(left, QB) ? 4 * at : kOut, stats + (buf * 2 + which) * SL + i % (SL / 64) * 64);
         }
     };
     int cur = -1, buf = 0;
@@ -406,15 +453,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_
         if constexpr (BIAS) {
             if (n / tiles != cur) {  // every wave has finished with the last head's line
                 cur = n / tiles;
-                rel_line(in.rel, kvh * in.shared + cur, line, tid, 256);
+                rel_line(in.rel, kvh * in.shared + cur, line, tid, 64 * NW);
                 __syncthreads();
             }
         }
         if (n + 1 < last) issue(n + 1, buf ^ 1);
-        const uint8_t* Qt = smem + buf * 2 * TILE;
+        const uint8_t* Qt = smem + buf * 2 * TILE + MY * wk * Tl::RB;
         const uint8_t* Gt = Qt + TILE;
-        const float* st = stats + buf * 2 * 64;
-        const int q0 = (n % tiles) * QB;
+        const float* st = stats + buf * 2 * SL + MY * wk;
+        const int q0 = (n % tiles) * QB + MY * wk;
         f32x16_t s[HALVES], ds[HALVES];
         FragParts<T> pf[HALVES][2], df[HALVES][2];
         auto scores = [&](auto hc, auto vc, auto side) {
@@ -435,7 +482,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_
             constexpr int hh = decltype(hc)::value;
             const int i0 = 32 * hh + 4 * g + 8 * i4;
             const float4 rf = *reinterpret_cast<const float4*>(st + i0);
-            const float4 dl = *reinterpret_cast<const float4*>(st + 64 + i0);
+            const float4 dl = *reinterpret_cast<const float4*>(st + SL + i0);
             const float ref[4] = {rf.x, rf.y, rf.z, rf.w}, delta[4] = {dl.x, dl.y, dl.z, dl.w};
             float p[4], d[4];
 #pragma unroll
@@ -483,6 +530,31 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DP == 64 ? 2 : 1) void attn_
         }
         grads(H1{}, None{}, NoSide{});
         buf ^= 1;
+    }
+    if constexpr (WK > 1) {  // the other waves' sums, in wave order
+        float* part = reinterpret_cast<float*>(smem) + lane;
+        constexpr int N = 2 * Tl::BLOCKS * 16 * 64;
+        __syncthreads();  // every wave has read its last tile
+        if (wk > 0) {
+#pragma unroll
+            for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    part[((wk - 1) * WR + wr) * N + (32 * d + e) * 64] = dk[d][e];
+                    part[((wk - 1) * WR + wr) * N + (32 * d + 16 + e) * 64] = dv[d][e];
+                }
+        }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+            for (int d = 0; d < Tl::BLOCKS; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    dk[d][e] += part[(w * WR + wr) * N + (32 * d + e) * 64];
+                    dv[d][e] += part[(w * WR + wr) * N + (32 * d + 16 + e) * 64];
+                }
     }
     if (!inside) return;
     if (!keep) {
@@ -556,42 +628,71 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(const BwdArgs a) {
 
 // ---- launch ------------------------------------------------------------------------------
 struct Plan {
+    int row_high, key_high;     // rows (keys) of a workgroup: 128, or 32 with waves that share them
+    bool row_pairs;             // 128 rows by eight waves
     int row_blocks, key_blocks, ranges;
     int64_t stat_floats, table_floats, kv_floats;  // workspace, in this order (ref and delta first)
 };
 
 int64_t up4(int64_t n) { return (n + 3) / 4 * 4; }
 
-Plan plan(const AttnIn& in, int buckets, int cus) {
+Plan plan(const AttnIn& in, bool bf16_io, int buckets, int cus) {
     Plan p{};
     const int dp = in.dim <= 64 ? 64 : 128;
-    p.row_blocks = (in.seq_q + 127) / 128;
-    p.key_blocks = (in.seq_kv + 127) / 128;
-    const int64_t blocks = (int64_t)p.key_blocks * in.kv_heads * in.batch, tiles = (int64_t)((in.seq_q + 63) / 64) * in.shared;
-    // Ranges of the queries until every CU has a workgroup, each of at least two tiles.
+    const int64_t rows = (int64_t)in.heads * in.batch, keys = (int64_t)in.kv_heads * in.batch;
+    // 128 rows a workgroup while that gives half the CUs one; up to one per CU by eight waves
+    // (bf16 without a bias, whose lines take the second tile's place).
+    const int64_t wide = (int64_t)((in.seq_q + 127) / 128) * rows;
+    p.row_high = wide * 2 >= cus ? 128 : 32;
+    p.row_pairs = p.row_high == 128 && wide <= cus && bf16_io && buckets == 0 && in.seq_kv > 64;
+    p.row_blocks = (in.seq_q + p.row_high - 1) / p.row_high;
+    // 128 keys, whose queries can be shared in up to 16 ranges of at least 128, while that gives
+    // every CU a workgroup.
+    const int64_t tall = (int64_t)((in.seq_kv + 127) / 128) * keys;
+    int64_t most = (int64_t)((in.seq_q + 127) / 128) * in.shared;
+    if (most > 16) most = 16;
+    p.key_high = tall * most >= cus ? 128 : 32;
+    p.key_blocks = (in.seq_kv + p.key_high - 1) / p.key_high;
+    const int64_t blocks = p.key_blocks * keys;
     int64_t s = blocks > 0 ? cus / blocks : 1;
-    if (s > tiles / 2) s = tiles / 2;
-    if (s > 16) s = 16;
+    if (s > most) s = most;
     p.ranges = s < 2 ? 1 : (int)s;
-    p.stat_floats = up4((int64_t)in.batch * in.heads * in.seq_q);
-    p.table_floats = buckets ? up4((int64_t)in.batch * in.heads * p.row_blocks * buckets) : 0;
-    p.kv_floats = p.ranges > 1 ? (int64_t)p.ranges * 2 * in.batch * in.kv_heads * in.seq_kv * dp : 0;
+    p.stat_floats = up4(rows * in.seq_q);
+    p.table_floats = buckets ? up4(rows * p.row_blocks * buckets) : 0;
+    p.kv_floats = p.ranges > 1 ? (int64_t)p.ranges * 2 * keys * in.seq_kv * dp : 0;
     return p;
+}
+
+template <typename T, int DP, bool BIAS, int WR, int WK, int HALVES>
+void launch_dq(const BwdArgs& a, int64_t blocks, hipStream_t st) {
+    const size_t lds = 4 * 32 * HALVES * WK * Tile<T, DP>::RB +
+                       (BIAS ? (1 + WR * WK) * rel_line_len(a.in.rel.reach) + WR * WK * kScratch : 0) * sizeof(float);
+    hipLaunchKernelGGL((attn_dq_kernel<T, DP, BIAS, WR, WK, HALVES>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, st, a);
+}
+template <typename T, int DP, bool BIAS, int WR, int WK, int HALVES>
+void launch_dkv(const BwdArgs& a, int64_t blocks, hipStream_t st) {
+    constexpr int QB = 32 * HALVES * WK;
+    const size_t lds = 4 * QB * Tile<T, DP>::RB + (4 * (QB < 64 ? 64 : QB) + (BIAS ? rel_line_len(a.in.rel.reach) : 0)) * sizeof(float);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, BIAS, WR, WK, HALVES>), dim3((unsigned)blocks), dim3(64 * WR * WK), lds, st, a);
 }
 
 template <typename T, int DP, bool BIAS>
 int launch(const BwdArgs& a, const Plan& p, hipStream_t st) {
     const char* who = "dt_attn_bwd";
     const AttnIn& in = a.in;
-    const size_t tiles = 4 * tile_rows<T, DP>() * Tile<T, DP>::RB;
-    const int line = rel_line_floats(in.rel);
     const int64_t dq_blocks = (int64_t)p.row_blocks * in.heads * in.batch;
     const int64_t dkv_blocks = (int64_t)p.key_blocks * p.ranges * in.kv_heads * in.batch;
     DT_REQUIRE(dq_blocks < (1ll << 31) && dkv_blocks < (1ll << 31), "%s: grid too large", who);
+    constexpr int H = halves<T, DP>(), FEW = few_waves<T, DP, BIAS>();
     int rc = DT_OK;
     if (dq_blocks > 0) {
-        const size_t lds = tiles + (BIAS ? 5 * line + 4 * kScratch : 0) * sizeof(float);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, BIAS>), dim3((unsigned)dq_blocks), dim3(256), lds, st, a);
+        if (p.row_high == 32) {
+            launch_dq<T, DP, BIAS, 1, FEW, 1>(a, dq_blocks, st);
+        } else if (p.row_pairs) {
+            if constexpr (sizeof(T) == 2 && !BIAS) launch_dq<T, DP, BIAS, 4, 2, 2>(a, dq_blocks, st);
+        } else {
+            launch_dq<T, DP, BIAS, 4, 1, H>(a, dq_blocks, st);
+        }
         rc = check_launch(who);
     }
     if (!rc && BIAS && a.d_table && in.heads > 0) {
@@ -599,8 +700,8 @@ int launch(const BwdArgs& a, const Plan& p, hipStream_t st) {
         rc = check_launch(who);
     }
     if (rc || dkv_blocks == 0) return rc;
-    const size_t lds = tiles + (4 * 64 + (BIAS ? line : 0)) * sizeof(float);
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, BIAS>), dim3((unsigned)dkv_blocks), dim3(256), lds, st, a);
+    if (p.key_high == 32) launch_dkv<T, DP, BIAS, 1, Tile<T, DP>::RB <= 256 ? 4 : 2, 1>(a, dkv_blocks, st);
+    else launch_dkv<T, DP, BIAS, 4, 1, H>(a, dkv_blocks, st);
     rc = check_launch(who);
     if (rc || p.ranges == 1) return rc;
     const int64_t n = (int64_t)in.batch * in.kv_heads * in.seq_kv * (DP / 4);
@@ -624,7 +725,7 @@ extern "C" size_t dt_attn_bwd_workspace_bytes(const dt_attn_args* x) {
     using namespace dit::attn;
     AttnIn in;
     if (prepare_in(x, "dt_attn_bwd_workspace_bytes", &in)) return 0;
-    return (size_t)total_floats(plan(in, x->rel_table ? x->rel_buckets : 0, cu_count())) * sizeof(float);
+    return (size_t)total_floats(plan(in, x->io_type == DT_TYPE_BF16, x->rel_table ? x->rel_buckets : 0, cu_count())) * sizeof(float);
 }
 
 extern "C" int dt_attn_bwd(const dt_attn_args* x, const dt_attn_grads* y, void* workspace, size_t workspace_bytes,
@@ -648,7 +749,7 @@ extern "C" int dt_attn_bwd(const dt_attn_args* x, const dt_attn_grads* y, void* 
     DT_REQUIRE(!x->rel_table || !y->d_rel_table || (((uintptr_t)y->d_rel_table & 3) == 0 && y->d_rel_table_stride >= x->heads),
                "%s: d_rel_table must be 4-byte aligned with rows of at least heads", who);
     a.buckets = x->rel_table ? x->rel_buckets : 0;
-    const Plan p = plan(in, a.buckets, cu_count());
+    const Plan p = plan(in, x->io_type == DT_TYPE_BF16, a.buckets, cu_count());
     const size_t need = (size_t)total_floats(p) * sizeof(float);
     DT_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", who, need, workspace ? workspace_bytes : 0);
