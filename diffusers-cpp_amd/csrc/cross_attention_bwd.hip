@@ -36,7 +36,7 @@ struct BwdArgs {
     float* part_kv;     // [ranges][2][batch][kv_heads][seq_kv][DP]
     float* d_table;
     int64_t d_table_stride;
-    int32_t row_blocks, key_blocks, ranges, buckets;
+    int32_t row_blocks, key_blocks, ranges, buckets, table_blocks;
 };
 
 // 32-row halves of a wave's part of a tile with four waves side by side; waves that share rows
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
     float* const line = scratch + NW * kScratch;
     // Then the waves' table gradients, a line each as the bias's; scratch first, for its alignment.
     float* const grad = line + line_len;
-    __shared__ float far_sum[2][NW];
+    __shared__ float far_sum[2][NW], part_delta[NW][32];
 
     const uint32_t bid = xcd_block();
     const int blk = (int)(bid % (uint32_t)a.row_blocks), bh = (int)(bid / (uint32_t)a.row_blocks);
@@ -103,6 +103,18 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
         }
     };
 
+    Kept<KB> kept;
+    const int len = kept_len(in, b);
+    auto first_tile = [&]() {
+        kept.start(in, b, len, 0, in.seq_kv, 1, lane);
+        return kept.next(lane);
+    };
+    // Which of this wave's keys of the tile are kept.
+    auto mine = [&]() { return (MY * wk < 64 ? kept.word[0] : kept.word[Kept<KB>::W - 1]) >> (MY * wk & 63); };
+    int t = first_tile(), buf = 0;
+    uint64_t word = mine();
+    if (t >= 0) issue(t, kept.word, 0);
+
     typename Tl::Frag qf[Tl::STEPS], of[Tl::STEPS];
     const int64_t stat = ((int64_t)b * in.heads + h) * in.seq_q + tok;
     float ref = a.lse[stat] * kLog2e;
@@ -127,7 +139,6 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
     }
     const typename Tl::Cols cols = Tl::cols(lane);
     const int at = row + (BIAS ? rel_position(in.rel, b) : 0);  // rows past the last one too: the block's offsets stay together
-    const int len = kept_len(in, b);
 
     // S and dP of one 32-key half of a tile.
     auto scores = [&](const uint8_t* Kt, const uint8_t* Vt, int hh, f32x16_t& s, f32x16_t& d, auto vc, auto side) {
@@ -158,23 +169,21 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
         for (int i = 0; i < 16; ++i)
             if (!(w & (1u << (8 * (i >> 2) + (i & 3))))) d[i] = 0.f;
     };
-    // Tiles with a kept key, the next one's DMA in flight behind each; body has this wave's
-    // rows of K and V, its first key and which of its keys are kept.
-    auto walk = [&](auto body) {
-        Kept<KB> kept;
-        kept.start(in, b, len, 0, in.seq_kv, 1, lane);
-        int t = kept.next(lane), buf = 0;
-        auto mine = [&]() {
-            return (MY * wk < 64 ? kept.word[0] : kept.word[Kept<KB>::W - 1]) >> (MY * wk & 63);
-        };
-        uint64_t word = mine();
-        if (t >= 0) issue(t, kept.word, 0);
-        while (t >= 0) {
+    // A pass over the tiles with a kept key, the next one's DMA in flight behind each (behind the
+    // last one the next pass's first); body has this wave's rows of K and V, its first key
+    // and which of its keys are kept.
+    auto walk = [&](auto body, bool again) {
+        bool more = t >= 0;
+        while (more) {
             wait_vmem<0>();
             wait_lds();
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            const int t_next = kept.next(lane);
+            int t_next = kept.next(lane);
+            if (t_next < 0) {
+                more = false;
+                if (again) t_next = first_tile();
+            }
             if (t_next >= 0) issue(t_next, kept.word, buf ^ 1);
             const uint8_t* Kt = smem + buf * 2 * TILE + MY * wk * Tl::RB;
             if (WK == 1 || (HALVES == 2 ? word != 0 : (uint32_t)word != 0)) body(Kt, Kt + TILE, t * KB + MY * wk, word);
@@ -182,8 +191,6 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
             word = mine();
             buf ^= 1;
         }
-        wait_lds();
-        __builtin_amdgcn_s_barrier();
     };
 
     // dS of a tile's halves: the first half's weights between the second one's products.
@@ -217,16 +224,14 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += d[hh][i];
             }
-        });
+        }, true);
         delta = sum + swap32(sum);
-        if constexpr (WK > 1) {  // of all keys, in wave order (the tiles are free)
-            float* part = reinterpret_cast<float*>(smem);
-            if (g == 0) part[wave * 32 + r] = delta;
+        if constexpr (WK > 1) {  // of all keys, in wave order
+            if (g == 0) part_delta[wave][r] = delta;
             __syncthreads();
-            delta = part[wr * 32 + r];
+            delta = part_delta[wr][r];
 #pragma unroll
-            for (int w = 1; w < WK; ++w) delta += part[(w * WR + wr) * 32 + r];
-            __syncthreads();
+            for (int w = 1; w < WK; ++w) delta += part_delta[w * WR + wr][r];
         }
     }
     if (live && g == 0 && wk == 0) {
@@ -284,11 +289,12 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
                 [&](int i) { return Tl::col_frag(Kt, 32 * hh + 16 * (i / Tl::BLOCKS), i % Tl::BLOCKS, cols); },
                 [&](int i, const typename Tl::Frag& f) { dq[i % Tl::BLOCKS] = mma(f, f2[i / Tl::BLOCKS], dq[i % Tl::BLOCKS]); });
         }
-    });
+    }, false);
 
     if constexpr (WK > 1) {  // the other waves' sums, in wave order
         float* part = reinterpret_cast<float*>(smem) + lane;
         constexpr int N = Tl::BLOCKS * 16 * 64;
+        __syncthreads();  // every wave has read its last tile
         if (wk > 0) {
 #pragma unroll
             for (int d = 0; d < Tl::BLOCKS; ++d)
@@ -334,24 +340,25 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
             grad[i] = sum;
         }
         __syncthreads();
-        // A bucket per wave at a time: its offsets over the lanes.
+        // Sixteen lanes a bucket, its offsets over them.
         float* out = a.part_table + (((int64_t)b * in.heads + h) * a.row_blocks + blk) * a.buckets;
-        for (int t = wave; t < a.buckets; t += NW) {
+        for (int t0 = 0; t0 < a.buckets; t0 += 4 * NW) {
+            const int bucket = t0 + (tid >> 4), t = min(bucket, a.buckets - 1), i = tid & 15;
             const bool ahead = in.rel.two_sided && t >= in.rel.side;
             const int u = ahead ? t - in.rel.side : t;
-            const bool last = u == in.rel.side - 1;
+            const bool last = u == in.rel.side - 1, rest = !in.rel.two_sided && u == 0;
             // Distances [lo, hi) of the bucket.  Without the two sides every key ahead is at distance 0.
             const int lo = in.rel.start[u], hi = last ? mid + 1 : in.rel.start[u + 1];
             float sum = 0.f;
-            for (int dist = lo + lane; dist < hi; dist += 64)
+            for (int dist = lo + i; dist < hi; dist += 16)
                 if (!ahead || dist > 0) sum += grad[mid + (ahead ? dist : -dist)];
-            if (!in.rel.two_sided && u == 0)
-                for (int dist = 1 + lane; dist <= mid; dist += 64) sum += grad[mid + dist];
-            sum = wave_sum(sum);
-            if (lane == 0) {
+            if (rest)
+                for (int dist = 1 + i; dist <= mid; dist += 16) sum += grad[mid + dist];
+            sum = row16_sum(sum);
+            if (i == 0 && bucket < a.buckets) {
                 if (last)
                     for (int w = 0; w < NW; ++w) sum += far_sum[ahead][w];
-                if (!in.rel.two_sided && u == 0)
+                if (rest)
                     for (int w = 0; w < NW; ++w) sum += far_sum[1][w];
                 out[t] = sum;
             }
@@ -360,8 +367,9 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
 }
 
 // dtable[t][h] = the sum of its partial sums over batch entries and row blocks: a wave per (t, h), in 64 bits.
-__global__ __launch_bounds__(64) void attn_dtable_kernel(const BwdArgs a) {
-    const int t = blockIdx.x % a.buckets, h = blockIdx.x / a.buckets, lane = threadIdx.x;
+__device__ __forceinline__ void sum_table(const BwdArgs& a, int id, int lane) {
+    if (id >= a.buckets * a.in.heads) return;
+    const int t = id % a.buckets, h = id / a.buckets;
     double sum = 0.0;
     const int n = a.in.batch * a.row_blocks;
     for (int i = lane; i < n; i += 64) {
@@ -385,10 +393,15 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 && DP == 64 ? 2 : 1) v
     float* const stats = reinterpret_cast<float*>(smem + 4 * TILE);  // [buffer][2][SL]
     float* const line = stats + 2 * 2 * SL;
 
-    const uint32_t bid = xcd_block();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // The launch's first workgroups add up the table's gradient.
+    if (BIAS && blockIdx.x < (uint32_t)a.table_blocks) {
+        sum_table(a, (int)blockIdx.x * NW + wave, lane);
+        return;
+    }
+    const uint32_t bid = BIAS ? blockIdx.x - a.table_blocks : xcd_block();
     const int blk = (int)(bid % (uint32_t)a.key_blocks), rest = (int)(bid / (uint32_t)a.key_blocks);
     const int range = rest % a.ranges, bh = rest / a.ranges, b = bh % in.batch, kvh = bh / in.batch;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, g = lane >> 5, wr = wave % WR, wk = wave / WR;
     const int key = (blk * WR + wr) * 32 + r, len = kept_len(in, b);
     const bool keep = key < len && (!in.kv_mask || in.kv_mask[b * in.mask_stride + key] != 0);
@@ -695,15 +708,17 @@ int launch(const BwdArgs& a, const Plan& p, hipStream_t st) {
         }
         rc = check_launch(who);
     }
-    if (!rc && BIAS && a.d_table && in.heads > 0) {
-        hipLaunchKernelGGL(attn_dtable_kernel, dim3((unsigned)(a.buckets * in.heads)), dim3(64), 0, st, a);
-        rc = check_launch(who);
-    }
-    if (rc || dkv_blocks == 0) return rc;
-    if (p.key_high == 32) launch_dkv<T, DP, BIAS, 1, Tile<T, DP>::RB <= 256 ? 4 : 2, 1>(a, dkv_blocks, st);
-    else launch_dkv<T, DP, BIAS, 4, 1, H>(a, dkv_blocks, st);
+    constexpr int KW = Tile<T, DP>::RB <= 256 ? 4 : 2;
+    BwdArgs k = a;
+    const int waves = p.key_high == 32 ? KW : 4;
+    k.table_blocks = BIAS && a.d_table ? (a.buckets * in.heads + waves - 1) / waves : 0;
+    const int64_t blocks = dkv_blocks + k.table_blocks;
+    DT_REQUIRE(blocks < (1ll << 31), "%s: grid too large", who);
+    if (rc || blocks == 0) return rc;
+    if (p.key_high == 32) launch_dkv<T, DP, BIAS, 1, KW, 1>(k, blocks, st);
+    else launch_dkv<T, DP, BIAS, 4, 1, H>(k, blocks, st);
     rc = check_launch(who);
-    if (rc || p.ranges == 1) return rc;
+    if (rc || p.ranges == 1 || dkv_blocks == 0) return rc;
     const int64_t n = (int64_t)in.batch * in.kv_heads * in.seq_kv * (DP / 4);
     hipLaunchKernelGGL((attn_dkv_join_kernel<T, DP>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     return check_launch(who);
