@@ -152,7 +152,8 @@ constexpr uint32_t kOut = 0x80000000u;  // an offset out of every buffer's range
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint8_t* lds) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
-}__device__ __forceinline__ void dma4(const void* base, uint32_t off, void* lds) {  // 4 bytes a lane
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, void* lds) {  // 4 bytes a lane
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
 }
@@ -432,7 +433,7 @@ __device__ __forceinline__ int rel_position(const RelArgs& r, int b) {
 
 // ---- host ---------------------------------------------------------------------------
 constexpr int64_t kMaxSeq = 1 << 28;
-constexpr int64_t kMaxRowStride = (1 << 23) - 128;  // 64 fp32 rows stay below kOut bytes
+constexpr int64_t kMaxRowBytes = (1 << 24) - 256;  // a tile's 128 rows stay below kOut bytes
 // Checks the shared arguments and fills `in` (cross_attention.hip).
 int prepare_in(const dt_attn_args* args, const char* who, AttnIn* in);
 // Checks one strided operand [batch][seq][heads][head_dim]; `out`: no element twice.

@@ -606,7 +606,7 @@ int check_rows(const dt_attn_args* x, const void* p, const int64_t* strides, int
     if (x->batch == 0 || heads == 0 || seq == 0) return DT_OK;  // no element
     DT_REQUIRE(p != nullptr && strides != nullptr, "%s: null %s", who, name);
     DT_REQUIRE(aligned16(p), "%s: %s must be 16-byte aligned", who, name);
-    const int64_t n[3] = {x->batch, seq, heads}, step = x->io_type == DT_TYPE_F32 ? 4 : 8;
+    const int64_t n[3] = {x->batch, seq, heads}, step = x->io_type == DT_TYPE_F32 ? 4 : 8;  // elements of 16 bytes
     int64_t reach = x->head_dim;  // of the dimensions with smaller strides
     bool done[3] = {false, false, false};
     for (int pass = 0; pass < 3; ++pass) {
@@ -617,7 +617,7 @@ int check_rows(const dt_attn_args* x, const void* p, const int64_t* strides, int
         if (n[at] == 1) continue;
         const int64_t s = strides[at];
         DT_REQUIRE(s % step == 0, "%s: %s strides must keep rows 16-byte aligned", who, name);
-        DT_REQUIRE(s >= 0 && s < (at == 1 ? kMaxRowStride : 1ll << 40), "%s: %s stride %lld unsupported", who, name, (long long)s);
+        DT_REQUIRE(s >= 0 && s < (at == 1 ? kMaxRowBytes / 16 * step : 1ll << 40), "%s: %s stride %lld unsupported", who, name, (long long)s);
         if (!out) continue;
         DT_REQUIRE(s >= reach, "%s: elements of %s overlap", who, name);
         reach = s * (n[at] - 1) + reach;
@@ -633,8 +633,8 @@ int prepare_in(const dt_attn_args* x, const char* who, AttnIn* out) {
                "%s: head_dim %lld unsupported (a multiple of 8 up to 128)", who, (long long)x->head_dim);
     DT_REQUIRE(x->heads == 0 || (x->kv_heads > 0 && x->heads % x->kv_heads == 0),
                "%s: %lld query heads do not share %lld key heads evenly", who, (long long)x->heads, (long long)x->kv_heads);
-    DT_REQUIRE(x->batch < (1 << 20) && x->heads < (1 << 16) && x->seq_q < kMaxSeq && x->seq_kv < kMaxSeq,
-               "%s: size too large", who);
+    DT_REQUIRE(x->batch < (1 << 20) && x->heads < (1 << 16) && x->seq_q < kMaxSeq && x->seq_kv < kMaxSeq &&
+                   x->seq_q * (x->heads == 0 ? 1 : x->heads / x->kv_heads) < (1ll << 30), "%s: size too large", who);
     DT_REQUIRE(x->scale >= 0.f && x->scale < INFINITY, "%s: scale must be >= 0 and finite (got %g)", who, (double)x->scale);
     int rc = check_rows(x, x->q, x->q_strides, x->heads, x->seq_q, false, "q", who);
     if (!rc) rc = check_rows(x, x->k, x->k_strides, x->kv_heads, x->seq_kv, false, "k", who);
@@ -730,8 +730,7 @@ extern "C" int dt_attn_fwd(const dt_attn_args* x, void* o, const int64_t* o_stri
     a.lse = lse;
     Plan p = plan(a.in, x->io_type == DT_TYPE_BF16, cu_count());
     if (p.splits > 1 && (!workspace || workspace_bytes < (size_t)p.part_floats * sizeof(float) || !aligned16(workspace))) p.splits = 1;
-    DT_REQUIRE((int64_t)a.in.seq_q * p.pack < (1ll << 31) &&
-                   (int64_t)p.row_blocks * p.splits * p.groups * a.in.batch < (1ll << 31) &&
+    DT_REQUIRE((int64_t)p.row_blocks * p.splits * p.groups * a.in.batch < (1ll << 31) &&
                    (int64_t)a.in.batch * a.in.heads * a.in.seq_q < (1ll << 36), "%s: grid too large", who);
     a.pack = p.pack;
     a.pack_div = make_fastdiv((uint32_t)p.pack);

@@ -473,7 +473,7 @@ int dt_flash_attn_f32(const float *q, const float *k, const float *v, float *o, 
  * the gradients; products of bf16 operands, or of fp32 ones on the fp32 matrix
  * cores, sums in fp32), head_dim a multiple of 8 up to 128, pointers and rows
  * 16-byte aligned (strides of dimensions of one element are not read; stride 0
- * repeats an input).
+ * repeats an input; tokens lie less than 16 MB - 256 bytes apart).
  * kv_len (int32 [batch], device) keeps keys below kv_len[b] (clamped to
  * [0, seq_kv]); kv_mask (uint8, key j of entry b at kv_mask[b*kv_mask_stride +
  * j], device) keeps keys with a nonzero byte; both given: both.  What a key that
