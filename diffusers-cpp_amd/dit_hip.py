@@ -214,6 +214,12 @@ class _Recorder:
         return call
 
 
+def _sizing():
+    """The library itself: a size asked for once is no part of what prepare() repeats."""
+    lib = load()
+    return lib._lib if isinstance(lib, _Recorder) else lib
+
+
 def prepare(wrapper, *args, **kwargs):
     """Run `wrapper(*args, **kwargs)` once (arguments checked, outputs
     allocated, the launch made) and return (result, launch): launch() repeats
@@ -838,7 +844,7 @@ def _lora_plan(x, w, scales, a, b, scale, rows, bias, addend, out, here):
     p = GemmProblem(None, ld(x, K), None, ld(w, K), None, ld(out, N), None, 0 if addend is None else ld(addend, N), None, M,
                     N, K, None, ld(scales, N) if q8 else 0)
     s = LoraArgs(None, ld(a, K), a[2][0], None, ld(b, rank), b[2][0], None, None, n, rank)
-    return bytes(p), bytes(s), load().dt_lora_gemm_workspace_bytes(M, N, K, rank), _IO_TYPES[out[0]]
+    return bytes(p), bytes(s), _sizing().dt_lora_gemm_workspace_bytes(M, N, K, rank), _IO_TYPES[out[0]]
 
 
 def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dtype=None):
@@ -942,7 +948,7 @@ def _attn_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, out,
     # The workspaces go by sizes alone; the pointers stand for the call's own.
     a.q = a.k = a.v = 16
     a.rel_table = None if table is None else 16
-    lib, p = load(), ctypes.addressof(a)
+    lib, p = _sizing(), ctypes.addressof(a)
     sizes = lib.dt_attn_fwd_workspace_bytes(p), lib.dt_attn_bwd_workspace_bytes(p)
     return bytes(a), *sizes, _i64x3(*out[2][:3])
 
