@@ -50,6 +50,14 @@ constexpr int few_waves() {
     return Tile<T, DP>::RB <= 128 || (Tile<T, DP>::RB == 256 && !BIAS) ? 4 : Tile<T, DP>::RB == 256 || !BIAS ? 2 : 1;
 }
 
+// delta = <dO, o> is off by the rounding of a bf16 o, and P spreads that over the row's dS: the
+// fewer the keys, the less it is averaged (error of dq and dk against 64 bits, in errors
+// of one rounding to bf16; two independent ones, of dS and of the result, are
+// 1.41: 9 keys 1.67, 16 keys 1.58, 40 keys 1.50, 77 keys 1.46, 200 keys 1.45).  Up to one tile
+// of keys sums P dP first (9 to 64 keys: 1.43); up to two would take 42.2 instead of 38.9 us for
+// a step of 1024 queries and 77 keys.
+constexpr int kExactKeys = 64;
+
 // A wave's dS block as its 63 diagonals (offsets -31 .. 31), each a row of 32 queries; what
 // lies outside the block stays 0.  Rows padded to 36: the block's writes (a step of 35
 // floats a lane) and a lane's reads of its row in 16 bytes spread over all banks.
@@ -211,8 +219,8 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
 
     // The table's gradient is kept in fp32, and a whole row's dS cancels in it: delta
     // from the rounded output (off by its rounding and P's) would show there, so it is
-    // summed from P and dP first.
-    if constexpr (BIAS && sizeof(T) == 2) {
+    // summed from P and dP first; so it is for few keys.
+    if (sizeof(T) == 2 && (BIAS || len <= kExactKeys)) {
         float sum = 0.f;
         delta = 0.f;
         walk([&](const uint8_t* Kt, const uint8_t* Vt, int key, uint64_t word) {
