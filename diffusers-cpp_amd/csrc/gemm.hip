@@ -1054,9 +1054,70 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
 // bf16, the value dt_dequant writes.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-template <typename TC, bool Q8, int KS, typename L = NoLora>
+// The adapters of a wave's 16 rows over the KS waves, in parts of one adapter and 32 of its rank,
+// four at a time.  Each product is kept in its own rows.
+template <int KS>
+struct LoraParts {
+    static constexpr int N = 4;
+    const uint16_t* t;
+    const uint16_t* u0;
+    uint64_t left;
+    int rows, turn, wave, g, a, k;
+    int of[N];  // the part's adapter, -2: no part
+    bf16x8_t u[N], x[N][2];
+
+    __device__ __forceinline__ void start(const LoraTile& l, int& mine, int w, const uint16_t* t_row, const uint16_t* u_row, int lg) {
+        if (mine >= l.adapters) mine = -1;
+        left = __builtin_amdgcn_ballot_w64(mine >= 0);
+        t = t_row;
+        u0 = u_row;
+        wave = w;
+        g = lg;
+        turn = a = 0;
+        k = l.rank;
+        rows = mine;
+    }
+    __device__ __forceinline__ bool next(const LoraTile& l) {
+        k += 32;
+        if (k < l.rank) return true;
+        while (left) {
+            a = __builtin_amdgcn_readlane(rows, (int)__builtin_ctzll(left));
+            left &= ~__builtin_amdgcn_ballot_w64(rows == a);
+            if (turn++ % KS != wave) continue;
+            k = 0;
+            return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ void fetch(const LoraTile& l) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            of[i] = -2;
+            if (next(l)) {
+                of[i] = a;
+                u[i] = lora_up(l, u0 + a * l.u_stride, k + 8 * g);
+                x[i][0] = lora_t(t + k);
+                x[i][1] = lora_t(t + l.rp + k);
+            }
+        }
+    }
+    // Adds the parts fetched last; whether there were as many as could be.
+    __device__ __forceinline__ bool add(int mine, f32x4_t& acc) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (of[i] < 0) return false;
+            f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i][0], d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i][1], d, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += mine == of[i] ? d[e] : 0.f;
+        }
+        return true;
+    }
+};
+
+template <typename TC, bool Q8, int KS, typename L = NoLora, int UNR = 4>  // UNR 64-k blocks loaded together
 __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, const L lora) {
-    constexpr int UNR = 4;      // 64-k blocks loaded together
     constexpr int LD = 16 + 4;  // padded row of the partial sums
     __shared__ float part[KS][16 * LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1067,6 +1128,7 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
     const int r = lane & 15, g = lane >> 4;
     int mine = -1;  // the adapter of row r, read ahead of the weights
     if constexpr (L::on) mine = r < p.M ? lora.row_adapter[r] : -1;
+    LoraParts<KS> parts;
 
     const int nblk = p.K / 64, per = (nblk + KS - 1) / KS;
     const int b0 = min(wave * per, nblk), b1 = min(b0 + per, nblk);
@@ -1077,8 +1139,8 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
     const float* sp = Q8 ? p.Bs + n + (g >> 1) * p.ldbs : nullptr;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 
-    // U blocks from block b.
-    auto step = [&](int b, auto uc) {
+    // U blocks from block b; meanwhile: what is issued behind their loads.
+    auto step = [&](int b, auto uc, auto meanwhile) {
         constexpr int U = decltype(uc)::value;
         uint4 w[U][2], x[U][2];
         float d[U];
@@ -1095,6 +1157,7 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 #pragma unroll
             for (int h = 0; h < 2; ++h) x[u][h] = *reinterpret_cast<const uint4*>(xp + k + 8 * h);
         }
+        meanwhile();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if constexpr (Q8) {
@@ -1118,28 +1181,30 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
                                                               __builtin_bit_cast(bf16x8_t, x[u][h]), acc, 0, 0, 0);
         }
     };
+    const auto start = [&]() {  // the adapters' first parts
+        if constexpr (L::on) {
+            parts.start(lora, mine, wave, lora.t + (int64_t)min(r, p.M - 1) * 2 * lora.rp + 8 * g, lora.u + n * lora.ldu, g);
+            parts.fetch(lora);
+        }
+    };
+    const auto nothing = [] {};
     int b = b0;
-    for (; b + UNR <= b1; b += UNR) step(b, std::integral_constant<int, UNR>{});
-    for (; b < b1; ++b) step(b, std::integral_constant<int, 1>{});
+    if constexpr (UNR == 8) {  // behind the weights' loads: registers to spare
+        if (b + UNR <= b1) {
+            step(b, std::integral_constant<int, UNR>{}, start);
+            b += UNR;
+        } else {
+            start();
+        }
+    }
+    for (; b + UNR <= b1; b += UNR) step(b, std::integral_constant<int, UNR>{}, nothing);
+    if constexpr (UNR == 8)
+        for (; b + 4 <= b1; b += 4) step(b, std::integral_constant<int, 4>{}, nothing);
+    for (; b < b1; ++b) step(b, std::integral_constant<int, 1>{}, nothing);
 
     if constexpr (L::on) {
-        // The rows' adapters over the waves, each product kept in its own rows.
-        const uint16_t* t = lora.t + (int64_t)min(r, p.M - 1) * 2 * lora.rp + 8 * g;
-        const uint16_t* u0 = lora.u + n * lora.ldu;
-        uint64_t left = __builtin_amdgcn_ballot_w64(mine >= 0 && mine < lora.adapters);
-        for (int turn = 0; left; ++turn) {
-            const int a = __builtin_amdgcn_readlane(mine, (int)__builtin_ctzll(left));
-            left &= ~__builtin_amdgcn_ballot_w64(mine == a);
-            if (turn % KS != wave) continue;
-            f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < lora.rank; k += 32) {
-                const bf16x8_t u = lora_up(lora, u0 + a * lora.u_stride, k + 8 * g);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, lora_t(t + k), d, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u, lora_t(t + lora.rp + k), d, 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += mine == a ? d[e] : 0.f;
-        }
+        if constexpr (UNR != 8) start();
+        while (parts.add(mine, acc)) parts.fetch(lora);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[wave][r * LD + 4 * g + e] = acc[e];
@@ -1371,6 +1436,8 @@ int launch_skinny(const Problem* ps, int n, const L& lora, hipStream_t st) {
     // Eight waves a workgroup until there are four workgroups per CU.
     if (total >= 4 * cu_count())
         hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 4, L>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
+    else if (L::on && total <= cu_count())
+        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8, L, L::on ? 8 : 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
     else
         hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8, L>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
     return check_launch("dt_gemm_bf16");
