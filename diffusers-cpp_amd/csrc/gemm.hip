@@ -1037,21 +1037,14 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
 }
 
 // ---- few rows: 16 weight rows per workgroup, K split over its waves -------------
-// M <= 16 (a conditioning vector's Linear): the product is a stream of the
-// weight.  With 128 x 128 tiles its 18432 x 3072 (113 MB) took 40.8 us at M = 1 with
-// 576 waves, each holding one k-tile in flight behind a barrier; here 27.4 us
-// (4.1 TB/s), 3072 x 9216 101 -> 19 us.
-// Every wave reads its weights straight into the MFMA's operand registers,
-// without LDS or barriers: a workgroup owns 16 weight rows, its KS waves one K
-// range each, and a wave loads four blocks of 64 k (16 rows x 128 bytes, whole
-// lines) at once; the partial sums meet in LDS and are added in wave order.
-// The activations (L2-resident) are read the same way by every workgroup.
+// M <= 16 (a conditioning vector's Linear, a decoding step): the product is a stream of the
+// weight.  A workgroup owns 16 weight rows, its KS waves one K range each; the
+// partial sums meet in LDS and are added in wave order.  The activations (L2-resident)
+// are read straight into the operands' registers by every workgroup.
 // v_mfma_f32_16x16x32_bf16 with the weights as A: lane l supplies row l % 16,
 // k = 64 b + 16 (l / 16) + 8 s + [0, 8) in step s of block b -- for both
 // operands, so the sum only meets its terms in another order -- and holds
 // C[m = l % 16][n = 4 (l / 16) + i].
-// Q8: 16 codes of one row per lane and block, w = fma(u, d, -128 d) rounded to
-// bf16, the value dt_dequant writes.
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // The adapters of a wave's 16 rows over the KS waves, in parts of one adapter and 32 of its rank,
@@ -1065,6 +1058,7 @@ struct LoraParts {
     int rows, turn, wave, g, a, k;
     int of[N];  // the part's adapter, -2: no part
     bf16x8_t u[N], x[N][2];
+    bool past[N];  // the lane's ranks lie past the last one
 
     __device__ __forceinline__ void start(const LoraTile& l, int& mine, int w, const uint16_t* t_row, const uint16_t* u_row, int lg) {
         if (mine >= l.adapters) mine = -1;
@@ -1090,15 +1084,33 @@ struct LoraParts {
         return false;
     }
     __device__ __forceinline__ void fetch(const LoraTile& l) {
+        const bf16x8_t zero = __builtin_bit_cast(bf16x8_t, make_uint4(0, 0, 0, 0));
+        int at[N], from[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            of[i] = -2;
-            if (next(l)) {
-                of[i] = a;
-                u[i] = lora_up(l, u0 + a * l.u_stride, k + 8 * g);
-                x[i][0] = lora_t(t + k);
-                x[i][1] = lora_t(t + l.rp + k);
+            of[i] = next(l) ? a : -2;
+            if (i == 0 && of[0] < 0) return;
+            // No part: the one before once more (a line that is in the cache), not added.
+            at[i] = of[i] < 0 ? at[i - (i > 0)] : k;
+            from[i] = of[i] < 0 ? from[i - (i > 0)] : a;
+        }
+        if (l.vec) {  // all loads in a row: nothing between them waits
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint16_t* row = u0 + from[i] * l.u_stride;
+                u[i] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(row + min(at[i] + 8 * g, l.rank - 8)));
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) u[i] = lora_up(l, u0 + from[i] * l.u_stride, at[i] + 8 * g);
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            // Of the adapter's own rows: the vector cache looks up every lane that asks.
+            const bool own = rows == of[i];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[i][h] = own ? lora_t(t + h * l.rp + at[i]) : zero;
+            past[i] = at[i] + 8 * g >= l.rank;
         }
     }
     // Adds the parts fetched last; whether there were as many as could be.
@@ -1106,9 +1118,10 @@ struct LoraParts {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (of[i] < 0) return false;
+            const bf16x8_t v = past[i] ? __builtin_bit_cast(bf16x8_t, make_uint4(0, 0, 0, 0)) : u[i];
             f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i][0], d, 0, 0, 0);
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(u[i], x[i][1], d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x[i][0], d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x[i][1], d, 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[e] += mine == of[i] ? d[e] : 0.f;
         }
@@ -1116,7 +1129,9 @@ struct LoraParts {
     }
 };
 
-template <typename TC, bool Q8, int KS, typename L = NoLora, int UNR = 4>  // UNR 64-k blocks loaded together
+// Q8_0 weights: 16 codes of one row per lane and block, w = fma(u, d, -128 d) rounded to bf16, the
+// value dt_dequant writes; UNR blocks of 64 k loaded together, straight into registers.
+template <typename TC, int KS, typename L, int UNR>
 __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, const L lora) {
     constexpr int LD = 16 + 4;  // padded row of the partial sums
     __shared__ float part[KS][16 * LD];
@@ -1134,9 +1149,8 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
     const int b0 = min(wave * per, nblk), b1 = min(b0 + per, nblk);
     const uint16_t* xp = p.A + (int64_t)min(r, p.M - 1) * p.lda + 16 * g;
     const int64_t n = min(n0 + r, p.N - 1);
-    const uint16_t* wp = Q8 ? nullptr : p.B + n * p.ldb + 16 * g;
-    const uint8_t* qp = Q8 ? reinterpret_cast<const uint8_t*>(p.B) + n * p.ldb + 16 * g : nullptr;
-    const float* sp = Q8 ? p.Bs + n + (g >> 1) * p.ldbs : nullptr;
+    const uint8_t* qp = reinterpret_cast<const uint8_t*>(p.B) + n * p.ldb + 16 * g;
+    const float* sp = p.Bs + n + (g >> 1) * p.ldbs;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
 
     // U blocks from block b; meanwhile: what is issued behind their loads.
@@ -1147,34 +1161,27 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int64_t k = (int64_t)(b + u) * 64;
-            if constexpr (Q8) {
-                w[u][0] = ld_stream(qp + k);
-                d[u] = sp[2 * (int64_t)(b + u) * p.ldbs];
-            } else {
-                w[u][0] = ld_stream(wp + k);
-                w[u][1] = ld_stream(wp + k + 8);
-            }
+            w[u][0] = ld_stream(qp + k);
+            d[u] = sp[2 * (int64_t)(b + u) * p.ldbs];
 #pragma unroll
             for (int h = 0; h < 2; ++h) x[u][h] = *reinterpret_cast<const uint4*>(xp + k + 8 * h);
         }
         meanwhile();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if constexpr (Q8) {
-                const float m = -128.0f * d[u];
-                const uint32_t q4[4] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w};
-                uint32_t pk[8];
+            const float m = -128.0f * d[u];
+            const uint32_t q4[4] = {w[u][0].x, w[u][0].y, w[u][0].z, w[u][0].w};
+            uint32_t pk[8];
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    float v[4];
+            for (int h = 0; h < 4; ++h) {
+                float v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)((q4[h] >> (8 * e)) & 0xFFu), d[u], m);
-                    pk[2 * h] = pack_bf16x2(v[0], v[1]);
-                    pk[2 * h + 1] = pack_bf16x2(v[2], v[3]);
-                }
-                w[u][0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-                w[u][1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
+                for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf((float)((q4[h] >> (8 * e)) & 0xFFu), d[u], m);
+                pk[2 * h] = pack_bf16x2(v[0], v[1]);
+                pk[2 * h + 1] = pack_bf16x2(v[2], v[3]);
             }
+            w[u][0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            w[u][1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w[u][h]),
@@ -1217,6 +1224,124 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
         float v = part[0][m * LD + c];
 #pragma unroll
         for (int k = 1; k < KS; ++k) v += part[k][m * LD + c];
+        if (p.bias) v += p.bias[n0 + c];
+        if (Dm) v += load_c(Dm + (int64_t)m * p.ldd + n0 + c);
+        store1<TC>(C + (int64_t)m * p.ldc + n0 + c, v);
+    }
+}
+
+// bf16 weights go through LDS: each wave streams its weights by direct
+// DMA through R blocks of its own, 16 rows of whole 128-byte lines, and reads the operands above
+// from there.  Read straight into the operands' registers, lanes next to each other lie in
+// different rows and the vector cache looks up every lane for itself, 16 bytes a cycle:
+// 10 us of it for 100 MB, and as much for 16 rows of activations.  No barrier before the
+// partial sums: a wave waits for its own loads.
+template <int... S, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, S...>, F f) {
+    (f(std::integral_constant<int, S>{}), ...);
+}
+
+template <typename TC, int KS, typename L, int R>
+__global__ __launch_bounds__(64 * KS) void gemm_stream_kernel(const Group grp, const L lora) {
+    constexpr int LD = 16 + 4, BLOCK = 16 * 128;  // padded row of the partial sums; bytes of a block of 64 k
+    static_assert(16 * LD * 4 <= R * BLOCK, "a wave's partial sums take its blocks' place");
+    __shared__ __attribute__((aligned(16))) uint8_t ring[KS][R * BLOCK];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int pi = 0;
+    while (pi + 1 < grp.count && (int)blockIdx.x >= grp.tile_start[pi + 1]) ++pi;
+    const Problem& p = grp.p[pi];
+    const int n0 = ((int)blockIdx.x - grp.tile_start[pi]) * 16;
+    const int r = lane & 15, g = lane >> 4;
+    int mine = -1;  // the adapter of row r, read ahead of the weights
+    if constexpr (L::on) mine = r < p.M ? lora.row_adapter[r] : -1;
+
+    const int nblk = p.K / 64, per = (nblk + KS - 1) / KS;
+    const int b0 = min(wave * per, nblk), b1 = min(b0 + per, nblk);
+    const uint16_t* xp = p.A + (int64_t)min(r, p.M - 1) * p.lda + 16 * g;
+    // Instruction j covers rows 8 j .. + 7, lane i chunk i % 8 of row i / 8 at place chunk ^ (row & 7).
+    const int chunk = (lane & 7) ^ (lane >> 3);
+    const uint16_t* wp[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) wp[j] = p.B + (int64_t)min(n0 + 8 * j + (lane >> 3), p.N - 1) * p.ldb + 8 * chunk;
+    uint8_t* const mem = ring[wave];
+    const uint8_t* const at[2] = {mem + r * 128 + (((2 * g) ^ (r & 7)) << 4), mem + r * 128 + (((2 * g + 1) ^ (r & 7)) << 4)};
+    uint4 x[R][2];
+    auto issue = [&](int b, int s) {
+        const int64_t k = (int64_t)b * 64;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            __builtin_amdgcn_global_load_lds(wp[j] + k, mem + s * BLOCK + 1024 * j, 16, 0, 2);  // nt
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[s][h] = *reinterpret_cast<const uint4*>(xp + k + 8 * h);
+    };
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    // Behind the wait for the block's loads: those issued later are `after` blocks, four loads each.
+    auto block = [&](int s, auto after) {
+        constexpr int N = 4 * decltype(after)::value;
+        __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8_t w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = *reinterpret_cast<const bf16x8_t*>(at[h] + s * BLOCK);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[h], __builtin_bit_cast(bf16x8_t, x[s][h]), acc, 0, 0, 0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the block is read
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using After = std::integral_constant<int, R - 1>;
+    using None = std::integral_constant<int, 0>;
+    LoraParts<KS> parts;
+    auto start = [&]() {  // the adapters' first parts
+        if constexpr (L::on) {
+            const int64_t n = min(n0 + r, p.N - 1);
+            parts.start(lora, mine, wave, lora.t + (int64_t)min(r, p.M - 1) * 2 * lora.rp + 8 * g, lora.u + n * lora.ldu, g);
+            parts.fetch(lora);
+        }
+    };
+    int b = b0;
+    if (b + R <= b1) {
+#pragma unroll
+        for (int s = 0; s < R; ++s) issue(b + s, s);
+        if constexpr (R != 3) start();  // behind the weights' loads: registers to spare
+        for (; b + 2 * R <= b1; b += R) {
+#pragma unroll
+            for (int s = 0; s < R; ++s) {
+                block(s, After{});
+                issue(b + R + s, s);
+            }
+        }
+        const int more = b1 - b - R;  // below R
+        each_of(std::make_integer_sequence<int, R>{}, [&](auto s) {
+            block(s, std::integral_constant<int, R - 1 - s>{});
+            if (s < more) issue(b + R + s, s);
+        });
+        b += R;
+    } else {
+#pragma unroll
+        for (int s = 0; s < R; ++s)
+            if (b + s < b1) issue(b + s, s);
+        if constexpr (R != 3) start();
+    }
+#pragma unroll
+    for (int s = 0; s < R; ++s)
+        if (b + s < b1) block(s, None{});
+    if constexpr (L::on) {
+        if constexpr (R == 3) start();
+        while (parts.add(mine, acc)) parts.fetch(lora);
+    }
+    float* const part = reinterpret_cast<float*>(mem);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[r * LD + 4 * g + e] = acc[e];
+    __syncthreads();
+    TC* C = reinterpret_cast<TC*>(p.C);
+    const TC* Dm = reinterpret_cast<const TC*>(p.D);
+    for (int u = tid; u < 16 * 16; u += 64 * KS) {
+        const int m = u >> 4, c = u & 15;
+        if (m >= p.M || n0 + c >= p.N) continue;
+        const float* sum = reinterpret_cast<const float*>(ring[0]) + m * LD + c;
+        float v = sum[0];
+#pragma unroll
+        for (int k = 1; k < KS; ++k) v += sum[k * (R * BLOCK / 4)];
         if (p.bias) v += p.bias[n0 + c];
         if (Dm) v += load_c(Dm + (int64_t)m * p.ldd + n0 + c);
         store1<TC>(C + (int64_t)m * p.ldc + n0 + c, v);
@@ -1434,12 +1559,17 @@ int launch_skinny(const Problem* ps, int n, const L& lora, hipStream_t st) {
     DT_REQUIRE(total < (1ll << 31), "dt_gemm_bf16: too many tiles");
     g.tile_start[n] = (int)total;
     // Eight waves a workgroup until there are four workgroups per CU.
-    if (total >= 4 * cu_count())
-        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 4, L>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
-    else if (L::on && total <= cu_count())
-        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8, L, L::on ? 8 : 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
-    else
-        hipLaunchKernelGGL((gemm_skinny_kernel<TC, Q8, 8, L>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
+    const bool four = total >= 4 * cu_count();
+    if constexpr (Q8) {
+        if (four) hipLaunchKernelGGL((gemm_skinny_kernel<TC, 4, L, 4>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
+        else if (L::on && total <= cu_count())
+            hipLaunchKernelGGL((gemm_skinny_kernel<TC, 8, L, L::on ? 8 : 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
+        else hipLaunchKernelGGL((gemm_skinny_kernel<TC, 8, L, 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
+    } else {
+        if (four) hipLaunchKernelGGL((gemm_stream_kernel<TC, 4, L, 3>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
+        else if (total <= cu_count()) hipLaunchKernelGGL((gemm_stream_kernel<TC, 8, L, 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
+        else hipLaunchKernelGGL((gemm_stream_kernel<TC, 8, L, 3>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
+    }
     return check_launch("dt_gemm_bf16");
 }
 

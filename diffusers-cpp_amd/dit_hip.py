@@ -533,6 +533,15 @@ def _scratch(nbytes, device):
     return ws
 
 
+def _scratch_by(t, nbytes):
+    """_scratch where t is."""
+    ws = t.new_empty(nbytes, dtype=_TORCH.uint8)
+    lib = load()
+    if isinstance(lib, _Recorder):
+        lib.keep.append(ws)
+    return ws
+
+
 def _gemm_ws(nbytes, M, N, K, a):
     """Scratch for a product taken over ranges of K, or None for one that is not split."""
     n = nbytes(M, N, K)
@@ -856,7 +865,7 @@ def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dty
     codes, scales = (w.codes, w.scales) if q8 else (w, None)
     a, b, scale = lora.a, lora.b, lora.scale
     if out is None:
-        out = torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype or torch.bfloat16, device=x.device)
+        out = x.new_empty((x.shape[0], w.shape[0]), dtype=out_dtype or torch.bfloat16)
     p, s, nbytes, out_type = _lora_plan(_meta(x), _meta(codes), _meta(scales), _meta(a), _meta(b), _meta(scale),
                                         _meta(row_adapter), _meta(bias), _meta(addend), _meta(out),
                                         torch.cuda.current_device())
@@ -871,7 +880,7 @@ def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dty
         p.b_scale = scales.data_ptr()
     if scale is not None:
         s.scale = scale.data_ptr()
-    ws = _scratch(nbytes, x.device) if nbytes else None
+    ws = _scratch_by(x, nbytes) if nbytes else None
     lib = load()
     check(lib.dt_lora_gemm(ctypes.addressof(p), ctypes.addressof(s), out_type, None if ws is None else ws.data_ptr(),
                            nbytes, stream()), "dt_lora_gemm")
@@ -976,11 +985,11 @@ def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out):
 def _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse):
     torch = _torch()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     a, n, _, o_strides = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out)
-    lse = torch.empty((a.batch, a.heads, a.seq_q), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((a.batch, a.heads, a.seq_q), dtype=torch.float32) if return_lse else None
     lib = load()
-    ws = _scratch(n, q.device) if n else None
+    ws = _scratch_by(q, n) if n else None
     check(lib.dt_attn_fwd(ctypes.addressof(a), out.data_ptr(), o_strides, None if lse is None else lse.data_ptr(),
                           None if ws is None else ws.data_ptr(), n, stream()), "dt_attn_fwd")
     if isinstance(lib, _Recorder):
@@ -1010,18 +1019,15 @@ def _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos):
     a, _, n, _ = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, o)
     y = AttnGrads.from_buffer_copy(_grads_plan(_meta(q), _meta(d_o), _meta(o), _meta(lse), _meta(k),
                                                torch.cuda.current_device()))
-    dtype, device = q.dtype, q.device
-    dq = torch.empty(q.shape, dtype=dtype, device=device)
-    dk = torch.empty(k.shape, dtype=dtype, device=device)
-    dv = torch.empty(k.shape, dtype=dtype, device=device)
+    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
     y.d_o, y.o, y.lse = d_o.data_ptr(), o.data_ptr(), lse.data_ptr()
     y.dq, y.dk, y.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     dt = None
     if rel is not None:
-        dt = torch.empty(rel.table.shape, dtype=torch.float32, device=device)
+        dt = rel.table.new_empty(rel.table.shape)
         y.d_rel_table = dt.data_ptr()
     lib = load()
-    ws = _scratch(n, device) if n else None
+    ws = _scratch_by(q, n) if n else None
     check(lib.dt_attn_bwd(ctypes.addressof(a), ctypes.addressof(y), None if ws is None else ws.data_ptr(), n, stream()), "dt_attn_bwd")
     if isinstance(lib, _Recorder):
         lib.keep.extend((a, y))

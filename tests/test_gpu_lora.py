@@ -81,6 +81,19 @@ SHAPES = [(1, 128, 64, 16, 1), (1, 4096, 1024, 8, 3), (5, 2048, 576, 64, 40), (1
           (700, 2304, 512, 96, 5), (1030, 4096, 128, 512, 2), (2100, 2500, 192, 12, 6)]
 
 
+# A stream of the weight: waves with no block of 64 k, fewer and more than they hold, uneven ends;
+# four and eight waves; ranks in one and several parts, more adapters than waves.
+@pytest.mark.parametrize("M,N,K,R,n", [(3, 200, 5184, 40, 2), (16, 130, 64, 16, 20), (2, 4096, 8192, 100, 1), (16, 8200, 4160, 64, 12),
+                                       (9, 5000, 1536, 33, 9), (7, 16500, 1216, 8, 3), (16, 16384, 2624, 200, 16)])
+def test_few_rows(M, N, K, R, n):
+    x, w, lora = case(121, M, N, K, R, n)
+    rows = (torch.arange(M, dtype=torch.int32, device="cuda") * 5 + 1) % (n + 1) - int(M > 4)
+    hold(dh.lora_gemm(x, w, lora, rows), x, w, lora, rows)
+    none = torch.full_like(rows, -7)
+    assert torch.equal(dh.lora_gemm(x, w, lora, none), dh.gemm(x, w))
+    hold(dh.gemm(x, w), x, w, lora, none)
+
+
 @pytest.mark.parametrize("how", ["one", "mixed", "requests"])
 @pytest.mark.parametrize("M,N,K,R,n", SHAPES)
 def test_adapters_beside_bf16_weights(M, N, K, R, n, how):
