@@ -165,8 +165,8 @@ __device__ __forceinline__ void epilogue(const Problem& p, const f32x16_t (&acc)
 // C[m, n] += sum_r T[m, r] U_a[n, r], a = adapter of row m: T = scale (A A_a^T) from
 // lora_down_kernel (lora.hip), U_a the adapter's up weights.  A tile's accumulators
 // start from it instead of 0, so the sum is rounded once, and its operands load
-// beside the first stages' (after the last k-step they found no registers, and each
-// tile waited for them: 4608 x 12288 x 4096 503-559 us instead of 420).  T is held
+// beside the first stages' (after the last k-step they found no registers, and each tile waited for
+// them: 4608 x 12288 x 4096, rank 32, 559 us instead of 500; 485 without adapters).  T is held
 // as two bf16 parts (16 significant bits), each a product of its own: beside K of
 // some thousands the second costs nothing that shows, and an fp32 C keeps its accuracy.
 // NoLora leaves a kernel as it is without.
@@ -1040,7 +1040,8 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
 // M <= 16 (a conditioning vector's Linear, a decoding step): the product is a stream of the
 // weight.  A workgroup owns 16 weight rows, its KS waves one K range each; the
 // partial sums meet in LDS and are added in wave order.  The activations (L2-resident)
-// are read straight into the operands' registers by every workgroup.
+// are read straight into the operands' registers by every workgroup.  18432 x 3072 (113 MB)
+// at M = 1: 40.8 us with 128 x 128 tiles, 19.2 us here (5.9 TB/s).
 // v_mfma_f32_16x16x32_bf16 with the weights as A: lane l supplies row l % 16,
 // k = 64 b + 16 (l / 16) + 8 s + [0, 8) in step s of block b -- for both
 // operands, so the sum only meets its terms in another order -- and holds
@@ -1130,7 +1131,8 @@ struct LoraParts {
 };
 
 // Q8_0 weights: 16 codes of one row per lane and block, w = fma(u, d, -128 d) rounded to bf16, the
-// value dt_dequant writes; UNR blocks of 64 k loaded together, straight into registers.
+// value dt_dequant writes; UNR blocks of 64 k loaded together, straight into registers: four, or
+// with adapters and at most one workgroup per CU eight (3072 x 9216, M = 1: 24.3 -> 21.0 us).
 template <typename TC, int KS, typename L, int UNR>
 __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, const L lora) {
     constexpr int LD = 16 + 4;  // padded row of the partial sums
@@ -1233,9 +1235,13 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 // bf16 weights go through LDS: each wave streams its weights by direct
 // DMA through R blocks of its own, 16 rows of whole 128-byte lines, and reads the operands above
 // from there.  Read straight into the operands' registers, lanes next to each other lie in
-// different rows and the vector cache looks up every lane for itself, 16 bytes a cycle:
-// 10 us of it for 100 MB, and as much for 16 rows of activations.  No barrier before the
-// partial sums: a wave waits for its own loads.
+// different rows and the vector cache looks up every lane for itself, 16 bytes a cycle
+// (12288 x 4096: 20.5 us at M = 1, 28.5 us at M = 16; so 16.5 and 21.7).  The activations still
+// are: through LDS too they take the weights' room (M = 16: 19.8 us, M = 8: 17.4 -> 19.8), and 32
+// weight rows a workgroup for one read of them leave it half as many waves (25.0 us).  No barrier
+// before the partial sums: a wave waits for its own loads.  R = 3 blocks let three workgroups of
+// eight waves share a CU; with at most one there, R = 4 and the adapters' first parts
+// behind them (4096 x 4096, M = 1: 8.5 -> 7.8 us).
 template <int... S, typename F>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, S...>, F f) {
     (f(std::integral_constant<int, S>{}), ...);
@@ -1444,7 +1450,7 @@ struct Config {
 // staged; 8, 9: configs 5 and 7 in eight waves of 128 x 64 (two per SIMD).
 // Chosen by size only, not by callers: 10: 128 x 128 in two k-groups (the rate puts it
 // below config 1's pair of tiles per CU only while one round of it holds every
-// tile); 11: few rows (gemm_skinny_kernel, which has no tiles and no row here).
+// tile); 11: few rows (gemm_stream_kernel, Q8_0 gemm_skinny_kernel, which has no tiles and no row here).
 constexpr int kAnyConfig = 4, kLastConfig = 9;
 constexpr int kSplitConfig = 10, kSkinnyConfig = 11;
 // Rows up to which the weight stream wins (Python call included, bf16 / Q8_0; the

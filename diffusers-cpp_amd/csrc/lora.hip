@@ -1,13 +1,13 @@
 // lora.hip -- the down projection of dt_lora_gemm: T[m, r] = scale_a sum_k x[m, k]
-// A_a[r, k], a = adapter of row m, as two bf16 parts for the product's epilogue
-// (lora_add in gemm.hip).
+// A_a[r, k], a = adapter of row m, as two bf16 parts for the product's
+// kernels (gemm.hip).
 //
 // A stream of x and of the used adapters with next to no arithmetic.  A workgroup takes 16
-// rows and 32 ranks; its waves take every NW-th 64 k and meet in LDS, in wave order.  Each
-// streams its 16 x 64 of x and 32 x 64 of the adapter through LDS buffers of its own by
+// or 32 rows and 32 ranks; its waves take every NW-th 64 k and meet in LDS, in wave order.  Each
+// streams its rows x 64 of x and 32 x 64 of the adapter through LDS buffers of its own by
 // direct DMA, whole 128-byte lines of a row side by side: read straight into the MFMA's
 // registers, lanes next to each other lie in different rows, and the vector cache
-// looks up every lane for itself, 16 bytes a cycle (4608 rows x 4096, rank 32: 27 us).
+// looks up every lane for itself, 16 bytes a cycle (4608 rows x 4096, rank 32: 27 us; so 16.5).
 // The adapters of the 16 rows are found by ballot and taken one after another, or,
 // when there are few rows, by workgroups of their own.
 #include "capi_util.hpp"
@@ -43,7 +43,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
 }
 
 constexpr int kRanks = 32;  // of a workgroup
-constexpr int kLine = 64;               // k a wave takes at a time
+constexpr int kLine = 64;   // k a wave takes at a time
 
 struct Out {  // a thread's element of T: row tid / 32, rank tid % 32
     const DownArgs& p;
