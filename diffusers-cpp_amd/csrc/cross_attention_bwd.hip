@@ -673,6 +673,12 @@ Plan plan(const AttnIn& in, bool bf16_io, int buckets, int cus) {
     int64_t most = (int64_t)((in.seq_q + 127) / 128) * in.shared;
     if (most > 16) most = 16;
     p.key_high = tall * most >= cus ? 128 : 32;
+    // bf16 with up to 2048 queries whose 32-key blocks give half the CUs a workgroup: those, with no
+    // ranges to join (16 heads x 4 batch entries, 64 wide, bwd: 1024 queries, 77 keys
+    // 28.2 -> 25.1 us; 2048, 512 keys, one entry 42.8 -> 35.4; 2048, 77 keys 44.8 -> 45.8; 4096, 77
+    // keys would be 72.1 -> 81.2: the four waves' query tiles are four times the loads).
+    const int64_t narrow = (int64_t)((in.seq_kv + 31) / 32) * keys;
+    if (bf16_io && (int64_t)in.seq_q * in.shared <= 2048 && tall * 2 <= cus && narrow * 2 >= cus) p.key_high = 32;
     p.key_blocks = (in.seq_kv + p.key_high - 1) / p.key_high;
     const int64_t blocks = p.key_blocks * keys;
     int64_t s = blocks > 0 ? cus / blocks : 1;
