@@ -962,11 +962,7 @@ def _attn_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, out,
     return bytes(a), *sizes, _i64x3(*out[2][:3])
 
 
-def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out):
-    table = None if rel is None else rel.table
-    plan, fwd, bwd, o_strides = _attn_plan(_meta(q), _meta(k), _meta(v), _meta(kv_len), _meta(kv_mask), _meta(table), _meta(q_pos),
-                      None if rel is None else rel.distance, None if rel is None else rel.two_sided, _meta(out),
-                      _torch().cuda.current_device())
+def _attn_pointers(plan, q, k, v, kv_len, kv_mask, scale, rel, q_pos):
     a = AttnArgs.from_buffer_copy(plan)
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
     if scale is not None:
@@ -975,19 +971,25 @@ def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out):
         a.kv_len = kv_len.data_ptr()
     if kv_mask is not None:
         a.kv_mask = kv_mask.data_ptr()
-    if table is not None:
-        a.rel_table = table.data_ptr()
+    if rel is not None:
+        a.rel_table = rel.table.data_ptr()
         if q_pos is not None:
             a.q_pos = q_pos.data_ptr()
-    return a, fwd, bwd, o_strides
+    return a
+
+
+def _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out):
+    plan, fwd, bwd, o_strides = _attn_plan(
+        _meta(q), _meta(k), _meta(v), _meta(kv_len), _meta(kv_mask), None if rel is None else _meta(rel.table), _meta(q_pos),
+        None if rel is None else rel.distance, None if rel is None else rel.two_sided, _meta(out), _torch().cuda.current_device())
+    return _attn_pointers(plan, q, k, v, kv_len, kv_mask, scale, rel, q_pos), fwd, bwd, o_strides
 
 
 def _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse):
-    torch = _torch()
     if out is None:
         out = q.new_empty(q.shape)
     a, n, _, o_strides = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out)
-    lse = q.new_empty((a.batch, a.heads, a.seq_q), dtype=torch.float32) if return_lse else None
+    lse = q.new_empty((a.batch, a.heads, a.seq_q), dtype=_TORCH.float32) if return_lse else None
     lib = load()
     ws = _scratch_by(q, n) if n else None
     check(lib.dt_attn_fwd(ctypes.addressof(a), out.data_ptr(), o_strides, None if lse is None else lse.data_ptr(),
@@ -998,10 +1000,10 @@ def _attn(q, k, v, kv_len, kv_mask, scale, rel, q_pos, out, return_lse):
 
 
 @functools.lru_cache(maxsize=512)
-def _grads_plan(q, d_o, o, lse, k, here):
-    for m, name in ((d_o, "d_o"), (o, "o")):
-        if m[1] != q[1] or m[0] != q[0] or m[2][3] != 1:
-            raise DtError(f"{name} must have q's shape and dtype, its head dim contiguous")
+def _grads_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, o, d_o, lse, here):
+    if o[1] != q[1] or o[0] != q[0] or o[2][3] != 1 or d_o[1] != q[1] or d_o[0] != q[0] or d_o[2][3] != 1:
+        raise DtError("o and d_o must have q's shape and dtype, their head dim contiguous")
+    plan, _, bwd, _ = _attn_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, o, here)
     B, Sq, H, D = q[1]
     if lse[0] != _torch().float32 or lse[1] != (B, H, Sq) or lse[2] != (H * Sq, Sq, 1) and 0 not in lse[1]:
         raise DtError("lse must be the forward pass's: contiguous fp32 [B, H, Sq]")
@@ -1011,14 +1013,15 @@ def _grads_plan(q, d_o, o, lse, k, here):
     y.dq_strides[:] = (Sq * H * D, H * D, D)
     y.dk_strides[:] = y.dv_strides[:] = (k[1][1] * k[1][2] * D, k[1][2] * D, D)
     y.d_rel_table_stride = H
-    return bytes(y)
+    return plan, bytes(y), bwd
 
 
 def _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos):
-    torch = _torch()
-    a, _, n, _ = _attn_args(q, k, v, kv_len, kv_mask, scale, rel, q_pos, o)
-    y = AttnGrads.from_buffer_copy(_grads_plan(_meta(q), _meta(d_o), _meta(o), _meta(lse), _meta(k),
-                                               torch.cuda.current_device()))
+    plan, grads, n = _grads_plan(
+        _meta(q), _meta(k), _meta(v), _meta(kv_len), _meta(kv_mask), None if rel is None else _meta(rel.table), _meta(q_pos),
+        None if rel is None else rel.distance, None if rel is None else rel.two_sided, _meta(o), _meta(d_o), _meta(lse),
+        _torch().cuda.current_device())
+    a, y = _attn_pointers(plan, q, k, v, kv_len, kv_mask, scale, rel, q_pos), AttnGrads.from_buffer_copy(grads)
     dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(k.shape)
     y.d_o, y.o, y.lse = d_o.data_ptr(), o.data_ptr(), lse.data_ptr()
     y.dq, y.dk, y.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
