@@ -338,13 +338,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attn_few_kernel(c
 #pragma unroll
         for (int c = 0; c < Tl::STEPS; ++c) qf[c] = live ? frag_global<T>(qp, c, g, in.dim) : frag_zero<T>();
     }
-    if constexpr (BIAS) {
-        rel_line(in.rel, h0, line, tid, 256);
-        wait_lds();  // not __syncthreads: K's DMA stays in flight
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-    }
     if (t >= 0) issue(vl, Vp, in.vs[1], t, word, Vt);
+    if constexpr (BIAS) {  // its loads behind the first tile's
+        rel_line(in.rel, h0, line, tid, 256);
+        __syncthreads();
+    }
     const typename Tl::Cols cols = Tl::cols(lane);
     Running<T, Tl::BLOCKS> run;
     run.clear();
