@@ -3,8 +3,8 @@
 // kernels (gemm.hip).
 //
 // A stream of x and of the used adapters with next to no arithmetic.  A workgroup takes 16
-// or 32 rows and 32 ranks; its waves take every NW-th 64 k and meet in LDS, in wave order.  Each
-// streams its rows x 64 of x and 32 x 64 of the adapter through LDS buffers of its own by
+// or 32 rows and 16 or 32 ranks; its waves take every NW-th 64 k and meet in LDS, in wave order.  Each
+// streams its rows and ranks x 64 of x and of the adapter through LDS buffers of its own by
 // direct DMA, whole 128-byte lines of a row side by side: read straight into the MFMA's
 // registers, lanes next to each other lie in different rows, and the vector cache
 // looks up every lane for itself, 16 bytes a cycle (4608 rows x 4096, rank 32: 27 us; so 16.5).
@@ -42,10 +42,9 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, int k, int K) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int kRanks = 32;  // of a workgroup
 constexpr int kLine = 64;   // k a wave takes at a time
 
-struct Out {  // a thread's element of T: row tid / 32, rank tid % 32
+struct Out {  // a thread's element of T: row tid / RANKS, rank tid % RANKS
     const DownArgs& p;
     int m, rank, theirs;
     __device__ __forceinline__ void put(float v) const {
@@ -68,26 +67,26 @@ __device__ __forceinline__ void down_dma(const void* base, uint32_t off, uint8_t
 }
 
 // VEC: rows in whole 16-byte chunks, through LDS.  Else element by element, for any layout.
-template <bool VEC, int ROWS, int NW, int NB>
+template <bool VEC, int ROWS, int NW, int NB, int RANKS>
 __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
-    constexpr int ROWB = kLine * 2, BUF = (ROWS + kRanks) * ROWB, RF = ROWS / 16;  // NB buffers of a wave
-    constexpr int DMAS = BUF / 1024, PARTB = NW * ROWS * (kRanks + 1) * 4;
+    constexpr int ROWB = kLine * 2, BUF = (ROWS + RANKS) * ROWB, RF = ROWS / 16, AF = RANKS / 16;  // NB buffers of a wave
+    constexpr int DMAS = BUF / 1024, PARTB = NW * ROWS * (RANKS + 1) * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[VEC && NW * NB * BUF > PARTB ? NW * NB * BUF : PARTB];
-    float(*const part)[ROWS][kRanks + 1] = reinterpret_cast<float(*)[ROWS][kRanks + 1]>(smem);
+    float(*const part)[ROWS][RANKS + 1] = reinterpret_cast<float(*)[ROWS][RANKS + 1]>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    const int m0 = blockIdx.x * ROWS, r0 = blockIdx.y * kRanks, slot = blockIdx.z;
+    const int m0 = blockIdx.x * ROWS, r0 = blockIdx.y * RANKS, slot = blockIdx.z;
     // Lane i < ROWS has row i's adapter.
     int mine = lane < ROWS && m0 + lane < p.M ? p.row_adapter[m0 + lane] : -1;
     if (mine >= p.adapters) mine = -1;
     const int lines = (p.K + kLine - 1) / kLine;
-    constexpr int OUTS = ROWS / (2 * NW) > 1 ? ROWS / (2 * NW) : 1;  // elements of T a thread has
+    constexpr int STEP = 64 * NW / RANKS, OUTS = ROWS / STEP > 1 ? ROWS / STEP : 1;  // elements of T a thread has
     auto each_out = [&](auto f) {
 #pragma unroll
         for (int o = 0; o < OUTS; ++o) {
-            const int row = (tid >> 5) + 2 * NW * o;
+            const int row = tid / RANKS + STEP * o;
             const int theirs = __shfl(mine, row & (ROWS - 1));
-            if (row < ROWS && m0 + row < p.M) f(Out{p, m0 + row, r0 + (tid & 31), theirs}, row);
+            if (row < ROWS && m0 + row < p.M) f(Out{p, m0 + row, r0 + tid % RANKS, theirs}, row);
         }
     };
     if (slot == 0)
@@ -101,14 +100,16 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
         const uint64_t of = __builtin_amdgcn_ballot_w64(mine == a);
         left &= ~of;
         if (turn % p.slots != slot) continue;
-        f32x4_t acc[RF][2];
+        f32x4_t acc[RF][AF];
 #pragma unroll
-        for (int f = 0; f < RF; ++f) acc[f][0] = acc[f][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        auto multiply = [&](const uint4 (&v)[RF + 2]) {  // 16 rows of x each, then 16 of the adapter each
+        for (int f = 0; f < RF; ++f)
+#pragma unroll
+            for (int h = 0; h < AF; ++h) acc[f][h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        auto multiply = [&](const uint4 (&v)[RF + AF]) {  // 16 rows of x each, then 16 of the adapter each
 #pragma unroll
             for (int f = 0; f < RF; ++f)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < AF; ++h)
                     acc[f][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v[RF + h]),
                                                                         __builtin_bit_cast(bf16x8_t, v[f]), acc[f][h], 0, 0, 0);
         };
@@ -141,11 +142,11 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
                 __builtin_amdgcn_s_waitcnt(((NB - 1) * DMAS & 15) | (((NB - 1) * DMAS >> 4) << 14) | 0x0F70);
                 __builtin_amdgcn_sched_barrier(0);
                 const uint8_t* t = mem + buf * BUF;
-                uint4 v[2][RF + 2];
+                uint4 v[2][RF + AF];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int h = 0; h < RF + 2; ++h)
+                    for (int h = 0; h < RF + AF; ++h)
                         v[s][h] = *reinterpret_cast<const uint4*>(t + (16 * h + r) * ROWB + (((4 * s + g) ^ (r & 7)) << 4));
 #pragma unroll
                 for (int s = 0; s < 2; ++s) multiply(v[s]);
@@ -155,17 +156,17 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
             }
             __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the DMA past the end is in LDS before it is used again
         } else {
-            const uint16_t* row[RF + 2];
+            const uint16_t* row[RF + AF];
 #pragma unroll
-            for (int h = 0; h < RF + 2; ++h)
+            for (int h = 0; h < RF + AF; ++h)
                 row[h] = h < RF ? p.x + (int64_t)min(m0 + 16 * h + r, p.M - 1) * p.ldx
                                 : p.a + a * p.a_stride + (int64_t)min(r0 + 16 * (h - RF) + r, p.rank - 1) * p.lda;
             for (int line = wave; line < lines; line += NW)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    uint4 v[RF + 2];
+                    uint4 v[RF + AF];
 #pragma unroll
-                    for (int h = 0; h < RF + 2; ++h) v[h] = load8(row[h], line * kLine + 32 * s + 8 * g, p.K);
+                    for (int h = 0; h < RF + AF; ++h) v[h] = load8(row[h], line * kLine + 32 * s + 8 * g, p.K);
                     multiply(v);
                 }
         }
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
 #pragma unroll
         for (int f = 0; f < RF; ++f)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < AF; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) part[wave][16 * f + r][16 * h + 4 * g + i] = acc[f][h][i];
         __syncthreads();
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
             if (o.theirs != a) return;
             float v = 0.f;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) v += part[w][row][tid & 31];
+            for (int w = 0; w < NW; ++w) v += part[w][row][tid % RANKS];
             if (o.rank >= p.rank) v = 0.f;
             o.put(p.scale ? v * p.scale[a] : v);
         });
@@ -206,23 +207,26 @@ int lora_down(const uint16_t* x, int64_t ldx, int64_t M, int64_t K, const dt_lor
     p.adapters = (int)l.adapters;
     p.rank = (int)l.rank;
     p.rp = (int)lora_rank_padded(l.rank);
+    // Rows in whole chunks, a tile's within 2^31 bytes.
+    const bool vec = K % 8 == 0 && ldx % 8 == 0 && l.lda % 8 == 0 && (l.a_stride % 8 == 0 || l.adapters == 1) &&
+                     aligned16(x) && aligned16(l.a) && ldx < (1 << 25) && l.lda < (1 << 25);
     // 16 rows a workgroup while that gives each CU one at most, else 32: the adapter is read
-    // again for every workgroup.
-    const int64_t blocks = p.rp / kRanks;
-    const bool small = (M + 15) / 16 * blocks <= cu_count();
-    const int64_t high = small ? 16 : 32, tiles = (M + high - 1) / high;
+    // again for every workgroup.  While 16 rows x 16 ranks give half the CUs one at most, those, by
+    // sixteen waves (K 4096, cold: 16 rows with 16 adapters of rank 64 11.8 -> 8.8 us, one row 8.5 -> 6.0;
+    // 1628 rows x 2560 would be 7.2 -> 8.6: x is read again for every 16 ranks).
+    const int64_t few = (M + 15) / 16;
+    const bool small = vec && few * (p.rp / 32) <= cu_count(), tiny = vec && few * (p.rp / 16) * 2 <= cu_count();
+    const int64_t high = small ? 16 : 32, tiles = (M + high - 1) / high, blocks = p.rp / (tiny ? 16 : 32);
     // Adapters of a tile side by side until the chip is full: at most one for each of its rows.
     int64_t slots = cu_count() / (tiles * blocks);
     const int64_t rows = M < high ? M : high, most = l.adapters < rows ? l.adapters : rows;
     slots = slots < 1 ? 1 : slots < most ? slots : most;
     p.slots = (int)slots;
-    // Rows in whole chunks, a tile's within 2^31 bytes.
-    const bool vec = K % 8 == 0 && ldx % 8 == 0 && l.lda % 8 == 0 && (l.a_stride % 8 == 0 || l.adapters == 1) &&
-                     aligned16(x) && aligned16(l.a) && ldx < (1 << 25) && l.lda < (1 << 25);
     const dim3 grid((unsigned)tiles, (unsigned)blocks, (unsigned)slots);
-    if (!vec) hipLaunchKernelGGL((lora_down_kernel<false, 32, 8, 1>), dim3((unsigned)((M + 31) / 32), (unsigned)blocks, (unsigned)slots), dim3(512), 0, st, p);
-    else if (small) hipLaunchKernelGGL((lora_down_kernel<true, 16, 8, 3>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((lora_down_kernel<true, 32, 8, 2>), grid, dim3(64 * 8), 0, st, p);
+    if (!vec) hipLaunchKernelGGL((lora_down_kernel<false, 32, 8, 1, 32>), grid, dim3(512), 0, st, p);
+    else if (tiny) hipLaunchKernelGGL((lora_down_kernel<true, 16, 16, 2, 16>), grid, dim3(1024), 0, st, p);
+    else if (small) hipLaunchKernelGGL((lora_down_kernel<true, 16, 8, 3, 32>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((lora_down_kernel<true, 32, 8, 2, 32>), grid, dim3(512), 0, st, p);
     return check_launch("dt_lora_gemm");
 }
 
