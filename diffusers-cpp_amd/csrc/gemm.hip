@@ -102,7 +102,7 @@ __device__ __forceinline__ void store1<bf16>(bf16* p, float v) { p->bits = (uint
 // per XCD, which is kept when the count per XCD is not a multiple of 4.
 // Then GROUP_M-row groups inside the problem.
 template <int BM, int BN>
-__device__ __forceinline__ const Problem& locate(const Group& g, int* tm, int* tn) {
+__device__ __forceinline__ const Problem& locate(const Group& g, int* tm, int* tn, int* which = nullptr) {
     uint32_t bid = blockIdx.x;
     const uint32_t nb = gridDim.x, q = nb >> 3;
     if (bid < (q << 3)) {
@@ -111,6 +111,7 @@ __device__ __forceinline__ const Problem& locate(const Group& g, int* tm, int* t
     }
     int pi = 0;
     while (pi + 1 < g.count && (int)bid >= g.tile_start[pi + 1]) ++pi;
+    if (which) *which = pi;
     const Problem& p = g.p[pi];
     const int local = (int)bid - g.tile_start[pi];
     const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
@@ -199,21 +200,25 @@ __device__ __forceinline__ bf16x8_t lora_t(const uint16_t* p) {
     return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(p));
 }
 
-// The adapter of each of this lane's rows (-1: none), read before the product's k-loop.
+// The adapter of each of this lane's rows (-1: none), read before the product's k-loop.  Where
+// several workgroups or wave groups sum parts of one tile, each takes a share of the adapters, by
+// their number alone (64 rows x 4096 x 4096 with 64 adapters of rank 16: 78 us with all of them
+// in the first, one part after another, 29 so and with two parts fetched together).
 template <int FM>
-__device__ __forceinline__ void lora_rows(const LoraTile& l, const Problem& p, int mw, int lane, int (&mine)[FM]) {
+__device__ __forceinline__ void lora_rows(const LoraTile& l, const Problem& p, int mw, int lane, int (&mine)[FM],
+                                          uint32_t share = 0, uint32_t shares = 1) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         const int m = mw + 32 * i + (lane & 31);
         const int a = m < p.M ? l.row_adapter[m] : -1;
-        mine[i] = a >= 0 && a < l.adapters ? a : -1;
+        mine[i] = a >= 0 && a < l.adapters && (uint32_t)a % shares == share ? a : -1;
     }
 }
 
 // The wave's FM x FN blocks of 32 x 32, which hold zeros.  Rows that all share an adapter:
 // the operands of 32 ranks at once.  Else block by block, an adapter at a time, each
 // kept in its own rows alone: what an adapter holds reaches no other request's rows.
-template <int FM, int FN>
+template <int FM, int FN, int PARTS = 1>
 __device__ __forceinline__ void lora_start(const LoraTile& l, const Problem& p, f32x16_t (&acc)[FN][FM],
                                            const int (&mine)[FM], int mw, int nw, int lane) {
     const int lrow = lane & 31, g = lane >> 5;
@@ -257,40 +262,84 @@ __device__ __forceinline__ void lora_start(const LoraTile& l, const Problem& p, 
         }
         return;
     }
+    constexpr int N = PARTS;  // parts of an adapter fetched together, while there are registers
+    const bf16x8_t zero = __builtin_bit_cast(bf16x8_t, make_uint4(0, 0, 0, 0));
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
         uint64_t left = __builtin_amdgcn_ballot_w64(mine[i] >= 0);
-        while (left) {
-            const int a = __builtin_amdgcn_readlane(mine[i], (int)__builtin_ctzll(left));
-            left &= ~__builtin_amdgcn_ballot_w64(mine[i] == a);
-            const int64_t at = a * l.u_stride;
-            f32x16_t d[FN];
+        int a = 0, r = l.rank;
+        f32x16_t d[FN];
+        bool more = left != 0;
+        while (more) {
+            int of[N], at[N];
 #pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) d[j][e] = 0.f;
-            for (int r = 0; r < l.rank; r += 32) {
-                bf16x8_t u[FN][2], t[2][2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) u[j][h] = lora_up(l, u0[j] + at, r + 16 * h + 8 * g);
-                    t[h][0] = lora_t(t0[i] + r + 16 * h);
-                    t[h][1] = lora_t(t0[i] + l.rp + r + 16 * h);
+            for (int n = 0; n < N; ++n) {
+                r += 32;
+                if (r >= l.rank && left) {  // the next adapter
+                    a = __builtin_amdgcn_readlane(mine[i], (int)__builtin_ctzll(left));
+                    left &= ~__builtin_amdgcn_ballot_w64(mine[i] == a);
+                    r = 0;
                 }
+                // No part: the one before once more (a line that is in the cache), not added.
+                of[n] = r < l.rank ? a : -2;
+                at[n] = r < l.rank ? r : at[n - (n > 0)];
+            }
+            if (of[0] < 0) break;
+            bf16x8_t u[N][FN][2], t[N][2][2];
+            if (l.vec) {  // all loads in a row: nothing between them waits
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (h && l.rank <= 16) continue;  // no rank there
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+                            u[n][j][h] = *reinterpret_cast<const bf16x8_t*>(
+                                u0[j] + (of[n] < 0 ? a : of[n]) * l.u_stride + min(at[n] + 16 * h + 8 * g, l.rank - 8));
+                    }
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+                            u[n][j][h] = lora_up(l, u0[j] + (of[n] < 0 ? a : of[n]) * l.u_stride, at[n] + 16 * h + 8 * g);
+            }
+            // Of the adapter's own rows: the vector cache looks up every lane that asks.
+#pragma unroll
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int part = 0; part < 2; ++part)
+                        t[n][h][part] = mine[i] == of[n] ? lora_t(t0[i] + part * l.rp + at[n] + 16 * h) : zero;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                more = of[n] >= 0;
+                if (!more) break;
+                if (at[n] == 0) {
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) d[j][e] = 0.f;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bool past = at[n] + 16 * h + 8 * g >= l.rank;
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
 #pragma unroll
                         for (int j = 0; j < FN; ++j)
-                            d[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[j][h], t[h][part], d[j], 0, 0, 0);
+                            d[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(past ? zero : u[n][j][h], t[n][h][part], d[j], 0, 0, 0);
+                }
+                if (at[n] + 32 < l.rank) continue;
+                const bool keep = mine[i] == of[n];
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[j][i][e] = keep ? d[j][e] : acc[j][i][e];
             }
-            const bool keep = mine[i] == a;
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[j][i][e] = keep ? d[j][e] : acc[j][i][e];
         }
     }
 }
@@ -455,12 +504,12 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp,
     // destination below is a scalar (M0 without a per-instruction
     // readfirstlane).
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int tm, tn;
-    const Problem& p = locate<BM, BN>(grp, &tm, &tn);
+    int tm, tn, which = 0;
+    const Problem& p = locate<BM, BN>(grp, &tm, &tn, L::on ? &which : nullptr);
     const int m0 = tm * BM, n0 = tn * BN;
     const int wm = (wave / WAVES_N) * (BM / WAVES_M), wn = (wave % WAVES_N) * (BN / WAVES_N);
     int mine[FM];
-    if constexpr (L::on) lora_rows<FM>(lora, p, m0 + wm, lane, mine);
+    if constexpr (L::on) lora_rows<FM>(lora, p, m0 + wm, lane, mine, (uint32_t)which * KG + kg, (uint32_t)grp.count * KG);
 
     // DMA sources: wave w fills A rows [BM/NW w, +BM/NW) and B rows
     // [256/NW w, +256/NW), instructions of 8 rows each; lane i covers row +
@@ -605,8 +654,7 @@ __global__ __launch_bounds__(64 * NW * KG) void gemm_k64_kernel(const Group grp,
     issue(ktile(0), 0);
     if constexpr (Q8) qwrite(0);
     if (nk > 1) issue(ktile(1), 1);
-    if constexpr (L::on)  // of several K ranges, and groups, in the first
-        if (&p == grp.p && kg == 0) lora_start<FM, FN>(lora, p, acc, mine, m0 + wm, n0 + wn, lane);
+    if constexpr (L::on) lora_start<FM, FN, FM <= 2 ? 2 : 1>(lora, p, acc, mine, m0 + wm, n0 + wn, lane);
     if (nk > 1) wait_vm<A_DMA + B_DMA>();  // Q8: QJ code and QJ scale loads stand in for the B_DMA B DMAs
     else wait_vm<0>();
     if constexpr (Q8) __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the B rows written

@@ -168,6 +168,21 @@ def test_same_bits_alone_and_in_a_batch():
         assert torch.equal(alone[64 * a:64 * a + 64], both[64 * a:64 * a + 64])
 
 
+@pytest.mark.parametrize("N,K", [(512, 2048), (4096, 4096), (2560, 192)])
+def test_many_adapters_in_a_tile(N, K):
+    """Each row another adapter, ranks in several parts, the adapters shared out over K
+    ranges: right, and a row's bits do not depend on whose rows share its tile."""
+    M, R, n = 64, 40, 64
+    x, w, lora = case(131, M, N, K, R, n)
+    rows = (torch.arange(M, dtype=torch.int32, device="cuda") * 29) % n
+    got = dh.lora_gemm(x, w, lora, rows)
+    hold(got, x, w, lora, rows)
+    for a in (0, 5, 63):
+        alone = dh.lora_gemm(x, w, lora, torch.full_like(rows, a))
+        at = (rows == a).nonzero()[0, 0]
+        assert torch.equal(alone[at], got[at])
+
+
 def test_captured_calls_replay():
     M, N, K, R, n = 200, 1024, 2048, 16, 4
     x, w, lora = case(91, M, N, K, R, n)
