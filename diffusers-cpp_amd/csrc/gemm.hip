@@ -211,7 +211,12 @@ __device__ __forceinline__ void lora_rows(const LoraTile& l, const Problem& p, i
     for (int i = 0; i < FM; ++i) {
         const int m = mw + 32 * i + (lane & 31);
         const int a = m < p.M ? l.row_adapter[m] : -1;
-        mine[i] = a >= 0 && a < l.adapters && (uint32_t)a % shares == share ? a : -1;
+        mine[i] = a >= 0 && a < l.adapters ? a : -1;
+    }
+    if (shares > 1) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+            if ((uint32_t)mine[i] % shares != share) mine[i] = -1;
     }
 }
 
