@@ -501,8 +501,10 @@ Plan plan(const AttnIn& in, bool bf16_io, int cus) {
     p.rows = in.seq_q * p.pack;
     const int64_t wide = (int64_t)((p.rows + 127) / 128) * p.groups * batch;
     const int64_t narrow = (int64_t)((p.rows + 31) / 32) * p.groups * batch;
-    // Blocks of 128 rows while they give every CU one, and are not three quarters empty.
-    p.few = wide < cus || p.rows <= 32;
+    // Blocks of 128 rows while they give three quarters of the CUs one, and are not three quarters
+    // empty (16 heads x 128, 512 keys: 192 blocks 16.4 us, in 32 rows 19.9; 128 blocks 15.8
+    // and 13.2).
+    p.few = wide * 4 < 3 * cus || p.rows <= 32;
     p.splits = p.kg = 1;
     if (!p.few) {
         p.row_blocks = (p.rows + 127) / 128;
@@ -512,7 +514,8 @@ Plan plan(const AttnIn& in, bool bf16_io, int cus) {
     }
     p.row_blocks = (p.rows + 31) / 32;
     int64_t s = 2 * cus / (narrow > 0 ? narrow : 1);
-    const int64_t most = in.seq_kv / 256;  // eight tiles of 32 a range: two a wave
+    // Eight tiles of 32 keys a range, two a wave; sixteen where every CU has a workgroup anyway.
+    const int64_t most = in.seq_kv / (narrow < cus ? 256 : 512);
     if (s > most) s = most;
     if (s > 64) s = 64;
     p.splits = s < 2 ? 1 : (int)s;

@@ -661,7 +661,8 @@ Plan plan(const AttnIn& in, bool bf16_io, int buckets, int cus) {
     Plan p{};
     const int dp = in.dim <= 64 ? 64 : 128;
     const int64_t rows = (int64_t)in.heads * in.batch, keys = (int64_t)in.kv_heads * in.batch;
-    // 128 rows a workgroup while that gives half the CUs one; up to one per CU by eight waves
+    // 128 rows a workgroup while that gives half the CUs one (bwd, 16 heads x 128, 512 keys: 128 blocks
+    // 43.0 us, in 32 rows 48.5; 64 blocks 36.9 and 30.8); up to one per CU by eight waves
     // (bf16 without a bias, whose lines take the second tile's place).
     const int64_t wide = (int64_t)((in.seq_q + 127) / 128) * rows;
     p.row_high = wide * 2 >= cus ? 128 : 32;
