@@ -477,6 +477,14 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 && DP == 64 ? 2 : 1) v
                 rel_line(in.rel, kvh * in.shared + cur, line, tid, 64 * NW);
                 __syncthreads();
             }
+            // Queries past the last one: their weight is 0 by a reference of +inf.  The bias of their
+            // offset is finite, but alone above 88.7 exp of it is not.
+            const int left = in.seq_q - (n % tiles) * QB;
+            if (left < QB) {
+                float* ref = stats + buf * 2 * SL;
+                for (int i = left + tid; i < QB; i += 64 * NW) ref[i] = INFINITY;
+                __syncthreads();
+            }
         }
         if (n + 1 < last) issue(n + 1, buf ^ 1);
         const uint8_t* Qt = smem + buf * 2 * TILE + MY * wk * Tl::RB;
@@ -497,8 +505,8 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 && DP == 64 ? 2 : 1) v
                 side);
         };
         // P and dS of elements 4 i4 .. + 3: queries q0 + 32 hh + 8 i4 + 4 g + e.  A query past the
-        // last one is all zeros (row, ref and delta), and so is what it adds; a key that is
-        // not kept has a lane of its own, which is not stored.
+        // last one is a row of zeros with weight 1 (its ref and delta are 0 too), with a bias of
+        // weight 0: it adds nothing; a key that is not kept has a lane of its own, which is not stored.
         auto weights = [&](auto hc, int i4) {
             constexpr int hh = decltype(hc)::value;
             const int i0 = 32 * hh + 4 * g + 8 * i4;

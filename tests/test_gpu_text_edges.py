@@ -1,0 +1,27 @@
+"""Calls at the edges of the text operators; formulas and bounds are
+test_gpu_attn_masked's and test_gpu_lora's."""
+import pytest
+import torch
+
+import dit_hip as dh
+from test_gpu_attn_masked import check, rand
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+# A softmax does not see what is added to the whole table, and exp of it alone is out of
+# range from 88.7 on: weights come from differences, also where the queries end inside a
+# tile.  The bound's 4 u of the scores' size holds: a weight's exponent is the sum of the
+# bias in log2 (one rounding), lse (the reference's addition and its scaling: two) and its
+# scaling back (one), and their difference is exact.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,H,Hkv,Sq,Skv,D", [(2, 2, 2, 1, 150, 64), (1, 2, 1, 33, 90, 128), (1, 4, 2, 37, 500, 64), (2, 2, 2, 70, 70, 64),
+                                              (1, 2, 2, 70, 200, 128), (1, 2, 2, 128, 130, 64), (1, 24, 24, 700, 700, 64),
+                                              (1, 24, 12, 701, 350, 128)])
+def test_bias_shifted_by_a_constant(dtype, B, H, Hkv, Sq, Skv, D):
+    print(f"shifted bias {dtype} {B, H, Hkv, Sq, Skv, D}", flush=True)
+    q, k, v = rand(1, (B, Sq, H, D), dtype, D ** -0.5), rand(2, (B, Skv, Hkv, D), dtype), rand(3, (B, Skv, Hkv, D), dtype)
+    do, table = rand(4, (B, Sq, H, D), dtype), rand(5, (32, H), F32)
+    for shift in (100.0, -100.0):
+        check(q, k, v, do, rel=dh.RelBias(table + shift, 128, True), scale=1.0)
