@@ -1101,8 +1101,10 @@ __global__ __launch_bounds__(256) void gemm_128_kernel(const Group grp, const L 
 // C[m = l % 16][n = 4 (l / 16) + i].
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// The adapters of a wave's 16 rows over the KS waves, in parts of one adapter and 32 of its rank,
-// four at a time.  Each product is kept in its own rows.
+// The adapters of the 16 rows over the KS waves in turn, in parts of one adapter and 32 of its rank,
+// four at a time.  Each product is kept in its own rows and apart from the wave's sum over its
+// K range: a row's adapter is one wave's, which one depends on the other rows, and the sum
+// of all waves' parts, zeros but for that one, does not.
 template <int KS>
 struct LoraParts {
     static constexpr int N = 4;
@@ -1189,7 +1191,7 @@ struct LoraParts {
 template <typename TC, int KS, typename L, int UNR>
 __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, const L lora) {
     constexpr int LD = 16 + 4;  // padded row of the partial sums
-    __shared__ float part[KS][16 * LD];
+    __shared__ float part[L::on ? 2 : 1][KS][16 * LD];  // the K ranges', the adapters'
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int pi = 0;
     while (pi + 1 < grp.count && (int)blockIdx.x >= grp.tile_start[pi + 1]) ++pi;
@@ -1264,21 +1266,30 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
         for (; b + 4 <= b1; b += 4) step(b, std::integral_constant<int, 4>{}, nothing);
     for (; b < b1; ++b) step(b, std::integral_constant<int, 1>{}, nothing);
 
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[0][wave][r * LD + 4 * g + e] = acc[e];
     if constexpr (L::on) {
         if constexpr (UNR != 8) start();
+        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
         while (parts.add(mine, acc)) parts.fetch(lora);
-    }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[wave][r * LD + 4 * g + e] = acc[e];
+        for (int e = 0; e < 4; ++e) part[1][wave][r * LD + 4 * g + e] = acc[e];
+    }
     __syncthreads();
     TC* C = reinterpret_cast<TC*>(p.C);
     const TC* Dm = reinterpret_cast<const TC*>(p.D);
     for (int u = tid; u < 16 * 16; u += 64 * KS) {
         const int m = u >> 4, c = u & 15;
         if (m >= p.M || n0 + c >= p.N) continue;
-        float v = part[0][m * LD + c];
+        float v = part[0][0][m * LD + c];
 #pragma unroll
-        for (int k = 1; k < KS; ++k) v += part[k][m * LD + c];
+        for (int k = 1; k < KS; ++k) v += part[0][k][m * LD + c];
+        if constexpr (L::on) {
+            float own = part[1][0][m * LD + c];
+#pragma unroll
+            for (int k = 1; k < KS; ++k) own += part[1][k][m * LD + c];
+            v += own;
+        }
         if (p.bias) v += p.bias[n0 + c];
         if (Dm) v += load_c(Dm + (int64_t)m * p.ldd + n0 + c);
         store1<TC>(C + (int64_t)m * p.ldc + n0 + c, v);
@@ -1292,18 +1303,18 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 // (12288 x 4096: 20.5 us at M = 1, 28.5 us at M = 16; so 16.5 and 21.7).  The activations still
 // are: through LDS too they take the weights' room (M = 16: 19.8 us, M = 8: 17.4 -> 19.8), and 32
 // weight rows a workgroup for one read of them leave it half as many waves (25.0 us).  No barrier
-// before the partial sums: a wave waits for its own loads.  R = 3 blocks let three workgroups of
-// eight waves share a CU; with at most one there, R = 4 and the adapters' first parts
-// behind them (4096 x 4096, M = 1: 8.5 -> 7.8 us).
+// before the partial sums: a wave waits for its own loads.  R = 3 blocks, and registers held to
+// 80, let three workgroups of eight waves share a CU; with at most one there, R = 4 and the
+// adapters' first parts behind them (4096 x 4096, M = 1: 8.5 -> 7.8 us).
 template <int... S, typename F>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, S...>, F f) {
     (f(std::integral_constant<int, S>{}), ...);
 }
 
 template <typename TC, int KS, typename L, int R>
-__global__ __launch_bounds__(64 * KS) void gemm_stream_kernel(const Group grp, const L lora) {
+__global__ __launch_bounds__(64 * KS, R == 3 ? 6 : 4) void gemm_stream_kernel(const Group grp, const L lora) {
     constexpr int LD = 16 + 4, BLOCK = 16 * 128;  // padded row of the partial sums; bytes of a block of 64 k
-    static_assert(16 * LD * 4 <= R * BLOCK, "a wave's partial sums take its blocks' place");
+    static_assert((L::on ? 2 : 1) * 16 * LD * 4 <= R * BLOCK, "a wave's partial sums take its blocks' place");
     __shared__ __attribute__((aligned(16))) uint8_t ring[KS][R * BLOCK];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int pi = 0;
@@ -1384,13 +1395,16 @@ __global__ __launch_bounds__(64 * KS) void gemm_stream_kernel(const Group grp, c
 #pragma unroll
     for (int s = 0; s < R; ++s)
         if (b + s < b1) block(s, None{});
-    if constexpr (L::on) {
-        if constexpr (R == 3) start();
-        while (parts.add(mine, acc)) parts.fetch(lora);
-    }
-    float* const part = reinterpret_cast<float*>(mem);
+    float* const part = reinterpret_cast<float*>(mem);  // the K range's, the adapters'
 #pragma unroll
     for (int e = 0; e < 4; ++e) part[r * LD + 4 * g + e] = acc[e];
+    if constexpr (L::on) {
+        if constexpr (R == 3) start();
+        acc = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        while (parts.add(mine, acc)) parts.fetch(lora);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[(16 + r) * LD + 4 * g + e] = acc[e];
+    }
     __syncthreads();
     TC* C = reinterpret_cast<TC*>(p.C);
     const TC* Dm = reinterpret_cast<const TC*>(p.D);
@@ -1401,6 +1415,12 @@ __global__ __launch_bounds__(64 * KS) void gemm_stream_kernel(const Group grp, c
         float v = sum[0];
 #pragma unroll
         for (int k = 1; k < KS; ++k) v += sum[k * (R * BLOCK / 4)];
+        if constexpr (L::on) {
+            float own = sum[16 * LD];
+#pragma unroll
+            for (int k = 1; k < KS; ++k) own += sum[k * (R * BLOCK / 4) + 16 * LD];
+            v += own;
+        }
         if (p.bias) v += p.bias[n0 + c];
         if (Dm) v += load_c(Dm + (int64_t)m * p.ldd + n0 + c);
         store1<TC>(C + (int64_t)m * p.ldc + n0 + c, v);

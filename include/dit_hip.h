@@ -539,8 +539,9 @@ int dt_attn_bwd(const dt_attn_args *args, const dt_attn_grads *grads, void *work
  *   C[m][n] = (dt_gemm_bf16 / dt_gemm_q8_0 of `problem`) +
  *             scale[a] * sum_r (sum_k A[m][k] a[a][r][k]) b[a][n][r],  a = row_adapter[m],
  * summed in fp32 and rounded once; a row whose row_adapter is outside [0,
- * adapters) has the shared product alone, and no adapter reaches another
- * adapter's rows.  a: bf16 [adapters][rank][K] (rows lda apart, adapters a_stride),
+ * adapters) has the shared product alone, no adapter reaches another
+ * adapter's rows, and which adapters the other rows have changes no bit of a
+ * row's result.  a: bf16 [adapters][rank][K] (rows lda apart, adapters a_stride),
  * b: bf16 [adapters][N][rank] (rows ldb, adapters b_stride), scale: fp32 [adapters]
  * or NULL (1), row_adapter: int32 [M]; all device memory.  Any rank up to 512
  * (adapters of smaller ranks are filled up with zeros); ranks, K and strides in

@@ -5,6 +5,7 @@ import torch
 
 import dit_hip as dh
 from test_gpu_attn_masked import check, rand
+from test_gpu_lora import case, hold, q8
 
 pytestmark = pytest.mark.gpu
 BF16, F32 = torch.bfloat16, torch.float32
@@ -25,3 +26,22 @@ def test_bias_shifted_by_a_constant(dtype, B, H, Hkv, Sq, Skv, D):
     do, table = rand(4, (B, Sq, H, D), dtype), rand(5, (32, H), F32)
     for shift in (100.0, -100.0):
         check(q, k, v, do, rel=dh.RelBias(table + shift, 128, True), scale=1.0)
+
+
+# The few-row products of four and of eight waves (one or several workgroups per CU), ranks in one
+# and several parts, in chunks of 8 and not.
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("N,K,R,n", [(4096, 1024, 16, 12), (8192, 256, 64, 20), (16384, 128, 20, 9), (4096, 2048, 100, 16)])
+def test_few_rows_have_the_same_bits_whoever_shares_the_step(N, K, R, n, quant):
+    M = 16
+    x, w, lora = case(11, M, N, K, R, n)
+    wq, value = q8(w) if quant else (w, w)
+    rows = (torch.arange(M, dtype=torch.int32, device="cuda") * 7 + 3) % (n + 1) - 1
+    both = dh.lora_gemm(x, wq, lora, rows)
+    hold(both, x, value, lora, rows)
+    for order in (torch.arange(M - 1, -1, -1, device="cuda"), (torch.arange(M, device="cuda") * 5 + 2) % M):
+        assert torch.equal(dh.lora_gemm(x[order].contiguous(), wq, lora, rows[order].contiguous()), both[order])
+    for m in range(M):
+        only = torch.where(torch.arange(M, device="cuda") == m, rows, -1).to(torch.int32)
+        assert torch.equal(dh.lora_gemm(x, wq, lora, only)[m], both[m]), f"row {m} beside rows without adapters"
+        assert torch.equal(dh.lora_gemm(x[m:m + 1], wq, lora, rows[m:m + 1])[0], both[m]), f"row {m} alone"
