@@ -57,11 +57,31 @@ constexpr int few_waves() {
 // of keys sums P dP first (9 to 64 keys: 1.43); up to two would take 42.2 instead of 38.9 us for
 // a step of 1024 queries and 77 keys.
 constexpr int kExactKeys = 64;
+// So do rows of more keys of which a mask keeps few, wherever they lie (9 of 500 1.63 -> 1.42, 32
+// 1.50 -> 1.42): the tiles that hold them are walked twice (1024 queries x 16 heads x 4, 32 of 500
+// keys in every tile, bwd 51.1 -> 63.1 us, side by side 39.8 -> 43.5; the count alone 0.2).
+constexpr int kExactKept = 32;
 
 // A wave's dS block as its 63 diagonals (offsets -31 .. 31), each a row of 32 queries; what
 // lies outside the block stays 0.  Rows padded to 36: the block's writes (a step of 35
 // floats a lane) and a lane's reads of its row in 16 bytes spread over all banks.
 constexpr int kDiag = 36, kScratch = 63 * kDiag;
+
+// The keys kept of 64 N mask bytes, fetched ahead of their count.
+template <int N>
+struct KeptCount {
+    uint32_t m[N];
+    __device__ __forceinline__ void fetch(const uint8_t* mask, int from, int len, int lane) {
+#pragma unroll
+        for (int w = 0; w < N; ++w) m[w] = from + 64 * w + lane < len ? mask[from + 64 * w + lane] : 0u;
+    }
+    __device__ __forceinline__ int count() const {
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < N; ++w) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(m[w] != 0));
+        return n;
+    }
+};
 
 // ---- dQ, delta, the table's gradient ---------------------------------------------------
 // WR waves of 32 rows each, times WK that share the rows and take HALVES x 32 keys each of
@@ -123,6 +143,10 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
     uint64_t word = mine();
     if (t >= 0) issue(t, kept.word, 0);
 
+    const bool counted = sizeof(T) == 2 && !BIAS && in.kv_mask && len > kExactKeys;
+    const uint8_t* const mask = in.kv_mask + b * in.mask_stride;
+    KeptCount<4> head;
+    if (counted) head.fetch(mask, 0, len, lane);
     typename Tl::Frag qf[Tl::STEPS], of[Tl::STEPS];
     const int64_t stat = ((int64_t)b * in.heads + h) * in.seq_q + tok;
     float ref = a.lse[stat] * kLog2e;
@@ -220,7 +244,17 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 ? 2 : 1) void attn_dq_
     // The table's gradient is kept in fp32, and a whole row's dS cancels in it: delta
     // from the rounded output (off by its rounding and P's) would show there, so it is
     // summed from P and dP first; so it is for few keys.
-    if (sizeof(T) == 2 && (BIAS || len <= kExactKeys)) {
+    bool exact = BIAS || len <= kExactKeys;
+    if (counted) {
+        int n = head.count();
+        for (int from = 256; n <= kExactKept && from < len; from += 1024) {
+            KeptCount<16> c;
+            c.fetch(mask, from, len, lane);
+            n += c.count();
+        }
+        exact = n <= kExactKept;
+    }
+    if (sizeof(T) == 2 && exact) {
         float sum = 0.f;
         delta = 0.f;
         walk([&](const uint8_t* Kt, const uint8_t* Vt, int key, uint64_t word) {

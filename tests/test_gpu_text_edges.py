@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_attn_masked import check, rand
+from test_gpu_attn_masked import check, oracle, rand
 from test_gpu_lora import case, hold, q8
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +45,22 @@ def test_few_rows_have_the_same_bits_whoever_shares_the_step(N, K, R, n, quant):
         only = torch.where(torch.arange(M, device="cuda") == m, rows, -1).to(torch.int32)
         assert torch.equal(dh.lora_gemm(x, wq, lora, only)[m], both[m]), f"row {m} beside rows without adapters"
         assert torch.equal(dh.lora_gemm(x[m:m + 1], wq, lora, rows[m:m + 1])[0], both[m]), f"row {m} alone"
+
+
+# As for calls of few keys: two independent roundings, 1.41 of one, within 1.5.  The kept keys lie side
+# by side (left padding) or anywhere.
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("kept,Skv,D", [(9, 77, 64), (9, 500, 64), (24, 500, 64), (40, 500, 64), (24, 1500, 64), (9, 300, 128)])
+def test_gradients_of_few_kept_keys_are_two_roundings_off(kept, Skv, D, apart):
+    B, H, Sq = 3, 16, 300
+    q, k, v, do = (rand(90 + i, (B, n, H, D), BF16) for i, n in enumerate((Sq, Skv, Skv, Sq)))
+    mask = torch.zeros((B, Skv), dtype=torch.uint8, device="cuda")
+    for b in range(B):
+        at = rand(94 + b, (Skv,), F32).argsort()[:kept] if apart else slice(Skv - kept, Skv)
+        mask[b, at] = 1
+    o, lse = dh.cross_attn(q, k, v, kv_mask=mask, return_lse=True)
+    want = oracle(q, k, v, do, kv_mask=mask)
+    for name, got in zip(("dq", "dk", "dv"), dh.cross_attn_bwd(do, q, k, v, o, lse, kv_mask=mask)):
+        w = want[name][0]
+        once = (w.to(BF16).double() - w).norm()
+        assert (got.double() - w).norm() <= 1.5 * once, f"{name}: {((got.double() - w).norm() / once).item():.2f}"
