@@ -1305,7 +1305,8 @@ __global__ __launch_bounds__(64 * KS) void gemm_skinny_kernel(const Group grp, c
 // weight rows a workgroup for one read of them leave it half as many waves (25.0 us).  No barrier
 // before the partial sums: a wave waits for its own loads.  R = 3 blocks, and registers held to
 // 80, let three workgroups of eight waves share a CU; with at most one there, R = 4 and the
-// adapters' first parts behind them (4096 x 4096, M = 1: 8.5 -> 7.8 us).
+// adapters' first parts behind them (4096 x 4096, M = 1: 8.5 -> 7.8 us).  Four waves that have a block
+// each at most, R = 1 and eight workgroups (M = 1, 65536 x 64 5.8 -> 4.9 us, x 256 8.6 -> 7.4).
 template <int... S, typename F>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, S...>, F f) {
     (f(std::integral_constant<int, S>{}), ...);
@@ -1645,7 +1646,10 @@ int launch_skinny(const Problem* ps, int n, const L& lora, hipStream_t st) {
             hipLaunchKernelGGL((gemm_skinny_kernel<TC, 8, L, L::on ? 8 : 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
         else hipLaunchKernelGGL((gemm_skinny_kernel<TC, 8, L, 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
     } else {
-        if (four) hipLaunchKernelGGL((gemm_stream_kernel<TC, 4, L, 3>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
+        bool one = !L::on;  // a wave has a block at most
+        for (int i = 0; i < n; ++i) one = one && ps[i].K <= 4 * 64;
+        if (four && one) hipLaunchKernelGGL((gemm_stream_kernel<TC, 4, L, L::on ? 3 : 1>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
+        else if (four) hipLaunchKernelGGL((gemm_stream_kernel<TC, 4, L, 3>), dim3((unsigned)total), dim3(256), 0, st, g, lora);
         else if (total <= cu_count()) hipLaunchKernelGGL((gemm_stream_kernel<TC, 8, L, 4>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
         else hipLaunchKernelGGL((gemm_stream_kernel<TC, 8, L, 3>), dim3((unsigned)total), dim3(512), 0, st, g, lora);
     }

@@ -64,3 +64,14 @@ def test_gradients_of_few_kept_keys_are_two_roundings_off(kept, Skv, D, apart):
         w = want[name][0]
         once = (w.to(BF16).double() - w).norm()
         assert (got.double() - w).norm() <= 1.5 * once, f"{name}: {((got.double() - w).norm() / once).item():.2f}"
+
+
+# A wide weight of few k: four waves with a block of 64 k at most, the last columns past N.
+@pytest.mark.parametrize("M", [1, 5, 16])
+@pytest.mark.parametrize("N,K", [(16500, 64), (16384, 192), (40000, 256), (16390, 320)])
+def test_few_rows_of_short_sums(N, K, M):
+    x, w, lora = case(31, M, N, K, 8, 1)
+    none = torch.full((M,), -1, dtype=torch.int32, device="cuda")
+    bias, add = rand(37, (N,), F32), rand(38, (M, N), F32)
+    hold(dh.gemm(x, w, bias=bias, addend=add, out_dtype=F32), x, w, lora, none, bias, add)
+    assert torch.equal(dh.gemm(x, w), dh.lora_gemm(x, w, lora, none))
