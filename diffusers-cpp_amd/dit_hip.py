@@ -837,6 +837,8 @@ def _lora_plan(x, w, scales, a, b, scale, rows, bias, addend, out, here):
     if (K > 1 and (x[2][1] != 1 or w[2][1] != 1 or a[2][2] != 1)) or (rank > 1 and b[2][2] != 1) or \
             (q8 and N > 1 and scales[2][1] != 1):
         raise DtError("rows of x, w and the adapters must be contiguous")
+    if rows is None:
+        raise DtError("row_adapter must be given (-1: no adapter)")
     _vector(rows, torch.int32, M, "row_adapter")
     _vector(scale, torch.float32, n, "scale")
     _vector(bias, torch.float32, N, "bias")

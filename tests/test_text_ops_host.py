@@ -272,3 +272,8 @@ def test_tensors_on_another_device_are_refused(monkeypatch):
         dh.cross_attn(q, k, k)
     with pytest.raises(dh.DtError, match="host"):
         dh.lora_gemm(z(8, 64), z(32, 64), dh.Lora(z(3, 16, 64), z(3, 32, 16)), z(8, dtype=torch.int32))
+
+
+def test_adapter_wrapper_refuses_no_rows(here):
+    with pytest.raises(dh.DtError, match="row_adapter"):
+        dh.lora_gemm(z(8, 64), z(32, 64), dh.Lora(z(3, 16, 64), z(3, 32, 16)), None)
