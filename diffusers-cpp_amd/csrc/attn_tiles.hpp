@@ -30,7 +30,7 @@ struct RelArgs {
     const float* table;   // [buckets][heads]; null: no bias
     int64_t table_stride;
     const int32_t* q_pos;  // position of query 0 per batch entry, or null (0)
-    int32_t side, two_sided, reach;  // buckets a side; reach = start[side - 1], offsets are clamped to it
+    int32_t side, two_sided, reach;  // buckets a side; reach = start[side - 1]: one bucket from there on
     int32_t start[kMaxSide];
 };
 
@@ -77,7 +77,7 @@ __device__ __forceinline__ f32x16_t mma(const Elem<float>::Frag& a, const Elem<f
 
 // Accumulator elements 8 j .. 8 j + 7 as the second operand of a product whose
 // terms are the accumulator's rows.  bf16 rounds them (the products' inputs are
-// bf16 anyway: each term is off by half a step, 2^-9 of itself, as the stored
+// bf16 anyway: each term is off by half a step at most, 2^-8 of itself, as the stored
 // result is; sums over them stay fp32).
 __device__ __forceinline__ void to_frag(const float (&p)[8], bf16x8_t& f) {
     f = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),

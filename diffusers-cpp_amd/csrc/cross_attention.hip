@@ -8,9 +8,9 @@
 // holds one query in both: the running maximum and sum of the softmax are
 // per-lane scalars, and P^T goes from the accumulator straight into the second
 // product.  One pass over the keys, no score is stored.  The bias is a line of
-// 2 reach + 1 values per head in LDS (offsets beyond the last bucket's start are
-// clamped), read by offset for each score of a tile that the band |offset| < reach
-// meets and once for any other.
+// 2 (reach + kMargin) + 1 values per head in LDS (one value from the last bucket's
+// start on), read by offset for each score of a 32 x 32 block that the band
+// |offset| < reach meets and once for any other.
 #include <float.h>
 #include <math.h>
 
@@ -503,7 +503,10 @@ Plan plan(const AttnIn& in, bool bf16_io, int cus) {
     const int64_t narrow = (int64_t)((p.rows + 31) / 32) * p.groups * batch;
     // Blocks of 128 rows while they give three quarters of the CUs one, and are not three quarters
     // empty (16 heads x 128, 512 keys: 192 blocks 16.4 us, in 32 rows 19.9; 128 blocks 15.8
-    // and 13.2).
+    // and 13.2; 8192 keys: 131 and 167; 144 and 98).  Workgroups of 32 rows come in rounds of
+    // their own, by which the line is off in places, in either direction: width 128, 160 blocks
+    // 15.4 and 18.5 at 512 keys, 131 and 162 at 8192; 192 blocks at width 64 and 2048 keys 27.7
+    // and 24.5, in fp32 165 and 121.
     p.few = wide * 4 < 3 * cus || p.rows <= 32;
     p.splits = p.kg = 1;
     if (!p.few) {

@@ -704,8 +704,10 @@ Plan plan(const AttnIn& in, bool bf16_io, int buckets, int cus) {
     const int dp = in.dim <= 64 ? 64 : 128;
     const int64_t rows = (int64_t)in.heads * in.batch, keys = (int64_t)in.kv_heads * in.batch;
     // 128 rows a workgroup while that gives half the CUs one (bwd, 16 heads x 128, 512 keys: 128 blocks
-    // 43.0 us, in 32 rows 48.5; 64 blocks 36.9 and 30.8); up to one per CU by eight waves
-    // (bf16 without a bias, whose lines take the second tile's place).
+    // 43.0 us, in 32 rows 48.5; 64 blocks 36.9 and 30.8; 128 blocks at 2048 keys 93 and 102, with a
+    // bias 187 and 207; but 128 blocks at width 64 59 and 53, in fp32 366 and 293, and 96 at width
+    // 128 84 and 91); up to one per CU by eight waves (bf16 without a bias, whose lines take the
+    // second tile's place).
     const int64_t wide = (int64_t)((in.seq_q + 127) / 128) * rows;
     p.row_high = wide * 2 >= cus ? 128 : 32;
     p.row_pairs = p.row_high == 128 && wide <= cus && bf16_io && buckets == 0 && in.seq_kv > 64;

@@ -861,7 +861,8 @@ def _lora_plan(x, w, scales, a, b, scale, rows, bias, addend, out, here):
 def lora_gemm(x, w, lora, row_adapter, bias=None, addend=None, out=None, out_dtype=None):
     """x: bf16 [M, K], w: bf16 [N, K] or Q8Weight -> x @ w.T (+ bias) (+ addend) +
     scale[a] * (x @ a[a].T) @ b[a].T, each row with the adapter a = row_adapter[m]
-    (int32 [M]; outside the adapters: none)."""
+    (int32 [M]; outside the adapters: none).  Autograd records nothing, and no
+    gradients of the adapters are offered."""
     torch = _torch()
     q8 = isinstance(w, Q8Weight)
     codes, scales = (w.codes, w.scales) if q8 else (w, None)
@@ -1043,8 +1044,9 @@ def cross_attn(q, k, v, kv_len=None, kv_mask=None, scale=None, out=None, return_
     """softmax over the kept keys of scale q k^T, times v: q [B, Sq, H, D], k and v
     [B, Skv, Hkv, D] (bf16 or fp32, Hkv a divisor of H, D a multiple of 8 up to 128,
     any strides with d contiguous) -> [B, Sq, H, D].  kv_len int32 [B] keeps keys
-    below it, kv_mask uint8 or bool [B, Skv] those that are set.  return_lse: also
-    the log of each softmax's sum, fp32 [B, H, Sq], for cross_attn_bwd."""
+    below it, kv_mask uint8 or bool [B, Skv] those that are set.  scale: >= 0, by
+    default D ** -0.5.  out must not overlap an input.  return_lse: also the log of
+    each softmax's sum, fp32 [B, H, Sq], for cross_attn_bwd: autograd records nothing."""
     return _attn(q, k, v, kv_len, kv_mask, scale, None, None, out, return_lse)
 
 

@@ -478,7 +478,7 @@ int dt_flash_attn_f32(const float *q, const float *k, const float *v, float *o, 
  * [0, seq_kv]); kv_mask (uint8, key j of entry b at kv_mask[b*kv_mask_stride +
  * j], device) keeps keys with a nonzero byte; both given: both.  What a key that
  * is not kept holds is not used (it may be NaN).  A query without kept keys, or
- * whose scores are all -inf, has o = 0 and lse = -inf.
+ * whose scores are all -inf, has o = 0 and lse = -inf.  scale: finite, >= 0.
  * rel_table (fp32 [rel_buckets][heads], rows rel_table_stride apart) adds a learned
  * bias by the bucket (dt_rel_bucket_fill) of key position j - query position
  * q_pos[b] + i (q_pos: int32 [batch], device, or NULL: 0).  rel_table NULL: none.
@@ -512,7 +512,8 @@ int dt_rel_bucket_fill(int32_t *bucket, int64_t n, int32_t buckets, int32_t dist
  * sum_j exp(s_ij) as fp32 [batch][heads][seq_q], which the gradients need.  Few
  * rows take their keys in ranges whose partial results go through `workspace`
  * (dt_attn_fwd_workspace_bytes, 0 for most calls; 16-byte aligned); with less,
- * or none, the ranges are one.  Same results for the same call: no atomics. */
+ * or none, the ranges are one.  Same results for the same call: no atomics.  o
+ * must not overlap an input. */
 size_t dt_attn_fwd_workspace_bytes(const dt_attn_args *args);
 int dt_attn_fwd(const dt_attn_args *args, void *o, const int64_t *o_strides, float *lse, void *workspace,
                 size_t workspace_bytes, dt_stream_t stream);
