@@ -146,18 +146,6 @@ __device__ __forceinline__ void wait_vmem() {
 }
 __device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(0xC07F); }
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-constexpr uint32_t kOut = 0x80000000u;  // an offset out of every buffer's range
-// 16 bytes a lane from base + off (zeros where off is out of range) to lds + 16 lane; base and lds uniform.
-__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint8_t* lds) {
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
-}
-__device__ __forceinline__ void dma4(const void* base, uint32_t off, void* lds) {  // 4 bytes a lane
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 4, off, 0, 0, 0);
-}
-
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) short4_t* lds_short4_p;
 __device__ __forceinline__ uint2 read_tr16(const uint8_t* p) {
@@ -192,7 +180,7 @@ struct Tile {
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 const int i = (wave * J + j) * 64 + lane, r = i / CPR, c = (i % CPR) ^ swz(r);
-                at[j] = c * Elem<T>::EPC < dim ? (uint32_t)((r * stride + c * Elem<T>::EPC) * (int64_t)sizeof(T)) : kOut;
+                at[j] = c * Elem<T>::EPC < dim ? (uint32_t)((r * stride + c * Elem<T>::EPC) * (int64_t)sizeof(T)) : kOutOfBuffer;
             }
         }
         __device__ __forceinline__ static int row(int wave, int lane, int j) { return ((wave * J + j) * 64 + lane) / CPR; }
@@ -200,12 +188,12 @@ struct Tile {
         // base: the tile's first row.
         __device__ __forceinline__ void issue_all(const T* base, uint8_t* lds, int wave) const {
 #pragma unroll
-            for (int j = 0; j < J; ++j) dma16(base, at[j], lds + (wave * J + j) * 1024);
+            for (int j = 0; j < J; ++j) lds_dma16(base, at[j], lds + (wave * J + j) * 1024);
         }
         template <typename Keep>
         __device__ __forceinline__ void issue(const T* base, uint8_t* lds, int wave, int lane, Keep keep) const {
 #pragma unroll
-            for (int j = 0; j < J; ++j) dma16(base, keep(row(wave, lane, j)) ? at[j] : kOut, lds + (wave * J + j) * 1024);
+            for (int j = 0; j < J; ++j) lds_dma16(base, keep(row(wave, lane, j)) ? at[j] : kOutOfBuffer, lds + (wave * J + j) * 1024);
         }
     };
     // Row operand: elements 16 c + 8 g .. + 7 of row r.
@@ -433,7 +421,7 @@ __device__ __forceinline__ int rel_position(const RelArgs& r, int b) {
 
 // ---- host ---------------------------------------------------------------------------
 constexpr int64_t kMaxSeq = 1 << 28;
-constexpr int64_t kMaxRowBytes = (1 << 24) - 256;  // a tile's 128 rows stay below kOut bytes
+constexpr int64_t kMaxRowBytes = (1 << 24) - 256;  // a tile's 128 rows stay below kOutOfBuffer bytes
 // Checks the shared arguments and fills `in` (cross_attention.hip).
 int prepare_in(const dt_attn_args* args, const char* who, AttnIn* in);
 // Checks one strided operand [batch][seq][heads][head_dim]; `out`: no element twice.

@@ -253,4 +253,16 @@ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
     return (__umulhi(n, f.m) + n) >> f.s;
 }
 
+// 16 (4) bytes a lane from base + off to lds + 16 (4) lane by direct DMA, zeros where off is out
+// of the buffer's range of 2^31 - 1 bytes; base and lds uniform.
+constexpr uint32_t kOutOfBuffer = 0x80000000u;
+__device__ __forceinline__ void lds_dma16(const void* base, uint32_t off, void* lds) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+}
+__device__ __forceinline__ void lds_dma4(const void* base, uint32_t off, void* lds) {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 4, off, 0, 0, 0);
+}
+
 }  // namespace dit

@@ -495,7 +495,7 @@ __global__ __launch_bounds__(64 * WR * WK, sizeof(T) == 2 && DP == 64 ? 2 : 1) v
             if (i % NW != wave) continue;
             const int which = i / (SL / 64), at = i % (SL / 64) * 64 + lane;
             const float* src = (which == 0 ? a.ref : a.delta) + ((int64_t)b * in.heads + h) * in.seq_q + q0;
-            dma4(src, at < min(left, QB) ? 4 * at : kOut, stats + (buf * 2 + which) * SL + i % (SL / 64) * 64);
+            lds_dma4(src, at < min(left, QB) ? 4 * at : kOutOfBuffer, stats + (buf * 2 + which) * SL + i % (SL / 64) * 64);
         }
     };
     int cur = -1, buf = 0;

@@ -58,14 +58,6 @@ struct Out {  // a thread's element of T: row tid / RANKS, rank tid % RANKS
     }
 };
 
-constexpr uint32_t kZero = 0x80000000u;  // an offset out of every buffer's range: reads zeros
-// 16 bytes a lane from base + off to lds + 16 lane; base and lds uniform.
-__device__ __forceinline__ void down_dma(const void* base, uint32_t off, uint8_t* lds) {
-    typedef __attribute__((address_space(3))) void* lds_ptr_t;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7FFFFFFF, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)lds, 16, off, 0, 0, 0);
-}
-
 // VEC: rows in whole 16-byte chunks, through LDS.  Else element by element, for any layout.
 template <bool VEC, int ROWS, int NW, int NB, int RANKS>
 __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
@@ -126,13 +118,13 @@ __global__ __launch_bounds__(64 * NW) void lora_down_kernel(const DownArgs p) {
             for (int j = 0; j < DMAS; ++j) {
                 const int row = 8 * j + (lane >> 3), rank = row - ROWS;
                 const bool there = row < ROWS ? (of >> row) & 1 : r0 + rank < p.rank;
-                off[j] = there ? (uint32_t)((row < ROWS ? row * p.ldx : rank * p.lda) * 2 + chunk * 16) : kZero;
+                off[j] = there ? (uint32_t)((row < ROWS ? row * p.ldx : rank * p.lda) * 2 + chunk * 16) : kOutOfBuffer;
             }
             auto issue = [&](int line, int buf) {
                 const bool tail = line * kLine + chunk * 8 >= p.K;  // lines past the last one too
 #pragma unroll
                 for (int j = 0; j < DMAS; ++j)
-                    down_dma((8 * j < ROWS ? xb : ab) + (int64_t)line * kLine, tail ? kZero : off[j], mem + buf * BUF + 1024 * j);
+                    lds_dma16((8 * j < ROWS ? xb : ab) + (int64_t)line * kLine, tail ? kOutOfBuffer : off[j], mem + buf * BUF + 1024 * j);
             };
 #pragma unroll
             for (int i = 0; i < NB - 1; ++i) issue(wave + i * NW, i);
