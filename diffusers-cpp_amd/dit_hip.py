@@ -1008,7 +1008,8 @@ def _grads_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, o, 
         raise DtError("o and d_o must have q's shape and dtype, their head dim contiguous")
     plan, _, bwd, _ = _attn_plan(q, k, v, kv_len, kv_mask, table, q_pos, distance, two_sided, o, here)
     B, Sq, H, D = q[1]
-    if lse[0] != _torch().float32 or lse[1] != (B, H, Sq) or lse[2] != (H * Sq, Sq, 1) and 0 not in lse[1]:
+    dense = all(n == 1 or s == want for n, s, want in zip(lse[1], lse[2], (H * Sq, Sq, 1)))
+    if lse[0] != _torch().float32 or lse[1] != (B, H, Sq) or not dense and 0 not in lse[1]:
         raise DtError("lse must be the forward pass's: contiguous fp32 [B, H, Sq]")
     _on_device((d_o, o, lse))
     y = AttnGrads()

@@ -277,3 +277,18 @@ def test_tensors_on_another_device_are_refused(monkeypatch):
 def test_adapter_wrapper_refuses_no_rows(here):
     with pytest.raises(dh.DtError, match="row_adapter"):
         dh.lora_gemm(z(8, 64), z(32, 64), dh.Lora(z(3, 16, 64), z(3, 32, 16)), None)
+
+
+def test_lse_of_one_entry_or_head_may_have_any_stride_there(here):
+    """Contiguous as torch counts it: the stride of a dimension of one element is none."""
+    for H, all_lse in ((1, z(1, 4, 5, dtype=torch.float32)), (4, z(1, 4, 1, 7, dtype=torch.float32)[..., 0])):
+        lse = all_lse[:, :H]
+        assert lse.is_contiguous() == (H == 1)
+        Sq = lse.shape[2]
+        q = z(1, Sq, H, 64)
+        args = [dh._meta(q)] * 3 + [None] * 6 + [dh._meta(q), dh._meta(q), dh._meta(lse), -1]
+        if H == 1:
+            dh._grads_plan(*args)
+        else:
+            with pytest.raises(dh.DtError, match="lse"):
+                dh._grads_plan(*args)
