@@ -75,3 +75,57 @@ def test_few_rows_of_short_sums(N, K, M):
     bias, add = rand(37, (N,), F32), rand(38, (M, N), F32)
     hold(dh.gemm(x, w, bias=bias, addend=add, out_dtype=F32), x, w, lora, none, bias, add)
     assert torch.equal(dh.gemm(x, w), dh.lora_gemm(x, w, lora, none))
+
+
+# A table entry of -inf leaves its bucket's keys out; a query that has none left is all zeros.  Two
+# kernels' results of one formula: each rounds its weights and its output, by u of v's size each.
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_bias_of_minus_infinity_leaves_keys_out(dtype):
+    B, H, Sq, Skv, D = 2, 2, 70, 300, 64
+    q, k, v, do = (rand(41 + i, (B, n, H, D), dtype) for i, n in enumerate((Sq, Skv, Skv, Sq)))
+    table = rand(45, (32, H), F32)
+    table[15] = table[31] = -torch.inf  # distance 113 and more, both sides
+    table[:, 1] = -torch.inf            # every key of the second head
+    rel = dh.RelBias(table, 128, True)
+    o, lse = dh.rel_attn(q, k, v, rel, return_lse=True)
+    dq, dk, dv, dt = dh.rel_attn_bwd(do, q, k, v, o, lse, rel)
+    for t in (o, dq, dk, dv):
+        assert torch.isfinite(t).all() and (t[:, :, 1] == 0).all()
+    assert (lse[:, 1] == -torch.inf).all() and (dt[:, 1] == 0).all() and (dt[[15, 31]] == 0).all()
+    # The same by a mask, query by query: keys of bucket 15 and 31 dropped for the first head.
+    buckets = dh.rel_buckets(Skv + Sq, 32, 128, True).cuda()
+    off = torch.arange(Skv, device="cuda")[None, :] - torch.arange(Sq, device="cuda")[:, None]
+    left_out = torch.isin(buckets[(off + Skv + Sq - 1).long()], torch.tensor([15, 31], device="cuda", dtype=torch.int32))
+    for i in (0, 33, 69):
+        part = table[:, :1].clone()
+        part[[15, 31]] = 0.0
+        mask = (~left_out[i])[None].expand(B, Skv).contiguous()
+        want = dh.rel_attn(q[:, i:i + 1, :1], k[:, :, :1], v[:, :, :1], dh.RelBias(part, 128, True),
+                           q_pos=torch.full((B,), i, dtype=torch.int32, device="cuda"), kv_mask=mask)
+        u = torch.finfo(dtype).eps / 2
+        err = (o[:, i, 0].double() - want[:, 0, 0].double()).abs().max().item()
+        assert err <= (4 * u if dtype == BF16 else 64 * u) * v.abs().max().item()
+
+
+def test_gradients_of_scale_zero():
+    B, H, Sq, Skv, D = 1, 2, 40, 90, 64
+    q, k, v, do = (rand(51 + i, (B, n, H, D), F32) for i, n in enumerate((Sq, Skv, Skv, Sq)))
+    check(q, k, v, do, scale=0.0)
+
+
+# Keys that lie more than 2^32 bytes apart, read and written.
+@pytest.mark.parametrize("Sq", [1, 130])
+def test_keys_beyond_four_gigabytes(Sq):
+    H, Skv, D = 2, 700, 64
+    step = (1 << 23) - 136  # elements from token to token, the most there may be: below 2^24 - 256 bytes
+    room = torch.zeros(Skv * step, dtype=BF16, device="cuda")
+    wide = room.as_strided((1, Skv, H, D), (Skv * step, step, D, 1))
+    q, k, v, do = (rand(61 + i, (1, n, H, D), BF16) for i, n in enumerate((Sq, Skv, Skv, Sq)))
+    wide.copy_(k)
+    assert (Skv - 1) * step * 2 > 1 << 32
+    o, lse = dh.cross_attn(q, wide, v, return_lse=True)
+    want, want_lse = dh.cross_attn(q, k, v, return_lse=True)
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+    assert torch.equal(dh.cross_attn(q, v, wide), dh.cross_attn(q, v, k))
+    for a, b in zip(dh.cross_attn_bwd(do, q, wide, v, o, lse), dh.cross_attn_bwd(do, q, k, v, o, lse)):
+        assert torch.equal(a, b)
