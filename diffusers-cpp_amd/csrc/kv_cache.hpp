@@ -1,0 +1,68 @@
+// kv_cache.hpp -- the paged key/value cache as its kernels see it (kv_cache.hip,
+// kv_attention.hip), e4m3 conversions, and the search for a row's sequence.
+#pragma once
+
+#include "capi_util.hpp"
+#include "common.hpp"
+#include "kv_index.hpp"
+
+namespace dit {
+namespace kv {
+
+struct e4m3 {
+    uint8_t bits;
+};
+
+struct Cache {
+    uint8_t* k;
+    uint8_t* v;
+    uint8_t* k_scale;  // null: bf16
+    uint8_t* v_scale;
+    int32_t kv_heads, page_log2, dim;
+    int64_t head_bytes;  // one page of one head: page * dim elements
+};
+
+// How many sequences b have key(seq_start[b], b) <= x, less one: with ascending keys, the one
+// that x belongs to.  By a whole wave.
+template <typename Key>
+__device__ __forceinline__ int find_seq(const Seqs& s, int64_t x, Key key) {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int b0 = 0; b0 < s.seqs; b0 += 64) {
+        const int b = b0 + lane;
+        const bool in = b < s.seqs && key(start_of(s, min(b, s.seqs)), b) <= x;
+        n += __popcll(__builtin_amdgcn_ballot_w64(in));
+    }
+    return n - 1;
+}
+
+// ---- e4m3: four bits of significand, 2^-9 to 448, NaN but no infinity --------------------
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+// Four values (at most 448 in size, or NaN) to codes, to nearest even.
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+__device__ __forceinline__ void from_e4m3x4(uint32_t w, float (&v)[4]) {
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = a[0];
+    v[1] = a[1];
+    v[2] = b[0];
+    v[3] = b[1];
+}
+
+// ---- host -------------------------------------------------------------------------------
+// Checks the descriptions and fills the kernels' own (kv_cache.hip).
+int prepare(const dt_kv_cache* cache, const dt_kv_seqs* seqs, const char* who, Cache* c, Seqs* s);
+// Rows of heads * dim elements of `es` bytes, strides {row, head}: `out`: no element twice.
+int check_rows(const void* p, const int64_t* strides, int64_t rows, int64_t heads, int64_t dim, int es, bool out,
+               const char* name, const char* who);
+
+}  // namespace kv
+
+namespace rotary {
+int check_rotary(const dt_rotary& r, int64_t head_dim, const char* who);  // rotary.hip
+}
+
+}  // namespace dit

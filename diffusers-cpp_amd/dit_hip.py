@@ -12,13 +12,14 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32, c_uint64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdit_hip.so")
 
 # ggml type ids
 F32, F16, Q8_0, Q4_K, I32, BF16 = 0, 1, 8, 12, 26, 30
+F8_E4M3 = 102  # a key/value cache's
 
 # dt_tensor.op ids
 (OP_NONE, OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_SCALE, OP_SIGMOID, OP_NORM, OP_RMS_NORM,
@@ -142,6 +143,12 @@ _SIGS = {
     "dt_attn_fwd": (c_int32, [c_void_p, c_void_p, _I64P, c_void_p, c_void_p, ctypes.c_size_t, _S]),
     "dt_attn_bwd_workspace_bytes": (ctypes.c_size_t, [c_void_p]),
     "dt_attn_bwd": (c_int32, [c_void_p, c_void_p, c_void_p, ctypes.c_size_t, _S]),
+    "dt_rotary_freq_fill": (c_int32, [c_void_p, c_int64, c_double, c_double, c_int64, c_double, c_double]),
+    "dt_rotary_apply": (c_int32, [c_void_p, _S]),
+    "dt_kv_append": (c_int32, [c_void_p, c_void_p, c_void_p, _S]),
+    "dt_kv_attn_workspace_bytes": (ctypes.c_size_t, [c_void_p, c_void_p, c_int64]),
+    "dt_kv_attn": (c_int32, [c_void_p, c_void_p, c_void_p, _I64P, c_int64, c_int32, c_float, c_void_p, _I64P,
+                             c_void_p, ctypes.c_size_t, _S]),
     "dt_op_binary": (c_int32, [c_int32, POINTER(DtTensor), POINTER(DtTensor), POINTER(DtTensor), _S]),
     "dt_op_unary": (c_int32, [c_int32, POINTER(DtTensor), POINTER(DtTensor), c_float, c_float, _S]),
     "dt_op_norm": (c_int32, [POINTER(DtTensor), POINTER(DtTensor), c_float, _S]),
@@ -1066,6 +1073,302 @@ def rel_attn(q, k, v, rel, q_pos=None, kv_len=None, kv_mask=None, scale=None, ou
 def rel_attn_bwd(d_o, q, k, v, o, lse, rel, q_pos=None, kv_len=None, kv_mask=None, scale=None):
     """(dq, dk, dv, dtable) of rel_attn's o for its gradient d_o; dtable fp32 [buckets, H]."""
     return _attn_bwd(d_o, q, k, v, o, lse, kv_len, kv_mask, scale, rel, q_pos)
+
+
+class RotaryStruct(ctypes.Structure):
+    _fields_ = [("freq", c_void_p), ("rot_dims", c_int64), ("half", c_int32), ("attn_factor", c_float)]
+
+
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("q_strides", _I64x3),
+                ("k_strides", _I64x3), ("q_out_strides", _I64x3), ("k_out_strides", _I64x3), ("batch", c_int64),
+                ("seq", c_int64), ("heads", c_int64), ("kv_heads", c_int64), ("head_dim", c_int64), ("pos", c_void_p),
+                ("pos_stride", c_int64), ("rotary", RotaryStruct), ("io_type", c_int32), ("backward", c_int32)]
+
+
+class Rotary:
+    """Rotary positions: pair i turns by position * freq[i] (fp32 [rot_dims / 2], rotary_freqs()
+    makes one); half: pairs (i, i + rot_dims / 2) instead of (2i, 2i + 1); what is rotated is
+    multiplied by attn_factor."""
+
+    def __init__(self, freq, half=False, attn_factor=1.0):
+        self.freq, self.half, self.attn_factor = freq, half, attn_factor
+
+
+def rotary_freqs(rot_dims, base=10000.0, factor=1.0, context=0, turns_low=1.0, turns_high=32.0, device="cuda"):
+    """Frequencies base^(-2i / rot_dims) for a context `factor` times as long: pairs of up to
+    turns_low turns within the original `context` are slowed by factor, those of turns_high or
+    more kept, the others blended; context 0: all are slowed."""
+    torch = _torch()
+    host = torch.empty(max(rot_dims // 2, 0), dtype=torch.float32)
+    check(load().dt_rotary_freq_fill(c_void_p(host.data_ptr()), rot_dims, base, factor, context, turns_low, turns_high),
+          "dt_rotary_freq_fill")
+    return host.to(device) if device != "cpu" else host
+
+
+def _freq_ok(freq):
+    if freq[0] != _torch().float32 or len(freq[1]) != 1 or (freq[1][0] > 1 and freq[2][0] != 1):
+        raise DtError("freq must be contiguous fp32 [rot_dims / 2]")
+
+
+def _four(m):
+    """Shape and strides of [tokens, heads, dim] or [batch, seq, heads, dim] as four dimensions."""
+    if len(m[1]) == 3:
+        return (1, *m[1]), (0, *m[2])
+    if len(m[1]) != 4:
+        raise DtError("q and k must be [tokens, heads, dim] or [batch, seq, heads, dim]")
+    return m[1], m[2]
+
+
+@functools.lru_cache(maxsize=512)
+def _rotary_plan(q, k, q_out, k_out, pos, freq, half, here):
+    torch = _torch()
+    a = RotaryArgs()
+    first = q if q is not None else k
+    if first is None:
+        raise DtError("q or k must be given")
+    (B, S, _, D), _ = _four(first)
+    if first[0] not in (torch.bfloat16, torch.float32):
+        raise DtError(f"q and k must be bf16 or fp32, not {first[0]}")
+    for x, y, name in ((q, q_out, "q"), (k, k_out, "k")):
+        if x is None:
+            continue
+        (b, s, h, d), st = _four(x)
+        if (b, s, d) != (B, S, D) or len(x[1]) != len(first[1]) or x[0] != first[0]:
+            raise DtError("q and k must share their tokens, width and dtype")
+        if y[1] != x[1] or y[0] != x[0] or (D > 1 and (st[3] != 1 or y[2][-1] != 1)):
+            raise DtError(f"{name} and its output must share shape and dtype, their head dim contiguous")
+        setattr(a, "heads" if name == "q" else "kv_heads", h)
+        getattr(a, name + "_strides")[:] = st[:3]
+        getattr(a, name + "_out_strides")[:] = _four(y)[1][:3]
+    want = first[1][:-2]
+    if pos[0] != torch.int32 or pos[1] != want or (S > 1 and pos[2][-1] != 1):
+        raise DtError(f"pos must be int32 {list(want)} with contiguous rows")
+    _freq_ok(freq)
+    _on_device((q, k, q_out, k_out, pos, freq))
+    a.batch, a.seq, a.head_dim = B, S, D
+    a.pos_stride = pos[2][0] if len(want) == 2 else 0
+    a.rotary.rot_dims, a.rotary.half = 2 * freq[1][0], 1 if half else 0
+    a.io_type = _IO_TYPES[first[0]]
+    return bytes(a)
+
+
+def _rotate(q, k, pos, rot, q_out, k_out, backward):
+    if q is not None and q_out is None:
+        q_out = q.new_empty(q.shape)
+    if k is not None and k_out is None:
+        k_out = k.new_empty(k.shape)
+    a = RotaryArgs.from_buffer_copy(_rotary_plan(_meta(q), _meta(k), None if q is None else _meta(q_out), None if k is None else _meta(k_out),
+                                                 _meta(pos), _meta(rot.freq), rot.half, _torch().cuda.current_device()))
+    if q is not None:
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if k is not None:
+        a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
+    a.pos, a.rotary.freq, a.rotary.attn_factor, a.backward = pos.data_ptr(), rot.freq.data_ptr(), rot.attn_factor, backward
+    lib = load()
+    check(lib.dt_rotary_apply(ctypes.addressof(a), stream()), "dt_rotary_apply")
+    if isinstance(lib, _Recorder):
+        lib.keep.append(a)
+    return q_out, k_out
+
+
+def rotary(q, k, pos, rot, q_out=None, k_out=None):
+    """q and k ([tokens, heads, dim] or [batch, seq, heads, dim], bf16 or fp32, any strides with
+    the head dim contiguous; either may be None) rotated by their positions pos (int32 [tokens] or
+    [batch, seq]) -> (q_out, k_out), which may be q and k themselves.  Autograd records nothing:
+    rotary_bwd makes the gradients."""
+    return _rotate(q, k, pos, rot, q_out, k_out, 0)
+
+
+def rotary_bwd(d_q, d_k, pos, rot, dq_out=None, dk_out=None):
+    """The gradients of rotary's q and k from those of its results."""
+    return _rotate(d_q, d_k, pos, rot, dq_out, dk_out, 1)
+
+
+_I64x2 = c_int64 * 2
+
+
+class KVCacheStruct(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("pages", c_int64),
+                ("kv_heads", c_int64), ("page", c_int64), ("head_dim", c_int64), ("type", c_int32)]
+
+
+class KVSeqs(ctypes.Structure):
+    _fields_ = [("table", c_void_p), ("table_stride", c_int64), ("table_pages", c_int64), ("seq_start", c_void_p),
+                ("past", c_void_p), ("seqs", c_int64), ("rows", c_int64)]
+
+
+class KVAppendArgs(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("q", c_void_p), ("q_out", c_void_p), ("k_strides", _I64x2),
+                ("v_strides", _I64x2), ("q_strides", _I64x2), ("q_out_strides", _I64x2), ("heads", c_int64),
+                ("rotary", c_void_p), ("pos", c_void_p), ("io_type", c_int32)]
+
+
+class KVCache:
+    """A pool of pages of keys and values: k [pages, kv_heads, page, dim] and v [pages, kv_heads,
+    dim, page], both bf16, or both float8_e4m3fn with the scales 2^(scale - 127) of each page and
+    head, uint8 [pages, kv_heads].  kv_cache() makes an empty one."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale")
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+
+def kv_cache(pages, kv_heads, page, dim, dtype=None, device="cuda"):
+    """A pool with room for `pages` pages of `page` tokens; dtype float8_e4m3fn (default) or bfloat16."""
+    torch = _torch()
+    dtype = dtype or torch.float8_e4m3fn
+    k = torch.zeros((pages, kv_heads, page, dim), dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype, device=device)
+    v = torch.zeros((pages, kv_heads, dim, page), dtype=k.dtype, device=device)
+    if dtype != torch.float8_e4m3fn:
+        return KVCache(k, v)
+    s = [torch.ones((pages, kv_heads), dtype=torch.uint8, device=device) for _ in range(2)]
+    return KVCache(k.view(dtype), v.view(dtype), *s)
+
+
+def _dense(m):
+    want = 1
+    for n, s in zip(reversed(m[1]), reversed(m[2])):
+        if n != 1 and s != want:
+            return False
+        want *= n
+    return True
+
+
+def _cache_plan(k, v, k_scale, v_scale, table, seq_start, past, rows):
+    torch = _torch()
+    if len(k[1]) != 4 or v[1] != (k[1][0], k[1][1], k[1][3], k[1][2]) or k[0] != v[0] or not _dense(k) or not _dense(v):
+        raise DtError("k must be [pages, kv_heads, page, dim], v [pages, kv_heads, dim, page], of one dtype and contiguous")
+    c = KVCacheStruct()
+    c.pages, c.kv_heads, c.page, c.head_dim = k[1]
+    if k[0] == torch.float8_e4m3fn:
+        c.type = F8_E4M3
+        for s in (k_scale, v_scale):
+            if s is None or s[0] != torch.uint8 or s[1] != k[1][:2] or not _dense(s):
+                raise DtError("an e4m3 cache needs k_scale and v_scale, contiguous uint8 [pages, kv_heads]")
+    elif k[0] == torch.bfloat16:
+        c.type = BF16
+    else:
+        raise DtError(f"a cache is float8_e4m3fn or bf16, not {k[0]}")
+    if table[0] != torch.int32 or len(table[1]) != 2 or (table[1][1] > 1 and table[2][1] != 1):
+        raise DtError("table must be int32 [seqs, pages] with contiguous rows")
+    n = table[1][0]
+    _vector(seq_start, torch.int32, n + 1, "seq_start")
+    _vector(past, torch.int32, n, "past")
+    _on_device((k, v, k_scale, v_scale, table, seq_start, past))
+    s = KVSeqs()
+    s.table_stride, s.table_pages, s.seqs, s.rows = table[2][0], table[1][1], n, rows
+    return c, s
+
+
+@functools.lru_cache(maxsize=512)
+def _append_plan(ck, cv, k_scale, v_scale, table, seq_start, past, k, v, q, q_out, pos, freq, half, here):
+    torch = _torch()
+    if len(k[1]) != 3 or v[1] != k[1] or k[1][1:] != (ck[1][1], ck[1][3]):
+        raise DtError(f"k {tuple(k[1])} and v {tuple(v[1])} must be [rows, kv_heads, dim] of the cache {tuple(ck[1])}")
+    if k[0] not in (torch.bfloat16, torch.float32) or v[0] != k[0] or k[2][2] != 1 or v[2][2] != 1:
+        raise DtError("k and v must share a dtype, bf16 or fp32, the head dim contiguous")
+    c, s = _cache_plan(ck, cv, k_scale, v_scale, table, seq_start, past, k[1][0])
+    a = KVAppendArgs()
+    a.k_strides[:], a.v_strides[:] = k[2][:2], v[2][:2]
+    a.io_type = _IO_TYPES[k[0]]
+    if q is not None:
+        if freq is None:
+            raise DtError("q needs a rotation")
+        if len(q[1]) != 3 or q[1][0] != k[1][0] or q[1][2] != k[1][2] or q[0] != k[0] or q[2][2] != 1:
+            raise DtError("q must be [rows, heads, dim] of k's rows, width and dtype, the head dim contiguous")
+        if q_out[1] != q[1] or q_out[0] != q[0] or q_out[2][2] != 1:
+            raise DtError("q_out must have q's shape and dtype, its head dim contiguous")
+        a.heads = q[1][1]
+        a.q_strides[:], a.q_out_strides[:] = q[2][:2], q_out[2][:2]
+    _vector(pos, torch.int32, k[1][0], "pos")
+    r = RotaryStruct()
+    if freq is not None:
+        _freq_ok(freq)
+        r.rot_dims, r.half = 2 * freq[1][0], 1 if half else 0
+    _on_device((k, v, q, q_out, pos, freq))
+    return bytes(c), bytes(s), bytes(a), bytes(r)
+
+
+def _cache_pointers(c, s, cache, table, seq_start, past):
+    c, s = KVCacheStruct.from_buffer_copy(c), KVSeqs.from_buffer_copy(s)
+    c.k, c.v = cache.k.data_ptr(), cache.v.data_ptr()
+    if cache.k_scale is not None:
+        c.k_scale, c.v_scale = cache.k_scale.data_ptr(), cache.v_scale.data_ptr()
+    s.table, s.seq_start, s.past = table.data_ptr(), seq_start.data_ptr(), past.data_ptr()
+    return c, s
+
+
+def cache_append(cache, k, v, table, seq_start, past, rot=None, pos=None, q=None, q_out=None):
+    """Store the new tokens' k and v ([rows, kv_heads, dim], bf16 or fp32, any strides with dim
+    contiguous), k rotated by rot (Rotary) on the way, and q ([rows, heads, dim]) rotated in the
+    same launch -> q_out (which may be q), or None without q.  Rows seq_start[b] up to seq_start[b + 1]
+    (int32 [seqs + 1]) are sequence b's tokens from place past[b] (int32 [seqs]) on; place t
+    lies in page table[b, t // page] (int32 [seqs, pages]).  Positions are the places, or pos
+    (int32 [rows]).  All of these are read on the device."""
+    if q is not None and q_out is None:
+        q_out = q.new_empty(q.shape)
+    freq = None if rot is None else rot.freq
+    plan = _append_plan(_meta(cache.k), _meta(cache.v), _meta(cache.k_scale), _meta(cache.v_scale), _meta(table), _meta(seq_start),
+                        _meta(past), _meta(k), _meta(v), _meta(q), None if q is None else _meta(q_out), _meta(pos), _meta(freq),
+                        None if rot is None else rot.half, _torch().cuda.current_device())
+    c, s = _cache_pointers(plan[0], plan[1], cache, table, seq_start, past)
+    a = KVAppendArgs.from_buffer_copy(plan[2])
+    a.k, a.v = k.data_ptr(), v.data_ptr()
+    if q is not None:
+        a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
+    if pos is not None:
+        a.pos = pos.data_ptr()
+    r = None
+    if rot is not None:
+        r = RotaryStruct.from_buffer_copy(plan[3])
+        r.freq, r.attn_factor = freq.data_ptr(), rot.attn_factor
+        a.rotary = ctypes.addressof(r)
+    lib = load()
+    check(lib.dt_kv_append(ctypes.addressof(c), ctypes.addressof(s), ctypes.addressof(a), stream()), "dt_kv_append")
+    if isinstance(lib, _Recorder):
+        lib.keep.extend((c, s, a, r))
+    return q_out if q is not None else None
+
+
+@functools.lru_cache(maxsize=512)
+def _cache_attn_plan(ck, cv, k_scale, v_scale, table, seq_start, past, q, out, here):
+    torch = _torch()
+    if len(q[1]) != 3 or q[1][2] != ck[1][3] or q[0] != torch.bfloat16 or q[2][2] != 1:
+        raise DtError("q must be bf16 [rows, heads, dim] of the cache's width, the head dim contiguous")
+    if out[1] != q[1] or out[0] != q[0] or out[2][2] != 1:
+        raise DtError("out must have q's shape and dtype, its head dim contiguous")
+    c, s = _cache_plan(ck, cv, k_scale, v_scale, table, seq_start, past, q[1][0])
+    if q[1][1] % c.kv_heads:
+        raise DtError(f"{q[1][1]} query heads do not share {c.kv_heads} key heads evenly")
+    _on_device((q, out))
+    plan = bytes(c), bytes(s)
+    # The size goes by sizes alone; the pointers stand for the call's own.
+    c.k = c.v = c.k_scale = c.v_scale = s.table = s.seq_start = s.past = 16
+    n = _sizing().dt_kv_attn_workspace_bytes(ctypes.addressof(c), ctypes.addressof(s), q[1][1])
+    return *plan, _I64x2(*q[2][:2]), _I64x2(*out[2][:2]), n
+
+
+def cache_attn(q, cache, table, seq_start, past, causal=True, scale=None, out=None):
+    """Attention of the new tokens' q (bf16 [rows, heads, dim], any strides with dim contiguous)
+    to what their sequences hold in the cache, the new tokens included: softmax(scale q k^T) v over
+    the tokens up to each row's own (causal) or over all -> bf16 [rows, heads, dim].  table,
+    seq_start and past as cache_append's (past: before the new tokens).  scale: >= 0, by default
+    dim ** -0.5.  Rows of no sequence are left as they are."""
+    if out is None:
+        out = q.new_empty(q.shape)
+    c, s, q_st, o_st, n = _cache_attn_plan(_meta(cache.k), _meta(cache.v), _meta(cache.k_scale), _meta(cache.v_scale), _meta(table),
+                                           _meta(seq_start), _meta(past), _meta(q), _meta(out), _torch().cuda.current_device())
+    c, s = _cache_pointers(c, s, cache, table, seq_start, past)
+    ws = _scratch_by(q, n) if n else None
+    lib = load()
+    check(lib.dt_kv_attn(ctypes.addressof(c), ctypes.addressof(s), q.data_ptr(), q_st, q.shape[1], 1 if causal else 0,
+                         c.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), o_st, None if ws is None else ws.data_ptr(),
+                         n, stream()), "dt_kv_attn")
+    if isinstance(lib, _Recorder):
+        lib.keep.extend((c, s))
+    return out
 
 
 # --------------------------------------------------------------------------

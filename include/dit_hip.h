@@ -60,7 +60,8 @@ extern "C" {
  * DT_TYPE_CONV2D_PACKED: a Conv2d weight [Co][Ci][K][K] packed by
  * dt_conv2d_pack_weights, the layout dt_conv2d reads (ne = {K, K, Ci, Co},
  * dt_conv2d_packed_bytes(Co, Ci, K) bytes; nb is not used).  As src0 of
- * DT_OP_CONV_2D_DIRECT it spares the executor a repack per call. */
+ * DT_OP_CONV_2D_DIRECT it spares the executor a repack per call.
+ * DT_TYPE_F8_E4M3: what a dt_kv_cache may hold (OCP e4m3, no infinities), no tensor's type. */
 enum {
     DT_TYPE_F32 = 0,
     DT_TYPE_F16 = 1,
@@ -69,7 +70,8 @@ enum {
     DT_TYPE_I32 = 26,
     DT_TYPE_BF16 = 30,
     DT_TYPE_Q8_0_SPLIT = 100,
-    DT_TYPE_CONV2D_PACKED = 101
+    DT_TYPE_CONV2D_PACKED = 101,
+    DT_TYPE_F8_E4M3 = 102
 };
 
 enum {
@@ -563,6 +565,118 @@ typedef struct dt_lora {
 size_t dt_lora_gemm_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t rank);
 int dt_lora_gemm(const dt_gemm_problem *problem, const dt_lora *lora, int32_t c_type, void *workspace,
                  size_t workspace_bytes, dt_stream_t stream);
+
+/* ---- text serving: rotary positions, a paged key/value cache, attention to it -- */
+
+/* Rotary positions: pair i of a head at position p turns by p * freq[i] radians,
+ *   (x, y) -> f (x cos - y sin, y cos + x sin),  f = attn_factor,
+ * the pair being elements (2i, 2i + 1), or (i, i + rot_dims / 2) with `half`; elements
+ * from rot_dims on stay as they are.  freq: fp32 [rot_dims / 2], device.  Angles are
+ * formed in 64 bits: positions may be any int32.  dt_rope_table_fill's rotation (the
+ * image model's, src/ggml/Runtime.hpp:281-293 in mode NORMAL) keeps ggml's fp32
+ * recurrence instead. */
+typedef struct dt_rotary {
+    const float *freq;
+    int64_t rot_dims;
+    int32_t half;
+    float attn_factor;
+} dt_rotary;
+
+/* Host-side: freq[i] = base^(-2i / rot_dims) (`freq` is HOST memory), scaled for a
+ * context `factor` times as long as the `context` tokens it was made for: a pair that
+ * makes up to turns_low turns within it is slowed by factor, one that makes
+ * turns_high or more is kept, those between are blended linearly in their turns.
+ * context 0: all are slowed.  factor 1: none. */
+int dt_rotary_freq_fill(float *freq, int64_t rot_dims, double base, double factor, int64_t context, double turns_low,
+                        double turns_high);
+
+/* Rotates q and k in one launch (either may be NULL).  Element (b, s, h, d) of q is
+ * q[b*q_strides[0] + s*q_strides[1] + h*q_strides[2] + d]; likewise k, which has
+ * kv_heads heads, and the outputs; position pos[b*pos_stride + s] (int32, device).
+ * An output may be its input (same pointer and strides) and else overlaps nothing.
+ * backward: the rotation back, which makes the gradients of dt_rotary_apply's inputs
+ * from those of its outputs.  Any head_dim up to 4096, alignment and strides (those of
+ * dimensions of one element are not read); whole 16-byte rows with head_dim % 16 == 0
+ * (and, with half, rot_dims % 16 == 0) are fast.  Computed in fp32, rounded once. */
+typedef struct dt_rotary_args {
+    const void *q, *k;
+    void *q_out, *k_out;
+    int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3];
+    int64_t batch, seq, heads, kv_heads, head_dim;
+    const int32_t *pos;
+    int64_t pos_stride;
+    dt_rotary rotary;
+    int32_t io_type, backward;
+} dt_rotary_args;
+int dt_rotary_apply(const dt_rotary_args *args, dt_stream_t stream);
+
+/* Keys and values in pages of `page` tokens (16, 32, 64, 128 or 256), a pool of `pages`
+ * of them:  k [pages][kv_heads][page][head_dim],  v [pages][kv_heads][head_dim][page]
+ * (a value's tokens side by side, as the product over them reads them), 16-byte
+ * aligned, head_dim a multiple of 16 up to 128.  type BF16, or F8_E4M3 with a power of
+ * two for each page and head: a code stands for code * 2^(scale - 127), k_scale and
+ * v_scale uint8 [pages][kv_heads], 1 to 254.  All device memory. */
+typedef struct dt_kv_cache {
+    void *k, *v;
+    uint8_t *k_scale, *v_scale;
+    int64_t pages, kv_heads, page, head_dim;
+    int32_t type;
+} dt_kv_cache;
+
+/* What a call works on: the new tokens of `seqs` sequences, side by side as `rows`
+ * rows.  Rows seq_start[b] .. seq_start[b + 1] - 1 (int32 [seqs + 1], device, ascending)
+ * belong to sequence b, which holds past[b] tokens already (int32 [seqs], device; below
+ * 0: 0); row seq_start[b] + i is its token past[b] + i, and token t lies in page
+ * table[b*table_stride + t / page] (int32 [seqs][table_pages], device), row t % page.
+ * Everything about lengths is read on the device: a captured launch serves
+ * other lengths and tables in place.  Rows of no sequence are neither read nor
+ * written.  A page number outside [0, pages) is no page, as is anything past the
+ * table: tokens there are not stored, and not attended to. */
+typedef struct dt_kv_seqs {
+    const int32_t *table;
+    int64_t table_stride, table_pages;
+    const int32_t *seq_start, *past;
+    int64_t seqs, rows;
+} dt_kv_seqs;
+
+/* Stores the new tokens' k and v (rows [kv_heads][head_dim], strides {row, head}), and
+ * rotates q (heads heads; NULL: none) into q_out in the same launch, which may be q.
+ * rotary NULL: nothing is rotated, and q must be NULL.  Positions are the tokens' places,
+ * or pos[row] (int32 [rows]) where pos is given.  With half, rot_dims is a multiple of 16.
+ * F8_E4M3: a page's scale is the least power of two (2^-126 at least) by which e4m3's
+ * 448 reaches every finite value of its tokens up to the last one stored; codes are
+ * the nearest e4m3 of value / scale, those of values that are not finite NaN.  Where
+ * a page's scale grows, its earlier codes are rounded again to the new one (which moves
+ * them only below 2^-6 of it).  A page that is begun anew (its first token is
+ * stored) forgets what it held.  A page that is written belongs to one sequence of
+ * the call.  k, v, q: io_type BF16 or F32, rows 16-byte aligned.  k is
+ * rotated in 64 bits and rounded once. */
+typedef struct dt_kv_append_args {
+    const void *k, *v, *q;
+    void *q_out;
+    int64_t k_strides[2], v_strides[2], q_strides[2], q_out_strides[2];
+    int64_t heads;
+    const dt_rotary *rotary;
+    const int32_t *pos;
+    int32_t io_type;
+} dt_kv_append_args;
+int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_append_args *args, dt_stream_t stream);
+
+/* Attention of the new tokens' q (bf16, rows [heads][head_dim], strides {row, head}; query
+ * head h reads key head h / (heads / kv_heads)) to what their sequences hold, the new
+ * tokens included (append them first):
+ *   o_i = sum_j softmax_j(scale <q_i, k_j>) v_j
+ * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
+ * not attended to holds is not used (it may be NaN); a row without any has o = 0.
+ * Operands bf16 (e4m3 codes times their scale are exact in it), the softmax's weights
+ * rounded to bf16 after their sum is taken, sums in fp32.  o: bf16; it must not overlap
+ * an input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
+ * aligned) is needed; its size goes by the number of rows, heads and sequences, not by the
+ * lengths.  No atomics: the same call gives the same bits. */
+size_t dt_kv_attn_workspace_bytes(const dt_kv_cache *cache, const dt_kv_seqs *seqs, int64_t heads);
+int dt_kv_attn(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const void *q, const int64_t *q_strides, int64_t heads,
+               int32_t causal, float scale, void *o, const int64_t *o_strides, void *workspace, size_t workspace_bytes,
+               dt_stream_t stream);
 
 /* ======================================================================== */
 /* (iii) unfused ggml-op kernels on ggml-shaped descriptors                 */
