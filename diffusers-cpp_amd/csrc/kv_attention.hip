@@ -19,18 +19,20 @@
 
 #include <type_traits>
 
+#include "attn_tiles.hpp"
 #include "kv_cache.hpp"
 
 namespace dit {
 namespace kv {
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+using attn::bf16x8_t;
+using attn::f32x16_t;
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kRows = 16;      // rows of a block
+constexpr int kRows = 16;      // rows of a block of the stream's
+constexpr int kFew = 32;       // beside the row blocks' kernel the stream takes sequences of up to so many rows
 
 struct Args {
     Cache c;
@@ -41,9 +43,13 @@ struct Args {
     int32_t heads, group, causal;
     FastDiv group_div;
     float scale_log2;
-    int32_t waves;        // a key head
+    int32_t few;          // sequences of up to so many rows (new tokens times heads of a group) are the stream's
+    int32_t splits;       // key ranges of the others' row blocks
+    int32_t waves;        // the stream's, a key head
     float* part_o;        // [kv_heads][waves][2][kRows][DP], unnormalised
     float* part_ml;       // [kv_heads][waves][2][kRows][2]: reference (log2), sum
+    float* rows_o;        // [splits][rows][heads][DP], as part_o
+    float* rows_ml;       // [splits][rows][heads][2]
 };
 
 // Units of sequence b, this lane's; 0 past the last sequence.
@@ -51,7 +57,7 @@ template <int STEP>
 __device__ __forceinline__ int64_t units_of(const Args& a, int b, int* tiles = nullptr) {
     if (b >= a.s.seqs) return 0;
     const Seq q(a.s, b);
-    if (q.n == 0) return 0;
+    if (q.n == 0 || q.n * (int64_t)a.group > a.few) return 0;
     const int t = max((q.len + STEP - 1) / STEP, 1);
     if (tiles) *tiles = t;
     return (int64_t)((q.n * (int64_t)a.group + kRows - 1) / kRows) * t;
@@ -204,6 +210,7 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                     qf[c][m] = __builtin_bit_cast(bf16x8_t, z);
                 }
         }
+        bool wild = false;
         float m = -INFINITY, l = 0.f;
         f32x4_t o[DB];
 #pragma unroll
@@ -271,8 +278,7 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d) vr[d] = leading<ES>(vr[d], holds);
             }
-            // So have those that only later rows of the block see; what is none is added to these rows below.
-            bool wild = false;
+            // So have those that only some rows of the block see; what is none is added to these rows at the end.
             if ((t + 1) * STEP > all) {
                 uint32_t any = 0;
 #pragma unroll
@@ -281,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                     any |= wx | wy | wz | ww;
                     vr[d] = make_uint4(vr[d].x & ~wx, vr[d].y & ~wy, vr[d].z & ~wz, vr[d].w & ~ww);
                 }
-                wild = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+                wild |= __builtin_amdgcn_ballot_w64(any != 0) != 0;
             }
 
             float mx = -INFINITY;
@@ -324,19 +330,18 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
 #pragma unroll
                 for (int mm = 0; mm < M; ++mm) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[mm], pf[mm], o[d], 0, 0, 0);
             }
-            if (wild) {
-                for (int key = t * STEP; key < min((t + 1) * STEP, sq.len); ++key) {
-                    const int p = page_of(a.s, b, key);
-                    if (p < 0 || key >= limit) continue;
-                    const uint8_t* at = a.c.v + ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes + (key & pmask) * ES;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (16 * d < dim) o[d][i] += Held<E>::value(at + (16 * d + 4 * g + i) * vrow);
-                }
-            }
         }
+        if (wild)
+            for (int key = max(t0, all / STEP) * STEP; key < min(t1 * STEP, sq.len); ++key) {
+                const int p = page_of(a.s, b, key);
+                if (p < 0 || key >= limit) continue;
+                const uint8_t* at = a.c.v + ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes + (key & pmask) * ES;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * d < dim) o[d][i] += Held<E>::value(at + (16 * d + 4 * g + i) * vrow);
+            }
 
         l = xor_sum(l);
         if (t0 == 0 && t1 == tiles) {
@@ -363,47 +368,50 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
     }
 }
 
-// The partial results of a row (token, head): TPR threads, each every PL-th wave's share of four elements.
+// The partial results of a row: TPR threads, each every PL-th wave's share of four elements.  Rows are
+// numbered as (token, head), or, beside the row blocks' kernel, as (sequence, key head, row of up to kFew).
 template <typename E, int DP, int TPR>
 __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
     constexpr int STEP = 4 * (16 / (int)sizeof(E)), LPD = DP / 4, PL = TPR / LPD;
     __shared__ float part[256][6];
     const int tid = threadIdx.x, sub = tid % TPR, pl = sub / LPD, d0 = (sub % LPD) * 4;
     const int64_t id = (int64_t)blockIdx.x * (256 / TPR) + __builtin_amdgcn_readfirstlane(tid / TPR);
-    const int r = (int)(id / a.heads), head = (int)(id - (int64_t)r * a.heads);
+    const bool by_seq = a.few == kFew;
+    const int r0 = by_seq ? 0 : (int)(id / a.heads);
+    int b = by_seq ? (int)(id / (a.c.kv_heads * kFew)) : r0 < a.s.rows ? find_seq(a.s, r0, [](int start, int) { return start; }) : -1;
+    if (b >= a.s.seqs) b = -1;
     float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     bool join = false;
-    if (r < a.s.rows) {
-        const int b = find_seq(a.s, r, [](int start, int) { return start; });
+    int r = 0, head = 0;
+    if (b >= 0) {
         const int64_t total = total_units<STEP>(a);
-        if (b >= 0 && total > 0) {
-            const Seq sq(a.s, b);
+        const Seq sq(a.s, b);
+        const int h = by_seq ? (int)(id / kFew % a.c.kv_heads) : (int)(id % a.heads) / a.group;
+        const int row = by_seq ? (int)(id % kFew) : (r0 - sq.row) * a.group + (int)(id % a.heads) % a.group;
+        r = sq.row + row / a.group;
+        head = h * a.group + row % a.group;
+        if (total > 0 && row < sq.n * (int64_t)a.group && sq.n * (int64_t)a.group <= a.few) {
             // The units before sequence b.
             const int lane = tid & 63;
             int64_t n = 0;
             for (int b0 = 0; b0 < b; b0 += 64) n += b0 + lane < b ? units_of<STEP>(a, b0 + lane) : 0;
             n = __shfl(scan64(n), 63, 64);
-            if (r - sq.row < sq.n) {
-                const int h = head / a.group, row = (r - sq.row) * a.group + head - h * a.group;
-                const int tiles = max((sq.len + STEP - 1) / STEP, 1);
-                const int64_t s0 = n + (int64_t)(row / kRows) * tiles, W = working(a, total);
-                const int w0 = (int)(((s0 + 1) * W - 1) / total), w1 = (int)(((s0 + tiles) * W - 1) / total);
-                join = w0 != w1;
-                if (join) {
-                    for (int w = w0 + pl; w <= w1; w += PL) {
-                        const int64_t at = (((int64_t)h * a.waves + w) * 2 + (w == w0 ? 1 : 0)) * kRows + row % kRows;
-                        const float m1 = a.part_ml[2 * at], l1 = a.part_ml[2 * at + 1];
-                        const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * DP + d0);
-                        const float to = fmaxf(m, m1), ref = to == -INFINITY ? 0.f : to;
-                        const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
-                        m = to;
-                        l = l * f0 + l1 * f1;
-                        v[0] = v[0] * f0 + x.x * f1;
-                        v[1] = v[1] * f0 + x.y * f1;
-                        v[2] = v[2] * f0 + x.z * f1;
-                        v[3] = v[3] * f0 + x.w * f1;
-                    }
-                }
+            const int tiles = max((sq.len + STEP - 1) / STEP, 1);
+            const int64_t s0 = n + (int64_t)(row / kRows) * tiles, W = working(a, total);
+            const int w0 = (int)(((s0 + 1) * W - 1) / total), w1 = (int)(((s0 + tiles) * W - 1) / total);
+            join = w0 != w1;
+            for (int w = w0 + pl; join && w <= w1; w += PL) {
+                const int64_t at = (((int64_t)h * a.waves + w) * 2 + (w == w0 ? 1 : 0)) * kRows + row % kRows;
+                const float m1 = a.part_ml[2 * at], l1 = a.part_ml[2 * at + 1];
+                const float4 x = *reinterpret_cast<const float4*>(a.part_o + at * DP + d0);
+                const float to = fmaxf(m, m1), ref = to == -INFINITY ? 0.f : to;
+                const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
+                m = to;
+                l = l * f0 + l1 * f1;
+                v[0] = v[0] * f0 + x.x * f1;
+                v[1] = v[1] * f0 + x.y * f1;
+                v[2] = v[2] * f0 + x.z * f1;
+                v[3] = v[3] * f0 + x.w * f1;
             }
         }
     }
@@ -431,32 +439,361 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
         make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
 }
 
+// ---- many rows: 256 rows per workgroup, 32 per wave, tiles of 64 keys ---------------------
+// The cache's tile is turned into bf16 once for the workgroup, on its way through registers
+// into LDS (two buffers), and every wave multiplies from there on v_mfma_f32_32x32x16_bf16, again
+// transposed: a lane holds one row.  LDS row 8 a + 4 g + c of a tile's 16 holds key 8 g + 4 a + c, so
+// that a lane's scores are those of 8 keys in order, and a value's operand one 16-byte piece.
+constexpr int kBlock = 256, kTile = 64;
+
+// The row blocks are numbered like the pages that are written (kv_index.hpp).
+__device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / kBlock + b; }
+
+template <typename E, int DP>
+__global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
+    typedef attn::Tile<bf16, DP> KT;
+    typedef attn::Tile<bf16, kTile> VT;
+    constexpr int ES = sizeof(E), KPL = 16 / ES, M = Held<E>::N;
+    constexpr int KCH = DP / KPL, VCH = kTile / KPL;                           // 16-byte pieces of a row
+    constexpr int J = (kTile * KCH + 511) / 512;                               // a thread's
+    constexpr int KBYTES = kTile * KT::RB, VBYTES = DP * VT::RB, BUF = KBYTES + VBYTES;
+    static_assert(kTile * KCH == DP * VCH, "pieces");
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];             // [buffer][K | V]
+    __shared__ uint32_t paged[2];                                              // a byte per 16 keys: whether they have a page
+    __shared__ int wild_seen;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, g = lane >> 5;
+
+    // Heads innermost: an XCD's workgroups share them.  The longest rows first.
+    const uint32_t bid = blockIdx.x, n_items = gridDim.x / (uint32_t)(a.c.kv_heads * a.splits);
+    const int h = (int)(bid % (uint32_t)a.c.kv_heads);
+    const uint32_t rest = bid / (uint32_t)a.c.kv_heads;
+    const int split = (int)(rest % (uint32_t)a.splits);
+    const int64_t item = (int64_t)n_items - 1 - rest / (uint32_t)a.splits;
+    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block(a, start, i); });
+    if (b < 0) return;
+    const Seq sq(a.s, b);
+    const int64_t all_rows = sq.n * (int64_t)a.group, row0 = (item - first_block(a, sq.row, b)) * kBlock;
+    if (all_rows <= a.few || row0 < 0 || row0 >= all_rows) return;
+    const int rows = (int)all_rows, last = min((int)row0 + kBlock, rows) - 1;
+    const int most = a.causal ? min(sq.past + (int)fdiv((uint32_t)last, a.group_div) + 1, sq.len) : sq.len;   // places some row sees
+    const int all = a.causal ? min(sq.past + (int)fdiv((uint32_t)row0, a.group_div) + 1, sq.len) : sq.len;  // and every row
+    const int tiles = (most + kTile - 1) / kTile;
+    const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+
+    const int row = (int)row0 + wave * 32 + r;
+    const bool live = row < rows;
+    const int tok = live ? (int)fdiv((uint32_t)row, a.group_div) : 0, head = h * a.group + (live ? row - tok * a.group : 0);
+    const int limit = !live ? all : a.causal ? min(sq.past + tok + 1, sq.len) : sq.len;
+    const int wave_last = min((int)row0 + wave * 32 + 31, rows - 1);  // below the wave's first row: it has none
+    const int wave_most = wave_last < (int)row0 + wave * 32 ? 0 : a.causal ? min(sq.past + (int)fdiv((uint32_t)wave_last, a.group_div) + 1, sq.len) : sq.len;
+
+    const int dim = a.c.dim, lg = a.c.page_log2, pmask = (1 << lg) - 1, krow = dim * ES, vrow = ES << lg;
+    struct Stage {
+        uint4 k[J], v[J];
+        float ks[J], vs[J];
+        int holds[J];
+    } st;
+    int kpage[J], vpage[J];  // of the next tile to be loaded
+    auto find_pages = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + 512 * j, kp = t * kTile + i / KCH, vp = t * kTile + i % VCH * KPL;
+            kpage[j] = kp < sq.len ? page_of(a.s, b, kp) : -1;
+            vpage[j] = vp < sq.len ? page_of(a.s, b, vp) : -1;
+        }
+    };
+    auto load = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + 512 * j;
+            st.k[j] = st.v[j] = make_uint4(0, 0, 0, 0);
+            st.ks[j] = st.vs[j] = 1.f;
+            st.holds[j] = 0;
+            if (kTile * KCH % 512 && i >= kTile * KCH) continue;
+            const int key = i / KCH, kc = i % KCH, d = i / VCH, vc = i % VCH;
+            const int kp = t * kTile + key, vp = t * kTile + vc * KPL;
+            if (kpage[j] >= 0 && 16 * kc < krow) {
+                const int64_t at = (int64_t)kpage[j] * a.c.kv_heads + h;
+                st.k[j] = *reinterpret_cast<const uint4*>(a.c.k + at * a.c.head_bytes + (kp & pmask) * (int64_t)krow + 16 * kc);
+                if constexpr (ES == 1) st.ks[j] = __uint_as_float((uint32_t)max((int)a.c.k_scale[at], 1) << 23);
+            }
+            if (vpage[j] >= 0) {
+                const int64_t at = (int64_t)vpage[j] * a.c.kv_heads + h;
+                if (d < dim) st.v[j] = *reinterpret_cast<const uint4*>(a.c.v + at * a.c.head_bytes + d * (int64_t)vrow + (vp & pmask) * ES);
+                if constexpr (ES == 1) st.vs[j] = __uint_as_float((uint32_t)max((int)a.c.v_scale[at], 1) << 23);
+                st.holds[j] = min(sq.len - vp, KPL);
+            }
+        }
+    };
+    auto store = [&](int t, int buf) {
+        uint8_t* kb = smem + buf * BUF;
+        uint8_t* vb = kb + KBYTES;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + 512 * j;
+            if (kTile * KCH % 512 && i >= kTile * KCH) continue;
+            const int key = i / KCH, kc = i % KCH, d = i / VCH, vc = i % VCH;
+            const int lr = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
+            uint4 v = st.v[j];
+            // What lies behind the sequence is anything: values of weight 0 have to be numbers.
+            if (__builtin_amdgcn_ballot_w64(st.holds[j] < KPL)) v = leading<ES>(v, st.holds[j]);
+            // So have those that only some rows see; what is none is added to those rows apart.
+            if ((t + 1) * kTile > all) {
+                const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
+                if (wx | wy | wz | ww) wild_seen = 1;
+                v = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
+            }
+            bf16x8_t kf[M], vf[M];
+            Held<E>::get(st.k[j], st.ks[j], kf);
+            Held<E>::get(v, st.vs[j], vf);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                *reinterpret_cast<bf16x8_t*>(kb + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) = kf[m];
+                *reinterpret_cast<bf16x8_t*>(vb + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) = vf[m];
+            }
+            if (d == 0 && vc * KPL % 16 == 0) reinterpret_cast<uint8_t*>(&paged[buf])[vc * KPL / 16] = st.holds[j] > 0;
+        }
+    };
+
+    typename KT::Frag qf[KT::STEPS];
+    {
+        const uint16_t* qp = a.q + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
+#pragma unroll
+        for (int c = 0; c < KT::STEPS; ++c)
+            qf[c] = live ? attn::frag_global<bf16>(reinterpret_cast<const bf16*>(qp), c, g, dim) : attn::frag_zero<bf16>();
+    }
+    if (tid == 0) wild_seen = 0;
+    attn::Running<bf16, KT::BLOCKS> run;
+    run.clear();
+    const float sc = a.scale_log2;
+    if (t0 < t1) {
+        find_pages(t0);
+        load(t0);
+        find_pages(t0 + 1);
+    }
+    __syncthreads();  // wild_seen is cleared
+    if (t0 < t1) store(t0, 0);
+    int buf = 0;
+    for (int t = t0; t < t1; ++t, buf ^= 1) {
+        __syncthreads();
+        if (t + 1 < t1) {
+            load(t + 1);
+            find_pages(t + 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* Kt = smem + buf * BUF;
+        const uint8_t* Vt = Kt + KBYTES;
+        if (t * kTile < wave_most) {
+            const uint32_t has = __builtin_amdgcn_readfirstlane(paged[buf]);
+            f32x16_t s[2] = {attn::zero16(), attn::zero16()};
+            attn::FragParts<bf16> p[2][2];
+            float sum[2] = {0.f, 0.f};
+            auto scores = [&](auto hc, auto vc, auto side) {
+                constexpr int hh = decltype(hc)::value;
+                attn::products<bf16, KT::STEPS, 1, decltype(vc)::value>(
+                    [&](int i) { return KT::row_frag(Kt, 32 * hh + r, i, g); },
+                    [&](int i, const typename KT::Frag& f) { s[hh] = attn::mma(f, qf[i], s[hh]); }, side);
+            };
+            // Element 8 j + e is key 16 j + 8 g + e of the half.
+            auto finish = [&](auto hc) {
+                constexpr int hh = decltype(hc)::value;
+                if ((t + 1) * kTile > all) {
+                    const int sees = limit - (t * kTile + 32 * hh + 8 * g);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (16 * (i >> 3) + (i & 7) >= sees) s[hh][i] = -INFINITY;
+                }
+                if (has != 0x01010101u) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (!(has >> (8 * (2 * hh + j)) & 1)) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) s[hh][8 * j + e] = -INFINITY;
+                        }
+                }
+            };
+            auto weights = [&](auto hc) {
+                return [&, hc](int part, int of) {
+#pragma unroll
+                    for (int i4 = 0; i4 < 4; ++i4)
+                        if (i4 * of / 4 == part) run.weigh(s[hc], sc, i4, p[hc], sum[hc]);
+                };
+            };
+            auto values = [&](auto hc, auto vc, auto side) {
+                constexpr int hh = decltype(hc)::value;
+                attn::products<bf16, 2 * KT::BLOCKS, 1, decltype(vc)::value>(
+                    [&](int i) { return VT::row_frag(Vt, 32 * (i % KT::BLOCKS) + r, 2 * hh + i / KT::BLOCKS, g); },
+                    [&](int i, const typename KT::Frag& f) {
+                        run.o[i % KT::BLOCKS] = attn::mma(f, p[hh][i / KT::BLOCKS].frag(), run.o[i % KT::BLOCKS]);
+                    },
+                    side);
+            };
+            using H0 = std::integral_constant<int, 0>;
+            using H1 = std::integral_constant<int, 1>;
+            using V = std::integral_constant<int, DP == 64 ? 12 : 6>;  // vector instructions per product
+            scores(H0{}, H0{}, attn::NoSide{});
+            finish(H0{});
+            run.look(s[0], sc);
+            scores(H1{}, V{}, weights(H0{}));
+            finish(H1{});
+            if (run.look(s[1], sc)) {  // the first half's weights again, by the new reference
+                sum[0] = 0.f;
+                weights(H0{})(0, 1);
+            }
+            values(H0{}, V{}, weights(H1{}));
+            values(H1{}, H0{}, attn::NoSide{});
+            run.l += sum[0] + sum[1];
+        }
+        if (t + 1 < t1) store(t + 1, buf ^ 1);
+    }
+    __syncthreads();
+    if (wild_seen)
+        for (int key = max(t0, all / kTile) * kTile; key < min(t1 * kTile, sq.len); ++key) {
+            const int p = page_of(a.s, b, key);
+            if (p < 0 || key >= limit) continue;
+            const uint8_t* at = a.c.v + ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes + (key & pmask) * ES;
+#pragma unroll
+            for (int d = 0; d < KT::BLOCKS; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int e = 32 * d + 8 * (i >> 2) + 4 * g + (i & 3);
+                    if (e < dim) run.o[d][i] += Held<E>::value(at + (int64_t)e * vrow);
+                }
+        }
+
+    const float l = run.l + attn::swap32(run.l);
+    if (!live) return;
+    if (a.splits == 1) {
+        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no place seen: 0; NaN stays
+        bf16* op = reinterpret_cast<bf16*>(a.o) + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
+#pragma unroll
+        for (int d = 0; d < KT::BLOCKS; ++d)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const int e0 = 32 * d + 8 * i4 + 4 * g;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = run.o[d][4 * i4 + e] * inv;
+                if (e0 < dim) attn::put4(op + e0, v);
+            }
+        return;
+    }
+    const int64_t at = ((int64_t)split * a.s.rows + sq.row + tok) * a.heads + head;
+#pragma unroll
+    for (int d = 0; d < KT::BLOCKS; ++d)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = run.o[d][4 * i4 + e];
+            attn::put4(a.rows_o + at * DP + 32 * d + 8 * i4 + 4 * g, v);
+        }
+    if (g == 0) {
+        a.rows_ml[2 * at] = run.m;
+        a.rows_ml[2 * at + 1] = l;
+    }
+}
+
+// The key ranges of a row, joined in their order: a thread per four elements.
+template <int DP>
+__global__ __launch_bounds__(256) void kv_rows_join_kernel(const Args a) {
+    constexpr int TPR = DP / 4;
+    const int64_t n = (int64_t)a.s.rows * a.heads, id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR;
+    const int d = (int)(threadIdx.x % TPR) * 4;
+    // The sequences of the wave's rows, one after the other, by the whole wave.
+    bool mine = false;
+#pragma unroll
+    for (int k = 0; k < 64 / TPR; ++k) {
+        const int r = min(__shfl((int)(id / a.heads), k * TPR, 64), a.s.rows - 1);
+        const int b = find_seq(a.s, r, [](int start, int) { return start; });
+        if (b < 0) continue;
+        const Seq sq(a.s, b);
+        if ((int)(threadIdx.x & 63) / TPR == k) mine = r - sq.row < sq.n && sq.n * (int64_t)a.group > a.few;
+    }
+    if (!mine || id >= n || d >= a.c.dim) return;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.rows_ml[((int64_t)s * n + id) * 2]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = a.rows_ml + ((int64_t)s * n + id) * 2;
+        const float w = __builtin_amdgcn_exp2f(p[0] - ref);
+        l += w * p[1];
+        const float4 x = *reinterpret_cast<const float4*>(a.rows_o + ((int64_t)s * n + id) * DP + d);
+        v[0] += w * x.x;
+        v[1] += w * x.y;
+        v[2] += w * x.z;
+        v[3] += w * x.w;
+    }
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    const int r = (int)(id / a.heads), head = (int)(id - (int64_t)r * a.heads);
+    attn::put4(reinterpret_cast<bf16*>(a.o) + (int64_t)r * a.os[0] + head * a.os[1] + d, v);
+}
+
 // ---- choice and launch --------------------------------------------------------------
 struct Plan {
-    int waves, dp;
-    int64_t floats;
+    bool stream, rows;
+    int few, waves, dp, splits;
+    int64_t blocks;             // of rows, at most
+    int64_t floats, row_floats;  // workspace: the stream's partial results, the row blocks'
 };
 
-Plan plan(const Cache& c, int cus) {
+// What a sequence's rows are is known on the device: with more rows than sequences both kernels
+// are launched, and each takes its own.
+Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     Plan p{};
-    // Two waves a SIMD in all, whole workgroups of four a key head.
-    p.waves = (8 * cus / c.kv_heads + 3) / 4 * 4;
-    if (p.waves < 4) p.waves = 4;
+    const int64_t group = heads / c.kv_heads, rows = s.rows * group;
     p.dp = c.dim <= 64 ? 64 : 128;
-    p.floats = (int64_t)c.kv_heads * p.waves * 2 * kRows * (p.dp + 2);
+    p.rows = s.rows > s.seqs && rows > kFew;
+    p.stream = !p.rows || s.seqs > 1;
+    p.few = !p.rows ? INT32_MAX : p.stream ? kFew : 0;
+    p.splits = 1;
+    if (p.stream) {
+        // Two waves a SIMD in all, whole workgroups of four a key head.
+        p.waves = (8 * cus / c.kv_heads + 3) / 4 * 4;
+        if (p.waves < 4) p.waves = 4;
+        p.floats = (int64_t)c.kv_heads * p.waves * 2 * kRows * (p.dp + 2);
+    }
+    if (p.rows) {
+        p.blocks = rows / kBlock + s.seqs;
+        const int64_t full = ((rows + kBlock - 1) / kBlock) * c.kv_heads;
+        int64_t n = cus / (full > 0 ? full : 1);
+        const int64_t longest = ((int64_t)s.table_pages << s.page_log2) / (8 * kTile);  // eight tiles a range
+        if (n > longest) n = longest;
+        if (n > 32) n = 32;
+        p.splits = n < 2 ? 1 : (int)n;
+        if (p.splits > 1) p.row_floats = (int64_t)p.splits * s.rows * heads * (p.dp + 2);
+    }
     return p;
 }
 
 template <typename E, int DP>
-int launch(const Args& a, hipStream_t st) {
+int launch(const Args& a, const Plan& p, hipStream_t st) {
+    const int64_t n = (int64_t)a.s.rows * a.heads;
+    if (p.rows) {
+        const dim3 grid((unsigned)(p.blocks * p.splits * a.c.kv_heads));
+        hipLaunchKernelGGL((kv_rows_kernel<E, DP>), grid, dim3(512), 2 * (size_t)(kTile * DP + DP * kTile) * 2, st, a);
+        int rc = check_launch("dt_kv_attn");
+        if (rc) return rc;
+        if (p.splits > 1) {
+            hipLaunchKernelGGL((kv_rows_join_kernel<DP>), dim3((unsigned)((n * (DP / 4) + 255) / 256)), dim3(256), 0, st, a);
+            rc = check_launch("dt_kv_attn");
+            if (rc) return rc;
+        }
+    }
+    if (!p.stream) return DT_OK;
     hipLaunchKernelGGL((kv_stream_kernel<E, DP>), dim3((unsigned)(a.c.kv_heads * (a.waves / 4))), dim3(256), 0, st, a);
     int rc = check_launch("dt_kv_attn");
     if (rc) return rc;
-    const int64_t n = (int64_t)a.s.rows * a.heads;
-    if (n <= 1024) {
-        hipLaunchKernelGGL((kv_join_kernel<E, DP, 256>), dim3((unsigned)n), dim3(256), 0, st, a);
+    // Few rows may each have many shares: a workgroup a row.
+    const int64_t joined = p.few == kFew ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
+    if (joined <= 1024) {
+        hipLaunchKernelGGL((kv_join_kernel<E, DP, 256>), dim3((unsigned)joined), dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((kv_join_kernel<E, DP, 64>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((kv_join_kernel<E, DP, 64>), dim3((unsigned)((joined + 3) / 4)), dim3(256), 0, st, a);
     }
     return check_launch("dt_kv_attn");
 }
@@ -472,7 +809,8 @@ extern "C" size_t dt_kv_attn_workspace_bytes(const dt_kv_cache* cache, const dt_
     Seqs s;
     if (prepare(cache, seqs, "dt_kv_attn_workspace_bytes", &c, &s)) return 0;
     if (s.rows == 0 || s.seqs == 0 || heads <= 0) return 0;
-    return (size_t)plan(c, cu_count()).floats * sizeof(float);
+    const Plan p = plan(c, s, heads, cu_count());
+    return (size_t)(p.floats + p.row_floats) * sizeof(float);
 }
 
 extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, const void* q, const int64_t* q_strides, int64_t heads,
@@ -492,9 +830,12 @@ extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, cons
     if (rc) return rc;
     if (a.s.rows == 0 || a.s.seqs == 0 || heads == 0) return DT_OK;
     DT_REQUIRE((int64_t)a.s.rows * heads < (1ll << 30), "%s: grid too large", who);
-    const Plan p = plan(a.c, cu_count());
-    DT_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= (size_t)p.floats * sizeof(float),
-               "%s: a 16-byte aligned workspace of %lld bytes is needed", who, (long long)(p.floats * sizeof(float)));
+    const Plan p = plan(a.c, a.s, heads, cu_count());
+    const size_t need = (size_t)(p.floats + p.row_floats) * sizeof(float);
+    DT_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+               "%s: a 16-byte aligned workspace of %lld bytes is needed", who, (long long)need);
+    DT_REQUIRE(p.blocks * p.splits * a.c.kv_heads < (1ll << 31) && (int64_t)a.s.seqs * a.c.kv_heads * kFew < (1ll << 31),
+               "%s: grid too large", who);
     a.q = (const uint16_t*)q;
     a.o = (uint16_t*)o;
     for (int i = 0; i < 2; ++i) {
@@ -506,11 +847,15 @@ extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, cons
     a.group_div = make_fastdiv((uint32_t)a.group);
     a.causal = causal != 0;
     // A scale of 0 as the least normal number: -inf times it is still -inf, every finite score next to 0.
-    a.scale_log2 = scale * kLog2e > FLT_MIN ? scale * kLog2e : FLT_MIN;
+    a.scale_log2 = scale * attn::kLog2e > FLT_MIN ? scale * attn::kLog2e : FLT_MIN;
+    a.few = p.few;
+    a.splits = p.splits;
     a.waves = p.waves;
     a.part_o = (float*)workspace;
     a.part_ml = a.part_o + (int64_t)a.c.kv_heads * p.waves * 2 * kRows * p.dp;
+    a.rows_o = a.part_o + p.floats;
+    a.rows_ml = a.rows_o + (int64_t)p.splits * a.s.rows * heads * p.dp;
     const hipStream_t st = (hipStream_t)stream;
-    if (a.c.k_scale) return p.dp == 64 ? launch<e4m3, 64>(a, st) : launch<e4m3, 128>(a, st);
-    return p.dp == 64 ? launch<bf16, 64>(a, st) : launch<bf16, 128>(a, st);
+    if (a.c.k_scale) return p.dp == 64 ? launch<e4m3, 64>(a, p, st) : launch<e4m3, 128>(a, p, st);
+    return p.dp == 64 ? launch<bf16, 64>(a, p, st) : launch<bf16, 128>(a, p, st);
 }

@@ -671,8 +671,8 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  * Operands bf16 (e4m3 codes times their scale are exact in it), the softmax's weights
  * rounded to bf16 after their sum is taken, sums in fp32.  o: bf16; it must not overlap
  * an input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
- * aligned) is needed; its size goes by the number of rows, heads and sequences, not by the
- * lengths.  No atomics: the same call gives the same bits. */
+ * aligned) is needed (0 for some calls); its size goes by the sizes given here, not by the
+ * lengths on the device.  No atomics: the same call gives the same bits. */
 size_t dt_kv_attn_workspace_bytes(const dt_kv_cache *cache, const dt_kv_seqs *seqs, int64_t heads);
 int dt_kv_attn(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const void *q, const int64_t *q_strides, int64_t heads,
                int32_t causal, float scale, void *o, const int64_t *o_strides, void *workspace, size_t workspace_bytes,
