@@ -62,6 +62,51 @@ __device__ __forceinline__ void finish_scores(f32x16_t& s, float sc, uint32_t wo
     }
 }
 
+// The running softmax of one query: reference m (log2), this lane's half of the sum.
+// Scores are in units of 1 / sc of log2 (sc > 0; 1 with a bias).
+template <typename T, int BLOCKS>
+struct Running {
+    float m, l;
+    f32x16_t o[BLOCKS];
+
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) o[b] = zero16();
+    }
+    // Whether the reference moved.  It does only when a score exceeds it by more than 2^8, so
+    // most tiles skip the rescale, and every weight stays <= 256.
+    __device__ __forceinline__ bool look(const f32x16_t& s, float sc) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, swap32(mx)) * sc;
+        const bool move = mx > m + 8.0f;
+        if (__builtin_amdgcn_ballot_w64(move) == 0) return false;
+        const float to = move ? mx : m;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        l *= alpha;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+        m = to;
+        return true;
+    }
+    // The weights of elements 4 i4 .. + 3 into their operand, and added to `sum` before that
+    // rounds them: lse, from which the gradients' weights come, stays fp32.
+    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i4, FragParts<T> (&p)[2], float& sum) const {
+        const float ref = m == -INFINITY ? 0.f : m;  // scores of -inf only, so far: weight 0
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], sc, -ref));
+        p[i4 / 2].set(i4 & 1, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[e];
+    }
+};
+
 // The lane's row of a row block.
 struct Row {
     int tok, h;

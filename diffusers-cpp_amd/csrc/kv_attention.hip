@@ -161,6 +161,26 @@ __device__ __forceinline__ uint4 leading(uint4 w, int n) {
     return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
+// Values that are not finite and were left out of the products are added to a row's stored result (or
+// its share, where part is given): elements d .. d + 3, places [from, to).  The lane that stored them
+// calls this.
+template <typename E>
+__device__ __forceinline__ void add_wild(const Args& a, int b, int h, int from, int to, int d, uint16_t* o, float* part) {
+#pragma unroll 1
+    for (int i = d; i < d + 4; ++i) {
+        float x = part ? part[i] : __uint_as_float((uint32_t)o[i] << 16);
+#pragma unroll 1
+        for (int key = from; key < to; ++key) {
+            const int p = page_of(a.s, b, key);
+            if (p < 0) continue;
+            const int64_t at = ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes;
+            x += Held<E>::value(a.c.v + at + (((int64_t)i << a.c.page_log2) + (key & ((1 << a.c.page_log2) - 1))) * sizeof(E));
+        }
+        if (part) part[i] = x;
+        else o[i] = (uint16_t)f32_to_bf16_bits(x);
+    }
+}
+
 template <typename E, int DP>
 __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
     constexpr int ES = sizeof(E), KPL = 16 / ES, STEP = 4 * KPL, M = Held<E>::N;
@@ -331,18 +351,6 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                 for (int mm = 0; mm < M; ++mm) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[mm], pf[mm], o[d], 0, 0, 0);
             }
         }
-        if (wild)
-            for (int key = max(t0, all / STEP) * STEP; key < min(t1 * STEP, sq.len); ++key) {
-                const int p = page_of(a.s, b, key);
-                if (p < 0 || key >= limit) continue;
-                const uint8_t* at = a.c.v + ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes + (key & pmask) * ES;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (16 * d < dim) o[d][i] += Held<E>::value(at + (16 * d + 4 * g + i) * vrow);
-            }
-
         l = xor_sum(l);
         if (t0 == 0 && t1 == tiles) {
             const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no place seen: 0; NaN stays
@@ -363,6 +371,13 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                 a.part_ml[2 * at] = m;
                 a.part_ml[2 * at + 1] = l;
             }
+        }
+        if (wild && live) {
+            uint16_t* op = a.o + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
+            float* part = t0 == 0 && t1 == tiles ? nullptr : a.part_o + ((((int64_t)h * a.waves + w) * 2 + (t0 == 0 ? 1 : 0)) * kRows + col) * DP;
+#pragma unroll 1
+            for (int d = 4 * g; d < dim; d += 16)
+                add_wild<E>(a, b, h, max(t0, all / STEP) * STEP, min(t1 * STEP, limit), d, op, part);
         }
         x = s0 + t1;
     }
@@ -441,24 +456,68 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
 
 // ---- many rows: 256 rows per workgroup, 32 per wave, tiles of 64 keys ---------------------
 // The cache's tile is turned into bf16 once for the workgroup, on its way through registers
-// into LDS (two buffers), and every wave multiplies from there on v_mfma_f32_32x32x16_bf16, again
-// transposed: a lane holds one row.  LDS row 8 a + 4 g + c of a tile's 16 holds key 8 g + 4 a + c, so
-// that a lane's scores are those of 8 keys in order, and a value's operand one 16-byte piece.
+// into LDS, and every wave multiplies from there on v_mfma_f32_32x32x16_bf16, again transposed: a lane
+// holds one row.  LDS row 8 a + 4 g + c of a tile's 16 holds key 8 g + 4 a + c, so that a lane's
+// scores are those of 8 keys in order, and a value's operand one 16-byte piece.
+//
+// The barrier of every tile keeps the waves in step, so each wave's matrix and vector
+// instructions have to overlap by themselves: a step takes 32 keys through three stages at once, the scores of the next 32, the softmax of
+// these, and the product with the values of the 32 before, none of which waits for another.
+// Keys therefore run a tile ahead of values in LDS (two buffers each).
 constexpr int kBlock = 256, kTile = 64;
 
 // The row blocks are numbered like the pages that are written (kv_index.hpp).
 __device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / kBlock + b; }
 
+// The softmax of 32 keys for one row: reference m (log2), this lane's half of the sum.
+template <int BLOCKS>
+struct Softmax {
+    float m, l, before, sum;
+    f32x16_t o[BLOCKS];
+    // The reference for scores s: it moves when one exceeds it by more than 2^8 (every weight stays
+    // <= 256), which the sums before follow in moved().
+    __device__ __forceinline__ bool refer(const f32x16_t& s, float sc) {
+        float mx = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, attn::swap32(mx)) * sc;
+        const bool move = mx > m + 8.0f;
+        before = m;
+        m = move ? mx : m;
+        sum = 0.f;
+        return __builtin_amdgcn_ballot_w64(move) != 0;
+    }
+    // Elements 4 i4 .. + 3 as weights, rounded to bf16 for the product after the sum took them as they are.
+    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i4, attn::FragParts<bf16> (&p)[2]) {
+        const float ref = m == -INFINITY ? 0.f : m;  // scores of -inf only, so far: weight 0
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], sc, -ref));
+        p[i4 / 2].set(i4 & 1, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += v[e];
+    }
+    __device__ __forceinline__ void moved() {
+        const float alpha = m == before ? 1.0f : __builtin_amdgcn_exp2f(before - m);
+        l *= alpha;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
+    }
+};
+
 template <typename E, int DP>
 __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     typedef attn::Tile<bf16, DP> KT;
     typedef attn::Tile<bf16, kTile> VT;
+    typedef typename KT::Frag Frag;
     constexpr int ES = sizeof(E), KPL = 16 / ES, M = Held<E>::N;
     constexpr int KCH = DP / KPL, VCH = kTile / KPL;                           // 16-byte pieces of a row
-    constexpr int J = (kTile * KCH + 511) / 512;                               // a thread's
-    constexpr int KBYTES = kTile * KT::RB, VBYTES = DP * VT::RB, BUF = KBYTES + VBYTES;
-    static_assert(kTile * KCH == DP * VCH, "pieces");
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];             // [buffer][K | V]
+    constexpr int PIECES = kTile * KCH, J = (PIECES + 511) / 512;               // of a tile, a thread's
+    constexpr int KBYTES = kTile * KT::RB, VBYTES = DP * VT::RB;
+    static_assert(PIECES == DP * VCH && (PIECES % 512 == 0 || J == 1), "pieces");
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];             // [2][K], [2][V]
     __shared__ uint32_t paged[2];                                              // a byte per 16 keys: whether they have a page
     __shared__ int wild_seen;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -475,223 +534,254 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     const Seq sq(a.s, b);
     const int64_t all_rows = sq.n * (int64_t)a.group, row0 = (item - first_block(a, sq.row, b)) * kBlock;
     if (all_rows <= a.few || row0 < 0 || row0 >= all_rows) return;
-    const int rows = (int)all_rows, last = min((int)row0 + kBlock, rows) - 1;
-    const int most = a.causal ? min(sq.past + (int)fdiv((uint32_t)last, a.group_div) + 1, sq.len) : sq.len;   // places some row sees
-    const int all = a.causal ? min(sq.past + (int)fdiv((uint32_t)row0, a.group_div) + 1, sq.len) : sq.len;  // and every row
+    const int rows = (int)all_rows, first = (int)row0, last = min(first + kBlock, rows) - 1;
+    // The places that a row sees are those below:
+    auto limit_of = [&](int row) { return a.causal ? min(sq.past + (int)fdiv((uint32_t)row, a.group_div) + 1, sq.len) : sq.len; };
+    const int most = limit_of(last), all = limit_of(first);  // some row sees, every row sees
     const int tiles = (most + kTile - 1) / kTile;
     const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
 
-    const int row = (int)row0 + wave * 32 + r;
+    const int row = first + wave * 32 + r;
     const bool live = row < rows;
     const int tok = live ? (int)fdiv((uint32_t)row, a.group_div) : 0, head = h * a.group + (live ? row - tok * a.group : 0);
-    const int limit = !live ? all : a.causal ? min(sq.past + tok + 1, sq.len) : sq.len;
-    const int wave_last = min((int)row0 + wave * 32 + 31, rows - 1);  // below the wave's first row: it has none
-    const int wave_most = wave_last < (int)row0 + wave * 32 ? 0 : a.causal ? min(sq.past + (int)fdiv((uint32_t)wave_last, a.group_div) + 1, sq.len) : sq.len;
+    const int limit = live ? limit_of(row) : all;
+    // This wave's tiles end where its last row sees no more.
+    const int wave_last = min(first + wave * 32 + 31, rows - 1);
+    const int w1 = wave_last < first + wave * 32 ? t0 : max(t0, min(t1, (limit_of(wave_last) + kTile - 1) / kTile));
 
     const int dim = a.c.dim, lg = a.c.page_log2, pmask = (1 << lg) - 1, krow = dim * ES, vrow = ES << lg;
-    struct Stage {
-        uint4 k[J], v[J];
-        float ks[J], vs[J];
-        int holds[J];
-    } st;
-    int kpage[J], vpage[J];  // of the next tile to be loaded
-    auto find_pages = [&](int t) {
+    // What is on its way stays as it is loaded: whatever looks at it would wait for it.  Threads
+    // without a piece, and places without a page, load another's.
+    uint4 kst[J], vst[J];
+    uint8_t kscale[J], vscale[J];
+    int kpage[J], vpage[J];  // the table's entries for the tiles that are loaded next
+    bool khas[J], vhas[J];   // of those that are stored next: whether they lie in a page
+    int krow_at[J], vrow_at[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int i = min(tid + 512 * j, PIECES - 1), kc = i % KCH, d = i / VCH;
+        krow_at[j] = 16 * kc < krow ? 16 * kc : 0;
+        vrow_at[j] = (d < dim ? d : 0) * vrow;
+    }
+    const int32_t* table = a.s.table + b * a.s.table_stride;
+    auto find_pages = [&](int kt, int vt) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int i = tid + 512 * j, kp = t * kTile + i / KCH, vp = t * kTile + i % VCH * KPL;
-            kpage[j] = kp < sq.len ? page_of(a.s, b, kp) : -1;
-            vpage[j] = vp < sq.len ? page_of(a.s, b, vp) : -1;
+            const int i = min(tid + 512 * j, PIECES - 1);
+            kpage[j] = table[min((kt * kTile + i / KCH) >> lg, a.s.table_pages - 1)];
+            vpage[j] = table[min((vt * kTile + i % VCH * KPL) >> lg, a.s.table_pages - 1)];
         }
     };
-    auto load = [&](int t) {
+    auto load = [&](const uint8_t* pool, const uint8_t* scales, int page, int place, int at, uint4& w, uint8_t& scale) {
+        const bool has = place < sq.len && (uint32_t)page < (uint32_t)a.s.pages;
+        const uint32_t n = (uint32_t)((has ? page : 0) * a.c.kv_heads + h);
+        w = *reinterpret_cast<const uint4*>(pool + (uint64_t)n * (uint32_t)a.c.head_bytes + (uint32_t)at);
+        if constexpr (ES == 1) scale = scales[n];
+        return has;
+    };
+    auto load_k = [&](int t) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int i = tid + 512 * j;
-            st.k[j] = st.v[j] = make_uint4(0, 0, 0, 0);
-            st.ks[j] = st.vs[j] = 1.f;
-            st.holds[j] = 0;
-            if (kTile * KCH % 512 && i >= kTile * KCH) continue;
-            const int key = i / KCH, kc = i % KCH, d = i / VCH, vc = i % VCH;
-            const int kp = t * kTile + key, vp = t * kTile + vc * KPL;
-            if (kpage[j] >= 0 && 16 * kc < krow) {
-                const int64_t at = (int64_t)kpage[j] * a.c.kv_heads + h;
-                st.k[j] = *reinterpret_cast<const uint4*>(a.c.k + at * a.c.head_bytes + (kp & pmask) * (int64_t)krow + 16 * kc);
-                if constexpr (ES == 1) st.ks[j] = __uint_as_float((uint32_t)max((int)a.c.k_scale[at], 1) << 23);
-            }
-            if (vpage[j] >= 0) {
-                const int64_t at = (int64_t)vpage[j] * a.c.kv_heads + h;
-                if (d < dim) st.v[j] = *reinterpret_cast<const uint4*>(a.c.v + at * a.c.head_bytes + d * (int64_t)vrow + (vp & pmask) * ES);
-                if constexpr (ES == 1) st.vs[j] = __uint_as_float((uint32_t)max((int)a.c.v_scale[at], 1) << 23);
-                st.holds[j] = min(sq.len - vp, KPL);
-            }
+            const int kp = t * kTile + min(tid + 512 * j, PIECES - 1) / KCH;
+            khas[j] = load(a.c.k, a.c.k_scale, kpage[j], kp, (kp & pmask) * krow + krow_at[j], kst[j], kscale[j]);
         }
     };
-    auto store = [&](int t, int buf) {
-        uint8_t* kb = smem + buf * BUF;
-        uint8_t* vb = kb + KBYTES;
+    auto load_v = [&](int t) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-            const int i = tid + 512 * j;
-            if (kTile * KCH % 512 && i >= kTile * KCH) continue;
-            const int key = i / KCH, kc = i % KCH, d = i / VCH, vc = i % VCH;
+            const int vp = t * kTile + min(tid + 512 * j, PIECES - 1) % VCH * KPL;
+            vhas[j] = load(a.c.v, a.c.v_scale, vpage[j], vp, vrow_at[j] + (vp & pmask) * ES, vst[j], vscale[j]);
+        }
+    };
+    auto factor = [](uint8_t scale) { return __uint_as_float(max((uint32_t)scale, 1u) << 23); };
+    auto store_k = [&](int t) {
+        uint8_t* kb = smem + (t & 1) * KBYTES;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + 512 * j, key = i / KCH, kc = i % KCH;
+            if (PIECES % 512 && i >= PIECES) continue;
             const int lr = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
-            uint4 v = st.v[j];
-            // What lies behind the sequence is anything: values of weight 0 have to be numbers.
-            if (__builtin_amdgcn_ballot_w64(st.holds[j] < KPL)) v = leading<ES>(v, st.holds[j]);
-            // So have those that only some rows see; what is none is added to those rows apart.
+            uint4 w = kst[j];
+            if (DP * ES > krow && 16 * kc >= krow) w = make_uint4(0, 0, 0, 0);  // beyond the head's width
+            bf16x8_t f[M];
+            Held<E>::get(w, ES == 1 ? factor(kscale[j]) : 1.f, f);
+#pragma unroll
+            for (int m = 0; m < M; ++m) *reinterpret_cast<bf16x8_t*>(kb + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) = f[m];
+            if (kc == 0 && key % 16 == 0) reinterpret_cast<uint8_t*>(&paged[t & 1])[key / 16] = khas[j] ? 1 : 0;
+        }
+    };
+    auto store_v = [&](int t) {
+        uint8_t* vb = smem + 2 * KBYTES + (t & 1) * VBYTES;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int i = tid + 512 * j, d = i / VCH, vc = i % VCH;
+            if (PIECES % 512 && i >= PIECES) continue;
+            uint4 v = vst[j];
+            float f32 = ES == 1 ? factor(vscale[j]) : 1.f;
+            // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
+            const int holds = vhas[j] ? sq.len - (t * kTile + vc * KPL) : 0;
+            if (__builtin_amdgcn_ballot_w64(holds < KPL)) {
+                v = leading<ES>(v, max(holds, 0));
+                if (!vhas[j]) f32 = 1.f;
+            }
+            // So have those that only some rows see; what is none is added to those rows at the end.
             if ((t + 1) * kTile > all) {
                 const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
                 if (wx | wy | wz | ww) wild_seen = 1;
                 v = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
             }
-            bf16x8_t kf[M], vf[M];
-            Held<E>::get(st.k[j], st.ks[j], kf);
-            Held<E>::get(v, st.vs[j], vf);
+            bf16x8_t f[M];
+            Held<E>::get(v, f32, f);
 #pragma unroll
-            for (int m = 0; m < M; ++m) {
-                *reinterpret_cast<bf16x8_t*>(kb + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) = kf[m];
-                *reinterpret_cast<bf16x8_t*>(vb + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) = vf[m];
-            }
-            if (d == 0 && vc * KPL % 16 == 0) reinterpret_cast<uint8_t*>(&paged[buf])[vc * KPL / 16] = st.holds[j] > 0;
+            for (int m = 0; m < M; ++m) *reinterpret_cast<bf16x8_t*>(vb + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) = f[m];
         }
     };
 
-    typename KT::Frag qf[KT::STEPS];
+    Frag qf[KT::STEPS];
     {
-        const uint16_t* qp = a.q + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
+        const bf16* qp = reinterpret_cast<const bf16*>(a.q) + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
 #pragma unroll
-        for (int c = 0; c < KT::STEPS; ++c)
-            qf[c] = live ? attn::frag_global<bf16>(reinterpret_cast<const bf16*>(qp), c, g, dim) : attn::frag_zero<bf16>();
+        for (int c = 0; c < KT::STEPS; ++c) qf[c] = live ? attn::frag_global<bf16>(qp, c, g, dim) : attn::frag_zero<bf16>();
     }
-    if (tid == 0) wild_seen = 0;
-    attn::Running<bf16, KT::BLOCKS> run;
-    run.clear();
+    Softmax<KT::BLOCKS> run;
+    run.m = -INFINITY;
+    run.l = 0.f;
+#pragma unroll
+    for (int d = 0; d < KT::BLOCKS; ++d) run.o[d] = attn::zero16();
     const float sc = a.scale_log2;
+    // Scores and weights of the even and of the odd 32 keys.
+    f32x16_t s[2];
+    attn::FragParts<bf16> p[2][2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[1][e] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[0][j].w[e] = 0;
+
+    // One step: the softmax of scores s[1 - hh], the product of weights p[hh] with half hh of the values at
+    // V, and the scores s[hh] of half hh of the keys at K, tile t.  Operands are read four ahead of
+    // their products.
+    auto step = [&](auto hc, const uint8_t* K, const uint8_t* V, int t, uint32_t has) {
+        constexpr int hh = decltype(hc)::value, NS = KT::STEPS, NV = 2 * KT::BLOCKS, G = 4, NG = (NS + NV) / G;
+        auto read = [&](int i) {
+            return i < NS ? KT::row_frag(K, 32 * hh + r, i, g)
+                          : VT::row_frag(V, 32 * ((i - NS) % KT::BLOCKS) + r, 2 * hh + (i - NS) / KT::BLOCKS, g);
+        };
+        bool move = false;
+        f32x16_t next = attn::zero16();
+        Frag f[2][G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) f[0][i] = read(i);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            if (n + 1 < NG) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) f[(n + 1) & 1][i] = read((n + 1) * G + i);
+            }
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                const int at = n * G + i;
+                if (at < NS) next = attn::mma(f[n & 1][i], qf[at], next);
+                else run.o[(at - NS) % KT::BLOCKS] = attn::mma(f[n & 1][i], p[hh][(at - NS) / KT::BLOCKS].frag(), run.o[(at - NS) % KT::BLOCKS]);
+            }
+            // Beside them the reference, then four quarters of weights, worked out here and not where they are first used.
+            if (n == 0) move = run.refer(s[1 - hh], sc);
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4)
+                if (i4 >= (n - 1) * 4 / (NG - 1) && i4 < n * 4 / (NG - 1)) {
+                    run.weigh(s[1 - hh], sc, i4, p[1 - hh]);
+                    uint32_t* w = p[1 - hh][i4 / 2].w + 2 * (i4 & 1);
+                    asm volatile("" : "+v"(w[0]), "+v"(w[1]));
+                }
+            if (n == 0) __builtin_amdgcn_sched_group_barrier(0x100, G, 0);
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS reads
+                __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);   // vector and transcendental ALU
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_expect(move, 0)) run.moved();
+        // Element 8 j + e is key 16 j + 8 g + e of the half.
+        if (__builtin_expect((t + 1) * kTile > all || t >= w1, 0)) {
+            const int sees = t >= w1 ? 0 : limit - (t * kTile + 32 * hh + 8 * g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) next[i] = 16 * (i >> 3) + (i & 7) < sees ? next[i] : -INFINITY;
+        }
+        if (__builtin_expect(has != 0x01010101u, 0)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool there = has >> (8 * (2 * hh + j)) & 1;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) next[8 * j + e] = there ? next[8 * j + e] : -INFINITY;
+            }
+        }
+        run.l += run.sum;
+        s[hh] = next;
+    };
+
+    // Before the first tile the weights are 0, and so have to be the values.
+    for (int i = tid; i < VBYTES / 16; i += 512)
+        *reinterpret_cast<uint4*>(smem + 2 * KBYTES + ((t0 + 1) & 1) * VBYTES + 16 * i) = make_uint4(0, 0, 0, 0);
+    if (tid == 0) wild_seen = 0;
     if (t0 < t1) {
-        find_pages(t0);
-        load(t0);
-        find_pages(t0 + 1);
+        find_pages(t0, t0);
+        load_k(t0);
+        find_pages(t0 + 1, t0);
+        store_k(t0);
     }
-    __syncthreads();  // wild_seen is cleared
-    if (t0 < t1) store(t0, 0);
-    int buf = 0;
-    for (int t = t0; t < t1; ++t, buf ^= 1) {
-        __syncthreads();
+    attn::wait_vmem<0>();  // the queries: their first use would wait for the loop's first loads too
+    // Keys a tile ahead: scores of tile t + 1, values of tile t.
+#pragma unroll 1
+    for (int t = t0 - 1; t < t1; ++t) {
+        __syncthreads();  // both are there, nobody reads those before
         if (t + 1 < t1) {
-            load(t + 1);
-            find_pages(t + 2);
+            load_k(t + 2);
+            load_v(t + 1);
+            find_pages(t + 3, t + 2);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const uint8_t* Kt = smem + buf * BUF;
-        const uint8_t* Vt = Kt + KBYTES;
-        if (t * kTile < wave_most) {
-            const uint32_t has = __builtin_amdgcn_readfirstlane(paged[buf]);
-            f32x16_t s[2] = {attn::zero16(), attn::zero16()};
-            attn::FragParts<bf16> p[2][2];
-            float sum[2] = {0.f, 0.f};
-            auto scores = [&](auto hc, auto vc, auto side) {
-                constexpr int hh = decltype(hc)::value;
-                attn::products<bf16, KT::STEPS, 1, decltype(vc)::value>(
-                    [&](int i) { return KT::row_frag(Kt, 32 * hh + r, i, g); },
-                    [&](int i, const typename KT::Frag& f) { s[hh] = attn::mma(f, qf[i], s[hh]); }, side);
-            };
-            // Element 8 j + e is key 16 j + 8 g + e of the half.
-            auto finish = [&](auto hc) {
-                constexpr int hh = decltype(hc)::value;
-                if ((t + 1) * kTile > all) {
-                    const int sees = limit - (t * kTile + 32 * hh + 8 * g);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (16 * (i >> 3) + (i & 7) >= sees) s[hh][i] = -INFINITY;
-                }
-                if (has != 0x01010101u) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        if (!(has >> (8 * (2 * hh + j)) & 1)) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) s[hh][8 * j + e] = -INFINITY;
-                        }
-                }
-            };
-            auto weights = [&](auto hc) {
-                return [&, hc](int part, int of) {
-#pragma unroll
-                    for (int i4 = 0; i4 < 4; ++i4)
-                        if (i4 * of / 4 == part) run.weigh(s[hc], sc, i4, p[hc], sum[hc]);
-                };
-            };
-            auto values = [&](auto hc, auto vc, auto side) {
-                constexpr int hh = decltype(hc)::value;
-                attn::products<bf16, 2 * KT::BLOCKS, 1, decltype(vc)::value>(
-                    [&](int i) { return VT::row_frag(Vt, 32 * (i % KT::BLOCKS) + r, 2 * hh + i / KT::BLOCKS, g); },
-                    [&](int i, const typename KT::Frag& f) {
-                        run.o[i % KT::BLOCKS] = attn::mma(f, p[hh][i / KT::BLOCKS].frag(), run.o[i % KT::BLOCKS]);
-                    },
-                    side);
-            };
-            using H0 = std::integral_constant<int, 0>;
-            using H1 = std::integral_constant<int, 1>;
-            using V = std::integral_constant<int, DP == 64 ? 12 : 6>;  // vector instructions per product
-            scores(H0{}, H0{}, attn::NoSide{});
-            finish(H0{});
-            run.look(s[0], sc);
-            scores(H1{}, V{}, weights(H0{}));
-            finish(H1{});
-            if (run.look(s[1], sc)) {  // the first half's weights again, by the new reference
-                sum[0] = 0.f;
-                weights(H0{})(0, 1);
-            }
-            values(H0{}, V{}, weights(H1{}));
-            values(H1{}, H0{}, attn::NoSide{});
-            run.l += sum[0] + sum[1];
+        const uint8_t* K = smem + ((t + 1) & 1) * KBYTES;
+        const uint8_t* V = smem + 2 * KBYTES + ((t + 2) & 1) * VBYTES;
+        if (t < w1) {
+            const uint32_t has = __builtin_amdgcn_readfirstlane(paged[(t + 1) & 1]);
+            step(std::integral_constant<int, 0>{}, K, V, t + 1, has);
+            step(std::integral_constant<int, 1>{}, K, V, t + 1, has);
         }
-        if (t + 1 < t1) store(t + 1, buf ^ 1);
+        if (t + 1 < t1) {
+            store_k(t + 2);
+            store_v(t + 1);
+        }
     }
     __syncthreads();
-    if (wild_seen)
-        for (int key = max(t0, all / kTile) * kTile; key < min(t1 * kTile, sq.len); ++key) {
-            const int p = page_of(a.s, b, key);
-            if (p < 0 || key >= limit) continue;
-            const uint8_t* at = a.c.v + ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes + (key & pmask) * ES;
-#pragma unroll
-            for (int d = 0; d < KT::BLOCKS; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int e = 32 * d + 8 * (i >> 2) + 4 * g + (i & 3);
-                    if (e < dim) run.o[d][i] += Held<E>::value(at + (int64_t)e * vrow);
-                }
-        }
-
     const float l = run.l + attn::swap32(run.l);
     if (!live) return;
-    if (a.splits == 1) {
-        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no place seen: 0; NaN stays
-        bf16* op = reinterpret_cast<bf16*>(a.o) + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
-#pragma unroll
-        for (int d = 0; d < KT::BLOCKS; ++d)
-#pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) {
-                const int e0 = 32 * d + 8 * i4 + 4 * g;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = run.o[d][4 * i4 + e] * inv;
-                if (e0 < dim) attn::put4(op + e0, v);
-            }
-        return;
-    }
+    const bool whole = a.splits == 1;
+    const float inv = !whole ? 1.f : l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no place seen: 0; NaN stays
+    bf16* op = reinterpret_cast<bf16*>(a.o) + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
     const int64_t at = ((int64_t)split * a.s.rows + sq.row + tok) * a.heads + head;
 #pragma unroll
     for (int d = 0; d < KT::BLOCKS; ++d)
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
+            const int e0 = 32 * d + 8 * i4 + 4 * g;
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = run.o[d][4 * i4 + e];
-            attn::put4(a.rows_o + at * DP + 32 * d + 8 * i4 + 4 * g, v);
+            for (int e = 0; e < 4; ++e) v[e] = run.o[d][4 * i4 + e] * inv;
+            if (!whole) attn::put4(a.rows_o + at * DP + e0, v);
+            else if (e0 < dim) attn::put4(op + e0, v);
         }
-    if (g == 0) {
+    if (!whole && g == 0) {
         a.rows_ml[2 * at] = run.m;
         a.rows_ml[2 * at + 1] = l;
+    }
+    if (wild_seen) {
+#pragma unroll 1
+        for (int e = 4 * g; e < dim; e += 8)
+            add_wild<E>(a, b, h, max(t0, all / kTile) * kTile, min(t1 * kTile, limit), e, reinterpret_cast<uint16_t*>(op),
+                        whole ? nullptr : a.rows_o + at * DP);
     }
 }
 

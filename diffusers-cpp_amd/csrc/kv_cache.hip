@@ -312,7 +312,7 @@ int prepare(const dt_kv_cache* x, const dt_kv_seqs* y, const char* who, Cache* c
                "%s: head_dim %lld unsupported (a multiple of 16 up to 128)", who, (long long)x->head_dim);
     DT_REQUIRE(x->page >= 16 && x->page <= 256 && (x->page & (x->page - 1)) == 0,
                "%s: pages of %lld tokens unsupported (16, 32, 64, 128 or 256)", who, (long long)x->page);
-    DT_REQUIRE(x->pages > 0 && x->pages < (1ll << 31) && x->kv_heads > 0 && x->kv_heads < (1 << 16),
+    DT_REQUIRE(x->pages > 0 && x->kv_heads > 0 && x->kv_heads < (1 << 16) && x->pages < (1ll << 31) / x->kv_heads,
                "%s: %lld pages of %lld heads unsupported", who, (long long)x->pages, (long long)x->kv_heads);
     DT_REQUIRE(x->k && x->v && aligned16(x->k) && aligned16(x->v), "%s: k and v must be given, 16-byte aligned", who);
     const bool f8 = x->type == DT_TYPE_F8_E4M3;
