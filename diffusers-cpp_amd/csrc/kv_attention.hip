@@ -120,17 +120,19 @@ template <typename E> struct Held;
 template <> struct Held<e4m3> {
     static constexpr int N = 2;
     // Codes times the power of two are exact in bf16.
-    __device__ __forceinline__ static void get(const uint4& w, float scale, bf16x8_t (&f)[2]) {
-        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    __device__ __forceinline__ static bf16x8_t part(const uint4& w, float scale, int m) {
+        const uint32_t x[2] = {m ? w.z : w.x, m ? w.w : w.y};
+        bf16x8_t f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const bf16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, false);
             const bf16x2_t hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i], scale, true);
-            f[i / 2][4 * (i & 1)] = lo[0];
-            f[i / 2][4 * (i & 1) + 1] = lo[1];
-            f[i / 2][4 * (i & 1) + 2] = hi[0];
-            f[i / 2][4 * (i & 1) + 3] = hi[1];
+            f[4 * i] = lo[0];
+            f[4 * i + 1] = lo[1];
+            f[4 * i + 2] = hi[0];
+            f[4 * i + 3] = hi[1];
         }
+        return f;
     }
     // Bits of the elements that are not finite.
     __device__ __forceinline__ static uint32_t wild(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
@@ -138,7 +140,7 @@ template <> struct Held<e4m3> {
 };
 template <> struct Held<bf16> {
     static constexpr int N = 1;
-    __device__ __forceinline__ static void get(const uint4& w, float, bf16x8_t (&f)[1]) { f[0] = __builtin_bit_cast(bf16x8_t, w); }
+    __device__ __forceinline__ static bf16x8_t part(const uint4& w, float, int) { return __builtin_bit_cast(bf16x8_t, w); }
     __device__ __forceinline__ static uint32_t wild(uint32_t w) {
         return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
     }
@@ -276,10 +278,9 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                     s[mm][hh] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int c = 0; c < KC; ++c) {
-                        bf16x8_t kf[M];
-                        Held<E>::get(kr[mm][hh][c], ks, kf);
 #pragma unroll
-                        for (int j = 0; j < M; ++j) s[mm][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[j], qf[c][j], s[mm][hh], 0, 0, 0);
+                        for (int j = 0; j < M; ++j)
+                            s[mm][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(kr[mm][hh][c], ks, j), qf[c][j], s[mm][hh], 0, 0, 0);
                     }
                 }
             // Key 8 mm + 4 hh + i of this lane's is seen below `sees`.
@@ -345,10 +346,9 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                bf16x8_t vf[M];
-                Held<E>::get(vr[d], vs, vf);
 #pragma unroll
-                for (int mm = 0; mm < M; ++mm) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[mm], pf[mm], o[d], 0, 0, 0);
+                for (int mm = 0; mm < M; ++mm)
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(vr[d], vs, mm), pf[mm], o[d], 0, 0, 0);
             }
         }
         l = xor_sum(l);
@@ -465,6 +465,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
 // these, and the product with the values of the 32 before, none of which waits for another.
 // Keys therefore run a tile ahead of values in LDS (two buffers each).
 constexpr int kBlock = 256, kTile = 64;
+constexpr uint32_t kOne = 127;  // a page's scale of 1
 
 // The row blocks are numbered like the pages that are written (kv_index.hpp).
 __device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / kBlock + b; }
@@ -474,28 +475,24 @@ template <int BLOCKS>
 struct Softmax {
     float m, l, before, sum;
     f32x16_t o[BLOCKS];
-    // The reference for scores s: it moves when one exceeds it by more than 2^8 (every weight stays
-    // <= 256), which the sums before follow in moved().
-    __device__ __forceinline__ bool refer(const f32x16_t& s, float sc) {
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, attn::swap32(mx)) * sc;
-        const bool move = mx > m + 8.0f;
+    // The reference for scores up to `top` (of this lane's half): it moves when one exceeds it by more than
+    // 2^8 (every weight stays <= 256), which the sums before follow in moved().
+    __device__ __forceinline__ bool refer(float top, float sc) {
+        top = fmaxf(top, attn::swap32(top)) * sc;
+        const bool move = top > m + 8.0f;
         before = m;
-        m = move ? mx : m;
+        m = move ? top : m;
         sum = 0.f;
         return __builtin_amdgcn_ballot_w64(move) != 0;
     }
-    // Elements 4 i4 .. + 3 as weights, rounded to bf16 for the product after the sum took them as they are.
-    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i4, attn::FragParts<bf16> (&p)[2]) {
+    // Elements 2 i and 2 i + 1 as weights, rounded to bf16 for the product after the sum took them as they are.
+    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i, uint32_t& w) {
         const float ref = m == -INFINITY ? 0.f : m;  // scores of -inf only, so far: weight 0
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i4 + e], sc, -ref));
-        p[i4 / 2].set(i4 & 1, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum += v[e];
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], sc, -ref)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], sc, -ref));
+        w = pack_bf16x2(x, y);
+        sum += x;
+        sum += y;
+        asm volatile("" : "+v"(w), "+v"(sum));  // made here, not where they are first used
     }
     __device__ __forceinline__ void moved() {
         const float alpha = m == before ? 1.0f : __builtin_amdgcn_exp2f(before - m);
@@ -507,7 +504,7 @@ struct Softmax {
     }
 };
 
-template <typename E, int DP>
+template <typename E, int DP, bool WIDE>
 __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     typedef attn::Tile<bf16, DP> KT;
     typedef attn::Tile<bf16, kTile> VT;
@@ -553,87 +550,105 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     // What is on its way stays as it is loaded: whatever looks at it would wait for it.  Threads
     // without a piece, and places without a page, load another's.
     uint4 kst[J], vst[J];
-    uint8_t kscale[J], vscale[J];
-    int kpage[J], vpage[J];  // the table's entries for the tiles that are loaded next
-    bool khas[J], vhas[J];   // of those that are stored next: whether they lie in a page
-    int krow_at[J], vrow_at[J];
+    uint32_t kscale[J], vscale[J];
+    bool khas[J], vhas[J];     // whether they lie in a page
+    int kpage[J], vpage[J];    // the table's entries for the tiles that are loaded next
+    uint32_t koff[J], voff[J];  // this thread's pieces in a page, from the tile's first place in it on
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int i = min(tid + 512 * j, PIECES - 1), kc = i % KCH, d = i / VCH;
-        krow_at[j] = 16 * kc < krow ? 16 * kc : 0;
-        vrow_at[j] = (d < dim ? d : 0) * vrow;
+        koff[j] = (i / KCH & pmask) * krow + (16 * kc < krow ? 16 * kc : 0);
+        voff[j] = (d < dim ? d : 0) * vrow + (i % VCH * KPL & pmask) * ES;
     }
     const int32_t* table = a.s.table + b * a.s.table_stride;
+    const int table_last = a.s.table_pages - 1;
+    // WIDE: a tile lies in one page, which is found and checked once for the wave.
+    constexpr int PJ = WIDE ? 1 : J;
     auto find_pages = [&](int kt, int vt) {
+        if constexpr (WIDE) {
+            kpage[0] = table[min(kt * kTile >> lg, table_last)];
+            vpage[0] = table[min(vt * kTile >> lg, table_last)];
+        } else {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = min(tid + 512 * j, PIECES - 1);
-            kpage[j] = table[min((kt * kTile + i / KCH) >> lg, a.s.table_pages - 1)];
-            vpage[j] = table[min((vt * kTile + i % VCH * KPL) >> lg, a.s.table_pages - 1)];
+            for (int j = 0; j < J; ++j) {
+                const int i = min(tid + 512 * j, PIECES - 1);
+                kpage[j] = table[min((kt * kTile + i / KCH) >> lg, table_last)];
+                vpage[j] = table[min((vt * kTile + i % VCH * KPL) >> lg, table_last)];
+            }
         }
     };
-    auto load = [&](const uint8_t* pool, const uint8_t* scales, int page, int place, int at, uint4& w, uint8_t& scale) {
-        const bool has = place < sq.len && (uint32_t)page < (uint32_t)a.s.pages;
-        const uint32_t n = (uint32_t)((has ? page : 0) * a.c.kv_heads + h);
-        w = *reinterpret_cast<const uint4*>(pool + (uint64_t)n * (uint32_t)a.c.head_bytes + (uint32_t)at);
-        if constexpr (ES == 1) scale = scales[n];
-        return has;
-    };
-    auto load_k = [&](int t) {
+    auto load = [&](const uint8_t* pool, const uint8_t* scales, int t, const int (&in_tile)[J], const int (&page)[J], const uint32_t (&off)[J],
+                    uint4 (&w)[J], uint32_t (&scale)[J], bool (&has)[J], int tile_bytes) {
+        const uint8_t* from[PJ];
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int kp = t * kTile + min(tid + 512 * j, PIECES - 1) / KCH;
-            khas[j] = load(a.c.k, a.c.k_scale, kpage[j], kp, (kp & pmask) * krow + krow_at[j], kst[j], kscale[j]);
+        for (int j = 0; j < PJ; ++j) {
+            const int pg = WIDE ? __builtin_amdgcn_readfirstlane(page[j]) : page[j];
+            has[j] = t * kTile + (WIDE ? 0 : in_tile[j]) < sq.len && (uint32_t)pg < (uint32_t)a.s.pages;
+            const uint32_t n = (uint32_t)((has[j] ? pg : 0) * a.c.kv_heads + h);
+            from[j] = pool + (uint64_t)n * (uint32_t)a.c.head_bytes + (uint32_t)((t * kTile & pmask) * tile_bytes);
+            if constexpr (ES == 1) scale[j] = scales[n];
         }
-    };
-    auto load_v = [&](int t) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int vp = t * kTile + min(tid + 512 * j, PIECES - 1) % VCH * KPL;
-            vhas[j] = load(a.c.v, a.c.v_scale, vpage[j], vp, vrow_at[j] + (vp & pmask) * ES, vst[j], vscale[j]);
-        }
+        for (int j = 0; j < J; ++j) w[j] = *reinterpret_cast<const uint4*>(from[WIDE ? 0 : j] + off[j]);
     };
-    auto factor = [](uint8_t scale) { return __uint_as_float(max((uint32_t)scale, 1u) << 23); };
-    auto store_k = [&](int t) {
-        uint8_t* kb = smem + (t & 1) * KBYTES;
+    int kin[J], vin[J];  // the pieces' first places in the tile
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int i = min(tid + 512 * j, PIECES - 1);
+        kin[j] = i / KCH;
+        vin[j] = i % VCH * KPL;
+    }
+    auto load_k = [&](int t) { load(a.c.k, a.c.k_scale, t, kin, kpage, koff, kst, kscale, khas, krow); };
+    auto load_v = [&](int t) { load(a.c.v, a.c.v_scale, t, vin, vpage, voff, vst, vscale, vhas, ES); };
+    auto factor = [](uint32_t scale) { return ES == 1 ? __uint_as_float(max(scale, 1u) << 23) : 1.f; };
+    // Part 0 or 1 of this thread's pieces into LDS: half a piece of codes, or every second piece.
+    constexpr int PARTS = J * M;
+    auto put_k = [&](int t, int part) {
+        const int j = part / M, m = part % M, i = tid + 512 * j, key = i / KCH, kc = i % KCH;
+        if (part >= PARTS || (PIECES % 512 && i >= PIECES)) return;
+        const int lr = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
+        *reinterpret_cast<bf16x8_t*>(smem + (t & 1) * KBYTES + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) =
+            Held<E>::part(kst[j], factor(kscale[WIDE ? 0 : j]), m);
+    };
+    auto put_v = [&](int t, int part) {
+        const int j = part / M, m = part % M, i = tid + 512 * j, d = i / VCH, vc = i % VCH;
+        if (part >= PARTS || (PIECES % 512 && i >= PIECES)) return;
+        *reinterpret_cast<bf16x8_t*>(smem + 2 * KBYTES + (t & 1) * VBYTES + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) =
+            Held<E>::part(vst[j], factor(vscale[WIDE ? 0 : j]), m);
+    };
+    // Before a tile's pieces are put: whether its keys have pages, and what may not enter a product.
+    auto mend_k = [&](int t) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int i = tid + 512 * j, key = i / KCH, kc = i % KCH;
-            if (PIECES % 512 && i >= PIECES) continue;
-            const int lr = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
-            uint4 w = kst[j];
-            if (DP * ES > krow && 16 * kc >= krow) w = make_uint4(0, 0, 0, 0);  // beyond the head's width
-            bf16x8_t f[M];
-            Held<E>::get(w, ES == 1 ? factor(kscale[j]) : 1.f, f);
-#pragma unroll
-            for (int m = 0; m < M; ++m) *reinterpret_cast<bf16x8_t*>(kb + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) = f[m];
-            if (kc == 0 && key % 16 == 0) reinterpret_cast<uint8_t*>(&paged[t & 1])[key / 16] = khas[j] ? 1 : 0;
+            if (DP * ES > krow && 16 * kc >= krow) kst[j] = make_uint4(0, 0, 0, 0);  // beyond the head's width
+            if (!WIDE && (PIECES % 512 == 0 || i < PIECES) && kc == 0 && key % 16 == 0)
+                reinterpret_cast<uint8_t*>(&paged[t & 1])[key / 16] = khas[j] ? 1 : 0;
         }
+        if (WIDE && tid == 0) paged[t & 1] = khas[0] ? 0x01010101u : 0;
     };
-    auto store_v = [&](int t) {
-        uint8_t* vb = smem + 2 * KBYTES + (t & 1) * VBYTES;
+    auto mend_v = [&](int t) {
+        // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
+        bool there = true;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + 512 * j, d = i / VCH, vc = i % VCH;
-            if (PIECES % 512 && i >= PIECES) continue;
-            uint4 v = vst[j];
-            float f32 = ES == 1 ? factor(vscale[j]) : 1.f;
-            // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
-            const int holds = vhas[j] ? sq.len - (t * kTile + vc * KPL) : 0;
-            if (__builtin_amdgcn_ballot_w64(holds < KPL)) {
-                v = leading<ES>(v, max(holds, 0));
-                if (!vhas[j]) f32 = 1.f;
+        for (int j = 0; j < PJ; ++j) there &= vhas[j];
+        if (__builtin_expect((t + 1) * kTile > sq.len || !(WIDE ? there : __builtin_amdgcn_ballot_w64(!there) == 0), 0)) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const bool has = vhas[WIDE ? 0 : j];
+                vst[j] = leading<ES>(vst[j], has ? max(sq.len - (t * kTile + vin[j]), 0) : 0);
+                if (!has) vscale[WIDE ? 0 : j] = kOne;
             }
-            // So have those that only some rows see; what is none is added to those rows at the end.
-            if ((t + 1) * kTile > all) {
+        }
+        // So have those that only some rows see; what is none is added to those rows at the end.
+        if (__builtin_expect((t + 1) * kTile > all, 0)) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const uint4 v = vst[j];
                 const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
                 if (wx | wy | wz | ww) wild_seen = 1;
-                v = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
+                vst[j] = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
             }
-            bf16x8_t f[M];
-            Held<E>::get(v, f32, f);
-#pragma unroll
-            for (int m = 0; m < M; ++m) *reinterpret_cast<bf16x8_t*>(vb + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) = f[m];
         }
     };
 
@@ -660,47 +675,46 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
         for (int e = 0; e < 4; ++e) p[0][j].w[e] = 0;
 
     // One step: the softmax of scores s[1 - hh], the product of weights p[hh] with half hh of the values at
-    // V, and the scores s[hh] of half hh of the keys at K, tile t.  Operands are read four ahead of
-    // their products.
-    auto step = [&](auto hc, const uint8_t* K, const uint8_t* V, int t, uint32_t has) {
-        constexpr int hh = decltype(hc)::value, NS = KT::STEPS, NV = 2 * KT::BLOCKS, G = 4, NG = (NS + NV) / G;
-        auto read = [&](int i) {
-            return i < NS ? KT::row_frag(K, 32 * hh + r, i, g)
-                          : VT::row_frag(V, 32 * ((i - NS) % KT::BLOCKS) + r, 2 * hh + (i - NS) / KT::BLOCKS, g);
-        };
+    // V, and the scores s[hh] of half hh of the keys at K, tile t.  Its products alternate, scores
+    // and values; beside each goes the read of the operand four products on (the first ones' are in
+    // f already) and a piece of the vector work, in this order.  (In larger pieces the compiler
+    // gathers the products, and each waits for the one before with the vector work behind it.)
+    constexpr int NS = KT::STEPS, N = 2 * NS, AHEAD = 4, RING = 8;
+    static_assert(NS == 2 * KT::BLOCKS, "as many products of either kind");
+    Frag f[RING];
+    auto read = [&](int hh, const uint8_t* K, const uint8_t* V, int i) {
+        const int n = i / 2;
+        f[i % RING] = i & 1 ? VT::row_frag(V, 32 * (n % KT::BLOCKS) + r, 2 * hh + n / KT::BLOCKS, g) : KT::row_frag(K, 32 * hh + r, n, g);
+    };
+    auto step = [&](auto hc, const uint8_t* K, const uint8_t* V, int t, uint32_t has, auto put) {
+        constexpr int hh = decltype(hc)::value;
+        float top = 0.f;
         bool move = false;
         f32x16_t next = attn::zero16();
-        Frag f[2][G];
+        // Twelve pieces: the reference (two), what goes to LDS (two), eight pairs of weights.
+        auto piece = [&](int k) {
+            const f32x16_t& now = s[1 - hh];
+            if (k == 0) {
+                top = now[0];
 #pragma unroll
-        for (int i = 0; i < G; ++i) f[0][i] = read(i);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-            if (n + 1 < NG) {
-#pragma unroll
-                for (int i = 0; i < G; ++i) f[(n + 1) & 1][i] = read((n + 1) * G + i);
+                for (int e = 1; e < 16; ++e) top = fmaxf(top, now[e]);
+            } else if (k == 1) {
+                move = run.refer(top, sc);
+            } else if (k < 4) {
+                put(k - 2);
+            } else {
+                run.weigh(now, sc, k - 4, p[1 - hh][(k - 4) / 4].w[(k - 4) % 4]);
             }
+        };
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                const int at = n * G + i;
-                if (at < NS) next = attn::mma(f[n & 1][i], qf[at], next);
-                else run.o[(at - NS) % KT::BLOCKS] = attn::mma(f[n & 1][i], p[hh][(at - NS) / KT::BLOCKS].frag(), run.o[(at - NS) % KT::BLOCKS]);
-            }
-            // Beside them the reference, then four quarters of weights, worked out here and not where they are first used.
-            if (n == 0) move = run.refer(s[1 - hh], sc);
+        for (int i = 0; i < N; ++i) {
+            if (i + AHEAD < N) read(hh, K, V, i + AHEAD);
+            else if (hh == 0) read(1, K, V, i + AHEAD - N);
+            if (i & 1) run.o[i / 2 % KT::BLOCKS] = attn::mma(f[i % RING], p[hh][i / 2 / KT::BLOCKS].frag(), run.o[i / 2 % KT::BLOCKS]);
+            else next = attn::mma(f[i % RING], qf[i / 2], next);
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4)
-                if (i4 >= (n - 1) * 4 / (NG - 1) && i4 < n * 4 / (NG - 1)) {
-                    run.weigh(s[1 - hh], sc, i4, p[1 - hh]);
-                    uint32_t* w = p[1 - hh][i4 / 2].w + 2 * (i4 & 1);
-                    asm volatile("" : "+v"(w[0]), "+v"(w[1]));
-                }
-            if (n == 0) __builtin_amdgcn_sched_group_barrier(0x100, G, 0);
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // MFMA
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // LDS reads
-                __builtin_amdgcn_sched_group_barrier(0x402, 6, 0);   // vector and transcendental ALU
-            }
+            for (int k = 0; k < 12; ++k)
+                if (k * N / 12 == i) piece(k);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (__builtin_expect(move, 0)) run.moved();
@@ -730,29 +744,42 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
         find_pages(t0, t0);
         load_k(t0);
         find_pages(t0 + 1, t0);
-        store_k(t0);
+        mend_k(t0);
+        put_k(t0, 0);
+        put_k(t0, 1);
+        load_k(t0 + 1);
+        load_v(t0);
+        find_pages(t0 + 2, t0 + 1);
     }
     attn::wait_vmem<0>();  // the queries: their first use would wait for the loop's first loads too
-    // Keys a tile ahead: scores of tile t + 1, values of tile t.
+    // Keys a tile ahead: at hand are those of tile t + 1 and the values of tile t, on their way to LDS those
+    // of tiles t + 2 and t + 1.
 #pragma unroll 1
     for (int t = t0 - 1; t < t1; ++t) {
         __syncthreads();  // both are there, nobody reads those before
-        if (t + 1 < t1) {
-            load_k(t + 2);
-            load_v(t + 1);
-            find_pages(t + 3, t + 2);
-        }
-        __builtin_amdgcn_sched_barrier(0);
         const uint8_t* K = smem + ((t + 1) & 1) * KBYTES;
         const uint8_t* V = smem + 2 * KBYTES + ((t + 2) & 1) * VBYTES;
-        if (t < w1) {
-            const uint32_t has = __builtin_amdgcn_readfirstlane(paged[(t + 1) & 1]);
-            step(std::integral_constant<int, 0>{}, K, V, t + 1, has);
-            step(std::integral_constant<int, 1>{}, K, V, t + 1, has);
-        }
+        const uint32_t has = __builtin_amdgcn_readfirstlane(paged[(t + 1) & 1]);
         if (t + 1 < t1) {
-            store_k(t + 2);
-            store_v(t + 1);
+            mend_k(t + 2);
+            mend_v(t + 1);
+        }
+        if (t < w1) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) read(0, K, V, i);
+            step(std::integral_constant<int, 0>{}, K, V, t + 1, has, [&](int part) { put_k(t + 2, part); });
+            step(std::integral_constant<int, 1>{}, K, V, t + 1, has, [&](int part) { put_v(t + 1, part); });
+        } else if (t + 1 < t1) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                put_k(t + 2, part);
+                put_v(t + 1, part);
+            }
+        }
+        if (t + 2 < t1) {
+            load_k(t + 3);
+            load_v(t + 2);
+            find_pages(t + 4, t + 3);
         }
     }
     __syncthreads();
@@ -865,7 +892,9 @@ int launch(const Args& a, const Plan& p, hipStream_t st) {
     const int64_t n = (int64_t)a.s.rows * a.heads;
     if (p.rows) {
         const dim3 grid((unsigned)(p.blocks * p.splits * a.c.kv_heads));
-        hipLaunchKernelGGL((kv_rows_kernel<E, DP>), grid, dim3(512), 2 * (size_t)(kTile * DP + DP * kTile) * 2, st, a);
+        const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
+        if (1 << a.c.page_log2 >= kTile) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true>), grid, dim3(512), lds, st, a);
+        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, false>), grid, dim3(512), lds, st, a);
         int rc = check_launch("dt_kv_attn");
         if (rc) return rc;
         if (p.splits > 1) {
