@@ -454,9 +454,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
         make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
 }
 
-// ---- many rows: 256 rows per workgroup, 32 per wave, tiles of 64 keys ---------------------
-// The cache's tile is turned into bf16 once for the workgroup, on its way through registers
-// into LDS, and every wave multiplies from there on v_mfma_f32_32x32x16_bf16, again transposed: a lane
+// ---- many rows: 256 or 128 rows per workgroup, 32 per wave, tiles of 64 keys --------------
+// Codes are turned into bf16 once for the workgroup, on their way through registers into LDS; bf16
+// comes there by direct DMA.  Every wave multiplies from there on v_mfma_f32_32x32x16_bf16, again transposed: a lane
 // holds one row.  LDS row 8 a + 4 g + c of a tile's 16 holds key 8 g + 4 a + c, so that a lane's
 // scores are those of 8 keys in order, and a value's operand one 16-byte piece.
 //
@@ -464,56 +464,67 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
 // instructions have to overlap by themselves: a step takes 32 keys through three stages at once, the scores of the next 32, the softmax of
 // these, and the product with the values of the 32 before, none of which waits for another.
 // Keys therefore run a tile ahead of values in LDS (two buffers each).
-constexpr int kBlock = 256, kTile = 64;
+constexpr int kTile = 64;
 constexpr uint32_t kOne = 127;  // a page's scale of 1
 
 // The row blocks are numbered like the pages that are written (kv_index.hpp).
-__device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / kBlock + b; }
+template <int BLOCK>
+__device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / BLOCK + b; }
 
 // The softmax of 32 keys for one row: reference m (log2), this lane's half of the sum.
 template <int BLOCKS>
 struct Softmax {
-    float m, l, before, sum;
+    float m, l, sum;
     f32x16_t o[BLOCKS];
-    // The reference for scores up to `top` (of this lane's half): it moves when one exceeds it by more than
-    // 2^8 (every weight stays <= 256), which the sums before follow in moved().
-    __device__ __forceinline__ bool refer(float top, float sc) {
+    __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
+    // Whether the weights by the reference as it is may stay: nearly always, and then their sizes are never
+    // looked at.  Weights whose sum in a lane is at most 2^12 are small enough; without a reference yet
+    // (ref() is then 0) they may all be too small.
+    __device__ __forceinline__ bool stays() const { return __builtin_amdgcn_ballot_w64(sum > 4096.0f || m == -INFINITY) == 0; }
+    // A reference for scores s: it moves when one exceeds it by more than 2^8, and the sums before follow.
+    __device__ __forceinline__ void refer(const f32x16_t& s, float sc) {
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
         top = fmaxf(top, attn::swap32(top)) * sc;
         const bool move = top > m + 8.0f;
-        before = m;
+        const float alpha = move ? __builtin_amdgcn_exp2f(m - top) : 1.0f;
         m = move ? top : m;
-        sum = 0.f;
-        return __builtin_amdgcn_ballot_w64(move) != 0;
-    }
-    // Elements 2 i and 2 i + 1 as weights, rounded to bf16 for the product after the sum took them as they are.
-    __device__ __forceinline__ void weigh(const f32x16_t& s, float sc, int i, uint32_t& w) {
-        const float ref = m == -INFINITY ? 0.f : m;  // scores of -inf only, so far: weight 0
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i], sc, -ref)), y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + 1], sc, -ref));
-        w = pack_bf16x2(x, y);
-        sum += x;
-        sum += y;
-        asm volatile("" : "+v"(w), "+v"(sum));  // made here, not where they are first used
-    }
-    __device__ __forceinline__ void moved() {
-        const float alpha = m == before ? 1.0f : __builtin_amdgcn_exp2f(before - m);
         l *= alpha;
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[b][e] *= alpha;
     }
+    // Elements 2 i and 2 i + 1 as weights, and those rounded to bf16 for the product.  The sum takes them as the product does.
+    __device__ __forceinline__ static void weigh(const f32x16_t& s, float sc, float minus_ref, int i, float (&x)[2]) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * i + e], sc, minus_ref));
+    }
+    __device__ __forceinline__ void pack(const float (&x)[2], uint32_t& w) {
+        w = pack_bf16x2(x[0], x[1]);
+        const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
+        sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), ones, sum, false);
+        asm volatile("" : "+v"(w), "+v"(sum));  // made here, not where they are first used
+    }
 };
 
-template <typename E, int DP, bool WIDE>
-__global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
+// 16 bytes a lane from `at` to lds + 16 lane (lds uniform) by direct DMA.
+__device__ __forceinline__ void dma16(const uint8_t* at, uint8_t* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+template <typename E, int DP, bool WIDE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
+    constexpr int kThreads = 64 * NW, kBlock = 32 * NW;
     typedef attn::Tile<bf16, DP> KT;
     typedef attn::Tile<bf16, kTile> VT;
     typedef typename KT::Frag Frag;
     constexpr int ES = sizeof(E), KPL = 16 / ES, M = Held<E>::N;
     constexpr int KCH = DP / KPL, VCH = kTile / KPL;                           // 16-byte pieces of a row
-    constexpr int PIECES = kTile * KCH, J = (PIECES + 511) / 512;               // of a tile, a thread's
+    constexpr int PIECES = kTile * KCH, J = (PIECES + kThreads - 1) / kThreads;               // of a tile, a thread's
     constexpr int KBYTES = kTile * KT::RB, VBYTES = DP * VT::RB;
-    static_assert(PIECES == DP * VCH && (PIECES % 512 == 0 || J == 1), "pieces");
+    static_assert(PIECES == DP * VCH && (PIECES % kThreads == 0 || J == 1), "pieces");
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];             // [2][K], [2][V]
     __shared__ uint32_t paged[2];                                              // a byte per 16 keys: whether they have a page
     __shared__ int wild_seen;
@@ -526,10 +537,10 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     const uint32_t rest = bid / (uint32_t)a.c.kv_heads;
     const int split = (int)(rest % (uint32_t)a.splits);
     const int64_t item = (int64_t)n_items - 1 - rest / (uint32_t)a.splits;
-    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block(a, start, i); });
+    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block<kBlock>(a, start, i); });
     if (b < 0) return;
     const Seq sq(a.s, b);
-    const int64_t all_rows = sq.n * (int64_t)a.group, row0 = (item - first_block(a, sq.row, b)) * kBlock;
+    const int64_t all_rows = sq.n * (int64_t)a.group, row0 = (item - first_block<kBlock>(a, sq.row, b)) * kBlock;
     if (all_rows <= a.few || row0 < 0 || row0 >= all_rows) return;
     const int rows = (int)all_rows, first = (int)row0, last = min(first + kBlock, rows) - 1;
     // The places that a row sees are those below:
@@ -547,38 +558,45 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     const int w1 = wave_last < first + wave * 32 ? t0 : max(t0, min(t1, (limit_of(wave_last) + kTile - 1) / kTile));
 
     const int dim = a.c.dim, lg = a.c.page_log2, pmask = (1 << lg) - 1, krow = dim * ES, vrow = ES << lg;
+    // This thread's pieces of a tile.  Codes come through registers: piece tid + kThreads j in the pool's
+    // order.  bf16 goes to LDS by direct DMA: the piece that belongs at place 64 (J wave + j) + lane there.
+    constexpr bool DMA = ES == 2;
+    static_assert(!DMA || PIECES % kThreads == 0, "pieces");
+    auto piece = [&](int j) { return DMA ? (wave * J + j) * 64 + lane : min(tid + kThreads * j, PIECES - 1); };
+    auto swapped = [](int key) { return (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1); };
+    auto k_key = [&](int j) { return DMA ? swapped(piece(j) / KCH) : piece(j) / KCH; };
+    auto k_col = [&](int j) { return DMA ? (piece(j) % KCH) ^ KT::swz(piece(j) / KCH) : piece(j) % KCH; };
+    auto v_dim = [&](int j) { return piece(j) / VCH; };
+    auto v_col = [&](int j) { return DMA ? (piece(j) % VCH) ^ VT::swz(v_dim(j)) : piece(j) % VCH; };
+
     // What is on its way stays as it is loaded: whatever looks at it would wait for it.  Threads
     // without a piece, and places without a page, load another's.
-    uint4 kst[J], vst[J];
+    uint4 kst[DMA ? 1 : J], vst[DMA ? 1 : J];
     uint32_t kscale[J], vscale[J];
     bool khas[J], vhas[J];     // whether they lie in a page
     int kpage[J], vpage[J];    // the table's entries for the tiles that are loaded next
     uint32_t koff[J], voff[J];  // this thread's pieces in a page, from the tile's first place in it on
+    int kin[J], vin[J];         // and their first places in the tile
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const int i = min(tid + 512 * j, PIECES - 1), kc = i % KCH, d = i / VCH;
-        koff[j] = (i / KCH & pmask) * krow + (16 * kc < krow ? 16 * kc : 0);
-        voff[j] = (d < dim ? d : 0) * vrow + (i % VCH * KPL & pmask) * ES;
+        kin[j] = k_key(j);
+        vin[j] = v_col(j) * KPL;
+        koff[j] = (kin[j] & pmask) * krow + (16 * k_col(j) < krow ? 16 * k_col(j) : 0);
+        voff[j] = (v_dim(j) < dim ? v_dim(j) : 0) * vrow + (vin[j] & pmask) * ES;
     }
     const int32_t* table = a.s.table + b * a.s.table_stride;
     const int table_last = a.s.table_pages - 1;
     // WIDE: a tile lies in one page, which is found and checked once for the wave.
     constexpr int PJ = WIDE ? 1 : J;
     auto find_pages = [&](int kt, int vt) {
-        if constexpr (WIDE) {
-            kpage[0] = table[min(kt * kTile >> lg, table_last)];
-            vpage[0] = table[min(vt * kTile >> lg, table_last)];
-        } else {
 #pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const int i = min(tid + 512 * j, PIECES - 1);
-                kpage[j] = table[min((kt * kTile + i / KCH) >> lg, table_last)];
-                vpage[j] = table[min((vt * kTile + i % VCH * KPL) >> lg, table_last)];
-            }
+        for (int j = 0; j < PJ; ++j) {
+            kpage[j] = table[min((kt * kTile + (WIDE ? 0 : kin[j])) >> lg, table_last)];
+            vpage[j] = table[min((vt * kTile + (WIDE ? 0 : vin[j])) >> lg, table_last)];
         }
     };
     auto load = [&](const uint8_t* pool, const uint8_t* scales, int t, const int (&in_tile)[J], const int (&page)[J], const uint32_t (&off)[J],
-                    uint4 (&w)[J], uint32_t (&scale)[J], bool (&has)[J], int tile_bytes) {
+                    uint4* w, uint8_t* lds, uint32_t (&scale)[J], bool (&has)[J], int tile_bytes) {
         const uint8_t* from[PJ];
 #pragma unroll
         for (int j = 0; j < PJ; ++j) {
@@ -589,65 +607,75 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
             if constexpr (ES == 1) scale[j] = scales[n];
         }
 #pragma unroll
-        for (int j = 0; j < J; ++j) w[j] = *reinterpret_cast<const uint4*>(from[WIDE ? 0 : j] + off[j]);
+        for (int j = 0; j < J; ++j) {
+            const uint8_t* at = from[WIDE ? 0 : j] + off[j];
+            if constexpr (DMA) dma16(at, lds + (wave * J + j) * 1024);
+            else w[j] = *reinterpret_cast<const uint4*>(at);
+        }
     };
-    int kin[J], vin[J];  // the pieces' first places in the tile
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int i = min(tid + 512 * j, PIECES - 1);
-        kin[j] = i / KCH;
-        vin[j] = i % VCH * KPL;
-    }
-    auto load_k = [&](int t) { load(a.c.k, a.c.k_scale, t, kin, kpage, koff, kst, kscale, khas, krow); };
-    auto load_v = [&](int t) { load(a.c.v, a.c.v_scale, t, vin, vpage, voff, vst, vscale, vhas, ES); };
+    auto k_buf = [&](int t) { return smem + (t & 1) * KBYTES; };
+    auto v_buf = [&](int t) { return smem + 2 * KBYTES + (t & 1) * VBYTES; };
+    auto load_k = [&](int t) { load(a.c.k, a.c.k_scale, t, kin, kpage, koff, kst, k_buf(t), kscale, khas, krow); };
+    auto load_v = [&](int t) { load(a.c.v, a.c.v_scale, t, vin, vpage, voff, vst, v_buf(t), vscale, vhas, ES); };
     auto factor = [](uint32_t scale) { return ES == 1 ? __uint_as_float(max(scale, 1u) << 23) : 1.f; };
-    // Part 0 or 1 of this thread's pieces into LDS: half a piece of codes, or every second piece.
-    constexpr int PARTS = J * M;
+    // Part `part` of this thread's pieces into LDS: half a piece of codes.
+    constexpr int PARTS = DMA ? 0 : J * M;
     auto put_k = [&](int t, int part) {
-        const int j = part / M, m = part % M, i = tid + 512 * j, key = i / KCH, kc = i % KCH;
-        if (part >= PARTS || (PIECES % 512 && i >= PIECES)) return;
-        const int lr = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
-        *reinterpret_cast<bf16x8_t*>(smem + (t & 1) * KBYTES + lr * KT::RB + (((M * kc + m) ^ KT::swz(lr)) << 4)) =
+        const int j = part / M, m = part % M, lr = swapped(k_key(j));
+        if (PIECES % kThreads && tid + kThreads * j >= PIECES) return;
+        *reinterpret_cast<bf16x8_t*>(k_buf(t) + lr * KT::RB + (((M * k_col(j) + m) ^ KT::swz(lr)) << 4)) =
             Held<E>::part(kst[j], factor(kscale[WIDE ? 0 : j]), m);
     };
     auto put_v = [&](int t, int part) {
-        const int j = part / M, m = part % M, i = tid + 512 * j, d = i / VCH, vc = i % VCH;
-        if (part >= PARTS || (PIECES % 512 && i >= PIECES)) return;
-        *reinterpret_cast<bf16x8_t*>(smem + 2 * KBYTES + (t & 1) * VBYTES + d * VT::RB + (((M * vc + m) ^ VT::swz(d)) << 4)) =
+        const int j = part / M, m = part % M, d = v_dim(j);
+        if (PIECES % kThreads && tid + kThreads * j >= PIECES) return;
+        *reinterpret_cast<bf16x8_t*>(v_buf(t) + d * VT::RB + (((M * v_col(j) + m) ^ VT::swz(d)) << 4)) =
             Held<E>::part(vst[j], factor(vscale[WIDE ? 0 : j]), m);
     };
-    // Before a tile's pieces are put: whether its keys have pages, and what may not enter a product.
+    // Before codes are put, after bf16 is there: whether keys have pages, and what may not enter a product.
     auto mend_k = [&](int t) {
+        if (DP * ES > krow) {  // beyond the head's width
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int i = tid + 512 * j, key = i / KCH, kc = i % KCH;
-            if (DP * ES > krow && 16 * kc >= krow) kst[j] = make_uint4(0, 0, 0, 0);  // beyond the head's width
-            if (!WIDE && (PIECES % 512 == 0 || i < PIECES) && kc == 0 && key % 16 == 0)
-                reinterpret_cast<uint8_t*>(&paged[t & 1])[key / 16] = khas[j] ? 1 : 0;
+            for (int j = 0; j < J; ++j)
+                if (16 * k_col(j) >= krow) {
+                    if constexpr (DMA) *reinterpret_cast<uint4*>(k_buf(t) + 16 * piece(j)) = make_uint4(0, 0, 0, 0);
+                    else kst[j] = make_uint4(0, 0, 0, 0);
+                }
         }
-        if (WIDE && tid == 0) paged[t & 1] = khas[0] ? 0x01010101u : 0;
+        if constexpr (WIDE) {
+            if (tid == 0) paged[t & 1] = khas[0] ? 0x01010101u : 0;
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if ((PIECES % kThreads == 0 || tid + kThreads * j < PIECES) && k_col(j) == 0 && kin[j] % 16 == 0)
+                    reinterpret_cast<uint8_t*>(&paged[t & 1])[kin[j] / 16] = khas[j] ? 1 : 0;
+        }
     };
     auto mend_v = [&](int t) {
-        // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
         bool there = true;
 #pragma unroll
         for (int j = 0; j < PJ; ++j) there &= vhas[j];
-        if (__builtin_expect((t + 1) * kTile > sq.len || !(WIDE ? there : __builtin_amdgcn_ballot_w64(!there) == 0), 0)) {
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const bool has = vhas[WIDE ? 0 : j];
-                vst[j] = leading<ES>(vst[j], has ? max(sq.len - (t * kTile + vin[j]), 0) : 0);
-                if (!has) vscale[WIDE ? 0 : j] = kOne;
-            }
-        }
+        // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
+        const bool tail = (t + 1) * kTile > sq.len || !(WIDE ? there : __builtin_amdgcn_ballot_w64(!there) == 0);
         // So have those that only some rows see; what is none is added to those rows at the end.
-        if (__builtin_expect((t + 1) * kTile > all, 0)) {
+        const bool some = (t + 1) * kTile > all;
+        if (__builtin_expect(tail || some, 0)) {
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const uint4 v = vst[j];
-                const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
-                if (wx | wy | wz | ww) wild_seen = 1;
-                vst[j] = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
+                uint4* const at = reinterpret_cast<uint4*>(v_buf(t) + 16 * piece(j));
+                uint4 v;
+                if constexpr (DMA) v = *at;
+                else v = vst[j];
+                const bool has = vhas[WIDE ? 0 : j];
+                v = leading<ES>(v, has ? max(sq.len - (t * kTile + vin[j]), 0) : 0);
+                if (some) {
+                    const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
+                    if (wx | wy | wz | ww) wild_seen = 1;
+                    v = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
+                }
+                if constexpr (DMA) *at = v;
+                else vst[j] = v;
+                if (!has) vscale[WIDE ? 0 : j] = kOne;
             }
         }
     };
@@ -679,45 +707,46 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     // and values; beside each goes the read of the operand four products on (the first ones' are in
     // f already) and a piece of the vector work, in this order.  (In larger pieces the compiler
     // gathers the products, and each waits for the one before with the vector work behind it.)
-    constexpr int NS = KT::STEPS, N = 2 * NS, AHEAD = 4, RING = 8;
+    constexpr int NS = KT::STEPS, N = 2 * NS, AHEAD = NW == 8 ? 4 : 3, RING = AHEAD + 1;  // three: what registers are left for
     static_assert(NS == 2 * KT::BLOCKS, "as many products of either kind");
     Frag f[RING];
     auto read = [&](int hh, const uint8_t* K, const uint8_t* V, int i) {
         const int n = i / 2;
-        f[i % RING] = i & 1 ? VT::row_frag(V, 32 * (n % KT::BLOCKS) + r, 2 * hh + n / KT::BLOCKS, g) : KT::row_frag(K, 32 * hh + r, n, g);
+        f[(hh * N + i) % RING] = i & 1 ? VT::row_frag(V, 32 * (n % KT::BLOCKS) + r, 2 * hh + n / KT::BLOCKS, g) : KT::row_frag(K, 32 * hh + r, n, g);
     };
     auto step = [&](auto hc, const uint8_t* K, const uint8_t* V, int t, uint32_t has, auto put) {
         constexpr int hh = decltype(hc)::value;
-        float top = 0.f;
-        bool move = false;
+        const f32x16_t& now = s[1 - hh];
         f32x16_t next = attn::zero16();
-        // Twelve pieces: the reference (two), what goes to LDS (two), eight pairs of weights.
-        auto piece = [&](int k) {
-            const f32x16_t& now = s[1 - hh];
-            if (k == 0) {
-                top = now[0];
-#pragma unroll
-                for (int e = 1; e < 16; ++e) top = fmaxf(top, now[e]);
-            } else if (k == 1) {
-                move = run.refer(top, sc);
-            } else if (k < 4) {
-                put(k - 2);
-            } else {
-                run.weigh(now, sc, k - 4, p[1 - hh][(k - 4) / 4].w[(k - 4) % 4]);
-            }
-        };
+        float x[8][2];
+        const float minus_ref = -run.ref();
+        run.sum = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (i + AHEAD < N) read(hh, K, V, i + AHEAD);
             else if (hh == 0) read(1, K, V, i + AHEAD - N);
-            if (i & 1) run.o[i / 2 % KT::BLOCKS] = attn::mma(f[i % RING], p[hh][i / 2 / KT::BLOCKS].frag(), run.o[i / 2 % KT::BLOCKS]);
-            else next = attn::mma(f[i % RING], qf[i / 2], next);
+            if (i & 1) run.o[i / 2 % KT::BLOCKS] = attn::mma(f[(hh * N + i) % RING], p[hh][i / 2 / KT::BLOCKS].frag(), run.o[i / 2 % KT::BLOCKS]);
+            else next = attn::mma(f[(hh * N + i) % RING], qf[i / 2], next);
+            // Two weights' exponentials, those of two products before into their operand, then what goes to LDS.
 #pragma unroll
-            for (int k = 0; k < 12; ++k)
-                if (k * N / 12 == i) piece(k);
+            for (int k = 0; k < 8; ++k) {
+                if (1 + k * N / 16 == i) run.weigh(now, sc, minus_ref, k, x[k]);
+                if (1 + N / 8 + k * N / 16 == i) run.pack(x[k], p[1 - hh][k / 4].w[k % 4]);
+            }
+#pragma unroll
+            for (int k = 0; k < PARTS; ++k)
+                if (N / 2 + 3 + k * (N / 2 - 3) / (PARTS ? PARTS : 1) == i) put(k);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (__builtin_expect(move, 0)) run.moved();
+        if (__builtin_expect(!run.stays(), 0)) {
+            run.refer(now, sc);
+            run.sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                run.weigh(now, sc, -run.ref(), k, x[k]);
+                run.pack(x[k], p[1 - hh][k / 4].w[k % 4]);
+            }
+        }
         // Element 8 j + e is key 16 j + 8 g + e of the half.
         if (__builtin_expect((t + 1) * kTile > all || t >= w1, 0)) {
             const int sees = t >= w1 ? 0 : limit - (t * kTile + 32 * hh + 8 * g);
@@ -737,47 +766,63 @@ __global__ __launch_bounds__(512, 2) void kv_rows_kernel(const Args a) {
     };
 
     // Before the first tile the weights are 0, and so have to be the values.
-    for (int i = tid; i < VBYTES / 16; i += 512)
+    for (int i = tid; i < VBYTES / 16; i += kThreads)
         *reinterpret_cast<uint4*>(smem + 2 * KBYTES + ((t0 + 1) & 1) * VBYTES + 16 * i) = make_uint4(0, 0, 0, 0);
     if (tid == 0) wild_seen = 0;
     if (t0 < t1) {
         find_pages(t0, t0);
         load_k(t0);
-        find_pages(t0 + 1, t0);
+        if constexpr (DMA) attn::wait_vmem<0>();
         mend_k(t0);
-        put_k(t0, 0);
-        put_k(t0, 1);
-        load_k(t0 + 1);
-        load_v(t0);
-        find_pages(t0 + 2, t0 + 1);
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) put_k(t0, part);
+        find_pages(t0 + 1, t0);
+        if constexpr (!DMA) {
+            load_k(t0 + 1);
+            load_v(t0);
+            find_pages(t0 + 2, t0 + 1);
+        }
     }
     attn::wait_vmem<0>();  // the queries: their first use would wait for the loop's first loads too
-    // Keys a tile ahead: at hand are those of tile t + 1 and the values of tile t, on their way to LDS those
-    // of tiles t + 2 and t + 1.
+    // Keys a tile ahead: at hand are those of tile t + 1 and the values of tile t.  Meanwhile those of tiles
+    // t + 2 and t + 1 come to LDS (codes by way of registers, a tile earlier), where nobody reads any more.
 #pragma unroll 1
     for (int t = t0 - 1; t < t1; ++t) {
-        __syncthreads();  // both are there, nobody reads those before
-        const uint8_t* K = smem + ((t + 1) & 1) * KBYTES;
-        const uint8_t* V = smem + 2 * KBYTES + ((t + 2) & 1) * VBYTES;
+        __syncthreads();
+        const uint8_t* K = k_buf(t + 1);
+        const uint8_t* V = v_buf(t + 2);
         const uint32_t has = __builtin_amdgcn_readfirstlane(paged[(t + 1) & 1]);
         if (t + 1 < t1) {
-            mend_k(t + 2);
-            mend_v(t + 1);
+            if constexpr (DMA) {
+                load_k(t + 2);
+                load_v(t + 1);
+                find_pages(t + 3, t + 2);
+            } else {
+                mend_k(t + 2);
+                mend_v(t + 1);
+            }
         }
         if (t < w1) {
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) read(0, K, V, i);
             step(std::integral_constant<int, 0>{}, K, V, t + 1, has, [&](int part) { put_k(t + 2, part); });
+            if (!DMA && t + 2 < t1) load_k(t + 3);
             step(std::integral_constant<int, 1>{}, K, V, t + 1, has, [&](int part) { put_v(t + 1, part); });
         } else if (t + 1 < t1) {
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
+            for (int part = 0; part < PARTS; ++part) {
                 put_k(t + 2, part);
                 put_v(t + 1, part);
             }
+            if (!DMA && t + 2 < t1) load_k(t + 3);
         }
-        if (t + 2 < t1) {
-            load_k(t + 3);
+        if constexpr (DMA) {
+            if (t + 1 < t1) {
+                attn::wait_vmem<0>();
+                mend_k(t + 2);
+                mend_v(t + 1);
+            }
+        } else if (t + 2 < t1) {
             load_v(t + 2);
             find_pages(t + 4, t + 3);
         }
@@ -853,7 +898,7 @@ __global__ __launch_bounds__(256) void kv_rows_join_kernel(const Args a) {
 // ---- choice and launch --------------------------------------------------------------
 struct Plan {
     bool stream, rows;
-    int few, waves, dp, splits;
+    int few, waves, dp, block, splits;
     int64_t blocks;             // of rows, at most
     int64_t floats, row_floats;  // workspace: the stream's partial results, the row blocks'
 };
@@ -875,10 +920,17 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
         p.floats = (int64_t)c.kv_heads * p.waves * 2 * kRows * (p.dp + 2);
     }
     if (p.rows) {
-        p.blocks = rows / kBlock + s.seqs;
-        const int64_t full = ((rows + kBlock - 1) / kBlock) * c.kv_heads;
-        int64_t n = cus / (full > 0 ? full : 1);
-        const int64_t longest = ((int64_t)s.table_pages << s.page_log2) / (8 * kTile);  // eight tiles a range
+        // Blocks of 256 rows, one workgroup a CU, where keys are many and so are blocks, or a single
+        // sequence's keys are shared out anyway (32 heads on 8 x 128: 4096 tokens 149 us against 159 in blocks
+        // of 128; 512 behind 30000 245 and 262).  Else, with pages of whole tiles, 128 rows and two workgroups
+        // a CU, of which one starts while the other works, and fewer rows are filled up (2048 tokens 62 us
+        // against 70; 8 x 1024 78 and 87; 4 x 300 behind 5000 101 and 127).
+        const int64_t keys = (int64_t)s.table_pages << s.page_log2;
+        p.block = 1 << c.page_log2 < kTile || (keys >= 4096 && (rows * c.kv_heads >= 512 * (int64_t)cus || s.seqs == 1)) ? 256 : 128;
+        p.blocks = rows / p.block + s.seqs;
+        const int64_t full = ((rows + p.block - 1) / p.block) * c.kv_heads;
+        int64_t n = (p.block == 128 ? 2 : 1) * cus / (full > 0 ? full : 1);
+        const int64_t longest = keys / (8 * kTile);  // eight tiles a range
         if (n > longest) n = longest;
         if (n > 32) n = 32;
         p.splits = n < 2 ? 1 : (int)n;
@@ -893,8 +945,11 @@ int launch(const Args& a, const Plan& p, hipStream_t st) {
     if (p.rows) {
         const dim3 grid((unsigned)(p.blocks * p.splits * a.c.kv_heads));
         const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
-        if (1 << a.c.page_log2 >= kTile) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true>), grid, dim3(512), lds, st, a);
-        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, false>), grid, dim3(512), lds, st, a);
+        const bool wide = 1 << a.c.page_log2 >= kTile;
+        const dim3 block(2 * p.block);
+        if (!wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 8>), grid, block, lds, st, a);
+        else if (p.block == 256) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
+        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 4>), grid, block, lds, st, a);
         int rc = check_launch("dt_kv_attn");
         if (rc) return rc;
         if (p.splits > 1) {
