@@ -32,6 +32,7 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;      // rows of a block of the stream's
+constexpr int kShort = 2048;   // places of a table up to which the stream's blocks of rows are not shared out
 constexpr int kFew = 32;       // beside the row blocks' kernel the stream takes sequences of up to so many rows
 
 struct Args {
@@ -52,17 +53,6 @@ struct Args {
     float* rows_ml;       // [splits][rows][heads][2]
 };
 
-// Units of sequence b, this lane's; 0 past the last sequence.
-template <int STEP>
-__device__ __forceinline__ int64_t units_of(const Args& a, int b, int* tiles = nullptr) {
-    if (b >= a.s.seqs) return 0;
-    const Seq q(a.s, b);
-    if (q.n == 0 || q.n * (int64_t)a.group > a.few) return 0;
-    const int t = max((q.len + STEP - 1) / STEP, 1);
-    if (tiles) *tiles = t;
-    return (int64_t)((q.n * (int64_t)a.group + kRows - 1) / kRows) * t;
-}
-
 __device__ __forceinline__ int64_t scan64(int64_t v) {  // inclusive sum over the wave's lanes
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -73,32 +63,68 @@ __device__ __forceinline__ int64_t scan64(int64_t v) {  // inclusive sum over th
     return v;
 }
 
-template <int STEP>
-__device__ __forceinline__ int64_t total_units(const Args& a) {
-    const int lane = threadIdx.x & 63;
-    int64_t n = 0;
-    for (int b0 = 0; b0 < a.s.seqs; b0 += 64) n += units_of<STEP>(a, b0 + lane);
-    return __shfl(scan64(n), 63, 64);
+// Blocks of rows are numbered like the pages that are written (kv_index.hpp).
+template <int BLOCK>
+__device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / BLOCK + b; }
+
+// One sequence, the same in all lanes.
+struct Mine {
+    int b, row, n, past, len;
+    int64_t before;  // units before it
+};
+
+__device__ __forceinline__ int64_t lane64(int64_t v, int l) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, l));
 }
 
-// The sequence that unit x (below the total) belongs to, and the units before it.
+// The stream's sequences in order, 64 at a time, one a lane.
 template <int STEP>
-__device__ __forceinline__ int find_unit(const Args& a, int64_t x, int64_t* before) {
-    const int lane = threadIdx.x & 63;
-    int64_t sum = 0;
-    for (int b0 = 0; b0 < a.s.seqs; b0 += 64) {
-        const int64_t u = units_of<STEP>(a, b0 + lane), end = sum + scan64(u);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(end > x);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            *before = __shfl(end - u, at, 64);
-            return b0 + at;
+struct Walk {
+    const Args& a;
+    int from, row, n, past, len;
+    int64_t units, end;  // of this lane's, and of all up to it
+    __device__ __forceinline__ explicit Walk(const Args& args) : a(args) {}
+    __device__ __forceinline__ static int tiles(int len) { return max((len + STEP - 1) / STEP, 1); }
+    __device__ __forceinline__ void load(int b0, int64_t before) {
+        from = b0;
+        const int b = b0 + (threadIdx.x & 63);
+        row = n = past = len = 0;
+        units = 0;
+        if (b < a.s.seqs) {
+            const Seq q(a.s, b);
+            row = q.row;
+            n = q.n;
+            past = q.past;
+            len = q.len;
+            if (n > 0 && n * (int64_t)a.group <= a.few) units = (n * (int64_t)a.group + kRows - 1) / kRows * tiles(len);
         }
-        sum = __shfl(end, 63, 64);
+        end = before + scan64(units);
     }
-    *before = sum;
-    return -1;
-}
+    __device__ __forceinline__ int64_t total() {
+        int64_t sum = 0;
+        for (int b0 = 0; b0 < a.s.seqs; b0 += 64) {
+            load(b0, sum);
+            sum = lane64(end, 63);
+        }
+        return sum;
+    }
+    __device__ __forceinline__ Mine mine(int l) const {
+        return {from + l, __builtin_amdgcn_readlane(row, l), __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(past, l),
+                __builtin_amdgcn_readlane(len, l), lane64(end - units, l)};
+    }
+    // The sequence that unit x (below the total) belongs to.
+    __device__ __forceinline__ Mine find(int64_t x) {
+        if (x < lane64(end - units, 0)) load(0, 0);
+        while (x >= lane64(end, 63)) load(from + 64, lane64(end, 63));
+        return mine(__builtin_ctzll(__builtin_amdgcn_ballot_w64(end > x)));
+    }
+    // Sequence b, wherever it is.
+    __device__ __forceinline__ Mine at(int b) {
+        if (b < from) load(0, 0);
+        while (b >= from + 64) load(from + 64, lane64(end, 63));
+        return mine(b - from);
+    }
+};
 
 // How many of the W waves work: two steps each at least.
 __device__ __forceinline__ int64_t working(const Args& a, int64_t total) {
@@ -183,93 +209,103 @@ __device__ __forceinline__ void add_wild(const Args& a, int b, int h, int from, 
     }
 }
 
-template <typename E, int DP>
-__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
-    constexpr int ES = sizeof(E), KPL = 16 / ES, STEP = 4 * KPL, M = Held<E>::N;
-    constexpr int KC = DP * ES / 64;  // 16-byte pieces of a key's row a lane group takes
-    constexpr int DB = DP / 16;
-    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int id = (int)(blockIdx.x * 4) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = id / a.waves, w = id - h * a.waves;
-    if (h >= a.c.kv_heads) return;
-    const int64_t total = total_units<STEP>(a);
-    if (total == 0) return;
-    const int64_t W = working(a, total);
-    if (w >= W) return;
-    const int64_t x1 = total * (w + 1) / W;
-    const int dim = a.c.dim, lg = a.c.page_log2, pmask = (1 << lg) - 1;
-    const int krow = dim * ES, vrow = ES << lg;
+// 16 rows' part of the softmax over steps t0, t0 + by .. < t1 of a sequence.  A step's keys are loaded while the
+// step before is in its second product, its values after that; nothing looks at what is on its way.
+// WIDE: a step's keys lie in one page, which is found and checked once for the wave.
+template <typename E, int DP, bool WIDE>
+struct Stream {
+    static constexpr int ES = sizeof(E), KPL = 16 / ES, STEP = 4 * KPL, M = Held<E>::N;
+    static constexpr int KC = DP * ES / 64;  // 16-byte pieces of a key's row a lane group takes
+    static constexpr int DB = DP / 16;
 
-    for (int64_t x = total * w / W; x < x1;) {
-        int64_t before;
-        const int b = find_unit<STEP>(a, x, &before);
-        if (b < 0) return;
-        const Seq sq(a.s, b);
-        const int tiles = max((sq.len + STEP - 1) / STEP, 1);
-        const int blk = (int)((x - before) / tiles);
-        const int64_t s0 = before + (int64_t)blk * tiles;
-        const int t0 = (int)(x - s0), t1 = (int)((x1 < s0 + tiles ? x1 : s0 + tiles) - s0);
+    int tok, head;  // this lane's row
+    bool live;
+    int limit, all;  // places that it sees are those below; those that every row of the block sees
+    bool wild;
+    float m, l;
+    f32x4_t o[DB];
 
-        const int row = blk * kRows + col, rows = sq.n * a.group;
-        const bool live = row < rows;
-        const int tok = live ? (int)fdiv((uint32_t)row, a.group_div) : 0;
-        const int head = h * a.group + (live ? row - tok * a.group : 0);
-        // The row sees places below this; rows past the last one all that the first row of the block sees.
-        const int tok0 = (int)fdiv((uint32_t)(blk * kRows), a.group_div);
-        const int limit = a.causal ? min(sq.past + (live ? tok : tok0) + 1, sq.len) : sq.len;
-        const int all = a.causal ? min(sq.past + tok0 + 1, sq.len) : sq.len;  // places that every row sees
-
-        bf16x8_t qf[KC][M];
-        {
-            const uint16_t* qp = a.q + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    const int d = KPL * (g + 4 * c) + 8 * m;
-                    uint4 z = make_uint4(0, 0, 0, 0);
-                    if (live && d < dim) z = *reinterpret_cast<const uint4*>(qp + d);
-                    qf[c][m] = __builtin_bit_cast(bf16x8_t, z);
-                }
-        }
-        bool wild = false;
-        float m = -INFINITY, l = 0.f;
-        f32x4_t o[DB];
+    __device__ __forceinline__ void run(const Args& a, const Mine& sq, int h, int blk, int t0, int t1, int by) {
+        const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+        const int dim = a.c.dim, lg = a.c.page_log2, pmask = (1 << lg) - 1, krow = dim * ES, vrow = ES << lg;
+        const int row = blk * kRows + col, tok0 = (int)fdiv((uint32_t)(blk * kRows), a.group_div);
+        live = row < sq.n * a.group;
+        tok = live ? (int)fdiv((uint32_t)row, a.group_div) : 0;
+        head = h * a.group + (live ? row - tok * a.group : 0);
+        all = a.causal ? min(sq.past + tok0 + 1, sq.len) : sq.len;
+        limit = !live ? all : a.causal ? min(sq.past + tok + 1, sq.len) : sq.len;
+        wild = false;
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-        for (int t = t0; t < t1; ++t) {
-            // This lane's keys' (scores, values) and its operand row's pages.
-            const int kb = t * STEP + KPL * (col >> 2), vb = t * STEP + KPL * g;
-            int kp = kb < sq.len ? page_of(a.s, b, kb) : -1, vp = vb < sq.len ? page_of(a.s, b, vb) : -1;
-            const bool paged = vp >= 0;
-            kp = max(kp, 0);
-            vp = max(vp, 0);
-            const int64_t kh = (int64_t)kp * a.c.kv_heads + h, vh = (int64_t)vp * a.c.kv_heads + h;
-            const uint8_t* ka = a.c.k + kh * a.c.head_bytes + ((kb & pmask) + (col & 3)) * (int64_t)krow + 16 * g;
-            const uint8_t* va = a.c.v + vh * a.c.head_bytes + (vb & pmask) * ES;
-            float ks = 1.f, vs = 1.f;
+        const int32_t* table = a.s.table + sq.b * a.s.table_stride;
+        const int table_last = a.s.table_pages - 1;
+        const int kin = KPL * (col >> 2), vin = KPL * g;  // first key of this lane's operand row's piece of four, of its scores and values
+        int kpage, vpage;
+        auto find_pages = [&](int t) {
+            kpage = table[max(min((t * STEP + (WIDE ? 0 : kin)) >> lg, table_last), 0)];
+            if constexpr (!WIDE) vpage = table[max(min((t * STEP + vin) >> lg, table_last), 0)];
+        };
+        uint4 kr[M][2][KC], vr[DB];
+        uint32_t kscale = 127, vscale = 127;
+        bool paged;            // this lane's scores and values
+        uint32_t vn = 0;       // page and head of the values
+        auto slot = [&](int page, int key, bool& has) {
+            has = key < sq.len && (uint32_t)page < (uint32_t)a.s.pages;
+            return (uint32_t)((has ? page : 0) * a.c.kv_heads + h);
+        };
+        const uint32_t koff = (uint32_t)(((WIDE ? kin : 0) + (col & 3)) * krow + 16 * g), voff = (uint32_t)(col * vrow + (WIDE ? vin * ES : 0));
+        auto load_k = [&](int t) {
+            bool has;
+            const uint32_t n = WIDE ? slot(__builtin_amdgcn_readfirstlane(kpage), t * STEP, has) : slot(kpage, t * STEP + kin, has);
+            if constexpr (WIDE) vn = n;
+            else vn = slot(vpage, t * STEP + vin, has);
+            paged = has;
+            const uint8_t* at = a.c.k + (uint64_t)n * (uint32_t)a.c.head_bytes + (uint32_t)((t * STEP + (WIDE ? 0 : kin)) & pmask) * (uint32_t)krow;
             if constexpr (ES == 1) {
-                ks = __uint_as_float((uint32_t)max((int)a.c.k_scale[kh], 1) << 23);
-                if (paged) vs = __uint_as_float((uint32_t)max((int)a.c.v_scale[vh], 1) << 23);  // any other page's may be NaN
+                kscale = a.c.k_scale[n];
+                vscale = a.c.v_scale[vn];
             }
-            uint4 kr[M][2][KC], vr[DB];
 #pragma unroll
             for (int mm = 0; mm < M; ++mm)
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
                     for (int c = 0; c < KC; ++c) {
-                        kr[mm][hh][c] = make_uint4(0, 0, 0, 0);
-                        if (16 * (g + 4 * c) < krow)
-                            kr[mm][hh][c] = *reinterpret_cast<const uint4*>(ka + (8 * mm + 4 * hh) * krow + 64 * c);
+                        // Pieces beyond the head's width are another's: their queries are 0, and they are cleared before use.
+                        const bool in = DP * ES == krow || 16 * (g + 4 * c) < krow;
+                        kr[mm][hh][c] = *reinterpret_cast<const uint4*>(at + (in ? koff + (8 * mm + 4 * hh) * krow + 64 * c : 0));
                     }
+        };
+        auto load_v = [&](int t) {
+            const uint8_t* at = a.c.v + (uint64_t)vn * (uint32_t)a.c.head_bytes + (uint32_t)((t * STEP + (WIDE ? 0 : vin)) & pmask) * ES;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
-                vr[d] = make_uint4(0, 0, 0, 0);
-                if (16 * d < dim) vr[d] = *reinterpret_cast<const uint4*>(va + (16 * d + col) * vrow);
+            for (int d = 0; d < DB; ++d) vr[d] = *reinterpret_cast<const uint4*>(at + (16 * d < dim ? 16 * d * vrow : 0) + voff);
+        };
+        if (t0 >= t1 || sq.len == 0) return;  // without a place there may be no table
+        find_pages(t0);
+        // Queries first: the keys' loads wait for the pages anyway.
+        bf16x8_t qf[KC][M];
+        const uint16_t* qp = a.q + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const int d = KPL * (g + 4 * c) + 8 * j;
+                uint4 z = make_uint4(0, 0, 0, 0);
+                if (live && d < dim) z = *reinterpret_cast<const uint4*>(qp + d);
+                qf[c][j] = __builtin_bit_cast(bf16x8_t, z);
             }
-
+        load_k(t0);
+        load_v(t0);
+        find_pages(t0 + by);
+        for (int t = t0; t < t1; t += by) {
+            const bool here = paged;
+            const float ks = ES == 1 ? __uint_as_float(max(kscale, 1u) << 23) : 1.f;
+            // Of a place in no page the scale may be NaN.
+            const float vs = ES == 1 && here ? __uint_as_float(max(vscale, 1u) << 23) : 1.f;
             f32x4_t s[M][2];
 #pragma unroll
             for (int mm = 0; mm < M; ++mm)
@@ -278,13 +314,20 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                     s[mm][hh] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int c = 0; c < KC; ++c) {
+                        uint4 w = kr[mm][hh][c];
+                        if (DP * ES != krow && 16 * (g + 4 * c) >= krow) w = make_uint4(0, 0, 0, 0);
 #pragma unroll
                         for (int j = 0; j < M; ++j)
-                            s[mm][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(kr[mm][hh][c], ks, j), qf[c][j], s[mm][hh], 0, 0, 0);
+                            s[mm][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(w, ks, j), qf[c][j], s[mm][hh], 0, 0, 0);
                     }
                 }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool more = t + by < t1;
+            if (more) load_k(t + by);
+            __builtin_amdgcn_sched_barrier(0);
+
             // Key 8 mm + 4 hh + i of this lane's is seen below `sees`.
-            const int sees = paged ? limit - vb : 0, holds = paged ? min(max(sq.len - vb, 0), KPL) : 0;
+            const int vb = t * STEP + vin, sees = here ? limit - vb : 0, holds = here ? min(max(sq.len - vb, 0), KPL) : 0;
             if (__builtin_amdgcn_ballot_w64(sees < KPL)) {
 #pragma unroll
                 for (int mm = 0; mm < M; ++mm)
@@ -294,23 +337,6 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                         for (int i = 0; i < 4; ++i)
                             if (8 * mm + 4 * hh + i >= sees) s[mm][hh][i] = -INFINITY;
             }
-            // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
-            if (__builtin_amdgcn_ballot_w64(holds < KPL)) {
-#pragma unroll
-                for (int d = 0; d < DB; ++d) vr[d] = leading<ES>(vr[d], holds);
-            }
-            // So have those that only some rows of the block see; what is none is added to these rows at the end.
-            if ((t + 1) * STEP > all) {
-                uint32_t any = 0;
-#pragma unroll
-                for (int d = 0; d < DB; ++d) {
-                    const uint32_t wx = Held<E>::wild(vr[d].x), wy = Held<E>::wild(vr[d].y), wz = Held<E>::wild(vr[d].z), ww = Held<E>::wild(vr[d].w);
-                    any |= wx | wy | wz | ww;
-                    vr[d] = make_uint4(vr[d].x & ~wx, vr[d].y & ~wy, vr[d].z & ~wz, vr[d].w & ~ww);
-                }
-                wild |= __builtin_amdgcn_ballot_w64(any != 0) != 0;
-            }
-
             float mx = -INFINITY;
 #pragma unroll
             for (int mm = 0; mm < M; ++mm)
@@ -344,43 +370,142 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                 pf[mm] = __builtin_bit_cast(bf16x8_t, make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]),
                                                                  pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7])));
             }
+            // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
+            if (__builtin_amdgcn_ballot_w64(holds < KPL)) {
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
+                for (int d = 0; d < DB; ++d) vr[d] = leading<ES>(vr[d], holds);
+            }
+            // So have those that only some rows of the block see; what is none is added to these rows at the end.
+            if ((t + 1) * STEP > all) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const uint32_t wx = Held<E>::wild(vr[d].x), wy = Held<E>::wild(vr[d].y), wz = Held<E>::wild(vr[d].z), ww = Held<E>::wild(vr[d].w);
+                    any |= wx | wy | wz | ww;
+                    vr[d] = make_uint4(vr[d].x & ~wx, vr[d].y & ~wy, vr[d].z & ~wz, vr[d].w & ~ww);
+                }
+                wild |= __builtin_amdgcn_ballot_w64(any != 0) != 0;
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
                 for (int mm = 0; mm < M; ++mm)
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(vr[d], vs, mm), pf[mm], o[d], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) {
+                load_v(t + by);
+                find_pages(t + 2 * by);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
         l = xor_sum(l);
-        if (t0 == 0 && t1 == tiles) {
-            const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // no place seen: 0; NaN stays
-            if (live) {
-                uint16_t* op = a.o + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-                    if (16 * d < dim)
-                        *reinterpret_cast<uint2*>(op + 16 * d + 4 * g) =
-                            make_uint2(pack_bf16x2(o[d][0] * inv, o[d][1] * inv), pack_bf16x2(o[d][2] * inv, o[d][3] * inv));
-            }
-        } else if (live) {
-            const int64_t at = (((int64_t)h * a.waves + w) * 2 + (t0 == 0 ? 1 : 0)) * kRows + col;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-                *reinterpret_cast<float4*>(a.part_o + at * DP + 16 * d + 4 * g) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
-            if (g == 0) {
-                a.part_ml[2 * at] = m;
-                a.part_ml[2 * at + 1] = l;
-            }
-        }
-        if (wild && live) {
-            uint16_t* op = a.o + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
-            float* part = t0 == 0 && t1 == tiles ? nullptr : a.part_o + ((((int64_t)h * a.waves + w) * 2 + (t0 == 0 ? 1 : 0)) * kRows + col) * DP;
-#pragma unroll 1
-            for (int d = 4 * g; d < dim; d += 16)
-                add_wild<E>(a, b, h, max(t0, all / STEP) * STEP, min(t1 * STEP, limit), d, op, part);
-        }
-        x = s0 + t1;
     }
+    __device__ __forceinline__ uint16_t* out(const Args& a, const Mine& sq) const {
+        return a.o + (int64_t)(sq.row + tok) * a.os[0] + head * a.os[1];
+    }
+};
+
+template <typename E, int DP, bool WIDE>
+__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
+    typedef Stream<E, DP, WIDE> St;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int id = (int)(blockIdx.x * 4) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = id / a.waves, w = id - h * a.waves;
+    if (h >= a.c.kv_heads) return;
+    Walk<St::STEP> walk(a);
+    const int64_t total = walk.total();
+    if (total == 0) return;
+    const int64_t W = working(a, total);
+    if (w >= W) return;
+    const int64_t x1 = total * (w + 1) / W;
+    for (int64_t x = total * w / W; x < x1;) {
+        const Mine sq = walk.find(x);
+        const int tiles = walk.tiles(sq.len), blk = (int)((x - sq.before) / tiles);
+        const int64_t s0 = sq.before + (int64_t)blk * tiles;
+        const int t0 = (int)(x - s0), t1 = (int)((x1 < s0 + tiles ? x1 : s0 + tiles) - s0);
+        x = s0 + t1;
+        St st;
+        st.run(a, sq, h, blk, t0, t1, 1);
+        if (!st.live) continue;
+        const bool whole = t0 == 0 && t1 == tiles;
+        const int64_t at = (((int64_t)h * a.waves + w) * 2 + (t0 == 0 ? 1 : 0)) * kRows + col;
+        const float inv = !whole ? 1.f : st.l > 0.f ? 1.0f / st.l : (st.l == 0.f ? 0.f : st.l);  // no place seen: 0; NaN stays
+        uint16_t* op = st.out(a, sq);
+#pragma unroll
+        for (int d = 0; d < St::DB; ++d) {
+            const int e = 16 * d + 4 * g;
+            const float v[4] = {st.o[d][0] * inv, st.o[d][1] * inv, st.o[d][2] * inv, st.o[d][3] * inv};
+            if (!whole) attn::put4(a.part_o + at * DP + e, v);
+            else if (16 * d < a.c.dim) attn::put4(reinterpret_cast<bf16*>(op) + e, v);
+        }
+        if (!whole && g == 0) {
+            a.part_ml[2 * at] = st.m;
+            a.part_ml[2 * at + 1] = st.l;
+        }
+        if (st.wild) {
+#pragma unroll 1
+            for (int d = 4 * g; d < a.c.dim; d += 16)
+                add_wild<E>(a, sq.b, h, max(t0, st.all / St::STEP) * St::STEP, min(t1 * St::STEP, st.limit), d, op, whole ? nullptr : a.part_o + at * DP);
+        }
+    }
+}
+
+// Short tables: a workgroup takes a block of rows whole, its eight waves every eighth step, and joins them in LDS.
+template <typename E, int DP, bool WIDE>
+__global__ __launch_bounds__(512, 2) void kv_short_kernel(const Args a) {
+    typedef Stream<E, DP, WIDE> St;
+    constexpr int LD = DP + 4;  // a row's floats in LDS: rows in other banks
+    extern __shared__ __attribute__((aligned(16))) float joined[];  // [8][kRows][LD]
+    __shared__ float ml[8][kRows][2];
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = (int)(blockIdx.x % (uint32_t)a.c.kv_heads);
+    const int64_t item = blockIdx.x / (uint32_t)a.c.kv_heads;
+    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block<kRows>(a, start, i); });
+    if (b < 0) return;
+    const Seq q(a.s, b);
+    const int64_t blk = item - first_block<kRows>(a, q.row, b), rows = q.n * (int64_t)a.group;
+    if (blk < 0 || blk * kRows >= rows || rows > a.few) return;
+    const Mine sq = {b, q.row, q.n, q.past, q.len, 0};
+    const int tiles = max((sq.len + St::STEP - 1) / St::STEP, 1);
+    St st;
+    st.run(a, sq, h, (int)blk, wave, tiles, 8);
+    float* mine = joined + (wave * kRows + col) * LD;
+#pragma unroll
+    for (int d = 0; d < St::DB; ++d) *reinterpret_cast<float4*>(mine + 16 * d + 4 * g) = make_float4(st.o[d][0], st.o[d][1], st.o[d][2], st.o[d][3]);
+    if (g == 0) {
+        ml[wave][col][0] = st.m;
+        ml[wave][col][1] = st.l;
+    }
+    __syncthreads();
+    const int n = min((int)(rows - blk * kRows), kRows);
+    for (int i = tid; i < n * (DP / 4); i += 512) {
+        const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+        if (d >= a.c.dim) continue;
+        float m = ml[0][r][0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) m = fmaxf(m, ml[w][r][0]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            const float f = __builtin_amdgcn_exp2f(ml[w][r][0] - ref);
+            const float4 x = *reinterpret_cast<const float4*>(joined + (w * kRows + r) * LD + d);
+            l += f * ml[w][r][1];
+            v[0] += f * x.x;
+            v[1] += f * x.y;
+            v[2] += f * x.z;
+            v[3] += f * x.w;
+        }
+        const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= inv;
+        const int row = (int)blk * kRows + r, tok = (int)fdiv((uint32_t)row, a.group_div);
+        attn::put4(reinterpret_cast<bf16*>(a.o) + (int64_t)(sq.row + tok) * a.os[0] + (h * a.group + row - tok * a.group) * a.os[1] + d, v);
+    }
+    if (!__syncthreads_or(st.wild) || wave != 0 || !st.live) return;
+#pragma unroll 1
+    for (int d = 4 * g; d < a.c.dim; d += 16)
+        add_wild<E>(a, b, h, st.all / St::STEP * St::STEP, min(tiles * St::STEP, st.limit), d, st.out(a, sq), nullptr);
 }
 
 // The partial results of a row: TPR threads, each every PL-th wave's share of four elements.  Rows are
@@ -399,20 +524,16 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
     bool join = false;
     int r = 0, head = 0;
     if (b >= 0) {
-        const int64_t total = total_units<STEP>(a);
-        const Seq sq(a.s, b);
+        Walk<STEP> walk(a);
+        const int64_t total = walk.total();
+        const Mine sq = walk.at(b);
         const int h = by_seq ? (int)(id / kFew % a.c.kv_heads) : (int)(id % a.heads) / a.group;
         const int row = by_seq ? (int)(id % kFew) : (r0 - sq.row) * a.group + (int)(id % a.heads) % a.group;
         r = sq.row + row / a.group;
         head = h * a.group + row % a.group;
         if (total > 0 && row < sq.n * (int64_t)a.group && sq.n * (int64_t)a.group <= a.few) {
-            // The units before sequence b.
-            const int lane = tid & 63;
-            int64_t n = 0;
-            for (int b0 = 0; b0 < b; b0 += 64) n += b0 + lane < b ? units_of<STEP>(a, b0 + lane) : 0;
-            n = __shfl(scan64(n), 63, 64);
-            const int tiles = max((sq.len + STEP - 1) / STEP, 1);
-            const int64_t s0 = n + (int64_t)(row / kRows) * tiles, W = working(a, total);
+            const int tiles = walk.tiles(sq.len);
+            const int64_t s0 = sq.before + (int64_t)(row / kRows) * tiles, W = working(a, total);
             const int w0 = (int)(((s0 + 1) * W - 1) / total), w1 = (int)(((s0 + tiles) * W - 1) / total);
             join = w0 != w1;
             for (int w = w0 + pl; join && w <= w1; w += PL) {
@@ -466,10 +587,6 @@ __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
 // Keys therefore run a tile ahead of values in LDS (two buffers each).
 constexpr int kTile = 64;
 constexpr uint32_t kOne = 127;  // a page's scale of 1
-
-// The row blocks are numbered like the pages that are written (kv_index.hpp).
-template <int BLOCK>
-__device__ __forceinline__ int64_t first_block(const Args& a, int start, int b) { return (int64_t)start * a.group / BLOCK + b; }
 
 // The softmax of 32 keys for one row: reference m (log2), this lane's half of the sum.
 template <int BLOCKS>
@@ -897,7 +1014,7 @@ __global__ __launch_bounds__(256) void kv_rows_join_kernel(const Args a) {
 
 // ---- choice and launch --------------------------------------------------------------
 struct Plan {
-    bool stream, rows;
+    bool stream, rows, whole;    // whole: the stream's blocks of rows are not shared out
     int few, waves, dp, block, splits;
     int64_t blocks;             // of rows, at most
     int64_t floats, row_floats;  // workspace: the stream's partial results, the row blocks'
@@ -913,7 +1030,8 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     p.stream = !p.rows || s.seqs > 1;
     p.few = !p.rows ? INT32_MAX : p.stream ? kFew : 0;
     p.splits = 1;
-    if (p.stream) {
+    p.whole = p.stream && ((int64_t)s.table_pages << s.page_log2) <= kShort;
+    if (p.stream && !p.whole) {
         // Two waves a SIMD in all, whole workgroups of four a key head.
         p.waves = (8 * cus / c.kv_heads + 3) / 4 * 4;
         if (p.waves < 4) p.waves = 4;
@@ -959,7 +1077,17 @@ int launch(const Args& a, const Plan& p, hipStream_t st) {
         }
     }
     if (!p.stream) return DT_OK;
-    hipLaunchKernelGGL((kv_stream_kernel<E, DP>), dim3((unsigned)(a.c.kv_heads * (a.waves / 4))), dim3(256), 0, st, a);
+    const bool wide = 1 << a.c.page_log2 >= Stream<E, DP, true>::STEP;
+    if (p.whole) {
+        const dim3 grid((unsigned)(((int64_t)a.s.rows * a.group / kRows + a.s.seqs) * a.c.kv_heads));
+        const size_t lds = 8 * kRows * (DP + 4) * sizeof(float);
+        if (wide) hipLaunchKernelGGL((kv_short_kernel<E, DP, true>), grid, dim3(512), lds, st, a);
+        else hipLaunchKernelGGL((kv_short_kernel<E, DP, false>), grid, dim3(512), lds, st, a);
+        return check_launch("dt_kv_attn");
+    }
+    const dim3 grid((unsigned)(a.c.kv_heads * (a.waves / 4)));
+    if (wide) hipLaunchKernelGGL((kv_stream_kernel<E, DP, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv_stream_kernel<E, DP, false>), grid, dim3(256), 0, st, a);
     int rc = check_launch("dt_kv_attn");
     if (rc) return rc;
     // Few rows may each have many shares: a workgroup a row.
@@ -1008,7 +1136,8 @@ extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, cons
     const size_t need = (size_t)(p.floats + p.row_floats) * sizeof(float);
     DT_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                "%s: a 16-byte aligned workspace of %lld bytes is needed", who, (long long)need);
-    DT_REQUIRE(p.blocks * p.splits * a.c.kv_heads < (1ll << 31) && (int64_t)a.s.seqs * a.c.kv_heads * kFew < (1ll << 31),
+    DT_REQUIRE(p.blocks * p.splits * a.c.kv_heads < (1ll << 31) &&
+                   ((int64_t)a.s.rows * (heads / a.c.kv_heads) / kRows + a.s.seqs) * a.c.kv_heads < (1ll << 31) && (int64_t)a.s.seqs * a.c.kv_heads * kFew < (1ll << 31),
                "%s: grid too large", who);
     a.q = (const uint16_t*)q;
     a.o = (uint16_t*)o;
