@@ -47,6 +47,8 @@ struct Args {
     int32_t few;          // sequences of up to so many rows (new tokens times heads of a group) are the stream's
     int32_t splits;       // key ranges of the others' row blocks
     int32_t waves;        // the stream's, a key head
+    int32_t stream_blocks;  // workgroups of the row blocks' kernel that are the stream's
+    int32_t join_blocks;    // workgroups of the join that are the stream's
     float* part_o;        // [kv_heads][waves][2][kRows][DP], unnormalised
     float* part_ml;       // [kv_heads][waves][2][kRows][2]: reference (log2), sum
     float* rows_o;        // [splits][rows][heads][DP], as part_o
@@ -409,11 +411,11 @@ struct Stream {
     }
 };
 
+// Wave id of all that share the stream out.
 template <typename E, int DP, bool WIDE>
-__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
+__device__ __forceinline__ void stream_part(const Args& a, int id) {
     typedef Stream<E, DP, WIDE> St;
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const int id = (int)(blockIdx.x * 4) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = id / a.waves, w = id - h * a.waves;
     if (h >= a.c.kv_heads) return;
     Walk<St::STEP> walk(a);
@@ -452,6 +454,11 @@ __global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
                 add_wild<E>(a, sq.b, h, max(t0, st.all / St::STEP) * St::STEP, min(t1 * St::STEP, st.limit), d, op, whole ? nullptr : a.part_o + at * DP);
         }
     }
+}
+
+template <typename E, int DP, bool WIDE>
+__global__ __launch_bounds__(256, 2) void kv_stream_kernel(const Args a) {
+    stream_part<E, DP, WIDE>(a, (int)(blockIdx.x * 4) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 
 // Short tables: a workgroup takes a block of rows whole, its eight waves every eighth step, and joins them in LDS.
@@ -512,11 +519,62 @@ __global__ __launch_bounds__(512, 2) void kv_short_kernel(const Args a) {
         add_wild<E>(a, b, h, st.all / St::STEP * St::STEP, min(tiles * St::STEP, st.limit), d, st.out(a, sq), nullptr);
 }
 
+// The key ranges of a row, joined in their order: a thread per four elements.
+template <int DP>
+__device__ __forceinline__ void join_ranges(const Args& a, int block) {
+    constexpr int TPR = DP / 4;
+    const int64_t n = (int64_t)a.s.rows * a.heads, id = ((int64_t)block * 256 + threadIdx.x) / TPR;
+    const int d = (int)(threadIdx.x % TPR) * 4;
+    // The sequences of the wave's rows, one after the other, by the whole wave.
+    bool mine = false;
+#pragma unroll
+    for (int k = 0; k < 64 / TPR; ++k) {
+        const int r = min(__shfl((int)(id / a.heads), k * TPR, 64), a.s.rows - 1);
+        const int b = find_seq(a.s, r, [](int start, int) { return start; });
+        if (b < 0) continue;
+        const Seq sq(a.s, b);
+        if ((int)(threadIdx.x & 63) / TPR == k) mine = r - sq.row < sq.n && sq.n * (int64_t)a.group > a.few;
+    }
+    if (!mine || id >= n || d >= a.c.dim) return;
+    float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        float2 ml[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // all on their way before the first is used
+            const int64_t at = (int64_t)min(s0 + i, a.splits - 1) * n + id;
+            ml[i] = *reinterpret_cast<const float2*>(a.rows_ml + 2 * at);
+            x[i] = *reinterpret_cast<const float4*>(a.rows_o + at * DP + d);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i >= a.splits) break;
+            const float to = fmaxf(m, ml[i].x), ref = to == -INFINITY ? 0.f : to;
+            const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(ml[i].x - ref);
+            m = to;
+            l = l * f0 + ml[i].y * f1;
+            v[0] = v[0] * f0 + x[i].x * f1;
+            v[1] = v[1] * f0 + x[i].y * f1;
+            v[2] = v[2] * f0 + x[i].z * f1;
+            v[3] = v[3] * f0 + x[i].w * f1;
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    const int r = (int)(id / a.heads), head = (int)(id - (int64_t)r * a.heads);
+    attn::put4(reinterpret_cast<bf16*>(a.o) + (int64_t)r * a.os[0] + head * a.os[1] + d, v);
+}
+
 // The partial results of a row: TPR threads, each every PL-th wave's share of four elements.  Rows are
 // numbered as (token, head), or, beside the row blocks' kernel, as (sequence, key head, row of up to kFew).
 template <typename E, int DP, int TPR>
 __global__ __launch_bounds__(256) void kv_join_kernel(const Args a) {
     constexpr int STEP = 4 * (16 / (int)sizeof(E)), LPD = DP / 4, PL = TPR / LPD;
+    if ((int)blockIdx.x >= a.join_blocks) {
+        join_ranges<DP>(a, (int)blockIdx.x - a.join_blocks);
+        return;
+    }
     __shared__ float part[256][6];
     const int tid = threadIdx.x, sub = tid % TPR, pl = sub / LPD, d0 = (sub % LPD) * 4;
     const int64_t id = (int64_t)blockIdx.x * (256 / TPR) + __builtin_amdgcn_readfirstlane(tid / TPR);
@@ -643,8 +701,14 @@ __device__ __forceinline__ void dma16(const uint8_t* at, uint8_t* lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)at, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
+// Its first workgroups share out the stream of the sequences of few rows, which waits for memory while
+// the others multiply.
 template <typename E, int DP, bool WIDE, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
+    if ((int)blockIdx.x < a.stream_blocks) {
+        stream_part<E, DP, WIDE>(a, (int)(blockIdx.x * NW) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+        return;
+    }
     constexpr int kThreads = 64 * NW, kBlock = 32 * NW;
     typedef attn::Tile<bf16, DP> KT;
     typedef attn::Tile<bf16, kTile> VT;
@@ -661,7 +725,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
     const int r = lane & 31, g = lane >> 5;
 
     // Heads innermost: an XCD's workgroups share them.  The longest rows first.
-    const uint32_t bid = blockIdx.x, n_items = gridDim.x / (uint32_t)(a.c.kv_heads * a.splits);
+    const uint32_t bid = blockIdx.x - a.stream_blocks, n_items = (gridDim.x - a.stream_blocks) / (uint32_t)(a.c.kv_heads * a.splits);
     const int h = (int)(bid % (uint32_t)a.c.kv_heads);
     const uint32_t rest = bid / (uint32_t)a.c.kv_heads;
     const int split = (int)(rest % (uint32_t)a.splits);
@@ -986,53 +1050,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
     }
 }
 
-// The key ranges of a row, joined in their order: a thread per four elements.
-template <int DP>
-__global__ __launch_bounds__(256) void kv_rows_join_kernel(const Args a) {
-    constexpr int TPR = DP / 4;
-    const int64_t n = (int64_t)a.s.rows * a.heads, id = ((int64_t)blockIdx.x * 256 + threadIdx.x) / TPR;
-    const int d = (int)(threadIdx.x % TPR) * 4;
-    // The sequences of the wave's rows, one after the other, by the whole wave.
-    bool mine = false;
-#pragma unroll
-    for (int k = 0; k < 64 / TPR; ++k) {
-        const int r = min(__shfl((int)(id / a.heads), k * TPR, 64), a.s.rows - 1);
-        const int b = find_seq(a.s, r, [](int start, int) { return start; });
-        if (b < 0) continue;
-        const Seq sq(a.s, b);
-        if ((int)(threadIdx.x & 63) / TPR == k) mine = r - sq.row < sq.n && sq.n * (int64_t)a.group > a.few;
-    }
-    if (!mine || id >= n || d >= a.c.dim) return;
-    float m = -INFINITY, l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < a.splits; s0 += 4) {
-        float2 ml[4];
-        float4 x[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // all on their way before the first is used
-            const int64_t at = (int64_t)min(s0 + i, a.splits - 1) * n + id;
-            ml[i] = *reinterpret_cast<const float2*>(a.rows_ml + 2 * at);
-            x[i] = *reinterpret_cast<const float4*>(a.rows_o + at * DP + d);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (s0 + i >= a.splits) break;
-            const float to = fmaxf(m, ml[i].x), ref = to == -INFINITY ? 0.f : to;
-            const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(ml[i].x - ref);
-            m = to;
-            l = l * f0 + ml[i].y * f1;
-            v[0] = v[0] * f0 + x[i].x * f1;
-            v[1] = v[1] * f0 + x[i].y * f1;
-            v[2] = v[2] * f0 + x[i].z * f1;
-            v[3] = v[3] * f0 + x[i].w * f1;
-        }
-    }
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= inv;
-    const int r = (int)(id / a.heads), head = (int)(id - (int64_t)r * a.heads);
-    attn::put4(reinterpret_cast<bf16*>(a.o) + (int64_t)r * a.os[0] + head * a.os[1] + d, v);
-}
-
 // ---- choice and launch --------------------------------------------------------------
 struct Plan {
     bool stream, rows, whole;    // whole: the stream's blocks of rows are not shared out
@@ -1051,11 +1068,13 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     p.stream = !p.rows || s.seqs > 1;
     p.few = !p.rows ? INT32_MAX : p.stream ? kFew : 0;
     p.splits = 1;
-    p.whole = p.stream && ((int64_t)s.table_pages << s.page_log2) <= kShort;
+    p.whole = !p.rows && ((int64_t)s.table_pages << s.page_log2) <= kShort;
     if (p.stream && !p.whole) {
-        // Two waves a SIMD in all, whole workgroups of four a key head.
-        p.waves = (8 * cus / c.kv_heads + 3) / 4 * 4;
-        if (p.waves < 4) p.waves = 4;
+        // Two waves a SIMD in all.  Beside blocks of rows a quarter of that, and so of the CUs at most: the
+        // stream is as fast as memory, and over before the products are (the same step with all of
+        // them first 128 us).
+        p.waves = ((p.rows ? 2 : 8) * cus / c.kv_heads + 7) / 8 * 8;
+        if (p.waves < 8) p.waves = 8;
         p.floats = (int64_t)c.kv_heads * p.waves * 2 * kRows * (p.dp + 2);
     }
     if (p.rows) {
@@ -1068,7 +1087,9 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
         p.block = 1 << c.page_log2 < kTile || (keys >= 4096 && (rows * c.kv_heads >= 512 * (int64_t)cus || s.seqs == 1)) ? 256 : 128;
         p.blocks = rows / p.block + s.seqs;
         const int64_t full = ((rows + p.block - 1) / p.block) * c.kv_heads;
-        int64_t n = (p.block == 128 ? 2 : 1) * cus / (full > 0 ? full : 1);
+        // Twice as many beside a stream, whose workgroups end at their own time (17 requests, two of them with
+        // 512 new tokens, behind 3500: 143 -> 124 us).
+        int64_t n = (p.block == 128 ? 2 : 1) * (p.stream ? 2 : 1) * cus / (full > 0 ? full : 1);
         const int64_t longest = keys / (8 * kTile);  // eight tiles a range
         if (n > longest) n = longest;
         if (n > 32) n = 32;
@@ -1079,45 +1100,37 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
 }
 
 template <typename E, int DP>
-int launch(const Args& a, const Plan& p, hipStream_t st) {
+int launch(Args& a, const Plan& p, hipStream_t st) {
     const int64_t n = (int64_t)a.s.rows * a.heads;
-    if (p.rows) {
-        const dim3 grid((unsigned)(p.blocks * p.splits * a.c.kv_heads));
-        const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
-        const bool wide = 1 << a.c.page_log2 >= kTile;
-        const dim3 block(2 * p.block);
-        if (!wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 8>), grid, block, lds, st, a);
-        else if (p.block == 256) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
-        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 4>), grid, block, lds, st, a);
-        int rc = check_launch("dt_kv_attn");
-        if (rc) return rc;
-        if (p.splits > 1) {
-            hipLaunchKernelGGL((kv_rows_join_kernel<DP>), dim3((unsigned)((n * (DP / 4) + 255) / 256)), dim3(256), 0, st, a);
-            rc = check_launch("dt_kv_attn");
-            if (rc) return rc;
-        }
-    }
-    if (!p.stream) return DT_OK;
-    const bool wide = 1 << a.c.page_log2 >= Stream<E, DP, true>::STEP;
+    const bool wide = 1 << a.c.page_log2 >= (p.rows ? kTile : Stream<E, DP, true>::STEP);
     if (p.whole) {
-        const dim3 grid((unsigned)(((int64_t)a.s.rows * a.group / kRows + a.s.seqs) * a.c.kv_heads));
+        const dim3 grid((unsigned)((n / a.c.kv_heads / kRows + a.s.seqs) * a.c.kv_heads));
         const size_t lds = 8 * kRows * (DP + 4) * sizeof(float);
         if (wide) hipLaunchKernelGGL((kv_short_kernel<E, DP, true>), grid, dim3(512), lds, st, a);
         else hipLaunchKernelGGL((kv_short_kernel<E, DP, false>), grid, dim3(512), lds, st, a);
         return check_launch("dt_kv_attn");
     }
-    const dim3 grid((unsigned)(a.c.kv_heads * (a.waves / 4)));
-    if (wide) hipLaunchKernelGGL((kv_stream_kernel<E, DP, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv_stream_kernel<E, DP, false>), grid, dim3(256), 0, st, a);
-    int rc = check_launch("dt_kv_attn");
-    if (rc) return rc;
-    // Few rows may each have many shares: a workgroup a row.
-    const int64_t joined = p.few == kFew ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
-    if (joined <= 1024) {
-        hipLaunchKernelGGL((kv_join_kernel<E, DP, 256>), dim3((unsigned)joined), dim3(256), 0, st, a);
+    if (p.rows) {
+        a.stream_blocks = p.stream ? a.c.kv_heads * a.waves / (p.block / 32) : 0;
+        const dim3 grid((unsigned)(a.stream_blocks + p.blocks * p.splits * a.c.kv_heads)), block(2 * p.block);
+        const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
+        if (!wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 8>), grid, block, lds, st, a);
+        else if (p.block == 256) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
+        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 4>), grid, block, lds, st, a);
     } else {
-        hipLaunchKernelGGL((kv_join_kernel<E, DP, 64>), dim3((unsigned)((joined + 3) / 4)), dim3(256), 0, st, a);
+        const dim3 grid((unsigned)(a.c.kv_heads * (a.waves / 4)));
+        if (wide) hipLaunchKernelGGL((kv_stream_kernel<E, DP, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((kv_stream_kernel<E, DP, false>), grid, dim3(256), 0, st, a);
     }
+    const int rc = check_launch("dt_kv_attn");
+    // Shares of the stream: few rows may each have many, then a workgroup a row.  Key ranges: four elements a thread.
+    const int64_t joined = !p.stream ? 0 : p.rows ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
+    const int64_t ranges = p.splits > 1 ? (n * (DP / 4) + 255) / 256 : 0;
+    if (rc || joined + ranges == 0) return rc;
+    a.join_blocks = (int32_t)(joined <= 1024 ? joined : (joined + 3) / 4);
+    const dim3 grid((unsigned)(a.join_blocks + ranges));
+    if (joined <= 1024) hipLaunchKernelGGL((kv_join_kernel<E, DP, 256>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv_join_kernel<E, DP, 64>), grid, dim3(256), 0, st, a);
     return check_launch("dt_kv_attn");
 }
 
@@ -1157,7 +1170,7 @@ extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, cons
     const size_t need = (size_t)(p.floats + p.row_floats) * sizeof(float);
     DT_REQUIRE(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                "%s: a 16-byte aligned workspace of %lld bytes is needed", who, (long long)need);
-    DT_REQUIRE(p.blocks * p.splits * a.c.kv_heads < (1ll << 31) &&
+    DT_REQUIRE((p.blocks + 1) * p.splits * a.c.kv_heads < (1ll << 30) &&
                    ((int64_t)a.s.rows * (heads / a.c.kv_heads) / kRows + a.s.seqs) * a.c.kv_heads < (1ll << 31) && (int64_t)a.s.seqs * a.c.kv_heads * kFew < (1ll << 31),
                "%s: grid too large", who);
     a.q = (const uint16_t*)q;
