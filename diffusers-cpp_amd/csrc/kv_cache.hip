@@ -34,7 +34,9 @@ struct Args {
     int32_t kv_blocks;               // workgroups before q's
     int32_t q_chunks;                // waves a row of q
     FastDiv head_div, chunk_div;
-    int32_t lds_row;                 // elements a dim's row of v takes in LDS
+    int32_t quads_per_pass;          // v: fours of tokens a pass
+    FastDiv quad_div;                // by the fours of dims of a row
+    int32_t lds_row;                 // words a dim's row of v takes in LDS
 };
 
 constexpr int kScaleLow = 1;   // 2^-126
@@ -118,81 +120,110 @@ __device__ void rotate_q(const Args& a) {
     }
 }
 
-// NP passes hold a page.
+// The largest of the workgroup's `most`.
+__device__ __forceinline__ float most_of_all(float most, float* of) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) of[threadIdx.x >> 6] = most;
+    __syncthreads();
+    return fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+}
+
+template <typename E>
+__device__ __forceinline__ uint4 stored8(const float (&x)[8], int shift) {
+    if constexpr (sizeof(E) == 1) {
+        float c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = scaled(x[e], shift);
+        return make_uint4(to_e4m3x4(c[0], c[1], c[2], c[3]), to_e4m3x4(c[4], c[5], c[6], c[7]), 0, 0);
+    } else {
+        return Io<bf16>::pack(x);
+    }
+}
+template <typename E>
+__device__ __forceinline__ void store8(uint8_t* y, uint4 w) {
+    if constexpr (sizeof(E) == 1) *reinterpret_cast<uint2*>(y) = make_uint2(w.x, w.y);
+    else *reinterpret_cast<uint4*>(y) = w;
+}
+
+// The scale of a page whose new values reach `most`, and by how much its earlier codes shrink.
+__device__ __forceinline__ int page_scale(float most, int before, bool has_before, int* grown) {
+    const int scale = scale_of(most);
+    *grown = has_before && scale > before ? scale - before : 0;
+    return has_before ? max(scale, before) : scale;
+}
+
+// k of one page and head.  Rotated in 32 bits, as values +- tol; only pairs of which an end is stored as another
+// code than the other end (one of ten thousand with e4m3) are rotated in 64 bits after all, and so is the page
+// where its scale is in doubt: what is stored is always the value's own rounding.
 template <typename T, typename E, int NP>
-__global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
+__device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int row0, int h, float* of) {
     constexpr bool F8 = sizeof(E) == 1;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // v: [dim][lds_row] elements
-    __shared__ float most_of[4];
-    if ((int)blockIdx.x >= a.kv_blocks) {
-        rotate_q<T>(a);
-        return;
-    }
-    // Workgroup: (number of a page, head, k or v), heads innermost: they share rows.
-    const int tid = threadIdx.x, wave = tid >> 6;
-    const bool is_v = blockIdx.x & 1;
-    const int item = (int)fdiv(blockIdx.x >> 1, a.head_div), h = (int)(blockIdx.x >> 1) - item * a.c.kv_heads;
-    const int page = 1 << a.c.page_log2, dim = a.c.dim;
-    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_item(a.s, start, i); });
-    if (b < 0) return;
-    const Seq q(a.s, b);
-    PageItem it;
-    if (!page_item(a.s, q, b, item, &it)) return;
-    const int first = it.first, last = it.last;
-
+    const int tid = threadIdx.x, dim = a.c.dim, first = it.first, last = it.last;
     const int t0 = (int)fdiv((uint32_t)tid, a.unit_div), u = tid - t0 * a.units;
-    const rotary::Unit at(u, is_v ? 0 : a.rot, a.half);
-    const T* src = reinterpret_cast<const T*>(is_v ? a.v : a.k) + h * (is_v ? a.vs[1] : a.ks[1]);
-    const int64_t stride = is_v ? a.vs[0] : a.ks[0];
-    const int row0 = q.row + it.begin - q.past;  // of the page's token 0 (there may be none)
-    float v[NP][16];
-    float most = 0.f;
+    const rotary::Unit at(u, a.rot, a.half);
+    const T* src = reinterpret_cast<const T*>(a.k) + h * a.ks[1];
+    const bool turned = 16 * u < a.rot, mine = t0 < a.per_pass;
+    auto place = [&](int t) { return a.pos ? a.pos[row0 + t] : it.begin + t; };
+    auto load = [&](int t, float (&v)[16]) {
+        const T* x = src + (int64_t)(row0 + t) * a.ks[0];
+        load8(x + at.a, v);
+        load8(x + at.b, v + 8);
+    };
+    auto exact = [&](int t, float (&v)[16]) {
+        load(t, v);
+        if (!turned) return;
+        rotary::Angles<double> w;
+        w.set(place(t), a.freq, u, a.rot, (double)a.mul);
+        double d[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = (double)v[e];
+        w.turn(d, u, a.rot, a.half, 1.0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = to_odd(d[e]);
+    };
+    auto largest = [&](const float (&v)[16], float most) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) most = fmaxf(most, finite(v[e]) ? fabsf(v[e]) : 0.f);
+        return most;
+    };
+    float v[NP][16], most = 0.f;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
-        if (t0 >= a.per_pass || t >= last) continue;
-        const T* x = src + (int64_t)(row0 + t) * stride;
-        load8(x + at.a, v[i]);
-        load8(x + at.b, v[i] + 8);
+        if (mine && t < last) load(t, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
-        if (t0 >= a.per_pass || t >= last) continue;
-        if (!is_v && 16 * u < a.rot) {
-            rotary::Angles<double> w;
-            w.set(a.pos ? a.pos[row0 + t] : it.begin + t, a.freq, u, a.rot, (double)a.mul);
-            double d[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) d[e] = (double)v[i][e];
-            w.turn(d, u, a.rot, a.half, 1.0);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[i][e] = to_odd(d[e]);
+        if (!mine || t >= last) continue;
+        if (turned) {
+            rotary::Angles<float> w;
+            w.set(place(t), a.freq, u, a.rot, a.mul);
+            w.turn(v[i], u, a.rot, a.half, 1.f);
         }
-        if constexpr (F8) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) most = fmaxf(most, finite(v[i][e]) ? fabsf(v[i][e]) : 0.f);
-        }
+        if constexpr (F8) most = largest(v[i], most);
     }
 
-    uint8_t* const out = (is_v ? a.c.v : a.c.k) + ((int64_t)it.page * a.c.kv_heads + h) * a.c.head_bytes;
-    int scale = kBias, grown = 0;  // grown: by how much the page's earlier codes shrink
+    uint8_t* const out = a.c.k + ((int64_t)it.page * a.c.kv_heads + h) * a.c.head_bytes;
+    int scale = kBias, grown = 0;
     if constexpr (F8) {
-        uint8_t* const held = (is_v ? a.c.v_scale : a.c.k_scale) + (int64_t)it.page * a.c.kv_heads + h;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, 64));
-        if ((tid & 63) == 0) most_of[wave] = most;
+        uint8_t* const held = a.c.k_scale + (int64_t)it.page * a.c.kv_heads + h;
         const int before = first ? (int)*held : 0;
-        __syncthreads();
-        scale = scale_of(fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3])));
-        if (first) {
-            if (scale > before) grown = scale - before;
-            scale = max(scale, before);
+        most = most_of_all(most, of);
+        if (scale_of(most * (1.f - 0x1p-19f)) != scale_of(most * (1.f + 0x1p-19f))) {
+            most = 0.f;
+#pragma unroll 1
+            for (int t = first + t0; mine && t < last; t += a.per_pass) {
+                float x[16];
+                exact(t, x);
+                most = largest(x, most);
+            }
+            most = most_of_all(most, of);
         }
-        if (tid == 0) *held = (uint8_t)scale;  // read by all before the barrier
-    }
-
-    if (!is_v) {
+        scale = page_scale(most, before, first > 0, &grown);
+        if (tid == 0) *held = (uint8_t)scale;  // read by all before the barriers
         if (grown)
             for (int i = tid; i < first * dim / 16; i += 256) {
                 uint4 w = *reinterpret_cast<const uint4*>(out + 16 * i);
@@ -202,43 +233,128 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
                 w.w = again(w.w, -grown);
                 *reinterpret_cast<uint4*>(out + 16 * i) = w;
             }
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int t = first + i * a.per_pass + t0;
-            if (t0 >= a.per_pass || t >= last) continue;
-#pragma unroll
-            for (int run = 0; run < 2; ++run) {
-                const float* x = v[i] + 8 * run;
-                uint8_t* y = out + ((int64_t)t * dim + (run ? at.b : at.a)) * sizeof(E);
-                if constexpr (F8) {
-                    float c[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) c[e] = scaled(x[e], kBias - scale);
-                    *reinterpret_cast<uint2*>(y) = make_uint2(to_e4m3x4(c[0], c[1], c[2], c[3]), to_e4m3x4(c[4], c[5], c[6], c[7]));
-                } else {
-                    *reinterpret_cast<uint4*>(y) = Io<bf16>::pack(x);
-                }
-            }
-        }
-        return;
     }
-
-    // v: codes to LDS by (dim, token), then whole 16-byte pieces of a dim's row.
-    E* const turned = reinterpret_cast<E*>(lds);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
-        if (t0 >= a.per_pass || t >= last) continue;
+        if (!mine || t >= last) continue;
+        // A rotation keeps a pair's length l: |x| + |y| <= sqrt(2) l <= sqrt(2) (|x'| + |y'|).  The cosine and sine
+        // are off by 2^-23.4 at most (2^-24.7 from the angle, two roundings at the end), products and
+        // sum add three roundings: below 2^-22.3 (|x| + |y|) in all, 2^-21.8 (|x'| + |y'|).
+        float tol[8];
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            if constexpr (F8) {
-                const uint32_t w = to_e4m3x4(scaled(v[i][e], kBias - scale), scaled(v[i][e + 1], kBias - scale),
-                                             scaled(v[i][e + 2], kBias - scale), scaled(v[i][e + 3], kBias - scale));
+        for (int e = 0; e < 8; ++e) {
+            const float x = a.half ? v[i][e] : v[i][2 * e], y = a.half ? v[i][8 + e] : v[i][2 * e + 1];
+            tol[e] = (fabsf(x) + fabsf(y)) * 0x1.4p-22f;
+        }
+        uint4 differ[2];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) turned[(16 * u + e + n) * a.lds_row + t].bits = (uint8_t)(w >> (8 * n));
+        for (int run = 0; run < 2; ++run) {
+            float y[8], lo[8], hi[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] = v[i][8 * run + e];
+                const float d = tol[a.half ? e : 4 * run + e / 2];
+                lo[e] = y[e] - d;
+                hi[e] = y[e] + d;
+            }
+            store8<E>(out + ((int64_t)t * dim + (run ? at.b : at.a)) * sizeof(E), stored8<E>(y, kBias - scale));
+            const uint4 p = stored8<E>(lo, kBias - scale), q = stored8<E>(hi, kBias - scale);
+            differ[run] = make_uint4(p.x ^ q.x, p.y ^ q.y, p.z ^ q.z, p.w ^ q.w);
+        }
+        if (!turned || !(differ[0].x | differ[0].y | differ[0].z | differ[0].w | differ[1].x | differ[1].y | differ[1].z | differ[1].w)) continue;
+        uint32_t pairs = 0;
+#pragma unroll
+        for (int run = 0; run < 2; ++run)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int per = 4 / (int)sizeof(E);
+                const uint32_t w[4] = {differ[run].x, differ[run].y, differ[run].z, differ[run].w};
+                if (w[e / per] << (32 - 8 * (int)sizeof(E) * (e % per + 1)) >> (32 - 8 * (int)sizeof(E))) pairs |= 1u << (a.half ? e : 4 * run + e / 2);
+            }
+        const T* x = src + (int64_t)(row0 + t) * a.ks[0];
+#pragma unroll 1
+        for (; pairs; pairs &= pairs - 1) {
+            const int e = __builtin_ctz(pairs), n = 8 * u + e;  // pair of the head
+            if (2 * n >= a.rot) continue;
+            const int d0 = a.half ? n : 2 * n, d1 = a.half ? n + a.rot / 2 : 2 * n + 1;
+            double c, s;
+            rotary::cos_sin(place(t), a.freq[n], (double)a.mul, &c, &s);
+            const double p = Io<T>::get(x + d0), q = Io<T>::get(x + d1);
+            const float w[2] = {to_odd(p * c - q * s), to_odd(q * c + p * s)};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint8_t* y = out + ((int64_t)t * dim + (k ? d1 : d0)) * sizeof(E);
+                if constexpr (F8) *y = (uint8_t)to_e4m3x4(scaled(w[k], kBias - scale), 0.f, 0.f, 0.f);
+                else Io<bf16>::put(reinterpret_cast<bf16*>(y), w[k]);
+            }
+        }
+    }
+}
+
+// v of one page and head: a thread takes four tokens by four dims, so that a dim's four codes are a word of its
+// row in LDS, from where whole 16-byte pieces of rows go out.
+template <typename T, typename E, int NP>
+__device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int row0, int h, float* of, uint32_t* turned) {
+    constexpr bool F8 = sizeof(E) == 1;
+    constexpr int WPT = sizeof(E);  // words of four tokens
+    const int tid = threadIdx.x, dim = a.c.dim, page = 1 << a.c.page_log2, first = it.first, last = it.last;
+    const int g0 = (int)fdiv((uint32_t)tid, a.quad_div), d0 = 4 * (tid - g0 * (dim / 4));
+    const T* src = reinterpret_cast<const T*>(a.v) + h * a.vs[1] + d0;
+    const bool mine = g0 < a.quads_per_pass;
+    const int start = first & ~3;  // tokens in fours, as they lie in the page
+    float v[NP][4][4], most = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int t = start + 4 * (i * a.quads_per_pass + g0) + k;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i][k][e] = 0.f;
+            if (!mine || t < first || t >= last) continue;
+            const T* x = src + (int64_t)(row0 + t) * a.vs[0];
+            if constexpr (sizeof(T) == 4) {
+                const float4 w = *reinterpret_cast<const float4*>(x);
+                v[i][k][0] = w.x;
+                v[i][k][1] = w.y;
+                v[i][k][2] = w.z;
+                v[i][k][3] = w.w;
             } else {
+                const uint2 w = *reinterpret_cast<const uint2*>(x);
+                v[i][k][0] = bf16_lo(w.x);
+                v[i][k][1] = bf16_hi(w.x);
+                v[i][k][2] = bf16_lo(w.y);
+                v[i][k][3] = bf16_hi(w.y);
+            }
+        }
+    uint8_t* const out = a.c.v + ((int64_t)it.page * a.c.kv_heads + h) * a.c.head_bytes;
+    int scale = kBias, grown = 0;
+    if constexpr (F8) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) Io<bf16>::put((bf16*)turned + (16 * u + e + n) * a.lds_row + t, v[i][e + n]);
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) most = fmaxf(most, finite(v[i][k][e]) ? fabsf(v[i][k][e]) : 0.f);
+        uint8_t* const held = a.c.v_scale + (int64_t)it.page * a.c.kv_heads + h;
+        const int before = first ? (int)*held : 0;
+        most = most_of_all(most, of);
+        scale = page_scale(most, before, first > 0, &grown);
+        if (tid == 0) *held = (uint8_t)scale;  // read by all before the barriers
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int t = start + 4 * (i * a.quads_per_pass + g0);
+        if (!mine || t >= last) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t* w = turned + (d0 + e) * a.lds_row + t / 4 * WPT;
+            if constexpr (F8) {
+                w[0] = to_e4m3x4(scaled(v[i][0][e], kBias - scale), scaled(v[i][1][e], kBias - scale),
+                                 scaled(v[i][2][e], kBias - scale), scaled(v[i][3][e], kBias - scale));
+            } else {
+                w[0] = pack_bf16x2(v[i][0][e], v[i][1][e]);
+                w[1] = pack_bf16x2(v[i][2][e], v[i][3][e]);
             }
         }
     }
@@ -249,9 +365,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
         const int d = i / pieces, c = (i & (pieces - 1)) * PER;
         if (c >= last || (c + PER <= first && !grown)) continue;
         uint8_t* y = out + ((int64_t)d * page + c) * sizeof(E);
-        const E* x = turned + d * a.lds_row + c;
+        const uint32_t* x = turned + d * a.lds_row + c * (int)sizeof(E) / 4;
         if (c >= first && c + PER <= last) {
-            *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(x);
+            *reinterpret_cast<uint4*>(y) = make_uint4(x[0], x[1], x[2], x[3]);
             continue;
         }
         if constexpr (F8) {
@@ -266,13 +382,34 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
                 }
             }
         }
-        for (int n = max(first - c, 0); n < min(last - c, PER); ++n) reinterpret_cast<E*>(y)[n] = x[n];
+        for (int n = max(first - c, 0); n < min(last - c, PER); ++n) reinterpret_cast<E*>(y)[n] = reinterpret_cast<const E*>(x)[n];
     }
+}
+
+// NP passes hold a page.
+template <typename T, typename E, int NP>
+__global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t turned[];  // v: [dim][lds_row] words
+    __shared__ float most_of[4];
+    if ((int)blockIdx.x >= a.kv_blocks) {
+        rotate_q<T>(a);
+        return;
+    }
+    // Workgroup: (number of a page, head, k or v), heads innermost: they share rows.
+    const int item = (int)fdiv(blockIdx.x >> 1, a.head_div), h = (int)(blockIdx.x >> 1) - item * a.c.kv_heads;
+    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_item(a.s, start, i); });
+    if (b < 0) return;
+    const Seq q(a.s, b);
+    PageItem it;
+    if (!page_item(a.s, q, b, item, &it)) return;
+    const int row0 = q.row + it.begin - q.past;  // of the page's token 0 (there may be none)
+    if (blockIdx.x & 1) append_v<T, E, NP>(a, it, row0, h, most_of, turned);
+    else append_k<T, E, NP>(a, it, row0, h, most_of);
 }
 
 template <typename T, typename E>
 int launch(const Args& a, int passes, dim3 grid, hipStream_t st) {
-    const size_t lds = (size_t)a.c.dim * a.lds_row * sizeof(E);
+    const size_t lds = (size_t)a.c.dim * a.lds_row * sizeof(uint32_t);
     if (passes <= 1) hipLaunchKernelGGL((kv_append_kernel<T, E, 1>), grid, dim3(256), lds, st, a);
     else if (passes <= 2) hipLaunchKernelGGL((kv_append_kernel<T, E, 2>), grid, dim3(256), lds, st, a);
     else if (passes <= 4) hipLaunchKernelGGL((kv_append_kernel<T, E, 4>), grid, dim3(256), lds, st, a);
@@ -406,13 +543,17 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
     a.chunk_div = make_fastdiv((uint32_t)a.q_chunks);
     const int64_t page = 1ll << a.c.page_log2;
     const bool f8 = a.c.k_scale != nullptr;
-    a.lds_row = (int32_t)page + 16 / (f8 ? 1 : 2);
+    // An odd number of words: dims lie in other banks.
+    a.lds_row = (int32_t)page * (f8 ? 1 : 2) / 4 + 1;
+    a.quads_per_pass = 256 / (a.c.dim / 4);
+    a.quad_div = make_fastdiv((uint32_t)(a.c.dim / 4));
     const int64_t kv_blocks = items(a.s) * a.c.kv_heads * 2;
     const int64_t q_blocks = turn_q ? ((int64_t)a.s.rows * a.q_chunks + 3) / 4 : 0;
     DT_REQUIRE(kv_blocks + q_blocks < (1ll << 31) && (int64_t)a.s.rows * a.q_chunks < (1ll << 31), "%s: grid too large", who);
     a.kv_blocks = (int32_t)kv_blocks;
     const dim3 grid((unsigned)(kv_blocks + q_blocks));
-    const int passes = ((int)page + a.per_pass - 1) / a.per_pass;
+    const int k_passes = ((int)page + a.per_pass - 1) / a.per_pass, v_passes = ((int)page / 4 + a.quads_per_pass - 1) / a.quads_per_pass;
+    const int passes = k_passes > v_passes ? k_passes : v_passes;
     const hipStream_t st = (hipStream_t)stream;
     if (x->io_type == DT_TYPE_F32)
         return f8 ? launch<float, e4m3>(a, passes, grid, st) : launch<float, bf16>(a, passes, grid, st);
