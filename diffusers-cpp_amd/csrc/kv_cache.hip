@@ -61,18 +61,38 @@ __device__ __forceinline__ float to_odd(double d) {
     return __uint_as_float(u | 1u);
 }
 
-// A value times 2^shift as an e4m3 code's input: NaN unless finite.
-__device__ __forceinline__ float scaled(float x, int shift) {
-    return finite(x) ? __builtin_amdgcn_ldexpf(x, shift) : __builtin_nanf("");
-}
+// A value that is not finite is held as NaN: the conversion would have the largest code for infinities.
+__device__ __forceinline__ float tame(float x) { return finite(x) ? x : __builtin_nanf(""); }
 
-// Codes times 2^shift, rounded again.
+__device__ __forceinline__ float power(int scale) { return __uint_as_float((uint32_t)scale << 23); }
+
+// Codes times 2^-shift, rounded again.
 __device__ __forceinline__ uint32_t again(uint32_t w, int shift) {
     float v[4];
     from_e4m3x4(w, v);
-    return to_e4m3x4(__builtin_amdgcn_ldexpf(v[0], shift), __builtin_amdgcn_ldexpf(v[1], shift),
-                     __builtin_amdgcn_ldexpf(v[2], shift), __builtin_amdgcn_ldexpf(v[3], shift));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_ldexpf(v[e], -shift);
+    return to_e4m3x4(v[0], v[1], v[2], v[3], 1.f);
 }
+
+// The largest size of N values, and whether all are finite: sizes of others do not count, which a second look sees to.
+struct Most {
+    float top = 0.f, zero = 0.f;  // zero: 0 while all are finite, then NaN
+    template <int N>
+    __device__ __forceinline__ void take(const float (&v)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            top = fmaxf(top, fabsf(v[e]));
+            zero = __builtin_fmaf(v[e], 0.f, zero);
+        }
+    }
+    __device__ __forceinline__ bool tame() const { return zero == 0.f; }
+    template <int N>
+    __device__ __forceinline__ void take_finite(const float (&v)[N]) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) top = fmaxf(top, finite(v[e]) ? fabsf(v[e]) : 0.f);
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float* v) {
@@ -92,7 +112,7 @@ __device__ void rotate_q(const Args& a) {
     const int slot = (int)fdiv(lane, a.unit_div), u = (int)lane - slot * a.units;
     if (slot >= a.slots) return;
     const int p = a.pos ? a.pos[row] : q.past + row - q.row;
-    const rotary::Unit at(u, a.rot, a.half);
+    const rotary::Unit<8> at(u, a.rot, a.half);
     constexpr int ITER = 4;
     const int first = chunk * ITER * a.slots + slot;
     float v[ITER][16];
@@ -104,13 +124,13 @@ __device__ void rotate_q(const Args& a) {
         load8(x + at.a, v[i]);
         load8(x + at.b, v[i] + 8);
     }
-    rotary::Angles<float> w;
-    w.set(p, a.freq, u, a.rot, a.mul);
+    rotary::Angles<float, 8> w;
+    w.set(p, a.freq, at, a.rot, a.mul);
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         const int h = first + i * a.slots;
         if (h >= a.heads) continue;
-        w.turn(v[i], u, a.rot, a.half, 1.f);
+        w.turn(v[i], at, a.rot, a.half, 1.f);
         T* y = reinterpret_cast<T*>(a.q_out) + row * a.os[0] + h * a.os[1];
 #pragma unroll
         for (int n = 0; n < 8 / Io<T>::EPV; ++n) {
@@ -131,12 +151,9 @@ __device__ __forceinline__ float most_of_all(float most, float* of) {
 }
 
 template <typename E>
-__device__ __forceinline__ uint4 stored8(const float (&x)[8], int shift) {
+__device__ __forceinline__ uint4 stored8(const float (&x)[8], float scale) {
     if constexpr (sizeof(E) == 1) {
-        float c[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = scaled(x[e], shift);
-        return make_uint4(to_e4m3x4(c[0], c[1], c[2], c[3]), to_e4m3x4(c[4], c[5], c[6], c[7]), 0, 0);
+        return make_uint4(to_e4m3x4(x[0], x[1], x[2], x[3], scale), to_e4m3x4(x[4], x[5], x[6], x[7], scale), 0, 0);
     } else {
         return Io<bf16>::pack(x);
     }
@@ -158,11 +175,11 @@ __device__ __forceinline__ int page_scale(float most, int before, bool has_befor
 // code than the other end (one of ten thousand with e4m3) are rotated in 64 bits after all, and so is the page
 // where its scale is in doubt: what is stored is always the value's own rounding.
 template <typename T, typename E, int NP>
-__device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int row0, int h, float* of) {
+__device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int row0, int page, int h, float* of) {
     constexpr bool F8 = sizeof(E) == 1;
     const int tid = threadIdx.x, dim = a.c.dim, first = it.first, last = it.last;
     const int t0 = (int)fdiv((uint32_t)tid, a.unit_div), u = tid - t0 * a.units;
-    const rotary::Unit at(u, a.rot, a.half);
+    const rotary::Unit<8> at(u, a.rot, a.half);
     const T* src = reinterpret_cast<const T*>(a.k) + h * a.ks[1];
     const bool turned = 16 * u < a.rot, mine = t0 < a.per_pass;
     auto place = [&](int t) { return a.pos ? a.pos[row0 + t] : it.begin + t; };
@@ -174,63 +191,65 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
     auto exact = [&](int t, float (&v)[16]) {
         load(t, v);
         if (!turned) return;
-        rotary::Angles<double> w;
-        w.set(place(t), a.freq, u, a.rot, (double)a.mul);
+        rotary::Angles<double, 8> w;
+        w.set(place(t), a.freq, at, a.rot, (double)a.mul);
         double d[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) d[e] = (double)v[e];
-        w.turn(d, u, a.rot, a.half, 1.0);
+        w.turn(d, at, a.rot, a.half, 1.0);
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = to_odd(d[e]);
     };
-    auto largest = [&](const float (&v)[16], float most) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) most = fmaxf(most, finite(v[e]) ? fabsf(v[e]) : 0.f);
-        return most;
-    };
-    float v[NP][16], most = 0.f;
+    float v[NP][16];
+    Most most;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
         if (mine && t < last) load(t, v[i]);
     }
+    if ((uint32_t)page >= (uint32_t)a.s.pages) return;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
         if (!mine || t >= last) continue;
         if (turned) {
-            rotary::Angles<float> w;
-            w.set(place(t), a.freq, u, a.rot, a.mul);
-            w.turn(v[i], u, a.rot, a.half, 1.f);
+            rotary::Angles<float, 8> w;
+            w.set(place(t), a.freq, at, a.rot, a.mul);
+            w.turn(v[i], at, a.rot, a.half, 1.f);
         }
-        if constexpr (F8) most = largest(v[i], most);
+        if constexpr (F8) most.take(v[i]);
     }
 
-    uint8_t* const out = a.c.k + ((int64_t)it.page * a.c.kv_heads + h) * a.c.head_bytes;
+    uint8_t* const out = a.c.k + ((int64_t)page * a.c.kv_heads + h) * a.c.head_bytes;
     int scale = kBias, grown = 0;
     if constexpr (F8) {
-        uint8_t* const held = a.c.k_scale + (int64_t)it.page * a.c.kv_heads + h;
+        uint8_t* const held = a.c.k_scale + (int64_t)page * a.c.kv_heads + h;
         const int before = first ? (int)*held : 0;
-        most = most_of_all(most, of);
-        if (scale_of(most * (1.f - 0x1p-19f)) != scale_of(most * (1.f + 0x1p-19f))) {
-            most = 0.f;
+        const bool tamed = __syncthreads_and(most.tame());
+        float top = most_of_all(most.top, of);
+        if (!tamed || scale_of(top * (1.f - 0x1p-19f)) != scale_of(top * (1.f + 0x1p-19f))) {
+            Most again;
 #pragma unroll 1
             for (int t = first + t0; mine && t < last; t += a.per_pass) {
                 float x[16];
                 exact(t, x);
-                most = largest(x, most);
+                again.take_finite(x);
             }
-            most = most_of_all(most, of);
+            top = most_of_all(again.top, of);
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[i][e] = tame(v[i][e]);
         }
-        scale = page_scale(most, before, first > 0, &grown);
+        scale = page_scale(top, before, first > 0, &grown);
         if (tid == 0) *held = (uint8_t)scale;  // read by all before the barriers
         if (grown)
             for (int i = tid; i < first * dim / 16; i += 256) {
                 uint4 w = *reinterpret_cast<const uint4*>(out + 16 * i);
-                w.x = again(w.x, -grown);
-                w.y = again(w.y, -grown);
-                w.z = again(w.z, -grown);
-                w.w = again(w.w, -grown);
+                w.x = again(w.x, grown);
+                w.y = again(w.y, grown);
+                w.z = again(w.z, grown);
+                w.w = again(w.w, grown);
                 *reinterpret_cast<uint4*>(out + 16 * i) = w;
             }
     }
@@ -238,28 +257,27 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
         if (!mine || t >= last) continue;
-        // A rotation keeps a pair's length l: |x| + |y| <= sqrt(2) l <= sqrt(2) (|x'| + |y'|).  The cosine and sine
-        // are off by 2^-23.4 at most (2^-24.7 from the angle, two roundings at the end), products and
-        // sum add three roundings: below 2^-22.3 (|x| + |y|) in all, 2^-21.8 (|x'| + |y'|).
+        // A rotation keeps a pair's length l: |x| + |y| <= sqrt(2) l <= sqrt(2) (|x'| + |y'|).  Cosine and sine are off by
+        // 2^-23 and the factor's rounding, products and sum add two roundings: below 5 2^-24 (|x| + |y|) in all,
+        // 1.8 2^-22 (|x'| + |y'|).
         float tol[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float x = a.half ? v[i][e] : v[i][2 * e], y = a.half ? v[i][8 + e] : v[i][2 * e + 1];
-            tol[e] = (fabsf(x) + fabsf(y)) * 0x1.4p-22f;
+            tol[e] = 2 * (8 * u + e) < a.rot ? (fabsf(x) + fabsf(y)) * 0x1p-21f : 0.f;
         }
         uint4 differ[2];
 #pragma unroll
         for (int run = 0; run < 2; ++run) {
-            float y[8], lo[8], hi[8];
+            float lo[8], hi[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                y[e] = v[i][8 * run + e];
                 const float d = tol[a.half ? e : 4 * run + e / 2];
-                lo[e] = y[e] - d;
-                hi[e] = y[e] + d;
+                lo[e] = v[i][8 * run + e] - d;
+                hi[e] = v[i][8 * run + e] + d;
             }
-            store8<E>(out + ((int64_t)t * dim + (run ? at.b : at.a)) * sizeof(E), stored8<E>(y, kBias - scale));
-            const uint4 p = stored8<E>(lo, kBias - scale), q = stored8<E>(hi, kBias - scale);
+            const uint4 p = stored8<E>(lo, power(scale)), q = stored8<E>(hi, power(scale));
+            store8<E>(out + ((int64_t)t * dim + (run ? at.b : at.a)) * sizeof(E), p);
             differ[run] = make_uint4(p.x ^ q.x, p.y ^ q.y, p.z ^ q.z, p.w ^ q.w);
         }
         if (!turned || !(differ[0].x | differ[0].y | differ[0].z | differ[0].w | differ[1].x | differ[1].y | differ[1].z | differ[1].w)) continue;
@@ -285,7 +303,7 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 uint8_t* y = out + ((int64_t)t * dim + (k ? d1 : d0)) * sizeof(E);
-                if constexpr (F8) *y = (uint8_t)to_e4m3x4(scaled(w[k], kBias - scale), 0.f, 0.f, 0.f);
+                if constexpr (F8) *y = (uint8_t)to_e4m3x4(tame(w[k]), 0.f, 0.f, 0.f, power(scale));
                 else Io<bf16>::put(reinterpret_cast<bf16*>(y), w[k]);
             }
         }
@@ -295,7 +313,7 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
 // v of one page and head: a thread takes four tokens by four dims, so that a dim's four codes are a word of its
 // row in LDS, from where whole 16-byte pieces of rows go out.
 template <typename T, typename E, int NP>
-__device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int row0, int h, float* of, uint32_t* turned) {
+__device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int row0, int in_page, int h, float* of, uint32_t* turned) {
     constexpr bool F8 = sizeof(E) == 1;
     constexpr int WPT = sizeof(E);  // words of four tokens
     const int tid = threadIdx.x, dim = a.c.dim, page = 1 << a.c.page_log2, first = it.first, last = it.last;
@@ -303,7 +321,7 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
     const T* src = reinterpret_cast<const T*>(a.v) + h * a.vs[1] + d0;
     const bool mine = g0 < a.quads_per_pass;
     const int start = first & ~3;  // tokens in fours, as they lie in the page
-    float v[NP][4][4], most = 0.f;
+    float v[NP][4][4];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -327,19 +345,29 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
                 v[i][k][3] = bf16_hi(w.y);
             }
         }
-    uint8_t* const out = a.c.v + ((int64_t)it.page * a.c.kv_heads + h) * a.c.head_bytes;
+    if ((uint32_t)in_page >= (uint32_t)a.s.pages) return;
+    uint8_t* const out = a.c.v + ((int64_t)in_page * a.c.kv_heads + h) * a.c.head_bytes;
     int scale = kBias, grown = 0;
     if constexpr (F8) {
+        Most most;
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k) most.take(v[i][k]);
+        if (!__syncthreads_and(most.tame())) {
+            most.top = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) most = fmaxf(most, finite(v[i][k][e]) ? fabsf(v[i][k][e]) : 0.f);
-        uint8_t* const held = a.c.v_scale + (int64_t)it.page * a.c.kv_heads + h;
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    most.take_finite(v[i][k]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[i][k][e] = tame(v[i][k][e]);
+                }
+        }
+        uint8_t* const held = a.c.v_scale + (int64_t)in_page * a.c.kv_heads + h;
         const int before = first ? (int)*held : 0;
-        most = most_of_all(most, of);
-        scale = page_scale(most, before, first > 0, &grown);
+        scale = page_scale(most_of_all(most.top, of), before, first > 0, &grown);
         if (tid == 0) *held = (uint8_t)scale;  // read by all before the barriers
     }
 #pragma unroll
@@ -350,8 +378,7 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
         for (int e = 0; e < 4; ++e) {
             uint32_t* w = turned + (d0 + e) * a.lds_row + t / 4 * WPT;
             if constexpr (F8) {
-                w[0] = to_e4m3x4(scaled(v[i][0][e], kBias - scale), scaled(v[i][1][e], kBias - scale),
-                                 scaled(v[i][2][e], kBias - scale), scaled(v[i][3][e], kBias - scale));
+                w[0] = to_e4m3x4(v[i][0][e], v[i][1][e], v[i][2][e], v[i][3][e], power(scale));
             } else {
                 w[0] = pack_bf16x2(v[i][0][e], v[i][1][e]);
                 w[1] = pack_bf16x2(v[i][2][e], v[i][3][e]);
@@ -375,7 +402,7 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
                 // Earlier tokens of the piece again; those that are not this call's stay.
                 for (int n = 0; n < 4; ++n) {
                     if (c + 4 * n >= first) break;
-                    const uint32_t w = reinterpret_cast<const uint32_t*>(y)[n], s = again(w, -grown);
+                    const uint32_t w = reinterpret_cast<const uint32_t*>(y)[n], s = again(w, grown);
                     const int left = first - c - 4 * n;
                     const uint32_t m = left >= 4 ? ~0u : (1u << (8 * left)) - 1;
                     reinterpret_cast<uint32_t*>(y)[n] = (s & m) | (w & ~m);
@@ -386,9 +413,9 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
     }
 }
 
-// NP passes hold a page.
+// NP passes hold a page.  Registers for four workgroups a CU where two passes do (8750 tokens of 32 + 8 heads: 57 us, 64 with three).
 template <typename T, typename E, int NP>
-__global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
+__global__ __launch_bounds__(256, NP <= 2 ? 4 : 2) void kv_append_kernel(const Args a) {
     extern __shared__ __attribute__((aligned(16))) uint32_t turned[];  // v: [dim][lds_row] words
     __shared__ float most_of[4];
     if ((int)blockIdx.x >= a.kv_blocks) {
@@ -403,8 +430,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const Args a) {
     PageItem it;
     if (!page_item(a.s, q, b, item, &it)) return;
     const int row0 = q.row + it.begin - q.past;  // of the page's token 0 (there may be none)
-    if (blockIdx.x & 1) append_v<T, E, NP>(a, it, row0, h, most_of, turned);
-    else append_k<T, E, NP>(a, it, row0, h, most_of);
+    // The page's number is looked at when the tokens are on their way.
+    const int page = a.s.table[b * a.s.table_stride + (it.begin >> a.s.page_log2)];
+    if (blockIdx.x & 1) append_v<T, E, NP>(a, it, row0, page, h, most_of, turned);
+    else append_k<T, E, NP>(a, it, row0, page, h, most_of);
 }
 
 template <typename T, typename E>

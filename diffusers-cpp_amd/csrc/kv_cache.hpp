@@ -39,10 +39,13 @@ __device__ __forceinline__ int find_seq(const Seqs& s, int64_t x, Key key) {
 // ---- e4m3: four bits of significand, 2^-9 to 448, NaN but no infinity --------------------
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
-// Four values (at most 448 in size, or NaN) to codes, to nearest even.
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+// Four values over `scale` (a power of two; at most 448 then, or NaN) to codes, to nearest even.
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d, float scale) {
+    s16x2_t w = {0, 0};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, scale, true);
+    return __builtin_bit_cast(uint32_t, w);
 }
 __device__ __forceinline__ void from_e4m3x4(uint32_t w, float (&v)[4]) {
     const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);

@@ -55,9 +55,9 @@ DT_KV_FN int page_of(const Seqs& s, int b, int t) {
 DT_KV_FN int64_t first_item(const Seqs& s, int start, int b) { return (int64_t)(start >> s.page_log2) + 2 * b; }
 DT_KV_FN int64_t items(const Seqs& s) { return first_item(s, s.rows, s.seqs); }
 
-// Item `item` of sequence b: its page, and which of the page's rows are new.  False: none.
+// Item `item` of sequence b: which rows of its page (page_of(begin)) are new.  False: none.
 struct PageItem {
-    int page, begin, first, last;  // begin: the place of the page's row 0; new rows [first, last)
+    int begin, first, last;  // begin: the place of the page's row 0; new rows [first, last)
 };
 DT_KV_FN bool page_item(const Seqs& s, const Seq& q, int b, int64_t item, PageItem* out) {
     const int64_t j = item - first_item(s, q.row, b) + (q.past >> s.page_log2), begin = j * (1 << s.page_log2);
@@ -66,9 +66,7 @@ DT_KV_FN bool page_item(const Seqs& s, const Seq& q, int b, int64_t item, PageIt
     out->begin = (int)begin;
     out->first = q.past > begin ? (int)(q.past - begin) : 0;
     out->last = q.len - begin < size ? (int)(q.len - begin) : size;
-    if (out->first >= out->last) return false;
-    out->page = page_of(s, b, (int)begin);
-    return out->page >= 0;
+    return out->first < out->last;
 }
 
 }  // namespace kv

@@ -2,7 +2,7 @@
 // rotation back): pair (x, y) -> (x c - y s, y c + x s), c = f cos(p w), s = f sin(p w).
 //
 // One pass: 16 bytes a lane and load.  A wave takes one token and up to ITER heads a lane;
-// lane l holds 16 elements (8 pairs) of every (64 / units)-th head, so the angles, which cost
+// lane l holds two vectors of 16 bytes of every (64 / units)-th head, so the angles, which cost
 // more than the rotation, are worked out once for ITER heads.
 #include <math.h>
 
@@ -30,18 +30,13 @@ struct Args {
     int64_t pos_stride;
     const float* freq;
     float mul, sign;
-    int32_t units, slots, chunks;  // 16-element units a head; heads side by side in a wave; waves a token
+    int32_t units, slots, chunks;  // units of two vectors a head; heads side by side in a wave; waves a token
     FastDiv unit_div, chunk_div;
-};
-
-template <typename T> struct Raw {
-    static constexpr int NV = 8 / Io<T>::EPV;
-    uint4 a[NV], b[NV];
 };
 
 template <typename T, int ITER>
 __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
-    constexpr int NV = Raw<T>::NV, EPV = Io<T>::EPV;
+    constexpr int EPV = Io<T>::EPV;
     const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t row = fdiv(wave, a.chunk_div), chunk = wave - row * a.chunks;
     if (row >= (uint64_t)a.rows) return;
@@ -50,10 +45,10 @@ __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
     if (slot >= (uint32_t)a.slots) return;
     const uint32_t b = fdiv(row, a.seq_div), tok = row - b * a.seq;
     const int p = a.pos[(int64_t)b * a.pos_stride + tok];
-    const Unit at(u, a.rot, a.half);
+    const Unit<EPV> at(u, a.rot, a.half, a.units);
     const int first = (int)(chunk * ITER * a.slots + slot);
 
-    Raw<T> raw[ITER];
+    uint4 raw[ITER][2];
     int64_t to[ITER];
     T* y[ITER];
 #pragma unroll
@@ -70,29 +65,20 @@ __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
         const T* x = reinterpret_cast<const T*>(k ? t1.x : t.x) + b * xb + tok * xt + h * xh;
         y[i] = reinterpret_cast<T*>(k ? t1.y : t.y);
         to[i] = b * yb + tok * yt + h * yh;
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            raw[i].a[n] = ld_stream(x + at.a + n * EPV);
-            raw[i].b[n] = ld_stream(x + at.b + n * EPV);
-        }
+        raw[i][0] = ld_stream(x + at.a);
+        raw[i][1] = ld_stream(x + at.b);
     }
-    Angles<float> w;
-    w.set(p, a.freq, u, a.rot, a.mul);
+    Angles<float, EPV> w;
+    w.set(p, a.freq, at, a.rot, a.mul);
 #pragma unroll
     for (int i = 0; i < ITER; ++i) {
         if (!y[i]) continue;
-        float v[16];
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            Io<T>::unpack(raw[i].a[n], v + n * EPV);
-            Io<T>::unpack(raw[i].b[n], v + 8 + n * EPV);
-        }
-        w.turn(v, u, a.rot, a.half, a.sign);
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            st_stream(y[i] + to[i] + at.a + n * EPV, Io<T>::pack(v + n * EPV));
-            st_stream(y[i] + to[i] + at.b + n * EPV, Io<T>::pack(v + 8 + n * EPV));
-        }
+        float v[2 * EPV];
+        Io<T>::unpack(raw[i][0], v);
+        Io<T>::unpack(raw[i][1], v + EPV);
+        w.turn(v, at, a.rot, a.half, a.sign);
+        st_stream(y[i] + to[i] + at.a, Io<T>::pack(v));
+        st_stream(y[i] + to[i] + at.b, Io<T>::pack(v + EPV));
     }
 }
 
@@ -232,7 +218,8 @@ extern "C" int dt_rotary_apply(const dt_rotary_args* x, dt_stream_t stream) {
     a.rot = (int32_t)x->rotary.rot_dims;
     a.half = x->rotary.half != 0;
     // Whole units, whose runs are whole vectors.
-    bool wide = a.dim % 16 == 0 && a.dim <= 1024 && (!a.half || a.rot % 16 == 0);
+    const int unit = 32 / elem_size(x->io_type);
+    bool wide = a.dim % unit == 0 && a.dim <= 64 * unit && (!a.half || a.rot % unit == 0);
     if (a.heads[0]) {
         rc = check_tensor(x, x->q, x->q_strides, x->heads, false, "q", &wide);
         if (!rc) rc = check_tensor(x, x->q_out, x->q_out_strides, x->heads, true, "q_out", &wide);
@@ -260,7 +247,7 @@ extern "C" int dt_rotary_apply(const dt_rotary_args* x, dt_stream_t stream) {
     a.freq = x->rotary.freq;
     a.mul = x->rotary.attn_factor;
     a.sign = x->backward ? -1.f : 1.f;
-    a.units = a.dim / 16;
+    a.units = a.dim / unit;
     a.slots = a.units ? 64 / a.units : 0;
     if (wide) a.unit_div = make_fastdiv((uint32_t)a.units);
     const hipStream_t st = (hipStream_t)stream;

@@ -19,11 +19,12 @@ struct Quarter {
 __device__ __forceinline__ Quarter quarter(int pos, float freq) {
     // 2 / pi in two parts: the second is what the first rounds off.
     constexpr double kHi = 0.63661977236758138, kLo = -3.9357353350364971e-17;
+    constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52: a sum with it ends in the nearest whole number
     const double t = (double)pos * (double)freq;
-    const double q = rint(t * kHi);
+    const double w = __builtin_fma(t, kHi, kWhole), q = w - kWhole;
     Quarter r;
     r.f = __builtin_fma(t, kLo, __builtin_fma(t, kHi, -q));
-    r.n = (int)(q - 4.0 * floor(q * 0.25));
+    r.n = (int)(uint32_t)__double_as_longlong(w) & 3;
     return r;
 }
 
@@ -35,10 +36,11 @@ __device__ __forceinline__ void unfold(int n, F co, F si, F mul, F* c, F* s) {
     *s = (n & 2) ? -b * mul : b * mul;
 }
 
-// In 32 bits: the terms left out are below 2e-9 of the result.
+// In 32 bits: off by 2^-23 of mul at most (the angle by 2^-24, two roundings at the end; the terms left
+// out are below 2e-9).
 __device__ __forceinline__ void cos_sin(int pos, float freq, float mul, float* c, float* s) {
     const Quarter r = quarter(pos, freq);
-    const float x = (float)(r.f * 1.5707963267948966), y = x * x;
+    const float x = (float)r.f * 1.57079632679f, y = x * x;
     float co = __builtin_fmaf(y, -1.f / 3628800, 1.f / 40320);
     co = __builtin_fmaf(y, co, -1.f / 720);
     co = __builtin_fmaf(y, co, 1.f / 24);
@@ -73,40 +75,46 @@ __device__ __forceinline__ void cos_sin(int pos, float freq, double mul, double*
     unfold(r.n, co, si, mul, c, s);
 }
 
-// The 16 elements a thread rotates: two runs of 8 at a and b.  Halves: run b holds the
-// partners of run a, pair e of the unit is (a[e], b[e]), and pair 8 u + e of the head.  Pairs:
-// the 16 are in order, pair e is (2 e, 2 e + 1).  Units behind the rotated part are in order too.
+// The 2 W elements a thread rotates: runs of W at a and b.  Halves: run b holds the partners of
+// run a, pair e of the unit is (a[e], b[e]).  Pairs: each run holds W / 2 of them, (2 e, 2 e + 1), and
+// run b follows run a, or lies `apart` units of W on (so that a wave's loads are whole rows).  Units
+// behind the rotated part of halves are in order too.
+template <int W>
 struct Unit {
     int a, b;
-    __device__ __forceinline__ Unit(int u, int rot, bool half) {
-        const bool split = half && 16 * u < rot;
-        a = split ? 8 * u : 16 * u;
-        b = split ? 8 * u + rot / 2 : 16 * u + 8;
+    int pa, pb;  // pairs of the head: the unit's first, and its W/2th
+    __device__ __forceinline__ Unit(int u, int rot, bool half, int apart = 0) {
+        const bool split = half && 2 * W * u < rot;
+        a = split || (!half && apart) ? W * u : 2 * W * u;
+        b = split ? a + rot / 2 : !half && apart ? a + W * apart : a + W;
+        pa = half ? W * u : a / 2;
+        pb = half ? pa + W / 2 : b / 2;
     }
+    __device__ __forceinline__ int pair(int e) const { return e < W / 2 ? pa + e : pb + e - W / 2; }
 };
 
-template <typename F>
+template <typename F, int W>
 struct Angles {
-    F c[8], s[8];
-    __device__ __forceinline__ void set(int pos, const float* freq, int u, int rot, F mul) {
+    F c[W], s[W];
+    __device__ __forceinline__ void set(int pos, const float* freq, const Unit<W>& at, int rot, F mul) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < W; ++e) {
             c[e] = mul;
             s[e] = 0;
-            if (2 * (8 * u + e) < rot) cos_sin(pos, freq[8 * u + e], mul, &c[e], &s[e]);
+            if (2 * at.pair(e) < rot) cos_sin(pos, freq[at.pair(e)], mul, &c[e], &s[e]);
         }
     }
     // v: run a, then run b.  Elements behind the rotated part stay as they are.
-    __device__ __forceinline__ void turn(F (&v)[16], int u, int rot, bool half, F sign) const {
+    __device__ __forceinline__ void turn(F (&v)[2 * W], const Unit<W>& at, int rot, bool half, F sign) const {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if (2 * (8 * u + e) >= rot) continue;
+        for (int e = 0; e < W; ++e) {
+            if (2 * at.pair(e) >= rot) continue;
             const F si = s[e] * sign;
-            F x = half ? v[e] : v[2 * e], y = half ? v[8 + e] : v[2 * e + 1];
+            F x = half ? v[e] : v[2 * e], y = half ? v[W + e] : v[2 * e + 1];
             const F x1 = x * c[e] - y * si, y1 = y * c[e] + x * si;
             if (half) {
                 v[e] = x1;
-                v[8 + e] = y1;
+                v[W + e] = y1;
             } else {
                 v[2 * e] = x1;
                 v[2 * e + 1] = y1;

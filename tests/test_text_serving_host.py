@@ -106,7 +106,7 @@ def cache(**kw):
 
 def seqs(**kw):
     s = dh.KVSeqs()
-    put(s, table=ADDR, table_stride=4, table_pages=4, seq_start=ADDR, past=ADDR, seqs=3, rows=7)
+    put(s, table=ADDR, table_stride=100, table_pages=100, seq_start=ADDR, past=ADDR, seqs=3, rows=7)
     return put(s, **kw)
 
 
@@ -192,6 +192,9 @@ def test_workspace_goes_by_sizes():
     n = ask(cache(), seqs(), 4)
     assert n > 0 and n % 8 == 0
     assert ask(cache(pages=1 << 20), seqs(table_pages=1 << 15), 4) == n
+    assert ask(cache(), seqs(table_pages=10), 4) == 0  # short tables: nothing is shared out
+    # more rows than sequences: the row blocks' key ranges too, more of them for longer tables
+    assert 0 < ask(cache(), seqs(rows=100), 4) < ask(cache(), seqs(rows=100, table_pages=1000), 4)
 
 
 # ---------------------------------------------------------- wrappers' refusals --
@@ -273,7 +276,9 @@ int main() {
         const Seq q(s, b);
         PageItem it;
         if (!page_item(s, q, b, item, &it)) continue;
-        printf("%d %d %d %d %d %d\n", b, it.page, it.begin, it.first, it.last, q.row + it.begin - q.past);
+        const int page = page_of(s, b, it.begin);
+        if (page < 0) continue;
+        printf("%d %d %d %d %d %d\n", b, page, it.begin, it.first, it.last, q.row + it.begin - q.past);
     }
 }
 """
