@@ -816,6 +816,16 @@ def _meta(t):
     return None if t is None else (t.dtype, t.shape, t.stride(), t.get_device())
 
 
+def _metas(*ts):
+    """_meta of each, without a call for each."""
+    return [None if t is None else (t.dtype, t.shape, t.stride(), t.get_device()) for t in ts]
+
+
+def _like(t):
+    torch = _torch()
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _on_device(metas):
     """The launch goes to the current device's current stream: every tensor has to be there."""
     here = _torch().cuda.current_device()
@@ -1155,11 +1165,12 @@ def _rotary_plan(q, k, q_out, k_out, pos, freq, half, here):
 
 def _rotate(q, k, pos, rot, q_out, k_out, backward):
     if q is not None and q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out = _like(q)
     if k is not None and k_out is None:
-        k_out = k.new_empty(k.shape)
-    a = RotaryArgs.from_buffer_copy(_rotary_plan(_meta(q), _meta(k), None if q is None else _meta(q_out), None if k is None else _meta(k_out),
-                                                 _meta(pos), _meta(rot.freq), rot.half, _torch().cuda.current_device()))
+        k_out = _like(k)
+    plan = _rotary_plan(*_metas(q, k, None if q is None else q_out, None if k is None else k_out, pos, rot.freq), rot.half,
+                        _torch().cuda.current_device())
+    a = RotaryArgs.from_buffer_copy(plan)
     if q is not None:
         a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
     if k is not None:
@@ -1308,10 +1319,10 @@ def cache_append(cache, k, v, table, seq_start, past, rot=None, pos=None, q=None
     lies in page table[b, t // page] (int32 [seqs, pages]).  Positions are the places, or pos
     (int32 [rows]).  All of these are read on the device."""
     if q is not None and q_out is None:
-        q_out = q.new_empty(q.shape)
+        q_out = _like(q)
     freq = None if rot is None else rot.freq
-    plan = _append_plan(_meta(cache.k), _meta(cache.v), _meta(cache.k_scale), _meta(cache.v_scale), _meta(table), _meta(seq_start),
-                        _meta(past), _meta(k), _meta(v), _meta(q), None if q is None else _meta(q_out), _meta(pos), _meta(freq),
+    plan = _append_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, k, v, q,
+                                None if q is None else q_out, pos, freq),
                         None if rot is None else rot.half, _torch().cuda.current_device())
     c, s = _cache_pointers(plan[0], plan[1], cache, table, seq_start, past)
     a = KVAppendArgs.from_buffer_copy(plan[2])
@@ -1357,9 +1368,9 @@ def cache_attn(q, cache, table, seq_start, past, causal=True, scale=None, out=No
     seq_start and past as cache_append's (past: before the new tokens).  scale: >= 0, by default
     dim ** -0.5.  Rows of no sequence are left as they are."""
     if out is None:
-        out = q.new_empty(q.shape)
-    c, s, q_st, o_st, n = _cache_attn_plan(_meta(cache.k), _meta(cache.v), _meta(cache.k_scale), _meta(cache.v_scale), _meta(table),
-                                           _meta(seq_start), _meta(past), _meta(q), _meta(out), _torch().cuda.current_device())
+        out = _like(q)
+    c, s, q_st, o_st, n = _cache_attn_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, q, out),
+                                           _torch().cuda.current_device())
     c, s = _cache_pointers(c, s, cache, table, seq_start, past)
     ws = _scratch_by(q, n) if n else None
     lib = load()
