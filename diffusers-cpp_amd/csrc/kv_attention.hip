@@ -471,9 +471,10 @@ __global__ __launch_bounds__(512, 2) void kv_short_kernel(const Args a) {
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = (int)(blockIdx.x % (uint32_t)a.c.kv_heads);
     const int64_t item = blockIdx.x / (uint32_t)a.c.kv_heads;
-    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block<kRows>(a, start, i); });
+    const Found of = find_seq(a.s, item, [&a](int start, int i) { return first_block<kRows>(a, start, i); });
+    const int b = of.b;
     if (b < 0) return;
-    const Seq q(a.s, b);
+    const Seq q = of.seq(a.s);
     const int64_t blk = item - first_block<kRows>(a, q.row, b), rows = q.n * (int64_t)a.group;
     if (blk < 0 || blk * kRows >= rows || rows > a.few) return;
     const Mine sq = {b, q.row, q.n, q.past, q.len, 0};
@@ -530,9 +531,9 @@ __device__ __forceinline__ void join_ranges(const Args& a, int block) {
 #pragma unroll
     for (int k = 0; k < 64 / TPR; ++k) {
         const int r = min(__shfl((int)(id / a.heads), k * TPR, 64), a.s.rows - 1);
-        const int b = find_seq(a.s, r, [](int start, int) { return start; });
-        if (b < 0) continue;
-        const Seq sq(a.s, b);
+        const Found of = find_seq(a.s, r, [](int start, int) { return start; });
+        if (of.b < 0) continue;
+        const Seq sq = of.seq(a.s);
         if ((int)(threadIdx.x & 63) / TPR == k) mine = r - sq.row < sq.n && sq.n * (int64_t)a.group > a.few;
     }
     if (!mine || id >= n || d >= a.c.dim) return;
@@ -730,9 +731,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
     const uint32_t rest = bid / (uint32_t)a.c.kv_heads;
     const int split = (int)(rest % (uint32_t)a.splits);
     const int64_t item = (int64_t)n_items - 1 - rest / (uint32_t)a.splits;
-    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_block<kBlock>(a, start, i); });
+    const Found of = find_seq(a.s, item, [&a](int start, int i) { return first_block<kBlock>(a, start, i); });
+    const int b = of.b;
     if (b < 0) return;
-    const Seq sq(a.s, b);
+    const Seq sq = of.seq(a.s);
     const int64_t all_rows = sq.n * (int64_t)a.group, row0 = (item - first_block<kBlock>(a, sq.row, b)) * kBlock;
     if (all_rows <= a.few || row0 < 0 || row0 >= all_rows) return;
     const int rows = (int)all_rows, first = (int)row0, last = min(first + kBlock, rows) - 1;

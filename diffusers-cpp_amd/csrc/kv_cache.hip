@@ -29,8 +29,11 @@ struct Args {
     const float* freq;
     float mul;
     int32_t rot, half;
-    int32_t units, per_pass, slots;  // 16-element units a row; tokens a pass of 256 threads; heads side by side in a wave
+    int32_t units, per_pass;         // 16-element units a row; tokens a pass of a workgroup
     FastDiv unit_div;
+    int32_t q_units, slots;          // q: units of two vectors a row; heads side by side in a wave
+    FastDiv q_unit_div;
+    int32_t threads;                 // of a workgroup
     int32_t kv_blocks;               // workgroups before q's
     int32_t q_chunks;                // waves a row of q
     FastDiv head_div, chunk_div;
@@ -102,42 +105,22 @@ __device__ __forceinline__ void load8(const T* p, float* v) {
 
 template <typename T>
 __device__ void rotate_q(const Args& a) {
-    const uint32_t wave = (blockIdx.x - a.kv_blocks) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t wave = (blockIdx.x - a.kv_blocks) * (a.threads >> 6) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int row = (int)fdiv(wave, a.chunk_div), chunk = (int)(wave - (uint32_t)row * a.q_chunks);
     if (row >= a.s.rows) return;
-    const int b = find_seq(a.s, row, [](int start, int) { return start; });
-    if (b < 0) return;
-    const Seq q(a.s, b);
+    const Found of = find_seq(a.s, row, [](int start, int) { return start; });
+    if (of.b < 0) return;
+    const Seq q = of.seq(a.s);
     if (row - q.row >= q.n) return;
-    const int slot = (int)fdiv(lane, a.unit_div), u = (int)lane - slot * a.units;
+    const int slot = (int)fdiv(lane, a.q_unit_div), u = (int)lane - slot * a.q_units;
     if (slot >= a.slots) return;
     const int p = a.pos ? a.pos[row] : q.past + row - q.row;
-    const rotary::Unit<8> at(u, a.rot, a.half);
-    constexpr int ITER = 4;
-    const int first = chunk * ITER * a.slots + slot;
-    float v[ITER][16];
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        const int h = first + i * a.slots;
-        if (h >= a.heads) continue;
-        const T* x = reinterpret_cast<const T*>(a.q) + row * a.qs[0] + h * a.qs[1];
-        load8(x + at.a, v[i]);
-        load8(x + at.b, v[i] + 8);
-    }
-    rotary::Angles<float, 8> w;
-    w.set(p, a.freq, at, a.rot, a.mul);
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        const int h = first + i * a.slots;
-        if (h >= a.heads) continue;
-        w.turn(v[i], at, a.rot, a.half, 1.f);
-        T* y = reinterpret_cast<T*>(a.q_out) + row * a.os[0] + h * a.os[1];
-#pragma unroll
-        for (int n = 0; n < 8 / Io<T>::EPV; ++n) {
-            Io<T>::store(y + at.a + n * Io<T>::EPV, v[i] + n * Io<T>::EPV);
-            Io<T>::store(y + at.b + n * Io<T>::EPV, v[i] + 8 + n * Io<T>::EPV);
-        }
-    }
+    const int first = chunk * 4 * a.slots + slot;
+    rotary::turn_heads<T, 4>(
+        p, a.freq, u, a.q_units, a.rot, a.half, a.mul, 1.f,
+        [&](int i) { return first + i * a.slots < a.heads; },
+        [&](int i) { return reinterpret_cast<const T*>(a.q) + row * a.qs[0] + (first + i * a.slots) * a.qs[1]; },
+        [&](int i) { return reinterpret_cast<T*>(a.q_out) + row * a.os[0] + (first + i * a.slots) * a.os[1]; });
 }
 
 // The largest of the workgroup's `most`.
@@ -147,7 +130,9 @@ __device__ __forceinline__ float most_of_all(float most, float* of) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) of[threadIdx.x >> 6] = most;
     __syncthreads();
-    return fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3]));
+    most = of[0];
+    for (uint32_t w = 1; w < blockDim.x >> 6; ++w) most = fmaxf(most, of[w]);
+    return most;
 }
 
 template <typename E>
@@ -188,18 +173,22 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
         load8(x + at.a, v);
         load8(x + at.b, v + 8);
     };
-    auto exact = [&](int t, float (&v)[16]) {
-        load(t, v);
-        if (!turned) return;
-        rotary::Angles<double, 8> w;
-        w.set(place(t), a.freq, at, a.rot, (double)a.mul);
-        double d[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] = (double)v[e];
-        w.turn(d, at, a.rot, a.half, 1.0);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = to_odd(d[e]);
+    // Pair e of the unit in 64 bits, rounded to odd, and where its ends lie in the row.
+    auto exact = [&](int t, int e, float (&w)[2], int (&d)[2]) {
+        const T* x = src + (int64_t)(row0 + t) * a.ks[0];
+        d[0] = at.a + (a.half ? e : 2 * e);
+        d[1] = a.half ? at.b + e : d[0] + 1;
+        w[0] = Io<T>::get(x + d[0]);
+        w[1] = Io<T>::get(x + d[1]);
+        const int n = at.pair(e);
+        if (2 * n >= a.rot) return;
+        double c, s;
+        rotary::cos_sin(place(t), a.freq[n], (double)a.mul, &c, &s);
+        const double p = w[0], q = w[1];
+        w[0] = to_odd(p * c - q * s);
+        w[1] = to_odd(q * c + p * s);
     };
+    rotary::Angles<float, 8> w(a.freq, at, a.rot);
     float v[NP][16];
     Most most;
 #pragma unroll
@@ -213,9 +202,8 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
         const int t = first + i * a.per_pass + t0;
         if (!mine || t >= last) continue;
         if (turned) {
-            rotary::Angles<float, 8> w;
-            w.set(place(t), a.freq, at, a.rot, a.mul);
-            w.turn(v[i], at, a.rot, a.half, 1.f);
+            w.set(place(t), a.mul);
+            w.turn(v[i], a.half, 1.f);
         }
         if constexpr (F8) most.take(v[i]);
     }
@@ -231,9 +219,13 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
             Most again;
 #pragma unroll 1
             for (int t = first + t0; mine && t < last; t += a.per_pass) {
-                float x[16];
-                exact(t, x);
-                again.take_finite(x);
+#pragma unroll 1
+                for (int e = 0; e < 8; ++e) {
+                    float w[2];
+                    int d[2];
+                    exact(t, e, w, d);
+                    again.take_finite(w);
+                }
             }
             top = most_of_all(again.top, of);
 #pragma unroll
@@ -244,7 +236,7 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
         scale = page_scale(top, before, first > 0, &grown);
         if (tid == 0) *held = (uint8_t)scale;  // read by all before the barriers
         if (grown)
-            for (int i = tid; i < first * dim / 16; i += 256) {
+            for (int i = tid; i < first * dim / 16; i += a.threads) {
                 uint4 w = *reinterpret_cast<const uint4*>(out + 16 * i);
                 w.x = again(w.x, grown);
                 w.y = again(w.y, grown);
@@ -290,19 +282,14 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
                 const uint32_t w[4] = {differ[run].x, differ[run].y, differ[run].z, differ[run].w};
                 if (w[e / per] << (32 - 8 * (int)sizeof(E) * (e % per + 1)) >> (32 - 8 * (int)sizeof(E))) pairs |= 1u << (a.half ? e : 4 * run + e / 2);
             }
-        const T* x = src + (int64_t)(row0 + t) * a.ks[0];
 #pragma unroll 1
         for (; pairs; pairs &= pairs - 1) {
-            const int e = __builtin_ctz(pairs), n = 8 * u + e;  // pair of the head
-            if (2 * n >= a.rot) continue;
-            const int d0 = a.half ? n : 2 * n, d1 = a.half ? n + a.rot / 2 : 2 * n + 1;
-            double c, s;
-            rotary::cos_sin(place(t), a.freq[n], (double)a.mul, &c, &s);
-            const double p = Io<T>::get(x + d0), q = Io<T>::get(x + d1);
-            const float w[2] = {to_odd(p * c - q * s), to_odd(q * c + p * s)};
+            float w[2];
+            int d[2];
+            exact(t, __builtin_ctz(pairs), w, d);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                uint8_t* y = out + ((int64_t)t * dim + (k ? d1 : d0)) * sizeof(E);
+                uint8_t* y = out + ((int64_t)t * dim + d[k]) * sizeof(E);
                 if constexpr (F8) *y = (uint8_t)to_e4m3x4(tame(w[k]), 0.f, 0.f, 0.f, power(scale));
                 else Io<bf16>::put(reinterpret_cast<bf16*>(y), w[k]);
             }
@@ -388,7 +375,7 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
     __syncthreads();
     constexpr int PER = 16 / sizeof(E);  // tokens of a piece
     const int pieces = page / PER;       // of a row: a power of two
-    for (int i = tid; i < dim * pieces; i += 256) {
+    for (int i = tid; i < dim * pieces; i += a.threads) {
         const int d = i / pieces, c = (i & (pieces - 1)) * PER;
         if (c >= last || (c + PER <= first && !grown)) continue;
         uint8_t* y = out + ((int64_t)d * page + c) * sizeof(E);
@@ -413,9 +400,10 @@ __device__ __forceinline__ void append_v(const Args& a, const PageItem& it, int 
     }
 }
 
-// NP passes hold a page.  Registers for four workgroups a CU where two passes do (8750 tokens of 32 + 8 heads: 57 us, 64 with three).
+// NP passes hold a page.  Registers for five workgroups a CU where two passes do: 8750 tokens of 32 + 8 heads of 128
+// 53 us, 56 with four, 59 with six.
 template <typename T, typename E, int NP>
-__global__ __launch_bounds__(256, NP <= 2 ? 4 : 2) void kv_append_kernel(const Args a) {
+__global__ __launch_bounds__(256, NP <= 2 ? 5 : 2) void kv_append_kernel(const Args a) {
     extern __shared__ __attribute__((aligned(16))) uint32_t turned[];  // v: [dim][lds_row] words
     __shared__ float most_of[4];
     if ((int)blockIdx.x >= a.kv_blocks) {
@@ -424,14 +412,14 @@ __global__ __launch_bounds__(256, NP <= 2 ? 4 : 2) void kv_append_kernel(const A
     }
     // Workgroup: (number of a page, head, k or v), heads innermost: they share rows.
     const int item = (int)fdiv(blockIdx.x >> 1, a.head_div), h = (int)(blockIdx.x >> 1) - item * a.c.kv_heads;
-    const int b = find_seq(a.s, item, [&a](int start, int i) { return first_item(a.s, start, i); });
-    if (b < 0) return;
-    const Seq q(a.s, b);
+    const Found of = find_seq(a.s, item, [&a](int start, int i) { return first_item(a.s, start, i); });
+    if (of.b < 0) return;
+    const Seq q = of.seq(a.s);
     PageItem it;
-    if (!page_item(a.s, q, b, item, &it)) return;
+    if (!page_item(a.s, q, of.b, item, &it)) return;
     const int row0 = q.row + it.begin - q.past;  // of the page's token 0 (there may be none)
     // The page's number is looked at when the tokens are on their way.
-    const int page = a.s.table[b * a.s.table_stride + (it.begin >> a.s.page_log2)];
+    const int page = a.s.table[of.b * a.s.table_stride + (it.begin >> a.s.page_log2)];
     if (blockIdx.x & 1) append_v<T, E, NP>(a, it, row0, page, h, most_of, turned);
     else append_k<T, E, NP>(a, it, row0, page, h, most_of);
 }
@@ -439,10 +427,10 @@ __global__ __launch_bounds__(256, NP <= 2 ? 4 : 2) void kv_append_kernel(const A
 template <typename T, typename E>
 int launch(const Args& a, int passes, dim3 grid, hipStream_t st) {
     const size_t lds = (size_t)a.c.dim * a.lds_row * sizeof(uint32_t);
-    if (passes <= 1) hipLaunchKernelGGL((kv_append_kernel<T, E, 1>), grid, dim3(256), lds, st, a);
-    else if (passes <= 2) hipLaunchKernelGGL((kv_append_kernel<T, E, 2>), grid, dim3(256), lds, st, a);
-    else if (passes <= 4) hipLaunchKernelGGL((kv_append_kernel<T, E, 4>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((kv_append_kernel<T, E, 8>), grid, dim3(256), lds, st, a);
+    if (passes <= 1) hipLaunchKernelGGL((kv_append_kernel<T, E, 1>), grid, dim3(a.threads), lds, st, a);
+    else if (passes <= 2) hipLaunchKernelGGL((kv_append_kernel<T, E, 2>), grid, dim3(a.threads), lds, st, a);
+    else if (passes <= 4) hipLaunchKernelGGL((kv_append_kernel<T, E, 4>), grid, dim3(a.threads), lds, st, a);
+    else hipLaunchKernelGGL((kv_append_kernel<T, E, 8>), grid, dim3(a.threads), lds, st, a);
     return check_launch("dt_kv_append");
 }
 
@@ -539,12 +527,13 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
         if (rc) return rc;
     }
     a.mul = 1.f;
+    a.freq = reinterpret_cast<const float*>(a.s.seq_start);
     if (x->rotary) {
         rc = rotary::check_rotary(*x->rotary, a.c.dim, who);
         if (rc) return rc;
         DT_REQUIRE(!x->rotary->half || x->rotary->rot_dims % 16 == 0, "%s: halves of %lld dims unsupported (a multiple of 16)", who,
                    (long long)x->rotary->rot_dims);
-        a.freq = x->rotary->freq;
+        if (x->rotary->rot_dims) a.freq = x->rotary->freq;
         a.mul = x->rotary->attn_factor;
         a.rot = (int32_t)x->rotary->rot_dims;
         a.half = x->rotary->half != 0;
@@ -564,8 +553,9 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
     a.heads = (int32_t)x->heads;
     a.pos = x->pos;
     a.units = a.c.dim / 16;
-    a.per_pass = 256 / a.units;
-    a.slots = 64 / a.units;
+    a.q_units = a.c.dim * es / 32;
+    a.slots = 64 / a.q_units;
+    a.q_unit_div = make_fastdiv((uint32_t)a.q_units);
     a.unit_div = make_fastdiv((uint32_t)a.units);
     a.head_div = make_fastdiv((uint32_t)a.c.kv_heads);
     a.q_chunks = turn_q ? (a.heads + 4 * a.slots - 1) / (4 * a.slots) : 1;
@@ -574,10 +564,16 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
     const bool f8 = a.c.k_scale != nullptr;
     // An odd number of words: dims lie in other banks.
     a.lds_row = (int32_t)page * (f8 ? 1 : 2) / 4 + 1;
-    a.quads_per_pass = 256 / (a.c.dim / 4);
+    // Threads for a pass over a page, which takes up to 256: pages of 16 tokens leave the rest without work (3003 tokens
+    // of 12 heads of 80, bf16: 25.5 us with 256, 19.9 with 128).
+    const int most = (int)page * a.units;
+    a.threads = most >= 256 ? 256 : (most + 63) / 64 * 64;
+    a.per_pass = a.threads / a.units;
+    a.quads_per_pass = a.threads / (a.c.dim / 4);
     a.quad_div = make_fastdiv((uint32_t)(a.c.dim / 4));
     const int64_t kv_blocks = items(a.s) * a.c.kv_heads * 2;
-    const int64_t q_blocks = turn_q ? ((int64_t)a.s.rows * a.q_chunks + 3) / 4 : 0;
+    const int64_t waves = a.threads / 64;
+    const int64_t q_blocks = turn_q ? ((int64_t)a.s.rows * a.q_chunks + waves - 1) / waves : 0;
     DT_REQUIRE(kv_blocks + q_blocks < (1ll << 31) && (int64_t)a.s.rows * a.q_chunks < (1ll << 31), "%s: grid too large", who);
     a.kv_blocks = (int32_t)kv_blocks;
     const dim3 grid((unsigned)(kv_blocks + q_blocks));

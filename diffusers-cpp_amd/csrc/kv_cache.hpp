@@ -22,18 +22,28 @@ struct Cache {
     int64_t head_bytes;  // one page of one head: page * dim elements
 };
 
-// How many sequences b have key(seq_start[b], b) <= x, less one: with ascending keys, the one
-// that x belongs to.  By a whole wave.
+// The last of the sequences b with key(seq_start[b], b) <= x, or -1: with ascending keys, the one
+// that x belongs to.  Its description as well, from lanes that read all of it at once: a load's wait
+// less than to look the sequence up after it is known.  By a whole wave.
+struct Found {
+    int b = -1, start = 0, end = 0, past = 0;
+    __device__ __forceinline__ Seq seq(const Seqs& s) const { return Seq(s, start, end, past); }
+};
 template <typename Key>
-__device__ __forceinline__ int find_seq(const Seqs& s, int64_t x, Key key) {
+__device__ __forceinline__ Found find_seq(const Seqs& s, int64_t x, Key key) {
     const int lane = threadIdx.x & 63;
-    int n = 0;
+    Found f;
     for (int b0 = 0; b0 < s.seqs; b0 += 64) {
-        const int b = b0 + lane;
-        const bool in = b < s.seqs && key(start_of(s, min(b, s.seqs)), b) <= x;
-        n += __popcll(__builtin_amdgcn_ballot_w64(in));
+        const int b = min(b0 + lane, s.seqs - 1);
+        const int start = s.seq_start[b], end = s.seq_start[b + 1], past = s.past[b];
+        const int n = __popcll(__builtin_amdgcn_ballot_w64(b0 + lane < s.seqs && key(clamped(start, 0, s.rows), b) <= x));
+        if (n == 0) break;
+        f.b = b0 + n - 1;
+        f.start = __builtin_amdgcn_readlane(start, n - 1);
+        f.end = __builtin_amdgcn_readlane(end, n - 1);
+        f.past = __builtin_amdgcn_readlane(past, n - 1);
     }
-    return n - 1;
+    return f;
 }
 
 // ---- e4m3: four bits of significand, 2^-9 to 448, NaN but no infinity --------------------

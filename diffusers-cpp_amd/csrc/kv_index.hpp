@@ -32,11 +32,12 @@ DT_KV_FN int start_of(const Seqs& s, int b) { return clamped(s.seq_start[b], 0, 
 struct Seq {
     int row, n;     // first row, rows
     int past, len;  // tokens before, and with the rows (places past the table's end are none)
-    DT_KV_FN Seq(const Seqs& s, int b) {
-        row = start_of(s, b);
-        const int end = start_of(s, b + 1);
+    DT_KV_FN Seq(const Seqs& s, int b) : Seq(s, s.seq_start[b], s.seq_start[b + 1], s.past[b]) {}
+    DT_KV_FN Seq(const Seqs& s, int start, int end, int before) {
+        row = clamped(start, 0, s.rows);
+        end = clamped(end, 0, s.rows);
         n = end > row ? end - row : 0;
-        past = clamped(s.past[b], 0, 1 << 30);
+        past = clamped(before, 0, 1 << 30);
         const int64_t cap = (int64_t)s.table_pages << s.page_log2;
         len = past + n < cap ? past + n : (int)cap;
     }

@@ -36,7 +36,6 @@ struct Args {
 
 template <typename T, int ITER>
 __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
-    constexpr int EPV = Io<T>::EPV;
     const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t row = fdiv(wave, a.chunk_div), chunk = wave - row * a.chunks;
     if (row >= (uint64_t)a.rows) return;
@@ -45,41 +44,24 @@ __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
     if (slot >= (uint32_t)a.slots) return;
     const uint32_t b = fdiv(row, a.seq_div), tok = row - b * a.seq;
     const int p = a.pos[(int64_t)b * a.pos_stride + tok];
-    const Unit<EPV> at(u, a.rot, a.half, a.units);
     const int first = (int)(chunk * ITER * a.slots + slot);
 
-    uint4 raw[ITER][2];
-    int64_t to[ITER];
-    T* y[ITER];
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        int h = first + i * a.slots;
-        y[i] = nullptr;
-        if (h >= a.heads[0] + a.heads[1]) continue;
-        const bool k = h >= a.heads[0];
-        if (k) h -= a.heads[0];
-        const Tensor& t = a.t[0];
-        const Tensor& t1 = a.t[1];
-        const int64_t xb = k ? t1.xs[0] : t.xs[0], xt = k ? t1.xs[1] : t.xs[1], xh = k ? t1.xs[2] : t.xs[2];
-        const int64_t yb = k ? t1.ys[0] : t.ys[0], yt = k ? t1.ys[1] : t.ys[1], yh = k ? t1.ys[2] : t.ys[2];
-        const T* x = reinterpret_cast<const T*>(k ? t1.x : t.x) + b * xb + tok * xt + h * xh;
-        y[i] = reinterpret_cast<T*>(k ? t1.y : t.y);
-        to[i] = b * yb + tok * yt + h * yh;
-        raw[i][0] = ld_stream(x + at.a);
-        raw[i][1] = ld_stream(x + at.b);
-    }
-    Angles<float, EPV> w;
-    w.set(p, a.freq, at, a.rot, a.mul);
-#pragma unroll
-    for (int i = 0; i < ITER; ++i) {
-        if (!y[i]) continue;
-        float v[2 * EPV];
-        Io<T>::unpack(raw[i][0], v);
-        Io<T>::unpack(raw[i][1], v + EPV);
-        w.turn(v, at, a.rot, a.half, a.sign);
-        st_stream(y[i] + to[i] + at.a, Io<T>::pack(v));
-        st_stream(y[i] + to[i] + at.b, Io<T>::pack(v + EPV));
-    }
+    // By value: a stride picked by its address would be a load.
+    const Tensor q = a.t[0], k = a.t[1];
+    auto at = [&](int i, int64_t qb, int64_t qt, int64_t qh, int64_t kb, int64_t kt, int64_t kh) {
+        const int h = first + i * a.slots;
+        const int64_t in_q = b * qb + tok * qt + h * qh, in_k = b * kb + tok * kt + (h - a.heads[0]) * kh;
+        return h < a.heads[0] ? in_q : in_k;
+    };
+    auto is_q = [&](int i) { return first + i * a.slots < a.heads[0]; };
+    turn_heads<T, ITER>(
+        p, a.freq, u, a.units, a.rot, a.half, a.mul, a.sign, [&](int i) { return first + i * a.slots < a.heads[0] + a.heads[1]; },
+        [&](int i) {
+            return reinterpret_cast<const T*>(is_q(i) ? q.x : k.x) + at(i, q.xs[0], q.xs[1], q.xs[2], k.xs[0], k.xs[1], k.xs[2]);
+        },
+        [&](int i) {
+            return reinterpret_cast<T*>(is_q(i) ? q.y : k.y) + at(i, q.ys[0], q.ys[1], q.ys[2], k.ys[0], k.ys[1], k.ys[2]);
+        });
 }
 
 // Any width, part and alignment: a thread per pair, or per element behind the rotated part.
@@ -244,7 +226,7 @@ extern "C" int dt_rotary_apply(const dt_rotary_args* x, dt_stream_t stream) {
     a.seq_div = make_fastdiv((uint32_t)x->seq);
     a.pos = x->pos;
     a.pos_stride = x->pos_stride;
-    a.freq = x->rotary.freq;
+    a.freq = a.rot ? x->rotary.freq : reinterpret_cast<const float*>(x->pos);
     a.mul = x->rotary.attn_factor;
     a.sign = x->backward ? -1.f : 1.f;
     a.units = a.dim / unit;

@@ -93,35 +93,72 @@ struct Unit {
     __device__ __forceinline__ int pair(int e) const { return e < W / 2 ? pa + e : pb + e - W / 2; }
 };
 
+// Without branches: the frequencies are on their way together, and what is behind the rotated part
+// is selected, never computed (0 times an infinity).
 template <typename F, int W>
 struct Angles {
     F c[W], s[W];
-    __device__ __forceinline__ void set(int pos, const float* freq, const Unit<W>& at, int rot, F mul) {
+    float f[W];
+    bool on[W];
+    // Before the loads of what is rotated: results come in the order of the loads.  freq: a word that can
+    // be read, also where nothing is rotated.
+    __device__ __forceinline__ Angles(const float* freq, const Unit<W>& at, int rot) {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-            c[e] = mul;
-            s[e] = 0;
-            if (2 * at.pair(e) < rot) cos_sin(pos, freq[at.pair(e)], mul, &c[e], &s[e]);
+            on[e] = 2 * at.pair(e) < rot;
+            f[e] = freq[max(min(at.pair(e), rot / 2 - 1), 0)];
         }
     }
-    // v: run a, then run b.  Elements behind the rotated part stay as they are.
-    __device__ __forceinline__ void turn(F (&v)[2 * W], const Unit<W>& at, int rot, bool half, F sign) const {
+    __device__ __forceinline__ void set(int pos, F mul) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) cos_sin(pos, f[e], mul, &c[e], &s[e]);
+    }
+    template <bool HALF>
+    __device__ __forceinline__ void turn_as(F (&v)[2 * W], F sign) const {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-            if (2 * at.pair(e) >= rot) continue;
-            const F si = s[e] * sign;
-            F x = half ? v[e] : v[2 * e], y = half ? v[W + e] : v[2 * e + 1];
-            const F x1 = x * c[e] - y * si, y1 = y * c[e] + x * si;
-            if (half) {
-                v[e] = x1;
-                v[W + e] = y1;
-            } else {
-                v[2 * e] = x1;
-                v[2 * e + 1] = y1;
-            }
+            F &x = HALF ? v[e] : v[2 * e], &y = HALF ? v[W + e] : v[2 * e + 1];
+            const F si = s[e] * sign, x1 = x * c[e] - y * si, y1 = y * c[e] + x * si;
+            x = on[e] ? x1 : x;
+            y = on[e] ? y1 : y;
         }
+    }
+    // v: run a, then run b.
+    __device__ __forceinline__ void turn(F (&v)[2 * W], bool half, F sign) const {
+        if (half) turn_as<true>(v, sign);
+        else turn_as<false>(v, sign);
     }
 };
+
+// Unit u of up to ITER heads of one token, whose angles are worked out once: x(i) is where the i-th
+// head is read if has(i), y(i) where it is written.
+template <typename T, int ITER, typename H, typename X, typename Y>
+__device__ __forceinline__ void turn_heads(int pos, const float* freq, int u, int units, int rot, bool half, float mul, float sign, H has, X x,
+                                           Y y) {
+    constexpr int W = Io<T>::EPV;
+    const Unit<W> at(u, rot, half, units);
+    Angles<float, W> w(freq, at, rot);
+    uint4 raw[ITER][2];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        if (!has(i)) continue;
+        const T* p = x(i);
+        raw[i][0] = ld_stream(p + at.a);
+        raw[i][1] = ld_stream(p + at.b);
+    }
+    w.set(pos, mul);
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        if (!has(i)) continue;
+        T* p = y(i);
+        float v[2 * W];
+        Io<T>::unpack(raw[i][0], v);
+        Io<T>::unpack(raw[i][1], v + W);
+        w.turn(v, half, sign);
+        st_stream(p + at.a, Io<T>::pack(v));
+        st_stream(p + at.b, Io<T>::pack(v + W));
+    }
+}
 
 }  // namespace rotary
 }  // namespace dit
