@@ -561,6 +561,88 @@ def test_attention_far_into_a_large_pool():
     assert ((got.to(F64) - want).abs() <= tol).all()
 
 
+BLOCKS = [  # heads, key heads, dim, page, (new tokens, past) of each sequence
+    (4, 2, 128, 64, [(300, 3900)]),  # one long sequence: its keys in ranges
+    (3, 3, 80, 128, [(70, 4200)]),
+    (16, 16, 64, 64, [(2100, 2000)]),  # rows enough without
+    (64, 8, 128, 64, [(1900, 2200), (1, 4096), (150, 3), (0, 9)]),
+    (8, 2, 128, 64, [(100, 2500), (1, 3000), (40, 0), (1, 5), (0, 70)]),  # few rows beside many, keys in ranges
+    (6, 1, 64, 256, [(3, 2100), (90, 1000), (1, 0)]),
+    (4, 1, 112, 32, [(70, 2000)]),  # small pages
+    (8, 4, 48, 16, [(150, 1200), (2, 900), (1, 3)]),
+    (2, 1, 64, 64, [(1, 7 * b) for b in range(70)] + [(0, 3), (65, 64), (17, 1)]),  # more sequences than lanes
+]
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS)
+def test_attention_of_many_rows(dtype, heads, kv_heads, dim, page, seqs):
+    new, past = zip(*seqs)
+    pool = filled(770, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
+    q = rand(771, (sum(new) + 3, heads, dim))
+    for causal in (True, False):
+        out = dh.cache_attn(q, pool.cache, pool.table, starts(new, 2), ints(*past), causal=causal, out=torch.full_like(q, 7.0))
+        assert (out[:2] == 7.0).all() and (out[2 + sum(new):] == 7.0).all()
+        check_attention(pool, q, new, past, out, causal, front=2)
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("page,new,past", [(64, (1, 1), (50, 200)), (64, (40, 3), (30, 64)), (128, (130, 1), (0, 9)), (64, (300,), (3900,)),
+                                           (256, (150, 1), (2000, 2500))])
+def test_attention_of_later_tokens_in_wide_pages(dtype, page, new, past):
+    """NaN, and with bf16 an infinity, in the last token of a sequence: for its last row alone."""
+    lens = [n + p for n, p in zip(new, past)]
+    clean, pool = filled(780, lens, 2, 128, page, dtype), filled(780, lens, 2, 128, page, dtype)
+    q = rand(781, (sum(new), 4, 128))
+    args = pool.table, starts(new), ints(*past)
+    base = dh.cache_attn(q, clean.cache, *args)
+    t, last = lens[0] - 1, new[0] - 1
+    p, off = pool.rows[0][t // page], t % page
+    for x in [math.nan] + [math.inf] * (dtype == BF16):
+        pool.cache.v[p, 1, 77, off] = x
+        want = base.clone()
+        want[last, 2:, 77] = x
+        same(dh.cache_attn(q, pool.cache, *args), want, f"v {x}")
+        pool.cache.v[p] = clean.cache.v[p]
+    pool.cache.k[p, 0, off, 99] = math.nan
+    want = base.clone()
+    want[last, :2] = math.nan
+    same(dh.cache_attn(q, pool.cache, *args), want, "k")
+
+
+def test_append_to_more_sequences_than_lanes():
+    new, past = zip(*[(b % 3, 5 * b % 40) for b in range(150)])
+    pool = Pool(790, [n + p for n, p in zip(new, past)], 2, 32, 16, BF16)
+    k, v, q = rand(791, (sum(new), 2, 32)), rand(792, (sum(new), 2, 32)), rand(793, (sum(new), 4, 32))
+    r = dh.Rotary(dh.rotary_freqs(32), half=True)
+    place = torch.cat([torch.arange(p, p + n, dtype=torch.int32) for n, p in zip(new, past)]).cuda()
+    out = dh.cache_append(pool.cache, k, v, pool.table, starts(new), ints(*past), rot=r, q=q)
+    check_turned(out, q, place, r.freq, True)
+    want = turned(k, place, r.freq, True)
+    for b, (n, p) in enumerate(zip(new, past)):
+        a = sum(new[:b])
+        got_k, got_v = (x[p:] for x in pool.held(b, n + p))
+        same(got_k, round_bf16(want[a:a + n]), f"k of {b}")
+        same(got_v, v[a:a + n].to(F64), f"v of {b}")
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams' calls on one cache, each with scratch of its own, hold what they do one after the other."""
+    jobs = []
+    for i, (new, past) in enumerate([((1, 1, 1), (3000, 50, 900)), ((100, 1, 40), (2500, 3000, 0))]):
+        pool = filled(800 + i, [n + p for n, p in zip(new, past)], 2, 128, 64, F8)
+        jobs.append((rand(810 + i, (sum(new), 8, 128)), pool, starts(new), ints(*past)))
+    want = [dh.cache_attn(q, p.cache, p.table, s, n) for q, p, s, n in jobs]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream() for _ in jobs], [[], []]
+    for _ in range(5):
+        for i, (q, p, s, n) in enumerate(jobs):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(dh.cache_attn(q, p.cache, p.table, s, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
+
+
 # ----------------------------------------------------------------- together --
 class Layer:
     """One layer of a text model on the operators: its projections' rows in, attention out."""
