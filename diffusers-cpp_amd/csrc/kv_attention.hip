@@ -1082,11 +1082,14 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     if (p.rows) {
         // Blocks of 256 rows, one workgroup a CU, where keys are many and so are blocks, or a single
         // sequence's keys are shared out anyway (32 heads on 8 x 128: 4096 tokens 149 us against 159 in blocks
-        // of 128; 512 behind 30000 245 and 262).  Else, with pages of whole tiles, 128 rows and two workgroups
-        // a CU, of which one starts while the other works, and fewer rows are filled up (2048 tokens 62 us
-        // against 70; 8 x 1024 78 and 87; 4 x 300 behind 5000 101 and 127).
+        // of 128; 512 behind 30000 245 and 262).  Else 128 rows and two workgroups a CU, of which one starts
+        // while the other works, and fewer rows are filled up (2048 tokens 62 us against 70; 8 x 1024 78 and 87;
+        // 4 x 300 behind 5000 101 and 127), but for codes in pages of less than a tile, whose 128 rows lack the
+        // registers (17 requests, two of them with 512 new tokens, behind 3500, pages of 16: 112 us against 99;
+        // in bf16 116 against 125, two requests alone 94 against 89).
         const int64_t keys = (int64_t)s.table_pages << s.page_log2;
-        p.block = 1 << c.page_log2 < kTile || (keys >= 4096 && (rows * c.kv_heads >= 512 * (int64_t)cus || s.seqs == 1)) ? 256 : 128;
+        const bool many = keys >= 4096 && (rows * c.kv_heads >= 512 * (int64_t)cus || s.seqs == 1);
+        p.block = many || (c.k_scale && 1 << c.page_log2 < kTile) ? 256 : 128;
         p.blocks = rows / p.block + s.seqs;
         const int64_t full = ((rows + p.block - 1) / p.block) * c.kv_heads;
         // Twice as many beside a stream, whose workgroups end at their own time (17 requests, two of them with
@@ -1116,9 +1119,14 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
         a.stream_blocks = p.stream ? a.c.kv_heads * a.waves / (p.block / 32) : 0;
         const dim3 grid((unsigned)(a.stream_blocks + p.blocks * p.splits * a.c.kv_heads)), block(2 * p.block);
         const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
-        if (!wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 8>), grid, block, lds, st, a);
-        else if (p.block == 256) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
-        else hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 4>), grid, block, lds, st, a);
+        if (p.block == 256) {
+            if (wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
+            else hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 8>), grid, block, lds, st, a);
+        } else if (wide) {
+            hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 4>), grid, block, lds, st, a);
+        } else if constexpr (sizeof(E) == 2) {
+            hipLaunchKernelGGL((kv_rows_kernel<E, DP, false, 4>), grid, block, lds, st, a);
+        }
     } else {
         const dim3 grid((unsigned)(a.c.kv_heads * (a.waves / 4)));
         if (wide) hipLaunchKernelGGL((kv_stream_kernel<E, DP, true>), grid, dim3(256), 0, st, a);

@@ -569,6 +569,7 @@ BLOCKS = [  # heads, key heads, dim, page, (new tokens, past) of each sequence
     (8, 2, 128, 64, [(100, 2500), (1, 3000), (40, 0), (1, 5), (0, 70)]),  # few rows beside many, keys in ranges
     (6, 1, 64, 256, [(3, 2100), (90, 1000), (1, 0)]),
     (4, 1, 112, 32, [(70, 2000)]),  # small pages
+    (6, 2, 128, 16, [(90, 4100)]),
     (8, 4, 48, 16, [(150, 1200), (2, 900), (1, 3)]),
     (2, 1, 64, 64, [(1, 7 * b) for b in range(70)] + [(0, 3), (65, 64), (17, 1)]),  # more sequences than lanes
 ]
@@ -588,8 +589,8 @@ def test_attention_of_many_rows(dtype, heads, kv_heads, dim, page, seqs):
 
 @pytest.mark.parametrize("dtype", [F8, BF16])
 @pytest.mark.parametrize("page,new,past", [(64, (1, 1), (50, 200)), (64, (40, 3), (30, 64)), (128, (130, 1), (0, 9)), (64, (300,), (3900,)),
-                                           (256, (150, 1), (2000, 2500))])
-def test_attention_of_later_tokens_in_wide_pages(dtype, page, new, past):
+                                           (256, (150, 1), (2000, 2500)), (32, (150,), (4000,))])
+def test_attention_of_later_tokens_in_pages_of_any_width(dtype, page, new, past):
     """NaN, and with bf16 an infinity, in the last token of a sequence: for its last row alone."""
     lens = [n + p for n, p in zip(new, past)]
     clean, pool = filled(780, lens, 2, 128, page, dtype), filled(780, lens, 2, 128, page, dtype)
