@@ -514,7 +514,9 @@ __global__ __launch_bounds__(512, 2) void kv_short_kernel(const Args a) {
         const int row = (int)blk * kRows + r, tok = (int)fdiv((uint32_t)row, a.group_div);
         attn::put4(reinterpret_cast<bf16*>(a.o) + (int64_t)(sq.row + tok) * a.os[0] + (h * a.group + row - tok * a.group) * a.os[1] + d, v);
     }
-    if (!__syncthreads_or(st.wild) || wave != 0 || !st.live) return;
+    if (!__syncthreads_or(st.wild)) return;
+    __syncthreads();  // the results that other waves stored are read
+    if (wave != 0 || !st.live) return;
 #pragma unroll 1
     for (int d = 4 * g; d < a.c.dim; d += 16)
         add_wild<E>(a, b, h, st.all / St::STEP * St::STEP, min(tiles * St::STEP, st.limit), d, st.out(a, sq), nullptr);

@@ -649,8 +649,8 @@ typedef struct dt_kv_seqs {
  * a page's scale grows, its earlier codes are rounded again to the new one (which moves
  * them only below 2^-6 of it).  A page that is begun anew (its first token is
  * stored) forgets what it held.  A page that is written belongs to one sequence of
- * the call.  k, v, q: io_type BF16 or F32, rows 16-byte aligned.  k is
- * rotated in 64 bits and rounded once. */
+ * the call.  k, v, q: io_type BF16 or F32, rows 16-byte aligned.  k is stored
+ * as its rotation in 64 bits rounded once; q as dt_rotary_apply has it. */
 typedef struct dt_kv_append_args {
     const void *k, *v, *q;
     void *q_out;
@@ -669,7 +669,8 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
  * Operands bf16 (e4m3 codes times their scale are exact in it), the softmax's weights
- * rounded to bf16 after their sum is taken, sums in fp32.  o: bf16; it must not overlap
+ * rounded to bf16 for the product (their sum takes them before, or, with many rows a
+ * sequence, as the product does), sums in fp32.  o: bf16; it must not overlap
  * an input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
  * aligned) is needed (0 for some calls); its size goes by the sizes given here, not by the
  * lengths on the device.  No atomics: the same call gives the same bits. */
