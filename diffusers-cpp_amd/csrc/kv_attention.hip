@@ -32,7 +32,7 @@ typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;      // rows of a block of the stream's
-constexpr int kShort = 2048;   // places of a table up to which the stream's blocks of rows are not shared out
+constexpr int kShort = 1 << 18;  // bytes of a key head's keys up to which the stream's blocks of rows are not shared out
 constexpr int kFew = 32;       // beside the row blocks' kernel the stream takes sequences of up to so many rows
 
 struct Args {
@@ -1072,7 +1072,12 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     p.stream = !p.rows || s.seqs > 1;
     p.few = !p.rows ? INT32_MAX : p.stream ? kFew : 0;
     p.splits = 1;
-    p.whole = !p.rows && ((int64_t)s.table_pages << s.page_log2) <= kShort;
+    // A workgroup's time goes by its own bytes, the stream's by all of them, with 5 to 8 us for its second launch
+    // (32 on 8 heads of 128, whole and shared out: bf16, one token to 800 14 and 17.5 us, 8 to 1500 27 and 20; e4m3, 16
+    // to 1500 17 and 21).  Blocks enough for every CU may be twice as long (e4m3, 32 tokens to 2300 23 and 30, 64
+    // to 3700 54 and 64; but 24 to 3900 of 16 heads of 64 in bf16 53 and 48).
+    const int64_t bytes = ((int64_t)s.table_pages << s.page_log2) * p.dp * (c.k_scale ? 1 : 2), blocks = (rows / kRows + s.seqs) * c.kv_heads;
+    p.whole = !p.rows && bytes <= (blocks >= cus ? 2 : 1) * (int64_t)kShort;
     if (p.stream && !p.whole) {
         // Two waves a SIMD in all.  Beside blocks of rows a quarter of that, and so of the CUs at most: the
         // stream is as fast as memory, and over before the products are (the same step with all of

@@ -572,12 +572,15 @@ BLOCKS = [  # heads, key heads, dim, page, (new tokens, past) of each sequence
     (6, 2, 128, 16, [(90, 4100)]),
     (8, 4, 48, 16, [(150, 1200), (2, 900), (1, 3)]),
     (2, 1, 64, 64, [(1, 7 * b) for b in range(70)] + [(0, 3), (65, 64), (17, 1)]),  # more sequences than lanes
+    (8, 2, 128, 64, [(1, 6000), (1, 0), (1, 4099)]),  # few rows, shared out
+    (32, 32, 128, 64, [(1, 3000 - 70 * b) for b in range(40)]),  # few rows and blocks for every CU
+    (64, 64, 64, 64, [(1, 6000 - 900 * b) for b in range(5)]),
 ]
 
 
 @pytest.mark.parametrize("dtype", [F8, BF16])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS)
-def test_attention_of_many_rows(dtype, heads, kv_heads, dim, page, seqs):
+def test_attention_of_many_rows_or_long_ones(dtype, heads, kv_heads, dim, page, seqs):
     new, past = zip(*seqs)
     pool = filled(770, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
     q = rand(771, (sum(new) + 3, heads, dim))

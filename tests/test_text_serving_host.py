@@ -106,7 +106,7 @@ def cache(**kw):
 
 def seqs(**kw):
     s = dh.KVSeqs()
-    put(s, table=ADDR, table_stride=100, table_pages=100, seq_start=ADDR, past=ADDR, seqs=3, rows=7)
+    put(s, table=ADDR, table_stride=400, table_pages=400, seq_start=ADDR, past=ADDR, seqs=3, rows=7)
     return put(s, **kw)
 
 
