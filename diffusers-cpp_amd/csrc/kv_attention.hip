@@ -33,7 +33,9 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kRows = 16;      // rows of a block of the stream's
 constexpr int kShort = 1 << 18;  // bytes of a key head's keys up to which the stream's blocks of rows are not shared out
-constexpr int kFew = 32;       // beside the row blocks' kernel the stream takes sequences of up to so many rows
+// Beside the row blocks' kernel the stream takes sequences of up to so many rows (20 sequences of 48 rows behind 4000, 32 on
+// 8 heads of 128: 56 us, with 64 88; 9 of 24 rows: 35, with 16 32, but of 48 rows 36).
+constexpr int kFew = 32;
 
 struct Args {
     Cache c;
@@ -1102,7 +1104,8 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
         // Twice as many beside a stream, whose workgroups end at their own time (17 requests, two of them with
         // 512 new tokens, behind 3500: 143 -> 124 us).
         int64_t n = (p.block == 128 ? 2 : 1) * (p.stream ? 2 : 1) * cus / (full > 0 ? full : 1);
-        const int64_t longest = keys / (8 * kTile);  // eight tiles a range
+        // Eight tiles a range (64 tokens behind 1000: 25.5 us, 22 with four, 32 with sixteen; 200: 30, 31, 34).
+        const int64_t longest = keys / (8 * kTile);
         if (n > longest) n = longest;
         if (n > 32) n = 32;
         p.splits = n < 2 ? 1 : (int)n;
@@ -1140,7 +1143,8 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
         else hipLaunchKernelGGL((kv_stream_kernel<E, DP, false>), grid, dim3(256), 0, st, a);
     }
     const int rc = check_launch("dt_kv_attn");
-    // Shares of the stream: few rows may each have many, then a workgroup a row.  Key ranges: four elements a thread.
+    // Shares of the stream: few rows may each have many, then a workgroup a row (24 tokens to 4000, 768 rows: 34 us, in
+    // fours 36; 4096 rows 129 and 122).  Key ranges: four elements a thread.
     const int64_t joined = !p.stream ? 0 : p.rows ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
     const int64_t ranges = p.splits > 1 ? (n * (DP / 4) + 255) / 256 : 0;
     if (rc || joined + ranges == 0) return rc;
