@@ -314,6 +314,12 @@ def stream():
     return c_void_p(raw(torch.cuda.current_device()))
 
 
+def _stream_of(device):
+    """stream() where the current device is known, as a plain number."""
+    raw = getattr(_torch()._C, "_cuda_getCurrentRawStream", None)
+    return stream() if raw is None else raw(device)
+
+
 def desc(t, op=OP_NONE) -> DtTensor:
     """ggml-ordered descriptor of a torch tensor (at most 4-D)."""
     if t.dim() > 4:
@@ -826,6 +832,15 @@ def _like(t):
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _like_meta(m):
+    """_meta of what _like makes."""
+    strides, step = [], 1
+    for n in reversed(m[1]):
+        strides.append(step)
+        step *= max(n, 1)
+    return m[0], m[1], tuple(reversed(strides)), m[3]
+
+
 def _on_device(metas):
     """The launch goes to the current device's current stream: every tensor has to be there."""
     here = _torch().cuda.current_device()
@@ -1132,7 +1147,9 @@ def _four(m):
 
 @functools.lru_cache(maxsize=512)
 def _rotary_plan(q, k, q_out, k_out, pos, freq, half, here):
+    """q_out, k_out None: _like q and k."""
     torch = _torch()
+    q_out, k_out = q_out or q and _like_meta(q), k_out or k and _like_meta(k)
     a = RotaryArgs()
     first = q if q is not None else k
     if first is None:
@@ -1164,12 +1181,12 @@ def _rotary_plan(q, k, q_out, k_out, pos, freq, half, here):
 
 
 def _rotate(q, k, pos, rot, q_out, k_out, backward):
+    here = _torch().cuda.current_device()
+    plan = _rotary_plan(*_metas(q, k, None if q is None else q_out, None if k is None else k_out, pos, rot.freq), rot.half, here)
     if q is not None and q_out is None:
         q_out = _like(q)
     if k is not None and k_out is None:
         k_out = _like(k)
-    plan = _rotary_plan(*_metas(q, k, None if q is None else q_out, None if k is None else k_out, pos, rot.freq), rot.half,
-                        _torch().cuda.current_device())
     a = RotaryArgs.from_buffer_copy(plan)
     if q is not None:
         a.q, a.q_out = q.data_ptr(), q_out.data_ptr()
@@ -1177,7 +1194,7 @@ def _rotate(q, k, pos, rot, q_out, k_out, backward):
         a.k, a.k_out = k.data_ptr(), k_out.data_ptr()
     a.pos, a.rotary.freq, a.rotary.attn_factor, a.backward = pos.data_ptr(), rot.freq.data_ptr(), rot.attn_factor, backward
     lib = load()
-    check(lib.dt_rotary_apply(ctypes.addressof(a), stream()), "dt_rotary_apply")
+    check(lib.dt_rotary_apply(ctypes.addressof(a), _stream_of(here)), "dt_rotary_apply")
     if isinstance(lib, _Recorder):
         lib.keep.append(a)
     return q_out, k_out
@@ -1275,7 +1292,9 @@ def _cache_plan(k, v, k_scale, v_scale, table, seq_start, past, rows):
 
 @functools.lru_cache(maxsize=512)
 def _append_plan(ck, cv, k_scale, v_scale, table, seq_start, past, k, v, q, q_out, pos, freq, half, here):
+    """q_out None: _like q."""
     torch = _torch()
+    q_out = q_out or q and _like_meta(q)
     if len(k[1]) != 3 or v[1] != k[1] or k[1][1:] != (ck[1][1], ck[1][3]):
         raise DtError(f"k {tuple(k[1])} and v {tuple(v[1])} must be [rows, kv_heads, dim] of the cache {tuple(ck[1])}")
     if k[0] not in (torch.bfloat16, torch.float32) or v[0] != k[0] or k[2][2] != 1 or v[2][2] != 1:
@@ -1318,12 +1337,11 @@ def cache_append(cache, k, v, table, seq_start, past, rot=None, pos=None, q=None
     (int32 [seqs + 1]) are sequence b's tokens from place past[b] (int32 [seqs]) on; place t
     lies in page table[b, t // page] (int32 [seqs, pages]).  Positions are the places, or pos
     (int32 [rows]).  All of these are read on the device."""
+    freq, here = None if rot is None else rot.freq, _torch().cuda.current_device()
+    plan = _append_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, k, v, q,
+                                None if q is None else q_out, pos, freq), None if rot is None else rot.half, here)
     if q is not None and q_out is None:
         q_out = _like(q)
-    freq = None if rot is None else rot.freq
-    plan = _append_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, k, v, q,
-                                None if q is None else q_out, pos, freq),
-                        None if rot is None else rot.half, _torch().cuda.current_device())
     c, s = _cache_pointers(plan[0], plan[1], cache, table, seq_start, past)
     a = KVAppendArgs.from_buffer_copy(plan[2])
     a.k, a.v = k.data_ptr(), v.data_ptr()
@@ -1337,7 +1355,7 @@ def cache_append(cache, k, v, table, seq_start, past, rot=None, pos=None, q=None
         r.freq, r.attn_factor = freq.data_ptr(), rot.attn_factor
         a.rotary = ctypes.addressof(r)
     lib = load()
-    check(lib.dt_kv_append(ctypes.addressof(c), ctypes.addressof(s), ctypes.addressof(a), stream()), "dt_kv_append")
+    check(lib.dt_kv_append(ctypes.addressof(c), ctypes.addressof(s), ctypes.addressof(a), _stream_of(here)), "dt_kv_append")
     if isinstance(lib, _Recorder):
         lib.keep.extend((c, s, a, r))
     return q_out if q is not None else None
@@ -1345,7 +1363,9 @@ def cache_append(cache, k, v, table, seq_start, past, rot=None, pos=None, q=None
 
 @functools.lru_cache(maxsize=512)
 def _cache_attn_plan(ck, cv, k_scale, v_scale, table, seq_start, past, q, out, here):
+    """out None: _like q."""
     torch = _torch()
+    out = out or _like_meta(q)
     if len(q[1]) != 3 or q[1][2] != ck[1][3] or q[0] != torch.bfloat16 or q[2][2] != 1:
         raise DtError("q must be bf16 [rows, heads, dim] of the cache's width, the head dim contiguous")
     if out[1] != q[1] or out[0] != q[0] or out[2][2] != 1:
@@ -1367,16 +1387,16 @@ def cache_attn(q, cache, table, seq_start, past, causal=True, scale=None, out=No
     the tokens up to each row's own (causal) or over all -> bf16 [rows, heads, dim].  table,
     seq_start and past as cache_append's (past: before the new tokens).  scale: >= 0, by default
     dim ** -0.5.  Rows of no sequence are left as they are."""
+    here = _torch().cuda.current_device()
+    c, s, q_st, o_st, n = _cache_attn_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, q, out), here)
     if out is None:
         out = _like(q)
-    c, s, q_st, o_st, n = _cache_attn_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, q, out),
-                                           _torch().cuda.current_device())
     c, s = _cache_pointers(c, s, cache, table, seq_start, past)
     ws = _scratch_by(q, n) if n else None
     lib = load()
     check(lib.dt_kv_attn(ctypes.addressof(c), ctypes.addressof(s), q.data_ptr(), q_st, q.shape[1], 1 if causal else 0,
                          c.head_dim ** -0.5 if scale is None else scale, out.data_ptr(), o_st, None if ws is None else ws.data_ptr(),
-                         n, stream()), "dt_kv_attn")
+                         n, _stream_of(here)), "dt_kv_attn")
     if isinstance(lib, _Recorder):
         lib.keep.extend((c, s))
     return out
