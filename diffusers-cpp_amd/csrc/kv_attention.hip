@@ -251,7 +251,7 @@ struct Stream {
         const int32_t* table = a.s.table + sq.b * a.s.table_stride;
         const int table_last = a.s.table_pages - 1;
         const int kin = KPL * (col >> 2), vin = KPL * g;  // first key of this lane's operand row's piece of four, of its scores and values
-        int kpage, vpage;
+        int kpage, vpage = 0;
         auto find_pages = [&](int t) {
             kpage = table[max(min((t * STEP + (WIDE ? 0 : kin)) >> lg, table_last), 0)];
             if constexpr (!WIDE) vpage = table[max(min((t * STEP + vin) >> lg, table_last), 0)];
@@ -294,6 +294,11 @@ struct Stream {
         };
         if (t0 >= t1 || sq.len == 0) return;  // without a place there may be no table
         find_pages(t0);
+        const int kpage0 = kpage, vpage0 = vpage;
+        find_pages(t0 + by);
+        const int kpage1 = kpage, vpage1 = vpage;
+        kpage = kpage0;
+        vpage = vpage0;
         // Queries first: the keys' loads wait for the pages anyway.
         bf16x8_t qf[KC][M];
         const uint16_t* qp = a.q + (int64_t)(sq.row + tok) * a.qs[0] + head * a.qs[1];
@@ -308,7 +313,8 @@ struct Stream {
             }
         load_k(t0);
         load_v(t0);
-        find_pages(t0 + by);
+        kpage = kpage1;
+        vpage = vpage1;
         for (int t = t0; t < t1; t += by) {
             const bool here = paged;
             const float ks = ES == 1 ? __uint_as_float(max(kscale, 1u) << 23) : 1.f;
@@ -401,8 +407,10 @@ struct Stream {
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Held<E>::part(vr[d], vs, mm), pf[mm], o[d], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
             if (more) {
-                load_v(t + by);
+                // Pages first: results come in the order of the loads, and the next keys' loads wait for them.
                 find_pages(t + 2 * by);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(t + by);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
