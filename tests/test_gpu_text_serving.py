@@ -372,6 +372,32 @@ def test_append_in_views_and_q_onto_itself():
         same(x, y, "pages")
 
 
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("half", [True, False])
+def test_append_with_nothing_to_rotate(dtype, half):
+    """A rotation of no dims: k as it is, q copied."""
+    a, b = Pool(8, [40, 3], 2, 48, 16, dtype), Pool(8, [40, 3], 2, 48, 16, dtype)
+    k, v, q = rand(84, (30, 2, 48)), rand(85, (30, 2, 48)), rand(86, (30, 4, 48))
+    args = ints(0, 28, 30), ints(10, 0)
+    dh.cache_append(a.cache, k, v, a.table, *args)
+    out = dh.cache_append(b.cache, k, v, b.table, *args, rot=dh.Rotary(torch.zeros(0, device="cuda"), half=half, attn_factor=3.0), q=q)
+    assert torch.equal(out, q)
+    for s, n in ((0, 38), (1, 2)):
+        for x, y in zip(a.held(s, n), b.held(s, n)):
+            same(x[10 if s == 0 else 0:], y[10 if s == 0 else 0:], "pages")
+
+
+def test_append_of_keys_that_share_rows():
+    """k and v one tensor, one head's rows standing for all (stride 0): sources may repeat."""
+    pool, flat = Pool(9, [20], 3, 32, 16, F8), Pool(9, [20], 3, 32, 16, F8)
+    x = rand(87, (20, 1, 32)).expand(20, 3, 32)
+    r = dh.Rotary(dh.rotary_freqs(32), half=True)
+    dh.cache_append(pool.cache, x, x, pool.table, ints(0, 20), ints(0), rot=r)
+    dh.cache_append(flat.cache, x.contiguous(), x.contiguous(), flat.table, ints(0, 20), ints(0), rot=r)
+    for x, y in zip(pool.held(0, 20), flat.held(0, 20)):
+        same(x, y, "pages")
+
+
 # ---------------------------------------------------------------- attention --
 def attended(q, k, v, past, causal, scale):
     """o [n, H, D] in 64 bits and its tolerance: q [n, H, D], k and v [held, KH, D]."""
