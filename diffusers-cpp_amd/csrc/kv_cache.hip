@@ -252,11 +252,18 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
         // A rotation keeps a pair's length l: |x| + |y| <= sqrt(2) l <= sqrt(2) (|x'| + |y'|).  Cosine and sine are off by
         // 2^-23 and the factor's rounding, products and sum add two roundings: below 5 2^-24 (|x| + |y|) in all,
         // 1.8 2^-22 (|x'| + |y'|).
-        float tol[8];
+        float tol[8], all = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float x = a.half ? v[i][e] : v[i][2 * e], y = a.half ? v[i][8 + e] : v[i][2 * e + 1];
             tol[e] = 2 * (8 * u + e) < a.rot ? (fabsf(x) + fabsf(y)) * 0x1p-21f : 0.f;
+            all += tol[e];
+        }
+        // A pair with an end that 32 bits could not hold (the 64 may, and its other end is held like any).
+        uint32_t pairs = 0;
+        if (!finite(all)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pairs |= finite(tol[e]) ? 0u : 1u << e;
         }
         uint4 differ[2];
 #pragma unroll
@@ -272,8 +279,7 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
             store8<E>(out + ((int64_t)t * dim + (run ? at.b : at.a)) * sizeof(E), p);
             differ[run] = make_uint4(p.x ^ q.x, p.y ^ q.y, p.z ^ q.z, p.w ^ q.w);
         }
-        if (!turned || !(differ[0].x | differ[0].y | differ[0].z | differ[0].w | differ[1].x | differ[1].y | differ[1].z | differ[1].w)) continue;
-        uint32_t pairs = 0;
+        if (!turned || !(pairs | differ[0].x | differ[0].y | differ[0].z | differ[0].w | differ[1].x | differ[1].y | differ[1].z | differ[1].w)) continue;
 #pragma unroll
         for (int run = 0; run < 2; ++run)
 #pragma unroll

@@ -650,7 +650,8 @@ typedef struct dt_kv_seqs {
  * them only below 2^-6 of it).  A page that is begun anew (its first token is
  * stored) forgets what it held.  A page that is written belongs to one sequence of
  * the call.  k, v, q: io_type BF16 or F32, rows 16-byte aligned.  k is stored
- * as its rotation in 64 bits rounded once; q as dt_rotary_apply has it. */
+ * as its rotation in 64 bits rounded once (an element beyond fp32's range is not
+ * finite, which its pair's other does not feel); q as dt_rotary_apply has it. */
 typedef struct dt_kv_append_args {
     const void *k, *v, *q;
     void *q_out;
