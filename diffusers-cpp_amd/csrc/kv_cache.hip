@@ -478,7 +478,7 @@ int prepare(const dt_kv_cache* x, const dt_kv_seqs* y, const char* who, Cache* c
     const bool f8 = x->type == DT_TYPE_F8_E4M3;
     DT_REQUIRE(!f8 || (x->k_scale && x->v_scale), "%s: an e4m3 cache needs k_scale and v_scale", who);
     DT_REQUIRE(y->seqs >= 0 && y->seqs < (1 << 20) && y->rows >= 0 && y->rows < (1 << 28), "%s: size out of range", who);
-    DT_REQUIRE(y->table_pages >= 0 && y->table_pages * x->page <= (1ll << 30), "%s: a table of %lld pages is too long", who,
+    DT_REQUIRE(y->table_pages >= 0 && y->table_pages <= (1ll << 30) / x->page, "%s: a table of %lld pages is too long", who,
                (long long)y->table_pages);
     if (y->seqs > 0 && y->rows > 0) {
         DT_REQUIRE(y->seq_start && y->past && ((uintptr_t)y->seq_start & 3) == 0 && ((uintptr_t)y->past & 3) == 0,

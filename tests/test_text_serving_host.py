@@ -150,6 +150,21 @@ def test_cache_refused(in_cache, in_seqs, says):
     assert lib.dt_kv_attn_workspace_bytes(ctypes.addressof(c), ctypes.addressof(s), 4) == 0
 
 
+@pytest.mark.parametrize("page", [16, 32, 256])
+@pytest.mark.parametrize("more", [0, 1, 5])
+def test_tables_of_any_number_of_pages_are_measured(page, more):
+    """Pages whose tokens pass 64 bits are too many, like any above 2^30 tokens; 2^30 are not."""
+    lib, a = dh.load(), append_args()
+    for n in ((1 << 30) // page + 1 + more, (1 << 64) // page + more, (1 << 63) // page - 1 - more, (1 << 63) - 1 - more):
+        if n >= 1 << 63:
+            continue
+        c, s = cache(page=page), seqs(table_pages=n)
+        assert "too long" in refused(lib.dt_kv_append, ctypes.addressof(c), ctypes.addressof(s), ctypes.addressof(a), None)
+        assert "too long" in refused(lib.dt_kv_attn, *attn_call(c, s))
+    c, s = cache(page=page), seqs(table_pages=(1 << 30) // page)
+    assert "workspace" in refused(lib.dt_kv_attn, *attn_call(c, s, ws=None))
+
+
 @pytest.mark.parametrize("change,says", [
     (dict(io_type=dh.F16), "io_type"), (dict(k=None), "null k"), (dict(v=None), "null v"), (dict(k=ADDR + 4), "aligned"),
     (dict(k_strides=(129, 64)), "aligned"), (dict(v_strides=(128, -64)), "stride"), (dict(q_out=None), "null q_out"),
