@@ -249,9 +249,9 @@ __device__ __forceinline__ void append_k(const Args& a, const PageItem& it, int 
     for (int i = 0; i < NP; ++i) {
         const int t = first + i * a.per_pass + t0;
         if (!mine || t >= last) continue;
-        // A rotation keeps a pair's length l: |x| + |y| <= sqrt(2) l <= sqrt(2) (|x'| + |y'|).  Cosine and sine are off by
-        // 2^-23 and the factor's rounding, products and sum add two roundings: below 5 2^-24 (|x| + |y|) in all,
-        // 1.8 2^-22 (|x'| + |y'|).
+        // A rotation by mul keeps a pair's length l but for mul: mul (|x| + |y|) <= sqrt(2) mul l <= sqrt(2) (|x'| + |y'|).  Cosine
+        // and sine are off by 2^-23 of mul, the products and their sum by two roundings of 2^-24 more: 4 2^-24 mul (|x| + |y|)
+        // in all, 1.42 2^-22 (|x'| + |y'|) of the 2 2^-22 that are taken.
         float tol[8], all = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

@@ -6,9 +6,27 @@ import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_text_serving import BF16, F8, F32, Pool, e4m3, ints, power, rand, round_bf16, same, turned
+from test_gpu_text_serving import BF16, F8, F32, F64, Pool, e4m3, ints, power, rand, round_bf16, same, turned
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------- rotary --
+@pytest.mark.parametrize("mul", [1.0, 0.9, 1.1, 1.25, 1.3465736])
+def test_rotary_cosine_and_sine(mul):
+    """(1, 0) turned is (cos, sin) times the factor: off by at most 2^-23 of it.  (The angle rounded to fp32 once, the
+    series, and the product by the factor: 2^-23.04 at most over every fp32 angle up to pi / 4.)"""
+    T, n = 60000, 64
+    x = torch.zeros((T, 1, 2 * n), dtype=F32, device="cuda")
+    x[..., :n] = 1.0
+    pos = torch.randint(0, 100000, (T,), dtype=torch.int32, generator=torch.Generator().manual_seed(1)).cuda()
+    freq = torch.rand(n, generator=torch.Generator().manual_seed(2)).cuda()
+    y, _ = dh.rotary(x, None, pos, dh.Rotary(freq, half=True, attn_factor=mul))
+    a = pos.to(F64)[:, None] * freq.to(F64)
+    f = torch.tensor(mul, dtype=F32).to(F64).item()
+    off = torch.stack(((y[:, 0, :n].to(F64) - f * torch.cos(a)).abs().amax(), (y[:, 0, n:].to(F64) - f * torch.sin(a)).abs().amax()))
+    # beside it the angles' own rounding in 64 bits, in the reference too
+    assert off.max().item() <= 2.0 ** -23 * f + 4 * 2.0 ** -53 * 1e5, f"2^{math.log2(off.max().item() / f):.3f} of the factor"
 
 
 # -------------------------------------------------------------------- cache --
