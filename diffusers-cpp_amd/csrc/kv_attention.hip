@@ -152,7 +152,8 @@ __device__ __forceinline__ float xor_sum(float v) {
 template <typename E> struct Held;
 template <> struct Held<e4m3> {
     static constexpr int N = 2;
-    // Codes times the power of two are exact in bf16.
+    // Codes times the power of two are exact in bf16 for scales from 3 (the least code is 2^-9, bf16's least value
+    // 2^-133) to 246 (the largest is 448, bf16's range below 2^128); past that the largest are infinite.
     __device__ __forceinline__ static bf16x8_t part(const uint4& w, float scale, int m) {
         const uint32_t x[2] = {m ? w.z : w.x, m ? w.w : w.y};
         bf16x8_t f;
@@ -167,18 +168,26 @@ template <> struct Held<e4m3> {
         }
         return f;
     }
+    // What takes the codes that are not finite to bit 7, in each byte: those from 2^(255 - scale) on, which is 8 (262 - scale), are
+    // infinite; NaN is 0x7f.
+    __device__ __forceinline__ static uint32_t past(uint32_t scale) { return 0x01010101u * (scale > 246 ? 128 - 8 * (262 - scale) : 1u); }
     // Bits of the elements that are not finite.
-    __device__ __forceinline__ static uint32_t wild(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu; }
-    __device__ __forceinline__ static float value(const uint8_t* p) { return (*p & 0x7f) == 0x7f ? __builtin_nanf("") : 0.f; }
+    __device__ __forceinline__ static uint32_t wild(uint32_t w, uint32_t past) { return ((((w & 0x7f7f7f7fu) + past) & 0x80808080u) >> 7) * 0xffu; }
+    // A value that is not finite; 0 for any other.
+    __device__ __forceinline__ static float value(const uint8_t* p, const uint8_t* scale) {
+        const uint32_t w = *p;
+        if (!wild(w, past(*scale))) return 0.f;
+        return (w & 0x7fu) == 0x7fu ? __builtin_nanf("") : w & 0x80u ? -INFINITY : INFINITY;
+    }
 };
 template <> struct Held<bf16> {
     static constexpr int N = 1;
     __device__ __forceinline__ static bf16x8_t part(const uint4& w, float, int) { return __builtin_bit_cast(bf16x8_t, w); }
-    __device__ __forceinline__ static uint32_t wild(uint32_t w) {
+    __device__ __forceinline__ static uint32_t past(uint32_t) { return 0; }
+    __device__ __forceinline__ static uint32_t wild(uint32_t w, uint32_t) {
         return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
     }
-    // A value that is not finite; 0 for any other.
-    __device__ __forceinline__ static float value(const uint8_t* p) {
+    __device__ __forceinline__ static float value(const uint8_t* p, const uint8_t*) {
         const uint32_t w = *reinterpret_cast<const uint16_t*>(p);
         return (w & 0x7f80u) == 0x7f80u ? __uint_as_float(w << 16) : 0.f;
     }
@@ -208,8 +217,9 @@ __device__ __forceinline__ void add_wild(const Args& a, int b, int h, int from, 
         for (int key = from; key < to; ++key) {
             const int p = page_of(a.s, b, key);
             if (p < 0) continue;
-            const int64_t at = ((int64_t)p * a.c.kv_heads + h) * a.c.head_bytes;
-            x += Held<E>::value(a.c.v + at + (((int64_t)i << a.c.page_log2) + (key & ((1 << a.c.page_log2) - 1))) * sizeof(E));
+            const int64_t n = (int64_t)p * a.c.kv_heads + h;
+            x += Held<E>::value(a.c.v + n * a.c.head_bytes + (((int64_t)i << a.c.page_log2) + (key & ((1 << a.c.page_log2) - 1))) * sizeof(E),
+                                sizeof(E) == 1 ? a.c.v_scale + n : nullptr);
         }
         if (part) part[i] = x;
         else o[i] = (uint16_t)f32_to_bf16_bits(x);
@@ -392,9 +402,11 @@ struct Stream {
             // So have those that only some rows of the block see; what is none is added to these rows at the end.
             if ((t + 1) * STEP > all) {
                 uint32_t any = 0;
+                const uint32_t past = Held<E>::past(__float_as_uint(vs) >> 23);  // vscale is the next step's by now
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    const uint32_t wx = Held<E>::wild(vr[d].x), wy = Held<E>::wild(vr[d].y), wz = Held<E>::wild(vr[d].z), ww = Held<E>::wild(vr[d].w);
+                    const uint32_t wx = Held<E>::wild(vr[d].x, past), wy = Held<E>::wild(vr[d].y, past), wz = Held<E>::wild(vr[d].z, past),
+                                   ww = Held<E>::wild(vr[d].w, past);
                     any |= wx | wy | wz | ww;
                     vr[d] = make_uint4(vr[d].x & ~wx, vr[d].y & ~wy, vr[d].z & ~wz, vr[d].w & ~ww);
                 }
@@ -876,7 +888,10 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_rows_kernel(const Args a) {
                 const bool has = vhas[WIDE ? 0 : j];
                 v = leading<ES>(v, has ? max(sq.len - (t * kTile + vin[j]), 0) : 0);
                 if (some) {
-                    const uint32_t wx = Held<E>::wild(v.x), wy = Held<E>::wild(v.y), wz = Held<E>::wild(v.z), ww = Held<E>::wild(v.w);
+                    uint32_t scale = ES == 1 ? vscale[WIDE ? 0 : j] : kOne;
+                    asm("" : "+v"(scale));  // a scalar would be made of it, and waited for, where it is loaded
+                    const uint32_t past = Held<E>::past(scale);
+                    const uint32_t wx = Held<E>::wild(v.x, past), wy = Held<E>::wild(v.y, past), wz = Held<E>::wild(v.z, past), ww = Held<E>::wild(v.w, past);
                     if (wx | wy | wz | ww) wild_seen = 1;
                     v = make_uint4(v.x & ~wx, v.y & ~wy, v.z & ~wz, v.w & ~ww);
                 }

@@ -615,7 +615,9 @@ int dt_rotary_apply(const dt_rotary_args *args, dt_stream_t stream);
  * (a value's tokens side by side, as the product over them reads them), 16-byte
  * aligned, head_dim a multiple of 16 up to 128.  type BF16, or F8_E4M3 with a power of
  * two for each page and head: a code stands for code * 2^(scale - 127), k_scale and
- * v_scale uint8 [pages][kv_heads], 1 to 254.  All device memory. */
+ * v_scale uint8 [pages][kv_heads], 1 to 254.  bf16 holds every code from scale 3 to 246
+ * exactly; dt_kv_attn reads those of 1 and 2 as the bf16 next to them, and those that
+ * 247 and more take to 2^128 as infinite.  All device memory. */
 typedef struct dt_kv_cache {
     void *k, *v;
     uint8_t *k_scale, *v_scale;
@@ -669,7 +671,7 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  *   o_i = sum_j softmax_j(scale <q_i, k_j>) v_j
  * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
- * Operands bf16 (e4m3 codes times their scale are exact in it), the softmax's weights
+ * Operands bf16 (e4m3 codes as dt_kv_cache has them), the softmax's weights
  * rounded to bf16 for the product (their sum takes them before, or, with many rows a
  * sequence, as the product does), sums in fp32.  o: bf16; it must not overlap
  * an input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte

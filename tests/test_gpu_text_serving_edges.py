@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_text_serving import BF16, F8, F32, F64, Pool, e4m3, ints, power, rand, round_bf16, same, turned
+from test_gpu_text_serving import BF16, F8, F32, F64, Pool, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,53 @@ def test_append_of_keys_next_to_the_end_of_fp32(dtype, io, mul, half, rot):
         e = power(torch.where(out, 0.0, x.abs()).amax())
         assert pool.cache.k_scale[p, 0].item() - 127 == e.item()
         same(got, e4m3(torch.where(out, math.nan, x) * torch.exp2(-e)), f"page {p}")
+
+
+# ---------------------------------------------------------------- attention --
+def test_attention_reads_every_code_at_every_scale():
+    """One token a sequence, so that o is its v: every code at every scale, as bf16 has it."""
+    n, D = 254, 128
+    c = dh.kv_cache(n, 2, 16, D)
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda")
+    c.v.view(torch.uint8)[:, :, :, 0] = codes.view(2, D)
+    scale = torch.arange(1, 255, dtype=torch.uint8, device="cuda")
+    c.v_scale.copy_(scale[:, None].expand(n, 2))
+    c.k_scale.fill_(127)
+    table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None]
+    o = dh.cache_attn(rand(6, (n, 2, D)), c, table, torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda"))
+    x = codes.view(F8).to(F32).to(F64) * torch.exp2(scale.to(F64) - 127)[:, None]
+    # from scale 3 on every code is a multiple of bf16's least value, from 247 on the largest are beyond its range
+    want = torch.where(x.abs() >= 2.0 ** 128, torch.copysign(torch.full_like(x, math.inf), x), x)
+    got = o.view(n, 256).to(F64)
+    for i in range(n):
+        if i + 1 >= 3:
+            same(got[i], want[i], f"scale {i + 1}")
+        else:
+            bad = (got[i] - want[i]).abs() > 2.0 ** -133
+            assert not bad.any(), f"scale {i + 1}: codes {bad.nonzero().flatten().tolist()}"
+
+
+@pytest.mark.parametrize("page,new,past", [(64, (1, 1), (50, 200)), (16, (2, 1), (50, 200)), (64, (40, 3), (30, 64)), (16, (40, 3), (30, 64)), (64, (300,), (3900,)),
+                                           (32, (150,), (4000,)), (64, (2, 3), (6000, 5000))])
+def test_attention_of_later_tokens_beyond_bf16(page, new, past):
+    """Codes of a token that their scale takes beyond bf16's range: infinite for the row that sees it, nothing to the others."""
+    lens = [n + p for n, p in zip(new, past)]
+    lens[0] = (lens[0] - 2) // page * page + 1  # the last token begins a page of its own
+    past = (lens[0] - new[0],) + tuple(past[1:])
+    clean, pool = filled(60, lens, 2, 128, page, F8), filled(60, lens, 2, 128, page, F8)
+    q = rand(61, (sum(new), 4, 128))
+    args = pool.table, starts(new), ints(*past)
+    t, last = lens[0] - 1, new[0] - 1
+    p, off = pool.rows[0][t // page], t % page
+    for c in (clean, pool):
+        c.cache.v[p, 1, :, off] = torch.zeros(128, device="cuda").to(F8)
+    base = dh.cache_attn(q, clean.cache, *args)
+    for scale, code, x in ((247, 256.0, math.inf), (250, -32.0, -math.inf), (254, 2.0, math.inf)):
+        pool.cache.v_scale[p, 1] = scale
+        pool.cache.v[p, 1, 77, off] = torch.tensor(code).to(F8)
+        want = base.clone()
+        want[last, 2:, 77] = x
+        same(dh.cache_attn(q, pool.cache, *args), want, f"scale {scale}")
+        pool.cache.v[p, 1, 77, off] = torch.tensor(code / 2).to(F8)
+        got = dh.cache_attn(q, pool.cache, *args)
+        assert torch.equal(got[:last], base[:last]), f"scale {scale}, code {code / 2}"
