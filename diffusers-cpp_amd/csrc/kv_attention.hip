@@ -21,6 +21,7 @@
 
 #include "attn_tiles.hpp"
 #include "kv_cache.hpp"
+#include "overlap.hpp"
 
 namespace dit {
 namespace kv {
@@ -1217,6 +1218,10 @@ extern "C" int dt_kv_attn(const dt_kv_cache* cache, const dt_kv_seqs* seqs, cons
     DT_REQUIRE((p.blocks + 1) * p.splits * a.c.kv_heads < (1ll << 30) &&
                    ((int64_t)a.s.rows * (heads / a.c.kv_heads) / kRows + a.s.seqs) * a.c.kv_heads < (1ll << 31) && (int64_t)a.s.seqs * a.c.kv_heads * kFew < (1ll << 31),
                "%s: grid too large", who);
+    // A row's q is read by the waves of its block alone, and o is stored where they all have it: o may be q.
+    const int64_t sizes[2] = {a.s.rows, heads};
+    const Strided q_rows(q, 2, 2, sizes, q_strides, a.c.dim), o_rows(o, 2, 2, sizes, o_strides, a.c.dim);
+    DT_REQUIRE(o_rows.same_as(q_rows) || !share_memory(o_rows, q_rows), "%s: o is partly q", who);
     a.q = (const uint16_t*)q;
     a.o = (uint16_t*)o;
     for (int i = 0; i < 2; ++i) {

@@ -10,6 +10,7 @@
 #include <math.h>
 
 #include "kv_cache.hpp"
+#include "overlap.hpp"
 #include "rotary.hpp"
 
 namespace dit {
@@ -546,6 +547,13 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
     }
     DT_REQUIRE(((uintptr_t)x->pos & 3) == 0, "%s: pos must be 4-byte aligned", who);
     if (a.s.rows == 0 || a.s.seqs == 0) return DT_OK;
+    if (turn_q) {
+        const int64_t q_sizes[2] = {a.s.rows, x->heads}, sizes[2] = {a.s.rows, a.c.kv_heads};
+        const Strided q(x->q, es, 2, q_sizes, x->q_strides, a.c.dim), out(x->q_out, es, 2, q_sizes, x->q_out_strides, a.c.dim);
+        DT_REQUIRE(out.same_as(q) || !share_memory(out, q), "%s: q_out is partly q", who);
+        DT_REQUIRE(!share_memory(out, Strided(x->k, es, 2, sizes, x->k_strides, a.c.dim)), "%s: q_out is partly k", who);
+        DT_REQUIRE(!share_memory(out, Strided(x->v, es, 2, sizes, x->v_strides, a.c.dim)), "%s: q_out is partly v", who);
+    }
     a.k = x->k;
     a.v = x->v;
     a.q = x->q;

@@ -8,6 +8,7 @@
 
 #include "capi_util.hpp"
 #include "common.hpp"
+#include "overlap.hpp"
 #include "rotary.hpp"
 
 namespace dit {
@@ -223,6 +224,17 @@ extern "C" int dt_rotary_apply(const dt_rotary_args* x, dt_stream_t stream) {
     }
     DT_REQUIRE(x->pos && ((uintptr_t)x->pos & 3) == 0, "%s: pos must be given, 4-byte aligned", who);
     DT_REQUIRE(x->batch <= 1 || (x->pos_stride >= 0 && x->pos_stride < (1ll << 40)), "%s: pos_stride unsupported", who);
+    const int64_t q_sizes[3] = {x->batch, x->seq, x->heads}, k_sizes[3] = {x->batch, x->seq, x->kv_heads};
+    const int es = elem_size(x->io_type);
+    const Strided q(x->q, es, 3, q_sizes, x->q_strides, x->head_dim), q_out(x->q_out, es, 3, q_sizes, x->q_out_strides, x->head_dim);
+    const Strided k(x->k, es, 3, k_sizes, x->k_strides, x->head_dim), k_out(x->k_out, es, 3, k_sizes, x->k_out_strides, x->head_dim);
+    if (a.heads[0]) DT_REQUIRE(q_out.same_as(q) || !share_memory(q_out, q), "%s: q_out is partly q", who);
+    if (a.heads[1]) DT_REQUIRE(k_out.same_as(k) || !share_memory(k_out, k), "%s: k_out is partly k", who);
+    if (a.heads[0] && a.heads[1]) {
+        DT_REQUIRE(!share_memory(q_out, k), "%s: q_out is partly k", who);
+        DT_REQUIRE(!share_memory(k_out, q), "%s: k_out is partly q", who);
+        DT_REQUIRE(!share_memory(q_out, k_out), "%s: q_out is partly k_out", who);
+    }
     a.seq = (int32_t)x->seq;
     a.seq_div = make_fastdiv((uint32_t)x->seq);
     a.pos = x->pos;

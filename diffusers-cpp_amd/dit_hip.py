@@ -1386,7 +1386,7 @@ def cache_attn(q, cache, table, seq_start, past, causal=True, scale=None, out=No
     to what their sequences hold in the cache, the new tokens included: softmax(scale q k^T) v over
     the tokens up to each row's own (causal) or over all -> bf16 [rows, heads, dim].  table,
     seq_start and past as cache_append's (past: before the new tokens).  scale: >= 0, by default
-    dim ** -0.5.  Rows of no sequence are left as they are."""
+    dim ** -0.5.  Rows of no sequence are left as they are.  out may be q itself."""
     here = _torch().cuda.current_device()
     c, s, q_st, o_st, n = _cache_attn_plan(*_metas(cache.k, cache.v, cache.k_scale, cache.v_scale, table, seq_start, past, q, out), here)
     if out is None:

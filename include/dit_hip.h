@@ -593,7 +593,8 @@ int dt_rotary_freq_fill(float *freq, int64_t rot_dims, double base, double facto
 /* Rotates q and k in one launch (either may be NULL).  Element (b, s, h, d) of q is
  * q[b*q_strides[0] + s*q_strides[1] + h*q_strides[2] + d]; likewise k, which has
  * kv_heads heads, and the outputs; position pos[b*pos_stride + s] (int32, device).
- * An output may be its input (same pointer and strides) and else overlaps nothing.
+ * An output may be its input (same pointer and strides) and else overlaps nothing; a call whose
+ * output is partly an input or the other output is refused.
  * backward: the rotation back, which makes the gradients of dt_rotary_apply's inputs
  * from those of its outputs.  Any head_dim up to 4096, alignment and strides (those of
  * dimensions of one element are not read); whole 16-byte rows with head_dim % 16 == 0
@@ -642,7 +643,8 @@ typedef struct dt_kv_seqs {
 } dt_kv_seqs;
 
 /* Stores the new tokens' k and v (rows [kv_heads][head_dim], strides {row, head}), and
- * rotates q (heads heads; NULL: none) into q_out in the same launch, which may be q.
+ * rotates q (heads heads; NULL: none) into q_out in the same launch, which may be q (same
+ * pointer and strides), but not a part of q, k or v.
  * rotary NULL: nothing is rotated, and q must be NULL.  Positions are the tokens' places,
  * or pos[row] (int32 [rows]) where pos is given.  With half, rot_dims is a multiple of 16.
  * F8_E4M3: a page's scale is the least power of two (2^-126 at least) by which e4m3's
@@ -673,8 +675,8 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
  * Operands bf16 (e4m3 codes as dt_kv_cache has them), the softmax's weights
  * rounded to bf16 for the product (their sum takes them before, or, with many rows a
- * sequence, as the product does), sums in fp32.  o: bf16; it must not overlap
- * an input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
+ * sequence, as the product does), sums in fp32.  o: bf16; it may be q (same pointer and
+ * strides) and else overlaps no input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
  * aligned) is needed (0 for some calls); its size goes by the sizes given here, not by the
  * lengths on the device.  No atomics: the same call gives the same bits. */
 size_t dt_kv_attn_workspace_bytes(const dt_kv_cache *cache, const dt_kv_seqs *seqs, int64_t heads);

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_text_serving import BF16, F8, F32, F64, Pool, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
+from test_gpu_text_serving import BF16, BLOCKS, F8, F32, F64, Pool, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,20 @@ def test_attention_of_later_tokens_beyond_bf16(page, new, past):
         pool.cache.v[p, 1, 77, off] = torch.tensor(code / 2).to(F8)
         got = dh.cache_attn(q, pool.cache, *args)
         assert torch.equal(got[:last], base[:last]), f"scale {scale}, code {code / 2}"
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS + [(8, 2, 128, 64, [(1, 1000), (1, 3)]), (40, 1, 96, 16, [(1, 70), (5, 0)]), (4, 4, 64, 32, [(9, 1500)])])
+def test_attention_onto_its_queries(dtype, heads, kv_heads, dim, page, seqs):
+    """o may be q, here inside wider rows: the bits of a call with a tensor of its own, and nothing else touched."""
+    new, past = zip(*seqs)
+    pool = filled(95, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
+    rows = rand(96, (sum(new) + 3, heads * dim + 64))
+    q = rows[:, :heads * dim].unflatten(1, (heads, dim))
+    args = pool.cache, pool.table, starts(new, 2), ints(*past)
+    for causal in (True, False):
+        before = rows.clone()
+        want = dh.cache_attn(q, *args, causal=causal, out=q.clone())
+        assert dh.cache_attn(q, *args, causal=causal, out=q) is q
+        assert torch.equal(q, want) and torch.equal(rows[:, heads * dim:], before[:, heads * dim:])
+        rows.copy_(before)

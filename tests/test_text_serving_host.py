@@ -362,3 +362,98 @@ def test_pages_that_are_none(index):
     got = index(40, 4, 4, [0, 40], [10], [[1, 0]])
     assert [(page, begin, first, last) for _, page, begin, first, last, _ in got] == [(1, 0, 10, 16), (0, 16, 0, 16)]
     assert index(40, 4, 4, [0, 40], [32], [[1, 0]]) == []
+
+
+# ------------------------------------------------------------------- overlaps --
+OVERLAP = r"""
+#include <stdio.h>
+#include "overlap.hpp"
+using namespace dit;
+// stdin: pairs of operands, each: address, element bytes, dims, their sizes and strides, width; stdout: 1 or 0 a pair, each way
+int main() {
+    for (;;) {
+        long long at[2], n[2][3], st[2][3], width[2];
+        int es[2], dims[2];
+        for (int k = 0; k < 2; ++k) {
+            if (scanf("%lld %d %d", &at[k], &es[k], &dims[k]) != 3) return 0;
+            for (int i = 0; i < dims[k]; ++i) scanf("%lld %lld", &n[k][i], &st[k][i]);
+            scanf("%lld", &width[k]);
+        }
+        int64_t sizes[2][3], strides[2][3];
+        for (int k = 0; k < 2; ++k)
+            for (int i = 0; i < dims[k]; ++i) sizes[k][i] = n[k][i], strides[k][i] = st[k][i];
+        const Strided a((void*)at[0], es[0], dims[0], sizes[0], strides[0], width[0]), b((void*)at[1], es[1], dims[1], sizes[1], strides[1], width[1]);
+        printf("%d %d\n", share_memory(a, b), share_memory(b, a));
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def overlap(tmp_path_factory):
+    d = tmp_path_factory.mktemp("overlap")
+    src, exe = d / "overlap.cpp", d / "overlap"
+    src.write_text(OVERLAP)
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", os.path.join(PKG, "csrc"), str(src),
+                           "-o", str(exe)])
+
+    def run(pairs):
+        text = "\n".join(" ".join(map(str, [at, es, len(n), *itertools.chain(*zip(n, st)), width])) for pair in pairs for at, es, n, st, width in pair)
+        out = subprocess.run([str(exe)], input=text, stdout=subprocess.PIPE, text=True, check=True).stdout
+        return [tuple(map(int, line.split())) for line in out.splitlines()]
+
+    return run
+
+
+def touched(at, es, n, st, width):
+    return {at + es * sum(i * s for i, s in zip(index, st)) + w for index in itertools.product(*map(range, n)) for w in range(width * es)}
+
+
+def test_operands_that_share_memory(overlap):
+    """Against every byte of either, over layouts of up to three dimensions in any order."""
+    rng = random.Random(7)
+    pairs = []
+    for _ in range(3000):
+        one = []
+        for _ in range(2):
+            width, n, st = rng.randint(1, 6), [rng.randint(1, 4) for _ in range(rng.randint(0, 3))], []
+            step = width + rng.choice([0, 0, rng.randint(0, 8), -width])
+            for k in n:
+                st.append(step)
+                step = step * k + rng.choice([0, 0, rng.randint(0, 20)])
+            order = rng.sample(range(len(n)), len(n))
+            one.append((rng.randint(0, 60), rng.choice([2, 4]), [n[i] for i in order], [st[i] for i in order], width))
+        if rng.random() < 0.5:  # one layout, at two places
+            one[1] = (one[1][0], *one[0][1:])
+        pairs.append(one)
+    want = [bool(touched(*a) & touched(*b)) for a, b in pairs]
+    assert 500 < sum(want) < 2500
+    assert overlap(pairs) == [(w, w) for w in want]
+
+
+def test_large_operands_that_share_memory(overlap):
+    T, H, K, D = 1 << 20, 40, 8, 128
+    R = (H + 2 * K) * D
+    q, k, v = (0, 2, [T, H], [R, D], D), (2 * H * D, 2, [T, K], [R, D], D), (2 * (H + K) * D, 2, [T, K], [R, D], D)
+    flat = (0, 2, [T, H], [H * D, D], D)
+    gaps = [(2 * D * i, 2, [T, H], [2 * H * D, 2 * D], D) for i in range(2)]  # two tensors' heads in turn
+    batch = [(2 * i * D, 2, [4, T, H], [3 * T * 2 * H * D, 2 * H * D, 2 * D], D) for i in range(2)]
+    pairs = [((q, k), 0), ((k, v), 0), ((q, q), 1), ((q, flat), 1), ((k, flat), 1), ((gaps[0], gaps[1]), 0), ((gaps[0], gaps[0]), 1),
+             ((gaps[0], flat), 1), ((batch[0], batch[1]), 0), ((batch[0], (2, *batch[1][1:])), 1), ((q, (2 * T * R, *flat[1:])), 0)]
+    assert overlap([p for p, _ in pairs]) == [(w, w) for _, w in pairs]
+
+
+def test_outputs_that_are_partly_inputs_are_refused():
+    lib = dh.load()
+    # 10 rows of 4 heads of 64 (bf16, 512 bytes); far: another buffer
+    far = ADDR + (1 << 20)
+    for change, says in ((dict(q_out=ADDR + 512), "q_out is partly q"), (dict(q_out_strides=(2560, 512, 64)), "q_out is partly q"),
+                         (dict(k=far, k_out=far + 128), "k_out is partly k"), (dict(k_out=far), "q_out is partly k"),
+                         (dict(k=far, k_out=ADDR), "k_out is partly q"),
+                         (dict(k=far, k_out=far + 2 ** 18, q_out=far + 2 ** 18), "q_out is partly k_out")):
+        assert says in refused(lib.dt_rotary_apply, ctypes.addressof(rotary_args(**change)), None)
+    for change, says in ((dict(q_out=ADDR + 512, k=far, v=far), "q_out is partly q"), (dict(v=far), "q_out is partly k"), (dict(k=far), "q_out is partly v"),
+                         (dict(q_out_strides=(512, 64), k=far, v=far), "q_out is partly q")):
+        assert says in refused(lib.dt_kv_append, ctypes.addressof(cache()), ctypes.addressof(seqs()), ctypes.addressof(append_args(**change)), None)
+    for change in (dict(o=ADDR + 512), dict(os_=(512, 64)), dict(o=ADDR + 128)):
+        assert "o is partly q" in refused(lib.dt_kv_attn, *attn_call(cache(), seqs(), **change))
