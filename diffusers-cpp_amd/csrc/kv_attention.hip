@@ -126,11 +126,15 @@ struct Walk {
         return {from + l, __builtin_amdgcn_readlane(row, l), __builtin_amdgcn_readlane(n, l), __builtin_amdgcn_readlane(past, l),
                 __builtin_amdgcn_readlane(len, l), lane64(end - units, l)};
     }
-    // The sequence that unit x (below the total) belongs to.
+    // The sequence that unit x (below the total) belongs to.  b = -1: none, which lengths that are written
+    // under the call may make of it.
     __device__ __forceinline__ Mine find(int64_t x) {
         if (x < lane64(end - units, 0)) load(0, 0);
-        while (x >= lane64(end, 63)) load(from + 64, lane64(end, 63));
-        return mine(__builtin_ctzll(__builtin_amdgcn_ballot_w64(end > x)));
+        while (x >= lane64(end, 63) && from + 64 < a.s.seqs) load(from + 64, lane64(end, 63));
+        const uint64_t behind = __builtin_amdgcn_ballot_w64(end > x);
+        Mine m = mine(behind ? __builtin_ctzll(behind) : 0);
+        if (!behind) m.b = -1;
+        return m;
     }
 };
 
@@ -449,6 +453,7 @@ __device__ __forceinline__ void stream_part(const Args& a, int id) {
     const int64_t x1 = total * (w + 1) / W;
     for (int64_t x = total * w / W; x < x1;) {
         const Mine sq = walk.find(x);
+        if (sq.b < 0) return;
         const int tiles = walk.tiles(sq.len), blk = (int)((x - sq.before) / tiles);
         const int64_t s0 = sq.before + (int64_t)blk * tiles;
         const int t0 = (int)(x - s0), t1 = (int)((x1 < s0 + tiles ? x1 : s0 + tiles) - s0);

@@ -631,8 +631,8 @@ typedef struct dt_kv_cache {
  * belong to sequence b, which holds past[b] tokens already (int32 [seqs], device; below
  * 0: 0); row seq_start[b] + i is its token past[b] + i, and token t lies in page
  * table[b*table_stride + t / page] (int32 [seqs][table_pages], device), row t % page.
- * Everything about lengths is read on the device: a captured launch serves
- * other lengths and tables in place.  Rows of no sequence are neither read nor
+ * Everything about lengths is read on the device, several times over, and stays as it is
+ * while the call runs: a captured launch serves other lengths and tables in place.  Rows of no sequence are neither read nor
  * written.  A page number outside [0, pages) is no page, as is anything past the
  * table: tokens there are not stored, and not attended to. */
 typedef struct dt_kv_seqs {
