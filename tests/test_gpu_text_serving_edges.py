@@ -1,12 +1,13 @@
 """The text-serving operators where they can go wrong: at the ends of their types' ranges, among thousands of keys, and
 behind tables wider than what is held.  Each against its definition in 64 bits."""
+import gc
 import math
 
 import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_text_serving import BF16, BLOCKS, F8, F32, F64, Pool, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
+from test_gpu_text_serving import BF16, BLOCKS, F8, F32, F64, Pool, check_attention, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +60,29 @@ def test_append_of_keys_next_to_the_end_of_fp32(dtype, io, mul, half, rot):
         same(got, e4m3(torch.where(out, math.nan, x) * torch.exp2(-e)), f"page {p}")
 
 
+@pytest.mark.parametrize("dtype", [F8, BF16])
+def test_prepared_appends_repeat(dtype):
+    """prepare() keeps what the call points to: its description of the rotation, the sequences and the pages."""
+    a, b = Pool(50, [40, 30], 2, 64, 16, dtype), Pool(50, [40, 30], 2, 64, 16, dtype)
+    k, v, q, pos = rand(51, (25, 2, 64)), rand(52, (25, 2, 64)), rand(53, (25, 4, 64)), ints(*range(7, 32))
+    freq, start, past = dh.rotary_freqs(64), ints(0, 20, 25), ints(3, 17)
+    for pool in (a, b):
+        for i, n in enumerate((3, 17)):
+            pool.fill(i, rand(54 + i, (n, 2, 64), F64), rand(56 + i, (n, 2, 64), F64))
+    out, launch = dh.prepare(dh.cache_append, a.cache, k, v, a.table, start, past, rot=dh.Rotary(freq, half=True, attn_factor=1.25), pos=pos, q=q)
+    gc.collect()
+    for i in range(3):
+        for t in (k, v, q):
+            t.copy_(rand(60 + i, t.shape))
+        out.fill_(7.0)
+        launch()
+        want = dh.cache_append(b.cache, k, v, b.table, start, past, rot=dh.Rotary(freq, half=True, attn_factor=1.25), pos=pos, q=q)
+        assert torch.equal(out, want)
+        for s, n in ((0, 23), (1, 22)):
+            for x, y in zip(a.held(s, n), b.held(s, n)):
+                same(x[3 if s == 0 else 17:], y[3 if s == 0 else 17:], "pages")
+
+
 # ---------------------------------------------------------------- attention --
 def test_attention_reads_every_code_at_every_scale():
     """One token a sequence, so that o is its v: every code at every scale, as bf16 has it."""
@@ -109,6 +133,84 @@ def test_attention_of_later_tokens_beyond_bf16(page, new, past):
         assert torch.equal(got[:last], base[:last]), f"scale {scale}, code {code / 2}"
 
 
+def key_dims(n, D):
+    """Of each place a dim, neighbours' unlike."""
+    j = torch.arange(n, device="cuda")
+    return (j * 5 + j // D * 3) % D
+
+
+@pytest.mark.parametrize("wide", [0, 200])
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS)
+def test_every_key_counts_once(dtype, heads, kv_heads, dim, page, seqs, wide):
+    """Keys of 0 weigh alike, and each value is 1 in one dim: o is how many of a row's keys have that dim, over their number.
+    One of N keys left out, or taken twice, changes a dim by D / N of it, where the result is rounded to 2^-8."""
+    new, past = zip(*seqs)
+    lens = [n + p for n, p in zip(new, past)]
+    assert max(lens) / dim < 100
+    pool = Pool(70, lens, kv_heads, dim, page, dtype)
+    ones = [torch.nn.functional.one_hot(key_dims(n, dim), dim).to(F64) for n in lens]
+    for b, n in enumerate(lens):
+        pool.fill(b, torch.zeros((n, kv_heads, dim), dtype=F64, device="cuda"), ones[b][:, None].expand(n, kv_heads, dim))
+    table = pool.table if not wide else torch.nn.functional.pad(pool.table, (0, wide), value=-1)
+    q = rand(71, (sum(new), heads, dim))
+    for causal in (True, False):
+        got = dh.cache_attn(q, pool.cache, table, starts(new), ints(*past), causal=causal).to(F64)
+        for b, (n, p) in enumerate(seqs):
+            if n == 0:
+                continue
+            seen = p + 1 + torch.arange(n, device="cuda") if causal else torch.full((n,), p + n, device="cuda")
+            want = (torch.cumsum(ones[b], 0)[seen - 1] / seen[:, None].to(F64))[:, None]
+            a = sum(new[:b])
+            # 1 / N and its product in fp32 (2^-24 each), the result's rounding; the counts are exact
+            over = (got[a:a + n] - want).abs() - (2.0 ** -8 + 4 * 2.0 ** -24) * want
+            assert over.max().item() <= 0, f"sequence {b}, row {int(over.amax((1, 2)).argmax())}"
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS)
+def test_a_row_finds_its_key(dtype, heads, kv_heads, dim, page, seqs):
+    """Keys of signs, and queries that are one key's each: o is that key's value, wherever it lies.  The first and the last key
+    that a row sees, those on both sides of the borders of pages and tiles, others anywhere."""
+    new, past = zip(*seqs)
+    lens = [n + p for n, p in zip(new, past)]
+    pool = Pool(80, lens, kv_heads, dim, page, dtype)
+    q, at = torch.zeros((sum(new), heads, dim), dtype=BF16, device="cuda"), []
+    g = torch.Generator().manual_seed(81)
+    for b, (n, p) in enumerate(seqs):
+        k = torch.where(torch.rand((n + p, kv_heads, dim), generator=g) < 0.5, 1.0, -1.0).to(F64).cuda()
+        pool.fill(b, k, rand(82 + b, (n + p, kv_heads, dim), F64))
+        if n == 0:
+            at.append(None)
+            continue
+        sees = (p + 1 + torch.arange(n))[:, None].expand(n, heads)
+        i = torch.arange(n * heads).view(n, heads)
+        edge = torch.randint(0, 10 ** 6, (n, heads), generator=g) % (-(-sees // page)) * page - (i // 4) % 2
+        edge = torch.where(edge < 0, 0, edge)
+        far = torch.randint(0, 10 ** 6, (n, heads), generator=g) % sees
+        j = torch.where(i % 4 == 0, sees - 1, torch.where(i % 4 == 1, edge, far)).clamp_max(sees - 1)
+        j[:, -1] = torch.where(torch.arange(n) % 3 == 0, 0, j[:, -1])
+        at.append(j.cuda())
+        kv = (torch.arange(heads, device="cuda") // (heads // kv_heads))[None].expand(n, heads)
+        q[sum(new[:b]):sum(new[:b]) + n] = k[at[b], kv].to(BF16)
+    # A key's own score is dim, others' a sum of dim signs: dim / 2 behind it is 28 standard deviations (4 at dim 64) ... times 4
+    got = dh.cache_attn(q, pool.cache, pool.table, starts(new), ints(*past), scale=4.0)
+    for b, (n, p) in enumerate(seqs):
+        if n == 0:
+            continue
+        a, (k, v) = sum(new[:b]), pool.held(b, n + p)
+        kv = (torch.arange(heads, device="cuda") // (heads // kv_heads))[None].expand(n, heads)
+        want = v[at[b], kv]
+        # equal keys share the weight: rows whose key is another's too are left out
+        x = 4.0 * torch.stack([q[a:a + n, h].to(F64) @ k[:, h * kv_heads // heads].t().contiguous() for h in range(heads)], 1)
+        x = x.masked_fill((torch.arange(n + p, device="cuda")[None] > p + torch.arange(n, device="cuda")[:, None])[:, None], -math.inf)
+        alone = (torch.exp(x - 4.0 * dim).sum(-1) - 1) <= 1e-6
+        assert alone.float().mean().item() > 0.9
+        # the weight's rounding to bf16 and the result's, beside what the others weigh (1e-6, of values up to 6)
+        over = ((got[a:a + n].to(F64) - want).abs() - (2 * 2.0 ** -8 + 2.0 ** -16 + 2.0 ** -20) * want.abs() - 2e-5).amax(-1)
+        assert over[alone].max().item() <= 0, f"sequence {b}: {(over * alone).argmax().item()}"
+
+
 @pytest.mark.parametrize("dtype", [F8, BF16])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", BLOCKS + [(8, 2, 128, 64, [(1, 1000), (1, 3)]), (40, 1, 96, 16, [(1, 70), (5, 0)]), (4, 4, 64, 32, [(9, 1500)])])
 def test_attention_onto_its_queries(dtype, heads, kv_heads, dim, page, seqs):
@@ -124,3 +226,19 @@ def test_attention_onto_its_queries(dtype, heads, kv_heads, dim, page, seqs):
         assert dh.cache_attn(q, *args, causal=causal, out=q) is q
         assert torch.equal(q, want) and torch.equal(rows[:, heads * dim:], before[:, heads * dim:])
         rows.copy_(before)
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", [
+    (8, 2, 128, 64, [(1, 1000)]), (8, 2, 128, 64, [(1, 1000), (1, 3), (1, 64)]), (8, 2, 128, 64, [(512, 0)]), (8, 2, 64, 16, [(100, 0), (1, 50), (3, 7)]),
+    (4, 4, 80, 128, [(64, 100)]), (4, 1, 128, 32, [(40, 700), (90, 0)]),
+])
+def test_tables_wider_than_what_is_held(dtype, heads, kv_heads, dim, page, seqs):
+    """A table made for the longest context: whatever it makes of the work, the results stay within their bounds."""
+    new, past = zip(*seqs)
+    pool = filled(90, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
+    q = rand(91, (sum(new), heads, dim))
+    for wide in (0, 30, 500, 4000):
+        table = torch.nn.functional.pad(pool.table, (0, wide), value=3)  # pages of others behind
+        for causal in (True, False):
+            check_attention(pool, q, new, past, dh.cache_attn(q, pool.cache, table, starts(new), ints(*past), causal=causal), causal)
