@@ -18,6 +18,9 @@ int check_launch(const char* what);
 // Multiprocessor (CU) count of the current device, cached per device.
 int cu_count();
 
+// Whether a launch in one dimension holds so many workgroups: past 2^32 - 1 threads it is cut short, without an error.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < (1ll << 31) && blocks * threads < (1ll << 32); }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline int elem_size(int32_t type) {

@@ -1148,15 +1148,25 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
     const int64_t n = (int64_t)a.s.rows * a.heads;
     const bool wide = 1 << a.c.page_log2 >= (p.rows ? kTile : Stream<E, DP, true>::STEP);
     if (p.whole) {
-        const dim3 grid((unsigned)((n / a.c.kv_heads / kRows + a.s.seqs) * a.c.kv_heads));
+        const int64_t blocks = (n / a.c.kv_heads / kRows + a.s.seqs) * a.c.kv_heads;
+        DT_REQUIRE(grid_fits(blocks, 512), "dt_kv_attn: grid too large");
+        const dim3 grid((unsigned)blocks);
         const size_t lds = 8 * kRows * (DP + 4) * sizeof(float);
         if (wide) hipLaunchKernelGGL((kv_short_kernel<E, DP, true>), grid, dim3(512), lds, st, a);
         else hipLaunchKernelGGL((kv_short_kernel<E, DP, false>), grid, dim3(512), lds, st, a);
         return check_launch("dt_kv_attn");
     }
+    // Shares of the stream: few rows may each have many, then a workgroup a row (24 tokens to 4000, 768 rows: 34 us, in
+    // fours 36; 4096 rows 129 and 122).  Key ranges: four elements a thread.
+    const int64_t joined = !p.stream ? 0 : p.rows ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
+    const int64_t ranges = p.splits > 1 ? (n * (DP / 4) + 255) / 256 : 0;
+    const int64_t join_blocks = joined <= 1024 ? joined : (joined + 3) / 4;
+    DT_REQUIRE(grid_fits(join_blocks + ranges, 256), "dt_kv_attn: grid too large");
     if (p.rows) {
         a.stream_blocks = p.stream ? a.c.kv_heads * a.waves / (p.block / 32) : 0;
-        const dim3 grid((unsigned)(a.stream_blocks + p.blocks * p.splits * a.c.kv_heads)), block(2 * p.block);
+        const int64_t blocks = a.stream_blocks + p.blocks * p.splits * a.c.kv_heads;
+        DT_REQUIRE(grid_fits(blocks, 2 * p.block), "dt_kv_attn: grid too large");
+        const dim3 grid((unsigned)blocks), block(2 * p.block);
         const size_t lds = 2 * (size_t)(kTile * DP + DP * kTile) * 2;
         if (p.block == 256) {
             if (wide) hipLaunchKernelGGL((kv_rows_kernel<E, DP, true, 8>), grid, block, lds, st, a);
@@ -1172,13 +1182,9 @@ int launch(Args& a, const Plan& p, hipStream_t st) {
         else hipLaunchKernelGGL((kv_stream_kernel<E, DP, false>), grid, dim3(256), 0, st, a);
     }
     const int rc = check_launch("dt_kv_attn");
-    // Shares of the stream: few rows may each have many, then a workgroup a row (24 tokens to 4000, 768 rows: 34 us, in
-    // fours 36; 4096 rows 129 and 122).  Key ranges: four elements a thread.
-    const int64_t joined = !p.stream ? 0 : p.rows ? (int64_t)a.s.seqs * a.c.kv_heads * kFew : n;
-    const int64_t ranges = p.splits > 1 ? (n * (DP / 4) + 255) / 256 : 0;
-    if (rc || joined + ranges == 0) return rc;
-    a.join_blocks = (int32_t)(joined <= 1024 ? joined : (joined + 3) / 4);
-    const dim3 grid((unsigned)(a.join_blocks + ranges));
+    if (rc || join_blocks + ranges == 0) return rc;
+    a.join_blocks = (int32_t)join_blocks;
+    const dim3 grid((unsigned)(join_blocks + ranges));
     if (joined <= 1024) hipLaunchKernelGGL((kv_join_kernel<E, DP, 256>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((kv_join_kernel<E, DP, 64>), grid, dim3(256), 0, st, a);
     return check_launch("dt_kv_attn");

@@ -588,7 +588,7 @@ extern "C" int dt_kv_append(const dt_kv_cache* cache, const dt_kv_seqs* seqs, co
     const int64_t kv_blocks = items(a.s) * a.c.kv_heads * 2;
     const int64_t waves = a.threads / 64;
     const int64_t q_blocks = turn_q ? ((int64_t)a.s.rows * a.q_chunks + waves - 1) / waves : 0;
-    DT_REQUIRE(kv_blocks + q_blocks < (1ll << 31) && (int64_t)a.s.rows * a.q_chunks < (1ll << 31), "%s: grid too large", who);
+    DT_REQUIRE(grid_fits(kv_blocks + q_blocks, a.threads) && (int64_t)a.s.rows * a.q_chunks < (1ll << 31), "%s: grid too large", who);
     a.kv_blocks = (int32_t)kv_blocks;
     const dim3 grid((unsigned)(kv_blocks + q_blocks));
     const int k_passes = ((int)page + a.per_pass - 1) / a.per_pass, v_passes = ((int)page / 4 + a.quads_per_pass - 1) / a.quads_per_pass;

@@ -33,11 +33,15 @@ struct Args {
     float mul, sign;
     int32_t units, slots, chunks;  // units of two vectors a head; heads side by side in a wave; waves a token
     FastDiv unit_div, chunk_div;
+    uint32_t grid_x;
 };
+
+// Workgroups in lines of grid_x: one dimension of a launch holds less than 2^32 threads, and is cut short past that.
+__device__ __forceinline__ uint32_t block_id(const Args& a) { return blockIdx.y * a.grid_x + blockIdx.x; }
 
 template <typename T, int ITER>
 __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
-    const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t wave = block_id(a) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t row = fdiv(wave, a.chunk_div), chunk = wave - row * a.chunks;
     if (row >= (uint64_t)a.rows) return;
     const uint32_t slot = fdiv(lane, a.unit_div);
@@ -69,7 +73,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(const Args a) {
 template <typename T>
 __global__ __launch_bounds__(256) void rotary_any_kernel(const Args a) {
     const int items = a.rot / 2 + a.dim - a.rot, heads = a.heads[0] + a.heads[1];
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t id = (int64_t)block_id(a) * 256 + threadIdx.x;
     const int64_t row = id / ((int64_t)items * heads);
     if (row >= a.rows) return;
     const int rest = (int)(id - row * items * heads);
@@ -95,13 +99,21 @@ __global__ __launch_bounds__(256) void rotary_any_kernel(const Args a) {
     Io<T>::put(y + d1, v * c + u * s);
 }
 
+// `blocks` workgroups of 256 threads in lines of equal length.
+dim3 lines_of(int64_t blocks, Args* a) {
+    const int64_t lines = (blocks + (1 << 23) - 1) >> 23;
+    a->grid_x = (uint32_t)((blocks + lines - 1) / lines);
+    return dim3(a->grid_x, (unsigned)lines);
+}
+
 template <typename T>
 int launch(Args& a, bool wide, hipStream_t st) {
     const int heads = a.heads[0] + a.heads[1];
     if (!wide) {
         const int64_t n = a.rows * heads * (a.rot / 2 + a.dim - a.rot);
         DT_REQUIRE((n + 255) / 256 < (1ll << 31), "dt_rotary_apply: grid too large");
-        hipLaunchKernelGGL((rotary_any_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+        const dim3 grid = lines_of((n + 255) / 256, &a);
+        hipLaunchKernelGGL((rotary_any_kernel<T>), grid, dim3(256), 0, st, a);
         return check_launch("dt_rotary_apply");
     }
     // Four heads a lane where that leaves every SIMD a wave; else one, whose loads are the shorter wait (40 heads of
@@ -111,8 +123,8 @@ int launch(Args& a, bool wide, hipStream_t st) {
     a.chunks = many ? four : (heads + a.slots - 1) / a.slots;
     a.chunk_div = make_fastdiv((uint32_t)a.chunks);
     const int64_t waves = a.rows * a.chunks;
-    DT_REQUIRE(waves < (1ll << 31), "dt_rotary_apply: grid too large");
-    const dim3 grid((unsigned)((waves + 3) / 4));
+    DT_REQUIRE(waves < (1ll << 30), "dt_rotary_apply: grid too large");
+    const dim3 grid = lines_of((waves + 3) / 4, &a);
     if (many) hipLaunchKernelGGL((rotary_kernel<T, 4>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((rotary_kernel<T, 1>), grid, dim3(256), 0, st, a);
     return check_launch("dt_rotary_apply");

@@ -30,6 +30,33 @@ def test_rotary_cosine_and_sine(mul):
     assert off.max().item() <= 2.0 ** -23 * f + 4 * 2.0 ** -53 * 1e5, f"2^{math.log2(off.max().item() / f):.3f} of the factor"
 
 
+@pytest.mark.parametrize("T,heads,dim,half", [(22600000, 64, 6, True), (70000000, 1, 16, False)])
+def test_rotary_of_more_threads_than_a_launch_holds(T, heads, dim, half):
+    """2^32 threads and more (a thread a pair, or a wave a token), in place: the first tokens, the last and some between."""
+    x = torch.ones((T, heads, dim), dtype=BF16, device="cuda")
+    at = torch.cat((torch.arange(200), T - 1 - torch.arange(200), torch.randint(0, T, (3000,), generator=torch.Generator().manual_seed(3)))).cuda()
+    rows = rand(4, (at.numel(), heads, dim))
+    x[at] = rows
+    rows = x[at]  # of a token drawn twice one of them
+    pos = (torch.arange(T, dtype=torch.int32, device="cuda") * 7) % 100003
+    freq = torch.rand(dim // 2, generator=torch.Generator().manual_seed(5)).cuda()
+    dh.rotary(x, None, pos, dh.Rotary(freq, half=half), q_out=x)
+    want = turned(rows, pos[at], freq, half)
+    assert ((x[at].to(F64) - want).abs() <= 2.0 ** -8 * want.abs() + 8 * 2.0 ** -24 * 12).all()  # terms of at most 6 each
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rotary_of_one_token_of_each_of_a_batch(dtype, half):
+    """[batch, 1, heads, dim] with a position each, k in the strides of a wider row: what the tokens side by side give."""
+    B, H, K, D = 37, 6, 2, 64
+    q, k = rand(7, (B, 1, H, D), dtype), rand(8, (B, 1, K, 2 * D), dtype)[..., D:]
+    pos = torch.randint(0, 100000, (B,), dtype=torch.int32, generator=torch.Generator().manual_seed(9)).cuda()
+    r = dh.Rotary(dh.rotary_freqs(D), half=half)
+    got, want = dh.rotary(q, k, pos[:, None], r), dh.rotary(q[:, 0], k[:, 0], pos, r)
+    assert torch.equal(got[0][:, 0], want[0]) and torch.equal(got[1][:, 0], want[1])
+
+
 # -------------------------------------------------------------------- cache --
 @pytest.mark.parametrize("half,rot", [(True, 64), (True, 32), (False, 64), (False, 38)])
 @pytest.mark.parametrize("mul", [1.0, 1.5, 0.75])

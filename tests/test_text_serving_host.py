@@ -212,6 +212,20 @@ def test_workspace_goes_by_sizes():
     assert 0 < ask(cache(), seqs(rows=100), 4) < ask(cache(), seqs(rows=100, table_pages=1000), 4)
 
 
+def test_launches_of_too_many_threads_are_refused():
+    """2^32 threads and more in one dimension would be cut short without an error."""
+    lib = dh.load()
+    rows = (1 << 28) - 1
+    c, s = cache(page=16, kv_heads=8), seqs(rows=rows, table_stride=1 << 26, table_pages=1 << 26)
+    a = append_args(q=None, k_strides=(512, 64), v_strides=(512, 64))
+    assert "grid too large" in refused(lib.dt_kv_append, ctypes.addressof(c), ctypes.addressof(s), ctypes.addressof(a), None)
+    c, n = cache(kv_heads=8), (1 << 20) - 1
+    for table_pages in (4, 4000):  # blocks of rows whole, and shared out
+        s = seqs(seqs=n, rows=n, table_stride=table_pages, table_pages=table_pages)
+        wide = (512 * 64, 64)
+        assert "grid too large" in refused(lib.dt_kv_attn, *attn_call(c, s, qs=wide, os_=wide, heads=512))
+
+
 # ---------------------------------------------------------- wrappers' refusals --
 def meta(dtype, *shape):
     t = torch.empty(shape, dtype=dtype)
