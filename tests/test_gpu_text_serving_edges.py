@@ -269,3 +269,20 @@ def test_tables_wider_than_what_is_held(dtype, heads, kv_heads, dim, page, seqs)
         table = torch.nn.functional.pad(pool.table, (0, wide), value=3)  # pages of others behind
         for causal in (True, False):
             check_attention(pool, q, new, past, dh.cache_attn(q, pool.cache, table, starts(new), ints(*past), causal=causal), causal)
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("wide", [0, 300])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs", [
+    (8, 2, 128, 64, [(0, 10)] * 30 + [(70, 500)] + [(0, 3)] * 39), (8, 2, 64, 16, [(0, 9), (3, 6000), (0, 0)]), (6, 6, 80, 32, [(9, 0)] + [(0, 0)] * 8),
+    (4, 1, 128, 128, [(2, 3000), (0, 5), (1, 2000), (0, 4000), (3, 1), (0, 0)]),
+])
+def test_as_many_rows_as_sequences_shared_unevenly(dtype, heads, kv_heads, dim, page, seqs, wide):
+    """What a step of one token each may become when it is replayed: the same numbers of rows and sequences, other lengths."""
+    new, past = zip(*seqs)
+    assert sum(new) == len(new)
+    pool = filled(97, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
+    table = torch.nn.functional.pad(pool.table, (0, wide), value=-1)
+    q = rand(98, (sum(new), heads, dim))
+    for causal in (True, False):
+        check_attention(pool, q, new, past, dh.cache_attn(q, pool.cache, table, starts(new), ints(*past), causal=causal), causal)
