@@ -673,9 +673,11 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  *   o_i = sum_j softmax_j(scale <q_i, k_j>) v_j
  * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
- * Operands bf16 (e4m3 codes as dt_kv_cache has them), the softmax's weights
- * rounded to bf16 for the product (their sum takes them before, or, with many rows a
- * sequence, as the product does), sums in fp32.  o: bf16; it may be q (same pointer and
+ * Operands bf16 (e4m3 codes as dt_kv_cache has them), sums in fp32.  The softmax's
+ * weights enter the product as two bf16 each (2^-16 of a weight is lost) where a
+ * sequence has up to 32 rows a key head (its new tokens times heads / kv_heads) or the
+ * call no more rows than sequences; else rounded to bf16, as their sum then takes them
+ * too.  o: bf16; it may be q (same pointer and
  * strides) and else overlaps no input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
  * aligned) is needed (0 for some calls); its size goes by the sizes given here, not by the
  * lengths on the device.  No atomics: the same call gives the same bits. */

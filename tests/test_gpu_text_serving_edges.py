@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import dit_hip as dh
-from test_gpu_text_serving import BF16, BLOCKS, F8, F32, F64, Pool, check_attention, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
+from test_gpu_text_serving import BF16, BLOCKS, F8, F32, F64, Pool, attended, check_attention, e4m3, filled, ints, power, rand, round_bf16, same, starts, turned
 
 pytestmark = pytest.mark.gpu
 
@@ -286,3 +286,27 @@ def test_as_many_rows_as_sequences_shared_unevenly(dtype, heads, kv_heads, dim, 
     q = rand(98, (sum(new), heads, dim))
     for causal in (True, False):
         check_attention(pool, q, new, past, dh.cache_attn(q, pool.cache, table, starts(new), ints(*past), causal=causal), causal)
+
+
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,seqs,wide", [
+    (32, 8, 128, 64, [(1, 1000)], 0), (8, 2, 128, 64, [(1, 1000), (1, 37), (1, 640)], 100), (16, 16, 64, 32, [(1, 2300 - 70 * b) for b in range(24)], 0),
+    (8, 1, 80, 16, [(1, 5000), (2, 300), (0, 7)], 0), (32, 8, 128, 64, [(1, 3000), (300, 0), (4, 2000), (1, 17)], 0), (4, 4, 112, 256, [(1, 4095)], 0),
+])
+def test_weights_of_few_rows_are_not_rounded_to_eight_bits(dtype, heads, kv_heads, dim, page, seqs, wide):
+    """Rows of sequences of up to 32 a key head take their weights as two bf16: 2^-16 of a weight is lost, not 2^-8."""
+    new, past = zip(*seqs)
+    pool = filled(99, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
+    table = torch.nn.functional.pad(pool.table, (0, wide), value=-1)
+    q = rand(100, (sum(new), heads, dim))
+    got = dh.cache_attn(q, pool.cache, table, starts(new), ints(*past)).to(F64)
+    for b, (n, p) in enumerate(seqs):
+        if n == 0 or n * heads // kv_heads > 32:
+            continue
+        a, (k, v) = sum(new[:b]), pool.held(b, n + p)
+        want, tol = attended(q[a:a + n], k, v, p, True, dim ** -0.5)
+        size, _ = attended(q[a:a + n], k, v.abs(), p, True, dim ** -0.5)
+        # the sums over keys have twice the terms
+        tol = tol - (2.0 ** -8 - 2.0 ** -16 - (n + p) * 2.0 ** -24) * size * (1 + 2.0 ** -7)
+        err = (got[a:a + n] - want).abs()
+        assert (err <= tol).all(), f"sequence {b}: {int((err > tol).sum())} of {err.numel()}, worst {(err / tol).max().item():.3g}"
