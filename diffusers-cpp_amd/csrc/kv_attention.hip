@@ -35,7 +35,9 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kRows = 16;      // rows of a block of the stream's
 constexpr int kShort = 1 << 18;  // bytes of a key head's keys up to which the stream's blocks of rows are not shared out
 // Beside the row blocks' kernel the stream takes sequences of up to so many rows (20 sequences of 48 rows behind 4000, 32 on
-// 8 heads of 128: 56 us, with 64 88; 9 of 24 rows: 35, with 16 32, but of 48 rows 36).
+// 8 heads of 128: 56 us, with 64 88; 9 of 24 rows: 35, with 16 32, but of 48 rows 36).  Where all are such sequences there is
+// nothing to run beside, and the stream's share of the CUs is too small (32 of 1, 2, 4 and 8 tokens behind 8000, e4m3: 66, 103,
+// 104 and 191 us): what the sequences' rows are is known on the device only.
 constexpr int kFew = 32;
 
 struct Args {
@@ -1111,16 +1113,17 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
     p.stream = !p.rows || s.seqs > 1;
     p.few = !p.rows ? INT32_MAX : p.stream ? kFew : 0;
     p.splits = 1;
-    // A workgroup's time goes by its own bytes, the stream's by all of them, with 5 to 8 us for its second launch
+    // By the table, as wide as it is: what is held is known on the device only (one token to 1001 10.9 us, with a table of 64
+    // pages of 64 16.6).  A workgroup's time goes by its own bytes, the stream's by all of them, with 5 to 8 us for its second launch
     // (32 on 8 heads of 128, whole and shared out: bf16, one token to 800 14 and 17.5 us, 8 to 1500 27 and 20; e4m3, 16
     // to 1500 17 and 21).  Blocks enough for every CU may be twice as long (e4m3, 32 tokens to 2300 23 and 30, 64
     // to 3700 54 and 64; but 24 to 3900 of 16 heads of 64 in bf16 53 and 48).
     const int64_t bytes = ((int64_t)s.table_pages << s.page_log2) * p.dp * (c.k_scale ? 1 : 2), blocks = (rows / kRows + s.seqs) * c.kv_heads;
     p.whole = !p.rows && bytes <= (blocks >= cus ? 2 : 1) * (int64_t)kShort;
     if (p.stream && !p.whole) {
-        // Two waves a SIMD in all.  Beside blocks of rows a quarter of that, and so of the CUs at most: the
-        // stream is as fast as memory, and over before the products are (the same step with all of
-        // them first 128 us).
+        // Two waves a SIMD in all.  Beside blocks of rows a quarter of that, and so of the CUs at most: where there are
+        // prompts the stream is over before the products are (with all of its waves first the step of 17 requests below
+        // took 128 us).
         p.waves = ((p.rows ? 2 : 8) * cus / c.kv_heads + 7) / 8 * 8;
         if (p.waves < 8) p.waves = 8;
         p.floats = (int64_t)c.kv_heads * p.waves * 2 * kRows * (p.dp + 2);
@@ -1133,7 +1136,7 @@ Plan plan(const Cache& c, const Seqs& s, int64_t heads, int cus) {
         // 4 x 300 behind 5000 101 and 127), but for codes in pages of less than a tile, whose 128 rows lack the
         // registers (17 requests, two of them with 512 new tokens, behind 3500, pages of 16: 112 us against 99;
         // in bf16 116 against 125, two requests alone 94 against 89).
-        const int64_t keys = (int64_t)s.table_pages << s.page_log2;
+        const int64_t keys = (int64_t)s.table_pages << s.page_log2;  // that the table has places for (see above)
         const bool many = keys >= 4096 && (rows * c.kv_heads >= 512 * (int64_t)cus || s.seqs == 1);
         p.block = many || (c.k_scale && 1 << c.page_log2 < kTile) ? 256 : 128;
         p.blocks = rows / p.block + s.seqs;

@@ -629,7 +629,7 @@ typedef struct dt_kv_cache {
 /* What a call works on: the new tokens of `seqs` sequences, side by side as `rows`
  * rows.  Rows seq_start[b] .. seq_start[b + 1] - 1 (int32 [seqs + 1], device, ascending)
  * belong to sequence b, which holds past[b] tokens already (int32 [seqs], device; below
- * 0: 0); row seq_start[b] + i is its token past[b] + i, and token t lies in page
+ * 0: 0, above 2^30: 2^30); row seq_start[b] + i is its token past[b] + i, and token t lies in page
  * table[b*table_stride + t / page] (int32 [seqs][table_pages], device), row t % page.
  * Everything about lengths is read on the device, several times over, and stays as it is
  * while the call runs: a captured launch serves other lengths and tables in place.  Rows of no sequence are neither read nor
@@ -674,13 +674,14 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
  * Operands bf16 (e4m3 codes as dt_kv_cache has them), sums in fp32.  The softmax's
- * weights enter the product as two bf16 each (2^-16 of a weight is lost) where a
- * sequence has up to 32 rows a key head (its new tokens times heads / kv_heads) or the
- * call no more rows than sequences; else rounded to bf16, as their sum then takes them
- * too.  o: bf16; it may be q (same pointer and
- * strides) and else overlaps no input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes (16-byte
- * aligned) is needed (0 for some calls); its size goes by the sizes given here, not by the
- * lengths on the device.  No atomics: the same call gives the same bits. */
+ * weights enter the product as two bf16 each (2^-16 of a weight is lost) in calls of no
+ * more rows than sequences, or of up to 32 rows times heads / kv_heads, and in calls of
+ * several sequences for those with up to 32 of these; else rounded to bf16, as their
+ * sum then takes them too.  o: bf16; it may be q (same pointer and strides) and else
+ * overlaps no input.  scale: finite, >= 0.  `workspace` of dt_kv_attn_workspace_bytes
+ * (16-byte aligned) is needed (0 for some calls); its size, and the kernels that are
+ * chosen, go by the sizes given here, not by the lengths on the device: a table no wider
+ * than a step needs is the faster one.  No atomics: the same call gives the same bits. */
 size_t dt_kv_attn_workspace_bytes(const dt_kv_cache *cache, const dt_kv_seqs *seqs, int64_t heads);
 int dt_kv_attn(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const void *q, const int64_t *q_strides, int64_t heads,
                int32_t causal, float scale, void *o, const int64_t *o_strides, void *workspace, size_t workspace_bytes,
