@@ -8,22 +8,22 @@ namespace dit {
 
 // Runs of `run` bytes at base + sum of i_k step_k, 0 <= i_k < n_k.
 struct Strided {
-    uintptr_t base;
-    int64_t run;
+    typedef __int128 wide;  // strides below 2^42 bytes times sizes below 2^30
+    wide base, run;
     int dims;
-    int64_t n[3], step[3];
+    wide n[3], step[3];
     // `count` dimensions of n elements and `strides` (in elements of es bytes) of rows of `width` elements.
     Strided(const void* p, int es, int count, const int64_t* sizes, const int64_t* strides, int64_t width)
-        : base((uintptr_t)p), run(width * es), dims(0) {
-        for (int i = 0; i < count; ++i) {  // by their steps, those of one element left out
-            if (sizes[i] == 1) continue;
+        : base((uintptr_t)p), run((wide)width * es), dims(0) {
+        for (int i = 0; i < count; ++i) {  // by their steps, those of one element, or of one element repeated, left out
+            if (sizes[i] == 1 || strides[i] == 0) continue;
             int at = dims++;
-            for (; at > 0 && step[at - 1] > strides[i] * es; --at) {
+            for (; at > 0 && step[at - 1] > (wide)strides[i] * es; --at) {
                 n[at] = n[at - 1];
                 step[at] = step[at - 1];
             }
             n[at] = sizes[i];
-            step[at] = strides[i] * es;
+            step[at] = (wide)strides[i] * es;
         }
         while (dims > 0 && step[0] == run) {  // one run after the other
             run *= n[0];
@@ -56,18 +56,18 @@ private:
 
 // True where a byte of a is shown to be one of b.  What lies apart is known at once; where the two are interleaved,
 // the distance of any two runs is b.base - a.base + sum of d_k step_k for whole d_k in a range each: the longest
-// range is solved, the others are tried, up to 4096 of them (rows of one buffer leave none to try).
+// range is solved, the others are tried, up to 4096 of them (rows of one buffer leave none to try, nor do heads in turn).
 inline bool share_memory(const Strided& a, const Strided& b) {
-    typedef __int128 wide;
-    wide a_end = (wide)a.base + a.run, b_end = (wide)b.base + b.run;
-    for (int i = 0; i < a.dims; ++i) a_end += (wide)a.step[i] * (a.n[i] - 1);
-    for (int i = 0; i < b.dims; ++i) b_end += (wide)b.step[i] * (b.n[i] - 1);
-    if ((wide)a.base >= b_end || (wide)b.base >= a_end) return false;
-    wide step[7] = {1}, lo[7] = {0}, hi[7] = {0}, d[7];  // the first: none, where there is no other
+    typedef Strided::wide wide;
+    wide a_end = a.base + a.run, b_end = b.base + b.run;
+    for (int i = 0; i < a.dims; ++i) a_end += a.step[i] * (a.n[i] - 1);
+    for (int i = 0; i < b.dims; ++i) b_end += b.step[i] * (b.n[i] - 1);
+    if (a.base >= b_end || b.base >= a_end) return false;
+    wide step[7] = {1}, lo[7] = {0}, hi[7] = {0}, tried[7] = {0};  // the first: none, where there is no other
     int dims = 1;
     for (int i = 0; i < a.dims; ++i, ++dims) {
         step[dims] = a.step[i];
-        lo[dims] = -(wide)(a.n[i] - 1);
+        lo[dims] = -(a.n[i] - 1);
         hi[dims] = 0;
     }
     for (int i = 0; i < b.dims; ++i) {
@@ -80,25 +80,40 @@ inline bool share_memory(const Strided& a, const Strided& b) {
         }
         hi[at] += b.n[i] - 1;
     }
-    int most = 0;
-    for (int i = 0; i < dims; ++i) {
-        if (step[i] > 0 && hi[i] - lo[i] > hi[most] - lo[most]) most = i;
-        d[i] = lo[i];
-    }
     auto floor_div = [](wide x, wide y) { return x / y - (x % y < 0); };
+    // Whether a distance within (-b.run, a.run) is base + a multiple of `by` that lies in [lo, hi].
+    auto meets = [&](wide base, wide by, wide lo, wide hi) {
+        const wide first = floor_div(-b.run - base, by) + 1, last = floor_div(a.run - 1 - base, by);
+        return (first < lo ? lo : first) <= (last > hi ? hi : last);
+    };
+    // Any distance is a multiple of the steps' common divisor from the bases' one: heads in turn are apart by that alone.
+    wide common = 0;
+    for (int i = 1; i < dims; ++i)
+        for (wide x = step[i]; x;) {
+            const wide y = common % x;
+            common = x;
+            x = y;
+        }
+    const wide any = (wide)1 << 100;
+    if (common && !meets(b.base - a.base, common, -any, any)) return false;
+    int most = 0;
+    for (int i = 0; i < dims; ++i)
+        if (step[i] > 0 && hi[i] - lo[i] > hi[most] - lo[most]) most = i;
+    // 0, 1, -1, 2, -2 .. until one side is done, then the rest of the other: runs of like indices meet soonest.
+    auto d_of = [&](int i) {
+        const wide c = tried[i], both = -lo[i] < hi[i] ? -lo[i] : hi[i];
+        if (c <= 2 * both) return c % 2 ? (c + 1) / 2 : -(c / 2);
+        return hi[i] > -lo[i] ? c - both : both - c;
+    };
     for (int tries = 0; tries < 4096; ++tries) {
-        wide x = (wide)b.base - (wide)a.base;
-        for (int i = 0; i < dims; ++i) x += i == most ? 0 : d[i] * step[i];
-        // Any d with -b.run < x + d step < a.run?
-        wide first = floor_div(-(wide)b.run - x, step[most]) + 1, last = floor_div((wide)a.run - 1 - x, step[most]);
-        if (first < lo[most]) first = lo[most];
-        if (last > hi[most]) last = hi[most];
-        if (first <= last) return true;
+        wide x = b.base - a.base;
+        for (int i = 0; i < dims; ++i) x += i == most ? 0 : d_of(i) * step[i];
+        if (meets(x, step[most], lo[most], hi[most])) return true;
         int i = 0;
         for (; i < dims; ++i) {
             if (i == most) continue;
-            if (++d[i] <= hi[i]) break;
-            d[i] = lo[i];
+            if (++tried[i] <= hi[i] - lo[i]) break;
+            tried[i] = 0;
         }
         if (i == dims) return false;
     }

@@ -454,6 +454,9 @@ def test_large_operands_that_share_memory(overlap):
     batch = [(2 * i * D, 2, [4, T, H], [3 * T * 2 * H * D, 2 * H * D, 2 * D], D) for i in range(2)]
     pairs = [((q, k), 0), ((k, v), 0), ((q, q), 1), ((q, flat), 1), ((k, flat), 1), ((gaps[0], gaps[1]), 0), ((gaps[0], gaps[0]), 1),
              ((gaps[0], flat), 1), ((batch[0], batch[1]), 0), ((batch[0], (2, *batch[1][1:])), 1), ((q, (2 * T * R, *flat[1:])), 0)]
+    # sizes and strides at their limits, whose products pass 64 bits
+    huge = [(at, 4, [1 << 29, 1 << 16], [(1 << 40) - 4, 1 << 35], 128) for at in (0, 4 * 128, 4 * 64)]
+    pairs += [((huge[0], huge[0]), 1), ((huge[0], huge[2]), 1), ((huge[0], (0, 4, [2, 1 << 29], [1 << 39, (1 << 40) - 4], 128)), 1)]
     assert overlap([p for p, _ in pairs]) == [(w, w) for _, w in pairs]
 
 
