@@ -397,13 +397,19 @@ struct Stream {
                     p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[mm][e / 4][e & 3], a.scale_log2, -ref));
                     l += p[e];
                 }
-                // As two bf16, rounded and what that leaves: 2^-16 of a weight is lost, not 2^-8, for 0.1 to 0.4 us (32 tokens to
-                // 8000 65.8 -> 66.2; against 64 bits 1.7e-3, the result's own rounding, instead of 2.2e-3).
-                const uint4 w = make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7]));
-                pf[mm] = __builtin_bit_cast(bf16x8_t, w);
-                pl[mm] = __builtin_bit_cast(
-                    bf16x8_t, make_uint4(pack_bf16x2(p[0] - bf16_lo(w.x), p[1] - bf16_hi(w.x)), pack_bf16x2(p[2] - bf16_lo(w.y), p[3] - bf16_hi(w.y)),
-                                         pack_bf16x2(p[4] - bf16_lo(w.z), p[5] - bf16_hi(w.z)), pack_bf16x2(p[6] - bf16_lo(w.w), p[7] - bf16_hi(w.w))));
+                // As two bf16, cut off and what that leaves: 2^-15 of a weight is lost, not 2^-8, for 0.1 to 0.4 us (32 tokens to
+                // 8000 65.8 -> 66.2; against 64 bits 1.7e-3, the result's own rounding, instead of 2.2e-3).  The second
+                // part is above 0 by 2^-23 of the weight, as 0 or less would make NaN of values that are infinite.
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x = __float_as_uint(p[2 * e]), y = __float_as_uint(p[2 * e + 1]);
+                    hi[e] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                    lo[e] = pack_bf16x2(__builtin_fmaf(p[2 * e], 1.f + 0x1p-23f, -__uint_as_float(x & 0xffff0000u)),
+                                        __builtin_fmaf(p[2 * e + 1], 1.f + 0x1p-23f, -__uint_as_float(y & 0xffff0000u)));
+                }
+                pf[mm] = __builtin_bit_cast(bf16x8_t, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                pl[mm] = __builtin_bit_cast(bf16x8_t, make_uint4(lo[0], lo[1], lo[2], lo[3]));
             }
             // What lies behind the sequence, or in no page, is anything: values of weight 0 have to be numbers.
             if (__builtin_amdgcn_ballot_w64(holds < KPL)) {

@@ -674,7 +674,7 @@ int dt_kv_append(const dt_kv_cache *cache, const dt_kv_seqs *seqs, const dt_kv_a
  * over tokens j <= i with `causal`, else over all of the sequence.  What a token that is
  * not attended to holds is not used (it may be NaN); a row without any has o = 0.
  * Operands bf16 (e4m3 codes as dt_kv_cache has them), sums in fp32.  The softmax's
- * weights enter the product as two bf16 each (2^-16 of a weight is lost) in calls of no
+ * weights enter the product as two bf16 each (2^-15 of a weight is lost) in calls of no
  * more rows than sequences, or of up to 32 rows times heads / kv_heads, and in calls of
  * several sequences for those with up to 32 of these; else rounded to bf16, as their
  * sum then takes them too.  o: bf16; it may be q (same pointer and strides) and else

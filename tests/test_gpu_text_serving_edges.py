@@ -160,6 +160,30 @@ def test_attention_of_later_tokens_beyond_bf16(page, new, past):
         assert torch.equal(got[:last], base[:last]), f"scale {scale}, code {code / 2}"
 
 
+@pytest.mark.parametrize("dtype", [F8, BF16])
+@pytest.mark.parametrize("wide", [0, 200])
+@pytest.mark.parametrize("page,new,past", [(64, (1, 1), (50, 200)), (16, (1, 2), (130, 70)), (64, (1, 1, 3), (3000, 900, 64)), (16, (40, 3), (90, 64)),
+                                           (64, (300,), (3900,)), (64, (2, 100), (700, 300)), (32, (1,), (4000,))])
+def test_attention_to_values_that_are_infinite(dtype, wide, page, new, past):
+    """An infinity that all rows see, alone in its page's dim: every row has it, and nothing else changes."""
+    lens = [n + p for n, p in zip(new, past)]
+    clean, pool = filled(62, lens, 2, 128, page, dtype), filled(62, lens, 2, 128, page, dtype)
+    q = rand(63, (sum(new), 4, 128))
+    table = torch.nn.functional.pad(pool.table, (0, wide), value=-1)
+    args = table, starts(new), ints(*past)
+    p, off = pool.rows[0][0], 7
+    for c in (clean, pool):
+        c.cache.v[p, 1] = torch.zeros((128, page), device="cuda").to(dtype)
+    base = dh.cache_attn(q, clean.cache, *args)
+    for x in (math.inf, -math.inf):
+        if dtype == F8:  # 256 times 2^120
+            pool.cache.v_scale[p, 1] = 247
+        pool.cache.v[p, 1, 77, off] = torch.tensor(math.copysign(256.0, x)).to(F8) if dtype == F8 else x
+        want = base.clone()
+        want[:new[0], 2:, 77] = x
+        same(dh.cache_attn(q, pool.cache, *args), want, f"{x}")
+
+
 def key_dims(n, D):
     """Of each place a dim, neighbours' unlike."""
     j = torch.arange(n, device="cuda")
@@ -294,7 +318,7 @@ def test_as_many_rows_as_sequences_shared_unevenly(dtype, heads, kv_heads, dim, 
     (8, 1, 80, 16, [(1, 5000), (2, 300), (0, 7)], 0), (32, 8, 128, 64, [(1, 3000), (300, 0), (4, 2000), (1, 17)], 0), (4, 4, 112, 256, [(1, 4095)], 0),
 ])
 def test_weights_of_few_rows_are_not_rounded_to_eight_bits(dtype, heads, kv_heads, dim, page, seqs, wide):
-    """Rows of sequences of up to 32 a key head take their weights as two bf16: 2^-16 of a weight is lost, not 2^-8."""
+    """Rows of sequences of up to 32 a key head take their weights as two bf16: 2^-15 of a weight is lost, not 2^-8."""
     new, past = zip(*seqs)
     pool = filled(99, [n + p for n, p in seqs], kv_heads, dim, page, dtype)
     table = torch.nn.functional.pad(pool.table, (0, wide), value=-1)
@@ -307,6 +331,6 @@ def test_weights_of_few_rows_are_not_rounded_to_eight_bits(dtype, heads, kv_head
         want, tol = attended(q[a:a + n], k, v, p, True, dim ** -0.5)
         size, _ = attended(q[a:a + n], k, v.abs(), p, True, dim ** -0.5)
         # the sums over keys have twice the terms
-        tol = tol - (2.0 ** -8 - 2.0 ** -16 - (n + p) * 2.0 ** -24) * size * (1 + 2.0 ** -7)
+        tol = tol - (2.0 ** -8 - 2.0 ** -15 - 2.0 ** -23 - (n + p) * 2.0 ** -24) * size * (1 + 2.0 ** -7)
         err = (got[a:a + n] - want).abs()
         assert (err <= tol).all(), f"sequence {b}: {int((err > tol).sum())} of {err.numel()}, worst {(err / tol).max().item():.3g}"
